@@ -269,6 +269,33 @@ int mh3_heads_partial_pool(const MH3HeadsArgs* args, const MH3CubeArgs* cubes, c
                            const float* k_w, const float* cos_t, const float* sin_t, const int32_t* map, uint16_t* q,
                            uint16_t* k, uint16_t* v, float* qc, float* kc, int32_t* counts, mh3_stream_t stream);
 
+/* ---- rotary positions with several axes ------------------------------------------------------------------------------
+ * The cos / sin tables of heads_partial made from integer positions on one to four axes (a video's time, height and
+ * width), and heads_partial with them made on the way. No counterpart in the reference, whose tables come from its host
+ * code. The rot / 2 pairs of a head go to the axes in order: the first pairs[0] to axis 0, the next pairs[1] to axis 1,
+ * ... Pair j of axis a at row r turns by
+ *   angle = pos[r][a] * step[a] * theta[a]^(-j / pairs[a])  (radians),
+ * with pos int32 [rows][axes] (device memory, any sign). The angle is taken modulo a turn in 64-bit fixed point, so far
+ * positions lose nothing: the tables are within 1e-7 of the exact cosine and sine at any int32 position for |step| up
+ * to 2 pi (a larger step loses as many bits as its turns a position have). */
+typedef struct MH3AxesArgs {
+    uint32_t axes;     /* 1 .. 4 */
+    uint32_t pairs[4]; /* rotary pairs of each axis (0 past the last axis); at most 64 in all */
+    uint32_t reserved;
+    double theta[4];   /* >= 1, finite (for the axes in use) */
+    double step[4];    /* what a position counts for: finite, |step| <= 1e6 */
+} MH3AxesArgs;
+/* cos_t and sin_t, float [rows][pairs in all], as mh3_heads_partial and mh3_heads_partial_pool read them (rot = twice
+ * the pairs). They may not overlap pos or each other (MH3_ERR_PARAM). */
+int mh3_rotary_axes(const MH3AxesArgs* args, uint32_t rows, const int32_t* pos, float* cos_t, float* sin_t,
+                    mh3_stream_t stream);
+/* mh3_rotary_axes and mh3_heads_partial in one pass with no tables in memory: the same bits as the two calls. pos is
+ * int32 [args->model_rows][axes->axes]; axes' pairs sum up to args->rot / 2 (MH3_ERR_PARAM otherwise; rot 0 takes no
+ * axes and no pos: both may be NULL). The rules of mh3_heads_partial hold, with pos in the place of the tables. */
+int mh3_heads_partial_axes(const MH3HeadsArgs* args, const MH3AxesArgs* axes, const uint16_t* qkv, const float* q_w,
+                           const float* k_w, const int32_t* pos, const int32_t* map, uint16_t* q, uint16_t* k,
+                           uint16_t* v, mh3_stream_t stream);
+
 /* ---- flash_attn_sparse_128 ---------------------------------------------------------------------------------------
  * Reference kernel `flash_attn_sparse_128` (mako-common; docs/architecture.md:123-130, docs/performance.md:162-181):
  * flash attention, head_dim 128, over the pass lists of cube_topk / cube_select. Per head h:
@@ -301,6 +328,56 @@ int mh3_flash_attn_sparse_128(const MH3AttnArgs* args, const uint16_t* q, const 
 int mh3_flash_attn_sparse_128_ordered(const MH3AttnArgs* args, const uint16_t* q, const uint16_t* k,
                                       const uint16_t* v, const int32_t* idx, const int32_t* cnt, const int32_t* order,
                                       uint16_t* out, mh3_stream_t stream);
+
+/* ---- flash_attn_128 ----------------------------------------------------------------------------------------------------
+ * Attention over whole rows, head_dim 128: a block without the sparse selection. The plain case is the reference's
+ * `flash_attn_coop_128_32` (mako-common; docs/performance.md); shared key heads, ranges, cap and bias have no counterpart
+ * in it. For query head h (key head h / (heads / kv_heads)) and query row i over the keys j in [lo_i, hi_i):
+ *   s[j] = scale q_i . k_j, under a cap (cap > 0) cap tanh(scale q_i . k_j / cap),
+ *          with slopes less slopes[h] |q_pos[i] - k_pos[j]|;
+ *   out_i = sum_j softmax(s)[j] v_j, float accumulation, rounded to bf16 once.
+ * A row without keys is zero. What lies in keys that a row does not attend has no effect on it, infinities and NaN
+ * included. Element (head, row, d) of q, k, v and out lies at head * head_stride + row * row_stride + d of each (strides
+ * in elements, multiples of 8, rows of 128 .. 2^23 - 1 elements apart), so head tiles, the model's [rows][heads * 128]
+ * order and slices of wider rows are all taken as they are.
+ *   ranges: int32 [q_rows][2], lo and hi of each query row, clamped to [0, kv_rows] (hi at least lo); 8-byte aligned;
+ *           NULL: every row attends all kv_rows. mh3_attn_ranges makes those of documents, prefixes and causal rows.
+ *   slopes: float [heads], or NULL: no bias. q_pos int32 [q_rows] and k_pos int32 [kv_rows]: both, or both NULL (the rows'
+ *           numbers); only with slopes (MH3_ERR_POINTER otherwise).
+ *   workspace: 16-byte aligned device memory of at least mh3_flash_attn_128_workspace_bytes(args) bytes (it may be 0, and
+ *           the pointer NULL; MH3_ERR_SHAPE if smaller). The call overwrites it, so calls that overlap in time, two
+ *           captured graphs among them, need their own.
+ * out may not overlap q, k, v, ranges, slopes, the positions or the workspace (each taken as the span from its start to
+ * the last row of its last head), else MH3_ERR_PARAM. */
+typedef struct MH3DenseAttnArgs {
+    uint32_t heads;    /* query heads, a multiple of kv_heads */
+    uint32_t kv_heads;
+    uint32_t head_dim; /* 128 */
+    uint32_t q_rows;   /* 0: nothing is done */
+    uint32_t kv_rows;  /* 0: every row is zero */
+    float scale;       /* score scale; 0 means 1 / sqrt(128) */
+    float cap;         /* tanh cap; 0: none */
+    uint32_t reserved;
+    uint64_t q_head_stride, q_row_stride, k_head_stride, k_row_stride;
+    uint64_t v_head_stride, v_row_stride, out_head_stride, out_row_stride;
+} MH3DenseAttnArgs;
+int64_t mh3_flash_attn_128_workspace_bytes(const MH3DenseAttnArgs* args); /* a negative code for invalid args */
+int mh3_flash_attn_128(const MH3DenseAttnArgs* args, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                       const int32_t* ranges, const float* slopes, const int32_t* q_pos, const int32_t* k_pos,
+                       void* workspace, uint64_t workspace_bytes, uint16_t* out, mh3_stream_t stream);
+/* The key ranges of documents packed into one batch. q_off and k_off (int32 [docs + 1], ascending) are the documents'
+ * first query and key rows and their ends: query rows q_off[d] .. q_off[d + 1] - 1 attend keys k_off[d] .. k_off[d + 1]
+ * - 1; rows of no document attend none. With causal 1 a document's last query row sits on its last key row and a row
+ * attends the keys up to its own, and the first prefix[d] of its document in any case (prefix int32 [docs], or NULL: no
+ * prefix; only with causal). ranges is int32 [q_rows][2], 8-byte aligned; it may not overlap an input (MH3_ERR_PARAM). */
+typedef struct MH3RangeArgs {
+    uint32_t q_rows;
+    uint32_t kv_rows; /* the ranges are clamped to [0, kv_rows] */
+    uint32_t docs;    /* >= 1 */
+    uint32_t causal;  /* 0 or 1 */
+} MH3RangeArgs;
+int mh3_attn_ranges(const MH3RangeArgs* args, const int32_t* q_off, const int32_t* k_off, const int32_t* prefix,
+                    int32_t* ranges, mh3_stream_t stream);
 
 /* ---- int8 weights: quant_rows_i8 (weight side) ---------------------------------------------------------------------
  * Reference kernel `quant_rows_i8` (mako-common; docs/performance.md:122-123, docs/architecture.md:54-56): each row
@@ -378,6 +455,34 @@ int mh3_gemm_gate_add(const MH3GemmArgs* args, uint32_t form, const void* x, con
 int mh3_gemm_gate_add_f32(const MH3GemmArgs* args, uint32_t form, const void* x, const float* x_scale, const void* w,
                           const float* w_scale, const float* gate, const uint8_t* set_of_row, float* residual,
                           mh3_stream_t stream);
+
+/* ---- 4-bit microscaled operands ----------------------------------------------------------------------------------------
+ * Products of 4-bit floats in blocks of 32 that share a power of two (OCP MX: e2m1 elements, E8M0 scales), beside the
+ * int8 forms; the reference stops at int8, so these have no counterpart in it. A matrix [rows][cols] is held as
+ *   q:     uint8 [rows][cols / 2], two values a byte, the lower column in the low half: bit 3 of a value its sign, bits
+ *          2..0 the magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6;
+ *   scale: uint8 [cols / 256][rows][8]: byte (c / 8, r, c % 8) scales columns 32 c .. 32 c + 31 of row r by
+ *          2^(byte - 127); 255 makes them NaN.
+ * mh3_quant_rows_mx4: w (float or bf16, `dtype`) to that form. A block's exponent is floor(log2(max |block|)) - 2, at
+ * least -127 (an all-zero block: -127), its values are rounded to nearest, ties to the even code, and saturate at 6; a
+ * block with an infinity or a NaN gets scale 255. cols % 256 == 0; 16-byte aligned pointers; q and scale may not overlap
+ * w or each other (MH3_ERR_PARAM). */
+int mh3_quant_rows_mx4(const MH3QuantArgs* args, const void* w, uint8_t* q, uint8_t* scale, mh3_stream_t stream);
+/* y = x w^T of two such matrices, x [m][k] and w [n][k] ([2n][k] for SwiGLU, gate rows then up rows), accumulated in
+ * float on the scaled MFMA, with the epilogues of mh3_gemm, mh3_gemm_w8a16_swiglu, mh3_gemm_gate_add and
+ * mh3_gemm_gate_add_f32. k % 256 == 0; n % 256 == 0 (n % 128 == 0 for SwiGLU); m >= 1; 16-byte aligned pointers; w, 256
+ * rows of x, and either's scales each below 2^31 bytes, else MH3_ERR_UNSUPPORTED. out (the residual) may overlap no
+ * operand (MH3_ERR_PARAM). */
+int mh3_gemm_mx4(const MH3GemmArgs* args, const uint8_t* x, const uint8_t* x_scale, const uint8_t* w,
+                 const uint8_t* w_scale, uint16_t* out, mh3_stream_t stream);
+int mh3_gemm_mx4_swiglu(const MH3GemmArgs* args, const uint8_t* x, const uint8_t* x_scale, const uint8_t* w,
+                        const uint8_t* w_scale, uint16_t* out, mh3_stream_t stream);
+int mh3_gemm_mx4_gate_add(const MH3GemmArgs* args, const uint8_t* x, const uint8_t* x_scale, const uint8_t* w,
+                          const uint8_t* w_scale, const float* gate, const uint8_t* set_of_row, uint16_t* residual,
+                          mh3_stream_t stream);
+int mh3_gemm_mx4_gate_add_f32(const MH3GemmArgs* args, const uint8_t* x, const uint8_t* x_scale, const uint8_t* w,
+                              const uint8_t* w_scale, const float* gate, const uint8_t* set_of_row, float* residual,
+                              mh3_stream_t stream);
 
 /* ---- time conditioning: the producer of the modulation table ---------------------------------------------------
  * What turns a step's distinct noise levels t = 1 - sigma (one to three in H3) into the [U][3][6][D] modulation

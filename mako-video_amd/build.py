@@ -36,7 +36,8 @@ COMMON = [
     f"-I{REPO / 'include'}",
     f"-I{CSRC}",
 ]
-SOURCES = ["rows.hip", "cond.hip", "heads.hip", "cubes.hip", "quant.hip", "gemm.hip", "attn.hip", "abi.cpp"]
+SOURCES = ["rows.hip", "cond.hip", "rotary.hip", "heads.hip", "cubes.hip", "quant.hip", "quant_mx4.hip", "gemm.hip", "gemm_mx4.hip", "attn.hip", "attn_dense.hip",
+           "abi.cpp"]
 # The streaming-bandwidth probe bench.py reports beside the kernels: its own library, not part of the C-ABI.
 PROBE_SOURCE = "probe/stream_probe.hip"
 PROBE_LIB = PKG / "lib" / "libmh3_stream_probe.so"

@@ -1,0 +1,307 @@
+// The block's products on 4-bit microscaled operands (OCP MX: blocks of 32 e2m1 values that share a power of two), on
+// v_mfma_scale_f32_16x16x128_f8f6f4, which takes both operands' block scales with them. The calls are those of the
+// int8 and bf16 forms (gemm.hip) with the same epilogues: a plain store (qkv), SwiGLU (fc1), gate_add_rows (out, fc2).
+//   y[r][c] = sum over the blocks b of 2^(sx[r][b] + sw[c][b] - 254) sum_{i in b} x[r][i] w[c][i], in float.
+//
+// Design (gfx950):
+// - The tile, the wave layout, the LDS swizzle and the XCD map are gemm_kernel's: a row of an LDS stage is 128 bytes of
+//   k, here 256 values, and one MFMA operand is 16 bytes a lane, here the 32 values of one block. So each lane has one
+//   scale byte an operand, and a K-step of 256 k is 64 MFMAs a wave with four times the bf16 kernel's products.
+// - The scale bytes come eight blocks (a K-step) of all rows at a time, [k / 256][rows][8]: a tile's are then one
+//   contiguous run a K-step, 4 bytes a lane of one DMA instruction a wave, and an operand's byte is one ds_read_u8.
+// - Both operands and their scales go out together, into a ring of stages each of which holds a whole K-step; the
+//   loads of tile kt + kStages start as soon as every wave has read tile kt, behind the barrier that publishes
+//   tile kt + 1.
+#include "gemm.hpp"
+
+#include <algorithm>
+
+namespace mh3 {
+namespace {
+
+typedef int int32x8 __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t kPastEnd = 0x80000000u; // a buffer offset past num_records: the load reads zeros
+
+template <int BM, int BN, int WM, int WN, int S>
+struct Mx4Ring {
+    static constexpr uint32_t kWaves = WM * WN, kStages = S;
+    static constexpr uint32_t kA = BM * 128u, kB = 2u * BN * 128u, kScale = kWaves * 256u; // bytes
+    static constexpr uint32_t kStage = kA + kB + 2u * kScale;
+    static constexpr size_t kEpi = size_t(BM) * gemm_epi_stride(BN) * sizeof(float);
+    static constexpr size_t kBytes = S * size_t(kStage) > kEpi ? S * size_t(kStage) : kEpi;
+    static_assert(BM * 8u <= kScale && 2u * BN * 8u <= kScale, "one scale DMA a wave covers a tile");
+    static_assert(kBytes <= 160u * 1024u, "the LDS");
+};
+
+template <int BM, int BN, int WM, int WN, int S, int EPI>
+__global__ __launch_bounds__(WM* WN * 64) void gemm_mx4_kernel(const uint8_t* __restrict__ x,
+                                                               const uint8_t* __restrict__ xs,
+                                                               const uint8_t* __restrict__ w,
+                                                               const uint8_t* __restrict__ ws,
+                                                               uint16_t* __restrict__ out, uint32_t M, uint32_t N,
+                                                               uint32_t K, uint32_t mt, uint32_t nt, GemmGate gg)
+{
+    using Ring = Mx4Ring<BM, BN, WM, WN, S>;
+    constexpr uint32_t kWaves = WM * WN;
+    constexpr int TM = BM / WM / 16, TN = BN / WN / 16; // MFMA tiles: rows, and gate (= up) columns
+    constexpr int FA = TM / 2;                          // row tiles a sub-step holds
+    static_assert(TM % 2 == 0);
+    extern __shared__ u32x4_t smem[];
+    char* const lds = reinterpret_cast<char*>(smem);
+    uint32_t tm, tn;
+    tile_of<BM>(mt, nt, tm, tn);
+    const uint32_t m0 = tm * uint32_t(BM);
+    const uint32_t w_lo = EPI == kSwiGLU ? tn * uint32_t(BN) : tn * 2u * BN;
+    const uint32_t w_hi = EPI == kSwiGLU ? N + w_lo : w_lo + uint32_t(BN);
+    const uint32_t w_rows = EPI == kSwiGLU ? 2u * N : N;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t wm = wave / WN, wn = wave % WN;
+    const uint32_t KB = K / 2u, KT = K / 256u; // bytes of a row, K-steps
+
+    // Operand loads: lane L of a wave's instruction i lands in chunk (wave AI + i) 64 + L = 8 row + physical chunk of
+    // the stage and fetches the logical chunk that the swizzle puts there. Rows past M read zeros.
+    constexpr int AI = BM * 8 / 64 / int(kWaves), BI = 2 * BN * 8 / 64 / int(kWaves);
+    static_assert(AI * 64 * int(kWaves) == BM * 8 && BI * 64 * int(kWaves) == 2 * BN * 8);
+    const uint64_t a_left = uint64_t(M - m0) * KB;
+    const __amdgpu_buffer_rsrc_t ra =
+        buffer_rsrc(x + uint64_t(m0) * KB, uint32_t(a_left < 0x7fffffffu ? a_left : 0x7fffffffu));
+    const __amdgpu_buffer_rsrc_t rb = buffer_rsrc(w, w_rows * KB);
+    uint32_t a_off[AI], b_off[BI];
+#pragma unroll
+    for (int i = 0; i < AI; ++i) {
+        const uint32_t row = (wave * AI + uint32_t(i)) * 8u + (lane >> 3), c = (lane & 7u) ^ ((row >> 1) & 7u);
+        a_off[i] = m0 + row < M ? row * KB + c * 16u : kPastEnd;
+    }
+#pragma unroll
+    for (int i = 0; i < BI; ++i) {
+        const uint32_t row = (wave * BI + uint32_t(i)) * 8u + (lane >> 3), c = (lane & 7u) ^ ((row >> 1) & 7u);
+        b_off[i] = (row < uint32_t(BN) ? w_lo + row : w_hi + (row - uint32_t(BN))) * KB + c * 16u;
+    }
+    // Scale loads: dword d = 64 wave + lane of the stage's scales is word d % 2 of row d / 2.
+    const __amdgpu_buffer_rsrc_t rsa = buffer_rsrc(xs, KT * M * 8u), rsb = buffer_rsrc(ws, KT * w_rows * 8u);
+    uint32_t sa_off, sb_off;
+    {
+        const uint32_t d = wave * 64u + lane, row = d >> 1;
+        const uint32_t wrow = row < uint32_t(BN) ? w_lo + row : w_hi + (row - uint32_t(BN));
+        sa_off = row < uint32_t(BM) && m0 + row < M ? (m0 + row) * 8u + (d & 1u) * 4u : kPastEnd;
+        sb_off = row < 2u * BN ? wrow * 8u + (d & 1u) * 4u : kPastEnd;
+    }
+    constexpr int kLoads = AI + BI + 2; // a wave's loads of one K-step
+    auto issue = [&](uint32_t kt) {
+        char* const stage = lds + (kt % S) * Ring::kStage;
+#pragma unroll
+        for (int i = 0; i < AI; ++i)
+            lds_dma16(ra, stage + (wave * AI + uint32_t(i)) * 1024u, a_off[i], int(kt * 128u));
+#pragma unroll
+        for (int i = 0; i < BI; ++i)
+            lds_dma16(rb, stage + Ring::kA + (wave * BI + uint32_t(i)) * 1024u, b_off[i], int(kt * 128u));
+        char* const sc = stage + Ring::kA + Ring::kB + wave * 256u;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr_t)sc, 4, sa_off, int(kt * M * 8u), 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb, (lds_ptr_t)(sc + Ring::kScale), 4, sb_off, int(kt * w_rows * 8u), 0,
+                                                 0);
+        __builtin_amdgcn_sched_barrier(0); // the waits count these loads
+    };
+
+    // Operands of sub-step ks (k-half h = ks / 2, the wave's row tiles (ks % 2) FA ..): 16 bytes a lane, row
+    // lane % 16 of a tile and block 4 h + lane / 16 of the K-step, and that block's scale byte.
+    // Every row a lane reads has the same swizzle, so a tile is a constant of 16 rows on.
+    const uint32_t rs = lane % 16u, kq = lane >> 4, fsx = (rs >> 1) & 7u;
+    const uint32_t arow = wm * uint32_t(BM / WM) + rs, brow = wn * 16u * TN + rs;
+    const uint32_t as_off = Ring::kA + Ring::kB + arow * 8u + kq;
+    const uint32_t bs_off = Ring::kA + Ring::kB + Ring::kScale + brow * 8u + kq;
+    uint32_t a_at[2], b_at[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        a_at[h] = arow * 128u + ((4u * h + kq) ^ fsx) * 16u;
+        b_at[h] = Ring::kA + brow * 128u + ((4u * h + kq) ^ fsx) * 16u;
+    }
+    auto frags_a = [&](uint32_t kt, uint32_t ks, u32x4_t (&fa)[FA], int (&sa)[FA]) {
+        const char* const stage = lds + (kt % S) * Ring::kStage;
+        const char* const A = stage + a_at[ks >> 1];
+        const char* const SA = stage + as_off;
+#pragma unroll
+        for (int t = 0; t < FA; ++t) {
+            const int tile = int(ks & 1u) * FA + t;
+            fa[t] = *reinterpret_cast<const u32x4_t*>(A + tile * 2048);
+            sa[t] = *reinterpret_cast<const uint8_t*>(SA + tile * 128 + 4 * int(ks >> 1));
+        }
+    };
+    auto frags_b = [&](uint32_t kt, uint32_t ks, u32x4_t (&fb)[2 * TN], int (&sb)[2 * TN]) {
+        const char* const stage = lds + (kt % S) * Ring::kStage;
+        const char* const B = stage + b_at[ks >> 1];
+        const char* const SB = stage + bs_off;
+#pragma unroll
+        for (int t = 0; t < 2 * TN; ++t) {
+            const int row = 16 * (t % TN) + (t >= TN ? BN : 0);
+            fb[t] = *reinterpret_cast<const u32x4_t*>(B + row * 128);
+            sb[t] = *reinterpret_cast<const uint8_t*>(SB + row * 8 + 4 * int(ks >> 1));
+        }
+    };
+
+    floatx4 acc[TM][2 * TN];
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < 2 * TN; ++b)
+            acc[a][b] = floatx4{};
+    u32x4_t fa[2][FA], fb[2][2 * TN]; // double buffers: A by sub-step, B by k-half
+    int sa[2][FA], sb[2][2 * TN];
+    auto widen = [](const u32x4_t& v) { return int32x8{int(v[0]), int(v[1]), int(v[2]), int(v[3]), 0, 0, 0, 0}; };
+    auto mfmas = [&](uint32_t ks, const u32x4_t (&a)[FA], const int (&as)[FA], const u32x4_t (&b)[2 * TN],
+                     const int (&bs)[2 * TN]) {
+        const int t0 = int(ks & 1u) * FA;
+#pragma unroll
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+            for (int j = 0; j < 2 * TN; ++j) // formats 4: e2m1
+                acc[t0 + i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(a[i]), widen(b[j]), acc[t0 + i][j],
+                                                                                 4, 4, 0, as[i], 0, bs[j]);
+    };
+
+    for (uint32_t t = 0; t < uint32_t(S); ++t)
+        if (t < KT)
+            issue(t);
+    if (KT >= uint32_t(S))
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm((S - 1) * kLoads));
+    else
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    asm volatile("" ::"s"(out), "s"(gg.gate), "s"(gg.set_of_row)); // no scalar load in flight in the loop
+    lds_barrier();
+    frags_a(0, 0, fa[0], sa[0]);
+    frags_b(0, 0, fb[0], sb[0]);
+    // One K-step of tile kt; more: tile kt + S exists; last: there is no tile kt + 1. No branch lies between the MFMAs (the
+    // compiler sinks them past one, to the step's end, and then spills the operands that all wait for it).
+    auto kstep = [&](uint32_t kt, auto more, auto last) {
+        constexpr bool kMore = decltype(more)::value, kLast = decltype(last)::value;
+        frags_a(kt, 1, fa[1], sa[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        mfmas(0, fa[0], sa[0], fb[0], sb[0]);
+        frags_a(kt, 2, fa[0], sa[0]);
+        frags_b(kt, 2, fb[1], sb[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        mfmas(1, fa[1], sa[1], fb[0], sb[0]);
+        frags_a(kt, 3, fa[1], sa[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        mfmas(2, fa[0], sa[0], fb[1], sb[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!kLast) {
+            // Loads complete in order: tile kt + 1 is there once only the later tiles' loads are left.
+            __builtin_amdgcn_s_waitcnt(waitcnt_vm(kMore ? (S - 2) * kLoads : 0));
+            lds_barrier();
+            frags_a(kt + 1, 0, fa[0], sa[0]);
+            frags_b(kt + 1, 0, fb[0], sb[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (kMore)
+                issue(kt + uint32_t(S)); // into the stage that every wave has read
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        mfmas(3, fa[1], sa[1], fb[1], sb[1]);
+    };
+    uint32_t kt = 0;
+    for (; kt + uint32_t(S) < KT; ++kt)
+        kstep(kt, std::true_type{}, std::false_type{});
+    for (; kt + 1u < KT; ++kt)
+        kstep(kt, std::false_type{}, std::false_type{});
+    kstep(kt, std::false_type{}, std::true_type{});
+
+    gemm_epilogue<BM, BN, WM, WN, kBf16, EPI, TM, TN>(acc, smem, M, N, m0, w_lo, w_hi, nullptr, nullptr, out, gg);
+}
+
+// The launch with tiles of BM rows and BN columns (2 BN where the epilogue pairs none).
+template <int BM, int BN, int WM, int WN, int S, int EPI>
+int launch_tile(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* xs, const uint8_t* w, const uint8_t* ws,
+                uint16_t* out, const GemmGate& gg, mh3_stream_t stream)
+{
+    const auto kernel = &gemm_mx4_kernel<BM, BN, WM, WN, S, EPI>;
+    constexpr size_t kLds = Mx4Ring<BM, BN, WM, WN, S>::kBytes;
+    if (const hipError_t e = host::allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds); e != hipSuccess)
+        return host::hip_error(e);
+    const uint32_t mt = (a->m + uint32_t(BM) - 1u) / uint32_t(BM), nt = a->n / (EPI == kSwiGLU ? BN : 2 * BN);
+    hipLaunchKernelGGL(kernel, dim3(mt * nt), dim3(WM * WN * 64), kLds, static_cast<hipStream_t>(stream), x, xs, w, ws,
+                       out, a->m, a->n, a->k, mt, nt, gg);
+    return host::check_launch();
+}
+
+// The checks of the four entry points and their launch.
+template <int EPI>
+int launch_mx4(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* xs, const uint8_t* w, const uint8_t* ws,
+               uint16_t* out, const GemmGate& gg, mh3_stream_t stream)
+{
+    constexpr uint32_t kCols = EPI == kSwiGLU ? kBN : 2u * kBN;
+    if (!a)
+        return MH3_ERR_POINTER;
+    if (a->m == 0 || a->k == 0 || a->n == 0 || a->k % 256u != 0 || a->n % kCols != 0)
+        return MH3_ERR_SHAPE;
+    const uint64_t w_rows = EPI == kSwiGLU ? 2ull * a->n : a->n;
+    if (a->m >= (1u << 31) || w_rows >= (uint64_t(1) << 31))
+        return MH3_ERR_SHAPE;
+    // 32-bit buffer offsets: a tile's rows of x, all of w, and all of either's scales.
+    if (uint64_t(a->k) / 2u * kBM >= (uint64_t(1) << 31) || w_rows * a->k / 2u >= (uint64_t(1) << 31) ||
+        uint64_t(a->m) * (a->k / 32u) >= (uint64_t(1) << 31))
+        return MH3_ERR_UNSUPPORTED;
+    if (!x || !xs || !w || !ws || !out)
+        return MH3_ERR_POINTER;
+    constexpr bool kGate = EPI == kGateAdd || EPI == kGateAddF32;
+    if (kGate && (!gg.gate || gg.n_sets == 0 || gg.n_sets > 256 || gg.gate_stride < a->n))
+        return gg.gate ? MH3_ERR_PARAM : MH3_ERR_POINTER;
+    if (!host::aligned16(x) || !host::aligned16(xs) || !host::aligned16(w) || !host::aligned16(ws) ||
+        !host::aligned16(out) || (kGate && reinterpret_cast<uintptr_t>(gg.gate) % 4u != 0u))
+        return MH3_ERR_ALIGN;
+    // The output may not overlap anything that other tiles still read.
+    const uint64_t x_bytes = uint64_t(a->m) * (a->k / 2u), w_bytes = w_rows * (a->k / 2u);
+    const host::Span in[] = {
+        {x, x_bytes},
+        {xs, x_bytes / 16u},
+        {w, w_bytes},
+        {ws, w_bytes / 16u},
+        {gg.gate, kGate ? (uint64_t(gg.n_sets) - 1u) * gg.gate_stride * 4u + a->n * 4ull : 0u},
+        {gg.set_of_row, kGate ? uint64_t(a->m) : 0u}};
+    const host::Span o[] = {{out, uint64_t(a->m) * a->n * (EPI == kGateAddF32 ? 4u : 2u)}};
+    if (host::any_overlap(in, o))
+        return MH3_ERR_PARAM;
+    const uint32_t nt = a->n / kCols;
+    if (uint64_t((a->m + 63u) / 64u) * nt * 4u >= (uint64_t(1) << 23)) // a launch holds under 2^32 threads
+        return MH3_ERR_SHAPE;
+    return launch_tile<256, kBN, 2, 4, 2, EPI>(a, x, xs, w, ws, out, gg, stream);
+}
+
+const GemmGate kNoGate{nullptr, nullptr, 0, 0};
+
+GemmGate gate_of(const MH3GemmArgs* a, const float* gate, const uint8_t* set_of_row)
+{
+    const uint32_t n_sets = a && a->n_sets ? a->n_sets : 1u;
+    const uint32_t stride = a && a->gate_stride ? a->gate_stride : (a ? a->n : 0u);
+    return GemmGate{gate, set_of_row, stride, n_sets};
+}
+
+} // namespace
+} // namespace mh3
+
+extern "C" int mh3_gemm_mx4(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* x_scale, const uint8_t* w,
+                            const uint8_t* w_scale, uint16_t* out, mh3_stream_t stream)
+{
+    return mh3::launch_mx4<mh3::kStore>(a, x, x_scale, w, w_scale, out, mh3::kNoGate, stream);
+}
+
+extern "C" int mh3_gemm_mx4_swiglu(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* x_scale, const uint8_t* w,
+                                   const uint8_t* w_scale, uint16_t* out, mh3_stream_t stream)
+{
+    return mh3::launch_mx4<mh3::kSwiGLU>(a, x, x_scale, w, w_scale, out, mh3::kNoGate, stream);
+}
+
+extern "C" int mh3_gemm_mx4_gate_add(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* x_scale, const uint8_t* w,
+                                     const uint8_t* w_scale, const float* gate, const uint8_t* set_of_row,
+                                     uint16_t* residual, mh3_stream_t stream)
+{
+    return mh3::launch_mx4<mh3::kGateAdd>(a, x, x_scale, w, w_scale, residual, mh3::gate_of(a, gate, set_of_row),
+                                          stream);
+}
+
+extern "C" int mh3_gemm_mx4_gate_add_f32(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* x_scale,
+                                         const uint8_t* w, const uint8_t* w_scale, const float* gate,
+                                         const uint8_t* set_of_row, float* residual, mh3_stream_t stream)
+{
+    return mh3::launch_mx4<mh3::kGateAddF32>(a, x, x_scale, w, w_scale, reinterpret_cast<uint16_t*>(residual),
+                                             mh3::gate_of(a, gate, set_of_row), stream);
+}

@@ -18,7 +18,9 @@
 // - A padding slot of the cube map writes zeros and reads nothing.
 // mh3_heads_partial_pool adds cube_pool to the same pass (heads_pool_kernel, some workgroups a cube): the selector's
 // cube means come from the values as they are stored, so q and k are not read back from HBM.
-#include "mh3_common.hpp"
+// mh3_heads_partial_axes makes the rows' cos / sin itself (rotary.hpp) where heads_kernel loads them from tables: 45
+// instructions for each of a row's 48 pairs, against some 30,000 values of q, k and v that the row streams.
+#include "rotary.hpp"
 
 namespace mh3 {
 namespace {
@@ -126,8 +128,11 @@ __device__ __forceinline__ void stage_weights(float* wt, const float* qw, const 
 
 // Output rows r0 .. r0 + nr - 1 (nr <= rows_per_block) by a workgroup of kHeadsThreads. LDS: the norm weights w [2][128]
 // (q, then k); the rows' model rows src [rows_per_block] (-1: padding); their cos and sin tables [rows_per_block][half]
-// each. The parameters go by value: through a reference the compiler reloads them (768p: 1.64 against 1.51 ms).
-__device__ __forceinline__ void heads_rows(const HeadsParams p, uint32_t r0, uint32_t nr, float* lds)
+// each, from the tables or computed (axes). The parameters go by value: through a reference the compiler reloads them
+// (768p: 1.64 against 1.51 ms).
+template <bool AXES = false>
+__device__ __forceinline__ void heads_rows(const HeadsParams p, uint32_t r0, uint32_t nr, float* lds,
+                                           const RotaryParams* axes = nullptr)
 {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, part = lane & 15u, group = tid >> 4;
     float* wt = lds;
@@ -145,8 +150,15 @@ __device__ __forceinline__ void heads_rows(const HeadsParams p, uint32_t r0, uin
     for (uint32_t i = tid; i < nr * p.half; i += kHeadsThreads) {
         const uint32_t r = i / p.half, c = i - r * p.half;
         const int32_t src = src_of(r);
-        ct[i] = src >= 0 ? p.cos_t[uint64_t(src) * p.half + c] : 0.0f;
-        st[i] = src >= 0 ? p.sin_t[uint64_t(src) * p.half + c] : 0.0f;
+        if constexpr (AXES) {
+            float cs, sn;
+            row_cos_sin(*axes, uint64_t(src >= 0 ? src : 0), c, cs, sn);
+            ct[i] = cs;
+            st[i] = sn;
+        } else {
+            ct[i] = src >= 0 ? p.cos_t[uint64_t(src) * p.half + c] : 0.0f;
+            st[i] = src >= 0 ? p.sin_t[uint64_t(src) * p.half + c] : 0.0f;
+        }
     }
     __syncthreads();
 
@@ -190,6 +202,13 @@ __global__ __launch_bounds__(kHeadsThreads) void heads_kernel(HeadsParams p)
     extern __shared__ float lds[];
     const uint32_t r0 = blockIdx.x * p.rows_per_block;
     heads_rows(p, r0, min(p.rows_per_block, p.rows - r0), lds);
+}
+
+__global__ __launch_bounds__(kHeadsThreads) void heads_axes_kernel(HeadsParams p, RotaryParams axes)
+{
+    extern __shared__ float lds[];
+    const uint32_t r0 = blockIdx.x * p.rows_per_block;
+    heads_rows<true>(p, r0, min(p.rows_per_block, p.rows - r0), lds, &axes);
 }
 
 // heads_partial fused with cube_pool over its output: a workgroup (512 threads) per cube and 8 consecutive head vectors
@@ -355,10 +374,11 @@ namespace {
 
 using namespace mh3;
 
-// The checks of mh3_heads_partial and the kernel parameters they give.
+// The checks of mh3_heads_partial and the kernel parameters they give. Under axes there are positions in the place of
+// the tables.
 int heads_setup(const MH3HeadsArgs* args, const uint16_t* qkv, const float* q_w, const float* k_w,
                 const float* cos_t, const float* sin_t, const int32_t* map, uint16_t* q, uint16_t* k, uint16_t* v,
-                HeadsParams& p)
+                HeadsParams& p, const MH3AxesArgs* axes = nullptr, const int32_t* pos = nullptr)
 {
     if (!args)
         return MH3_ERR_POINTER;
@@ -375,11 +395,12 @@ int heads_setup(const MH3HeadsArgs* args, const uint16_t* qkv, const float* q_w,
         return MH3_OK;
     if (a.rows >= (1u << 31) || a.model_rows == 0 || a.model_rows >= (1u << 31) || (!map && a.model_rows < a.rows))
         return MH3_ERR_SHAPE;
-    if (!qkv || !q || !k || (a.rot && (!cos_t || !sin_t)))
+    if (!qkv || !q || !k || (a.rot && (axes ? !pos : !cos_t || !sin_t)))
         return MH3_ERR_POINTER;
     if (a.qkv_stride % 8 != 0 || a.out_head_stride % 8 != 0 || a.out_row_stride % 8 != 0 || !host::aligned16(qkv) ||
         !host::aligned16(q) || !host::aligned16(k) || (v && !host::aligned16(v)) ||
-        (q_w && !host::aligned16(q_w)) || (k_w && !host::aligned16(k_w)))
+        (q_w && !host::aligned16(q_w)) || (k_w && !host::aligned16(k_w)) ||
+        (axes && reinterpret_cast<uintptr_t>(pos) % 4u != 0u))
         return MH3_ERR_ALIGN;
     // Outputs over qkv only in place: each output at its own input's position.
     const uint64_t qkv_bytes = ((uint64_t(a.model_rows) - 1) * a.qkv_stride + 3ull * a.heads * 128u) * 2u;
@@ -397,7 +418,8 @@ int heads_setup(const MH3HeadsArgs* args, const uint16_t* qkv, const float* q_w,
     // Nor may an output overlap the norm weights, the rotary tables or the map.
     const uint64_t tab = a.rot ? uint64_t(a.model_rows) * (a.rot / 2u) * 4u : 0u;
     const host::Span small_in[] = {
-        {q_w, 512u}, {k_w, 512u}, {cos_t, tab}, {sin_t, tab}, {map, map ? uint64_t(a.rows) * 4u : 0u}};
+        {q_w, 512u}, {k_w, 512u}, {cos_t, tab}, {sin_t, tab}, {map, map ? uint64_t(a.rows) * 4u : 0u},
+        {pos, axes ? uint64_t(a.model_rows) * axes->axes * 4u : 0u}};
     for (int t = 0; t < 3; ++t) {
         const host::Span o[] = {{outs[t], out_bytes}};
         if (host::any_overlap(small_in, o))
@@ -418,6 +440,25 @@ int heads_setup(const MH3HeadsArgs* args, const uint16_t* qkv, const float* q_w,
     return MH3_OK;
 }
 
+// The launch of heads_kernel, or under axes of heads_axes_kernel.
+int launch_heads(const HeadsParams& p, const RotaryParams* axes, mh3_stream_t stream)
+{
+    const uint64_t blocks = (uint64_t(p.rows) + p.rows_per_block - 1) / p.rows_per_block;
+    size_t lds = (256u + ((p.rows_per_block + 3u) & ~3u) + 2u * size_t(p.rows_per_block) * p.half) * sizeof(float);
+    if (lds < kHeadsLdsFloor)
+        lds = kHeadsLdsFloor;
+    const void* kernel =
+        axes ? reinterpret_cast<const void*>(&heads_axes_kernel) : reinterpret_cast<const void*>(&heads_kernel);
+    if (const hipError_t e = host::allow_dynamic_lds(kernel, lds); e != hipSuccess)
+        return host::hip_error(e);
+    const dim3 grid{uint32_t(blocks)}, block{kHeadsThreads};
+    if (axes)
+        hipLaunchKernelGGL(heads_axes_kernel, grid, block, lds, static_cast<hipStream_t>(stream), p, *axes);
+    else
+        hipLaunchKernelGGL(heads_kernel, grid, block, lds, static_cast<hipStream_t>(stream), p);
+    return host::check_launch();
+}
+
 } // namespace
 
 extern "C" int mh3_heads_partial(const MH3HeadsArgs* args, const uint16_t* qkv, const float* q_w, const float* k_w,
@@ -428,15 +469,28 @@ extern "C" int mh3_heads_partial(const MH3HeadsArgs* args, const uint16_t* qkv, 
     const int rc = heads_setup(args, qkv, q_w, k_w, cos_t, sin_t, map, q, k, v, p);
     if (rc != MH3_OK || args->rows == 0)
         return rc;
-    const uint64_t blocks = (uint64_t(p.rows) + p.rows_per_block - 1) / p.rows_per_block;
-    size_t lds = (256u + ((p.rows_per_block + 3u) & ~3u) + 2u * size_t(p.rows_per_block) * p.half) * sizeof(float);
-    if (lds < kHeadsLdsFloor)
-        lds = kHeadsLdsFloor;
-    if (const hipError_t e = host::allow_dynamic_lds(reinterpret_cast<const void*>(&heads_kernel), lds); e != hipSuccess)
-        return host::hip_error(e);
-    hipLaunchKernelGGL(heads_kernel, dim3(uint32_t(blocks)), dim3(kHeadsThreads), lds, static_cast<hipStream_t>(stream),
-                       p);
-    return host::check_launch();
+    return launch_heads(p, nullptr, stream);
+}
+
+extern "C" int mh3_heads_partial_axes(const MH3HeadsArgs* args, const MH3AxesArgs* axes, const uint16_t* qkv,
+                                      const float* q_w, const float* k_w, const int32_t* pos, const int32_t* map,
+                                      uint16_t* q, uint16_t* k, uint16_t* v, mh3_stream_t stream)
+{
+    if (!args)
+        return MH3_ERR_POINTER;
+    const MH3AxesArgs* const ax = args->rot ? axes : nullptr;
+    RotaryParams rp{};
+    if (args->rot) {
+        if (args->rot % 16u != 0 || args->rot > 2u * kMaxRotPairs)
+            return MH3_ERR_PARAM;
+        if (const int rc = host::rotary_setup(axes, pos, args->rot / 2u, rp); rc != MH3_OK)
+            return rc;
+    }
+    HeadsParams p;
+    const int rc = heads_setup(args, qkv, q_w, k_w, nullptr, nullptr, map, q, k, v, p, ax, pos);
+    if (rc != MH3_OK || args->rows == 0)
+        return rc;
+    return launch_heads(p, ax ? &rp : nullptr, stream);
 }
 
 extern "C" int mh3_heads_partial_pool(const MH3HeadsArgs* args, const MH3CubeArgs* cubes, const uint16_t* qkv,

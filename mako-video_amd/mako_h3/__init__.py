@@ -56,6 +56,21 @@ class HeadsArgs(C.Structure):
                 ("out_row_stride", C.c_uint64)]
 
 
+class AxesArgs(C.Structure):
+    _fields_ = [("axes", C.c_uint32), ("pairs", C.c_uint32 * 4), ("reserved", C.c_uint32), ("theta", C.c_double * 4),
+                ("step", C.c_double * 4)]
+
+
+class DenseAttnArgs(C.Structure):
+    _fields_ = [("heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("q_rows", C.c_uint32),
+                ("kv_rows", C.c_uint32), ("scale", C.c_float), ("cap", C.c_float), ("reserved", C.c_uint32)] + \
+               [(f"{t}_{d}_stride", C.c_uint64) for t in ("q", "k", "v", "out") for d in ("head", "row")]
+
+
+class RangeArgs(C.Structure):
+    _fields_ = [("q_rows", C.c_uint32), ("kv_rows", C.c_uint32), ("docs", C.c_uint32), ("causal", C.c_uint32)]
+
+
 class CubeMapArgs(C.Structure):
     _fields_ = [("grid_t", C.c_uint32), ("grid_h", C.c_uint32), ("grid_w", C.c_uint32), ("n_dense", C.c_uint32),
                 ("video_row0", C.c_uint64), ("dense_row0", C.c_uint64)]
@@ -113,6 +128,16 @@ def _load() -> C.CDLL:
         "mh3_heads_partial_pool": (I32, [C.POINTER(HeadsArgs), C.POINTER(CubeArgs)] + [P] * 13),
         "mh3_flash_attn_sparse_128": (I32, [C.POINTER(AttnArgs), P, P, P, P, P, P, P]),
         "mh3_flash_attn_sparse_128_ordered": (I32, [C.POINTER(AttnArgs), P, P, P, P, P, P, P, P]),
+        "mh3_rotary_axes": (I32, [C.POINTER(AxesArgs), U32, P, P, P, P]),
+        "mh3_heads_partial_axes": (I32, [C.POINTER(HeadsArgs), C.POINTER(AxesArgs)] + [P] * 9),
+        "mh3_flash_attn_128_workspace_bytes": (I64, [C.POINTER(DenseAttnArgs)]),
+        "mh3_flash_attn_128": (I32, [C.POINTER(DenseAttnArgs)] + [P] * 8 + [C.c_uint64, P, P]),
+        "mh3_attn_ranges": (I32, [C.POINTER(RangeArgs), P, P, P, P, P]),
+        "mh3_quant_rows_mx4": (I32, [C.POINTER(QuantArgs), P, P, P, P]),
+        "mh3_gemm_mx4": (I32, [C.POINTER(GemmArgs), P, P, P, P, P, P]),
+        "mh3_gemm_mx4_swiglu": (I32, [C.POINTER(GemmArgs), P, P, P, P, P, P]),
+        "mh3_gemm_mx4_gate_add": (I32, [C.POINTER(GemmArgs), P, P, P, P, P, P, P, P]),
+        "mh3_gemm_mx4_gate_add_f32": (I32, [C.POINTER(GemmArgs), P, P, P, P, P, P, P, P]),
         "mh3_quant_rows_i8": (I32, [C.POINTER(QuantArgs), P, P, P, P]),
         "mh3_gemm_w8a16_swiglu": (I32, [C.POINTER(GemmArgs), P, P, P, P, P]),
         "mh3_gemm_bf16_swiglu": (I32, [C.POINTER(GemmArgs), P, P, P, P]),
@@ -162,6 +187,31 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int) -> None:
         raise ValueError(f"{name}: must be contiguous")
     if t.numel() < numel:
         raise ValueError(f"{name}: {t.numel()} elements, the call touches {numel}")
+
+
+def _one_device(**tensors: torch.Tensor | None) -> torch.device:
+    """The GPU that all of the tensors (None skipped) are on."""
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a tensor")
+        if t.device.type != "cuda":
+            raise ValueError(f"{name}: must be on the GPU")
+        if device is not None and t.device != device:
+            raise ValueError(f"{name}: on {t.device}, other operands on {device}")
+        device = t.device
+    return device
+
+
+def _on(device: torch.device, call, what: str) -> None:
+    """call(stream) on `device` as the current one, with its current stream."""
+    if device.index == torch.cuda.current_device():
+        _check(call(_stream()), what)
+    else:
+        with torch.cuda.device(device):
+            _check(call(_stream()), what)
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -603,6 +653,160 @@ def heads_partial_pool(qkv, heads, grid, q_w=None, k_w=None, cos_t=None, sin_t=N
     return (*outs, qc, kc)
 
 
+# ---- rotary positions with several axes ------------------------------------------------------------------------------
+
+def _axes_args(pos, pairs, theta, step) -> AxesArgs:
+    axes = len(pairs)
+    if not 1 <= axes <= 4:
+        raise ValueError("one to four axes")
+    theta = (theta,) * axes if isinstance(theta, (int, float)) else tuple(theta)
+    step = (step,) * axes if isinstance(step, (int, float)) else tuple(step)
+    if len(theta) != axes or len(step) != axes:
+        raise ValueError("theta and step: one value, or one an axis")
+    if pos.dim() != 2 or pos.shape[1] != axes:
+        raise ValueError(f"pos must be [rows][{axes}]")
+    if any(int(n) != n or not 0 <= n <= 64 for n in pairs):
+        raise ValueError("pairs: 0 to 64 an axis")
+    _need(pos, "pos", torch.int32, pos.numel())
+    a = AxesArgs()
+    a.axes = axes
+    for i in range(axes):
+        a.pairs[i], a.theta[i], a.step[i] = int(pairs[i]), theta[i], step[i]
+    return a
+
+
+def rotary_axes(pos, pairs, *, theta=10000.0, step=1.0, cos=None, sin=None):
+    """The cos / sin tables of heads_partial from positions on one to four axes (time, height, width): pos int32
+    [rows][axes], the first pairs[0] of a head's pairs turned by axis 0, the next pairs[1] by axis 1, ...; pair j of
+    axis a by pos[:, a] step[a] theta[a]^(-j / pairs[a]) radians. Returns (cos, sin), float [rows][sum(pairs)]."""
+    a = _axes_args(pos, pairs, theta, step)
+    rows, half = pos.shape[0], sum(int(n) for n in pairs)
+    cos = torch.empty((rows, half), dtype=torch.float32, device=pos.device) if cos is None else cos
+    sin = torch.empty((rows, half), dtype=torch.float32, device=pos.device) if sin is None else sin
+    _need(cos, "cos", torch.float32, rows * half)
+    _need(sin, "sin", torch.float32, rows * half)
+    _on(_one_device(pos=pos, cos=cos, sin=sin),
+        lambda s: lib.mh3_rotary_axes(C.byref(a), rows, _ptr(pos), _ptr(cos), _ptr(sin), s), "rotary_axes")
+    return cos, sin
+
+
+def heads_partial_axes(qkv, heads, pos, pairs, q_w=None, k_w=None, *, theta=10000.0, step=1.0, eps=1e-6, map=None,
+                       with_v=True, layout="heads", q=None, k=None, v=None):
+    """heads_partial with the rotary positions of rotary_axes (pos int32 [model_rows][axes], rot = 2 sum(pairs)), in one
+    pass with no tables in memory: the same bits as the two calls. Returns (q, k, v)."""
+    ax = _axes_args(pos, pairs, theta, step)
+    if qkv.dim() == 2 and pos.shape[0] != qkv.shape[0]:
+        raise ValueError("pos: one row a row of qkv")
+    rot = 2 * sum(int(n) for n in pairs)
+    device = _one_device(qkv=qkv, pos=pos, q_w=q_w, k_w=k_w, map=map, q=q, k=k, v=v)
+    a, outs, ptrs = _heads_setup(qkv, heads, q_w, k_w, None, None, 0, eps, map, with_v, layout, q, k, v)
+    a.rot = rot
+    _on(device, lambda s: lib.mh3_heads_partial_axes(C.byref(a), C.byref(ax), *ptrs[:3], _ptr(pos), ptrs[5],
+                                                     *(_ptr(t) for t in outs), s), "heads_partial_axes")
+    return tuple(outs)
+
+
+# ---- flash_attn_128 --------------------------------------------------------------------------------------------------
+
+def _head_rows(t, name, layout):
+    """(heads, rows, head stride, row stride) of bf16 head rows: "heads" [heads][rows][128], "rows" [rows][heads * 128],
+    either with any strides of multiples of 8 elements and the last dimension contiguous."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor")
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected {torch.bfloat16}")
+    if t.dim() != (3 if layout == "heads" else 2):
+        raise ValueError(f"{name}: [heads][rows][128] for layout 'heads', [rows][heads * 128] for 'rows'")
+    if t.shape[-1] and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    if layout == "heads":
+        if t.shape[2] != 128:
+            raise ValueError(f"{name}: rows of 128 values")
+        # A dimension of one element may carry any stride: it is never stepped over.
+        return (t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 128)
+    if t.shape[1] == 0 or t.shape[1] % 128:
+        raise ValueError(f"{name}: rows of heads * 128 values")
+    return t.shape[1] // 128, t.shape[0], 128, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def attn_ranges(q_off, k_off, q_rows, kv_rows, *, prefix=None, causal=False, ranges=None):
+    """The key range of each query row for documents packed into one batch -> int32 [q_rows][2], flash_attn_128's
+    `ranges`. q_off and k_off int32 [docs + 1]: query rows q_off[d] .. q_off[d + 1] - 1 attend keys k_off[d] ..
+    k_off[d + 1] - 1; rows of no document none. causal: a document's last query row sits on its last key row and a row
+    attends the keys up to its own, and its document's first prefix[d] (int32 [docs]) in any case."""
+    docs = q_off.numel() - 1
+    _need(q_off, "q_off", torch.int32, docs + 1)
+    _need(k_off, "k_off", torch.int32, docs + 1)
+    if prefix is not None:
+        _need(prefix, "prefix", torch.int32, docs)
+    ranges = torch.empty((q_rows, 2), dtype=torch.int32, device=q_off.device) if ranges is None else ranges
+    _need(ranges, "ranges", torch.int32, 2 * q_rows)
+    if docs < 1:
+        raise ValueError("q_off: at least one document")
+    a = RangeArgs()
+    a.q_rows, a.kv_rows, a.docs, a.causal = q_rows, kv_rows, docs, int(bool(causal))
+    _on(_one_device(q_off=q_off, k_off=k_off, prefix=prefix, ranges=ranges),
+        lambda s: lib.mh3_attn_ranges(C.byref(a), _ptr(q_off), _ptr(k_off), _ptr(prefix), _ptr(ranges), s),
+        "attn_ranges")
+    return ranges
+
+
+def _dense_args(q, k, v, out, layout, out_layout, scale, cap) -> DenseAttnArgs:
+    heads, q_rows, qhs, qrs = _head_rows(q, "q", layout)
+    kv_heads, kv_rows, khs, krs = _head_rows(k, "k", layout)
+    if _head_rows(v, "v", layout)[:2] != (kv_heads, kv_rows):
+        raise ValueError("k and v: the same heads and rows")
+    if _head_rows(out, "out", out_layout)[:2] != (heads, q_rows):
+        raise ValueError("out: q's heads and rows")
+    a = DenseAttnArgs()
+    a.heads, a.kv_heads, a.head_dim, a.q_rows, a.kv_rows, a.scale, a.cap = heads, kv_heads, 128, q_rows, kv_rows, scale, cap
+    a.q_head_stride, a.q_row_stride, a.k_head_stride, a.k_row_stride = qhs, qrs, khs, krs
+    a.v_head_stride, a.v_row_stride = _head_rows(v, "v", layout)[2:]
+    a.out_head_stride, a.out_row_stride = _head_rows(out, "out", out_layout)[2:]
+    return a
+
+
+def flash_attn_128_workspace_bytes(q, k, v, *, layout="heads") -> int:
+    """Bytes of workspace that flash_attn_128 needs for these operands (0 where it needs none)."""
+    n = int(lib.mh3_flash_attn_128_workspace_bytes(C.byref(_dense_args(q, k, v, q, layout, layout, 0.0, 0.0))))
+    _check(min(n, 0), "flash_attn_128_workspace_bytes")
+    return n
+
+
+def flash_attn_128(q, k, v, *, ranges=None, scale=0.0, cap=0.0, slopes=None, q_pos=None, k_pos=None, layout="heads",
+                   out=None, out_layout=None, workspace=None):
+    """Attention over whole rows, head_dim 128, bf16: out_i = softmax_j(s_ij) v over the keys of ranges[i] (int32
+    [q_rows][2], [lo, hi); None: all), s = scale q k, under a cap cap tanh(s / cap), less slopes[h] |q_pos_i - k_pos_j|
+    (float [heads], int32 [q_rows] and [kv_rows], None: the rows' numbers). Fewer key heads than query heads are shared
+    in order; scale 0 is 1 / sqrt(128); a row without keys is zero. layout "heads": [heads][rows][128], "rows":
+    [rows][heads * 128] (slices of wider rows too); out_layout: out's, the same by default. `workspace` (uint8, at least
+    flash_attn_128_workspace_bytes) is allocated here when None. Returns out."""
+    out_layout = layout if out_layout is None else out_layout
+    if layout not in ("heads", "rows") or out_layout not in ("heads", "rows"):
+        raise ValueError("layout is 'heads' or 'rows'")
+    heads, q_rows = _head_rows(q, "q", layout)[:2]
+    device = _one_device(q=q, k=k, v=v, ranges=ranges, slopes=slopes, q_pos=q_pos, k_pos=k_pos, out=out,
+                         workspace=workspace)
+    if out is None:
+        out = torch.empty((heads, q_rows, 128) if out_layout == "heads" else (q_rows, heads * 128),
+                          dtype=torch.bfloat16, device=device)
+    a = _dense_args(q, k, v, out, layout, out_layout, scale, cap)
+    for name, t, dtype, n in (("ranges", ranges, torch.int32, 2 * q_rows), ("slopes", slopes, torch.float32, heads),
+                              ("q_pos", q_pos, torch.int32, q_rows), ("k_pos", k_pos, torch.int32, a.kv_rows)):
+        if t is not None:
+            _need(t, name, dtype, n)
+    nbytes = int(lib.mh3_flash_attn_128_workspace_bytes(C.byref(a)))
+    _check(min(nbytes, 0), "flash_attn_128")
+    if workspace is None and nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if workspace is not None:
+        _need(workspace, "workspace", torch.uint8, nbytes)
+    _on(device, lambda s: lib.mh3_flash_attn_128(
+        C.byref(a), _ptr(q), _ptr(k), _ptr(v), _ptr(ranges), _ptr(slopes), _ptr(q_pos), _ptr(k_pos), _ptr(workspace),
+        0 if workspace is None else workspace.numel(), _ptr(out), s), "flash_attn_128")
+    return out
+
+
 # ---- flash_attn_sparse_128 -------------------------------------------------------------------------------------------
 
 def flash_attn_sparse_128(a: CubeArgs, q, k, v, idx, cnt, *, dense_row0=0, n_dense=0, scale=0.0, out=None,
@@ -762,4 +966,79 @@ def gemm_gate_add(x, w, residual, gate, *, x_scale=None, w_scale=None, set_of_ro
     _check(fn(C.byref(a), form, _ptr(x), _ptr(x_scale if form == GEMM_W8A8 else None), _ptr(w),
               _ptr(w_scale if form != GEMM_BF16 else None), _ptr(gate), _ptr(set_of_row), _ptr(residual), _stream()),
            "gemm_gate_add")
+    return residual
+
+
+# ---- 4-bit microscaled operands --------------------------------------------------------------------------------------
+
+def quant_rows_mx4(w, *, q=None, scale=None):
+    """Each row to 4-bit floats in blocks of 32 columns that share a power of two (OCP MX: e2m1, E8M0): w f32 or bf16
+    [rows][cols], cols % 256 == 0 -> (q uint8 [rows][cols / 2], the lower column in a byte's low half; scale uint8
+    [cols / 256][rows][8], byte (c / 8, r, c % 8) scaling columns 32 c .. of row r by 2^(byte - 127))."""
+    if w.dim() != 2:
+        raise ValueError("w must be [rows][cols]")
+    a = QuantArgs()
+    a.rows, a.cols, a.dtype = w.shape[0], w.shape[1], _dt(w)
+    if a.cols == 0 or a.cols % 256:
+        raise ValueError("cols must be a multiple of 256")
+    _need(w, "w", w.dtype, w.numel())
+    q = torch.empty((a.rows, a.cols // 2), dtype=torch.uint8, device=w.device) if q is None else q
+    scale = torch.empty((a.cols // 256, a.rows, 8), dtype=torch.uint8, device=w.device) if scale is None else scale
+    _need(q, "q", torch.uint8, w.numel() // 2)
+    _need(scale, "scale", torch.uint8, w.numel() // 32)
+    _on(_one_device(w=w, q=q, scale=scale),
+        lambda s: lib.mh3_quant_rows_mx4(C.byref(a), _ptr(w), _ptr(q), _ptr(scale), s), "quant_rows_mx4")
+    return q, scale
+
+
+def _mx4_args(x, x_scale, w, w_scale) -> GemmArgs:
+    if x.dim() != 2 or w.dim() != 2 or w.shape[1] != x.shape[1]:
+        raise ValueError("x must be [m][k / 2] and w [n][k / 2]")
+    m, half = x.shape
+    n = w.shape[0]
+    for name, t, numel in (("x", x, m * half), ("x_scale", x_scale, m * half // 16), ("w", w, n * half),
+                           ("w_scale", w_scale, n * half // 16)):
+        _need(t, name, torch.uint8, numel)
+    a = GemmArgs()
+    a.m, a.n, a.k = m, n, 2 * half
+    return a
+
+
+def gemm_mx4(x, x_scale, w, w_scale, *, out=None):
+    """out = x w^T of two matrices as quant_rows_mx4 leaves them (x [m][k], w [n][k]), bf16 [m][n]."""
+    a = _mx4_args(x, x_scale, w, w_scale)
+    out = torch.empty((a.m, a.n), dtype=torch.bfloat16, device=x.device) if out is None else out
+    _need(out, "out", torch.bfloat16, a.m * a.n)
+    _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, out=out),
+        lambda s: lib.mh3_gemm_mx4(C.byref(a), _ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(out), s), "gemm_mx4")
+    return out
+
+
+def gemm_mx4_swiglu(x, x_scale, w, w_scale, *, out=None):
+    """fc1 + SwiGLU: w [2n][k] (gate rows then up rows), out = silu(x Wg^T) * (x Wu^T), bf16 [m][n]."""
+    a = _mx4_args(x, x_scale, w, w_scale)
+    if a.n % 2:
+        raise ValueError("w must be [2n][k / 2]")
+    a.n //= 2
+    out = torch.empty((a.m, a.n), dtype=torch.bfloat16, device=x.device) if out is None else out
+    _need(out, "out", torch.bfloat16, a.m * a.n)
+    _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, out=out),
+        lambda s: lib.mh3_gemm_mx4_swiglu(C.byref(a), _ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(out), s),
+        "gemm_mx4_swiglu")
+    return out
+
+
+def gemm_mx4_gate_add(x, x_scale, w, w_scale, residual, gate, *, set_of_row=None, n_sets=1):
+    """The out projection and fc2 with gate_add_rows folded in: residual += gate[s] * (x w^T), [m][n] in place, bf16 or
+    float; gate and set_of_row as gemm_gate_add takes them. Returns residual."""
+    a = _mx4_args(x, x_scale, w, w_scale)
+    f32 = residual.dtype == torch.float32
+    _need(residual, "residual", torch.float32 if f32 else torch.bfloat16, a.m * a.n)
+    a.n_sets, a.gate_stride = n_sets, _set_stride(gate, "gate", a.n, n_sets)
+    if set_of_row is not None:
+        _need(set_of_row, "set_of_row", torch.uint8, a.m)
+    fn = lib.mh3_gemm_mx4_gate_add_f32 if f32 else lib.mh3_gemm_mx4_gate_add
+    _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, residual=residual, gate=gate, set_of_row=set_of_row),
+        lambda s: fn(C.byref(a), _ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(gate), _ptr(set_of_row),
+                     _ptr(residual), s), "gemm_mx4_gate_add")
     return residual
