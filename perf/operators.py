@@ -27,6 +27,8 @@ E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
 def _lib():
+    if "mako_h3" in sys.modules:
+        return sys.modules["mako_h3"]
     root = str(Path(__file__).resolve().parent.parent / "mako-video_amd")
     if root not in sys.path:
         sys.path.insert(0, root)
