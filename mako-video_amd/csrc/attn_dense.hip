@@ -35,8 +35,6 @@ typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
-constexpr uint32_t kPastEnd = 0x80000000u; // a buffer offset past num_records: the load reads zeros
-constexpr uint32_t kRecords = 0x7fffffffu;
 constexpr uint32_t kTileBytes = 16384; // 64 keys of K, or of V
 
 struct DenseParams {
@@ -77,6 +75,17 @@ __device__ __forceinline__ void lds_barrier()
     asm volatile("" ::: "memory");
 }
 
+// 16 or 4 bytes a lane from a buffer straight into LDS, lane L's at lds + 16 L or 4 L. (Not in templates: the host's pass
+// checks the size again at each instantiation, as of its own target, and leaves the kernel out without a word.)
+__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t offset)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)lds, 16, offset, 0, 0, 0);
+}
+__device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t offset)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)lds, 4, offset, 0, 0, 0);
+}
+
 // The keys [lo, hi) of list row f, within [0, kv_rows]; none for a row past the list.
 __device__ __forceinline__ void range_of(const DenseParams& p, uint32_t f, uint32_t row, uint32_t& lo, uint32_t& hi)
 {
@@ -88,48 +97,34 @@ __device__ __forceinline__ void range_of(const DenseParams& p, uint32_t f, uint3
     }
 }
 
-// The sources of a wave's DMA instructions. Instruction i of a tile's 16 fills the LDS kilobyte 1024 i with keys
-// 4 i .. 4 i + 3: of K 256-byte rows whose 16-byte chunks are XOR-swizzled by the row, of V the four keys' 64-byte
-// pieces interleaved (so that operand and transposed reads hit distinct banks); each quad of lanes fetches one aligned
-// 64-byte piece of a row.
+// N of a tile's 16 DMA instructions of K (VALUE false) or V, the ones from i0 on. Instruction i fills the LDS kilobyte
+// 1024 i with keys 4 i .. 4 i + 3: of K 256-byte rows whose 16-byte chunks are XOR-swizzled by the row, of V the four keys'
+// 64-byte pieces interleaved (so that operand and transposed reads hit distinct banks); each quad of lanes fetches one
+// aligned 64-byte piece of a row. The descriptor ends behind the last key, so keys past it read zeros.
+template <int N, bool VALUE>
 struct TileLoads {
-    uint32_t k_row, v_key, k_off[4], v_off;
-    __device__ __forceinline__ TileLoads(const DenseParams& p, uint32_t lane)
+    const uint16_t* head;
+    uint64_t stride; // elements between keys
+    uint32_t off[N], i0;
+    __device__ __forceinline__ TileLoads(const uint16_t* h, uint64_t s, uint32_t first, uint32_t lane)
+        : head(h), stride(s), i0(first)
     {
-        k_row = lane >> 4, v_key = (lane >> 2) & 3u;
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u)
-            k_off[u] = k_row * uint32_t(p.krs) * 2u + 16u * ((lane & 15u) ^ (4u * u + k_row));
-        v_off = v_key * uint32_t(p.vrs) * 2u + 16u * (4u * (lane >> 4) + (lane & 3u));
-    }
-    // Instructions i0 .. i0 + N - 1 of the K or V tile at key t0, `live` of whose 64 keys exist.
-    template <int N>
-    __device__ __forceinline__ void k_tile(const DenseParams& p, const uint16_t* kh, char* dst, uint32_t t0, uint32_t i0,
-                                           uint32_t live) const
-    {
-        const __amdgpu_buffer_rsrc_t r = buffer_rsrc(kh + uint64_t(t0) * p.krs, kRecords);
 #pragma unroll
         for (uint32_t u = 0; u < uint32_t(N); ++u) {
-            const uint32_t i = i0 + u;
-            const int so = int(4u * i * uint32_t(p.krs) * 2u);
-            const uint32_t off = N % 4 == 0 ? k_off[u & 3u] : (i & 1u) ? ((i & 2u) ? k_off[3] : k_off[1])
-                                                                       : ((i & 2u) ? k_off[2] : k_off[0]);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(dst + 1024u * i), 16,
-                                                     live >= 64u || 4u * i + k_row < live ? off : kPastEnd, so, 0, 0);
+            const uint32_t i = first + u;
+            const uint32_t key = VALUE ? (lane >> 2) & 3u : lane >> 4;
+            const uint32_t chunk = VALUE ? 4u * (lane >> 4) + (lane & 3u) : (lane & 15u) ^ (4u * (i & 3u) + key);
+            off[u] = (4u * i + key) * uint32_t(s) * 2u + 16u * chunk;
         }
     }
-    template <int N>
-    __device__ __forceinline__ void v_tile(const DenseParams& p, const uint16_t* vh, char* dst, uint32_t t0, uint32_t i0,
-                                           uint32_t live) const
+    // The tile at key t0 < keys.
+    __device__ __forceinline__ void operator()(char* dst, uint32_t t0, uint32_t keys) const
     {
-        const __amdgpu_buffer_rsrc_t r = buffer_rsrc(vh + uint64_t(t0) * p.vrs, kRecords);
+        const uint32_t bytes = (min(64u, keys - t0) - 1u) * uint32_t(stride) * 2u + 256u;
+        const __amdgpu_buffer_rsrc_t r = buffer_rsrc(head + uint64_t(t0) * stride, bytes);
 #pragma unroll
-        for (uint32_t u = 0; u < uint32_t(N); ++u) {
-            const uint32_t i = i0 + u;
-            const int so = int(4u * i * uint32_t(p.vrs) * 2u);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(dst + 1024u * i), 16,
-                                                     live >= 64u || 4u * i + v_key < live ? v_off : kPastEnd, so, 0, 0);
-        }
+        for (uint32_t u = 0; u < uint32_t(N); ++u)
+            load_lds16(r, dst + 1024u * (i0 + u), off[u]);
     }
 };
 
@@ -143,6 +138,9 @@ struct WaveRows {
     uint32_t any_lo, any_hi;    // keys that some row attends lie in [any_lo, any_hi)
     float slope_log2;           // BIAS: the row's head's slope, in base-2 units
     int32_t q_pos;
+    // Whether the wave has work in the tile at key t0, and whether some row's range does not cover it.
+    __device__ __forceinline__ bool meets(uint32_t t0) const { return t0 < any_hi && t0 + 64u > any_lo; }
+    __device__ __forceinline__ bool masks(uint32_t t0) const { return t0 < all_lo || t0 + 64u > all_hi; }
 };
 
 template <bool BIAS>
@@ -176,21 +174,6 @@ __device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, ui
         w.slope_log2 = p.slopes[head] * kLog2e;
         w.q_pos = p.q_pos ? p.q_pos[row] : int32_t(row);
     }
-}
-
-// Whether the V tile in LDS holds an infinity or a NaN (wave-uniform).
-__device__ __forceinline__ bool tile_not_finite(const char* vt, uint32_t lane)
-{
-    uint32_t any = 0;
-#pragma unroll 4
-    for (uint32_t i = 0; i < kTileBytes / 1024u; ++i) {
-        const uint4 t = *reinterpret_cast<const uint4*>(vt + 1024u * i + 16u * lane);
-        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) // the exponent field of either half all ones: the sum carries into its sign bit
-            any |= ((w[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-    }
-    return __ballot(any != 0u) != 0;
 }
 
 // Scores of a tile at key t0 to base-2 units where a cap or a bias needs every one changed; kp: the tile's key positions
@@ -236,43 +219,61 @@ __device__ __forceinline__ void shape_scores(const DenseParams& p, const WaveRow
         }
 }
 
-// The non-finite values of a masked tile's V (the matrix cores took zeros for them), one key at a time into the rows that
-// attend it. pl: the wave's probabilities as they entered the MFMA, [row][key] bf16.
-__device__ __forceinline__ void add_not_finite(WaveRows& w, const char* vt, const uint16_t* pl, uint32_t t0, uint32_t lane)
-{
-    const uint32_t n = lane & 31u, hh = lane >> 5;
-#pragma unroll 1
-    for (uint32_t j = 0; j < 64u; ++j) {
-        const float pj = __uint_as_float(uint32_t(pl[n * 64u + j]) << 16);
-        const bool in = t0 + j >= w.lo && t0 + j < w.hi;
-        const char* const row = vt + 1024u * (j >> 2) + 64u * (j & 3u) + 8u * hh;
-#pragma unroll
-        for (int db = 0; db < 4; ++db)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const uint2 t = *reinterpret_cast<const uint2*>(row + 256 * db + 16 * g);
-                const float v[4] = {bf16_lo(t.x), bf16_hi(t.x), bf16_lo(t.y), bf16_hi(t.y)};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool add = in && (__float_as_uint(v[e]) & 0x7f800000u) == 0x7f800000u;
-                    w.o[db][4 * g + e] = add ? fmaf(pj, v[e], w.o[db][4 * g + e]) : w.o[db][4 * g + e];
-                }
-            }
+// Where a wave's lanes find their operands in a tile's LDS images.
+struct TileReads {
+    uint32_t k_lane, v_lane;
+    __device__ __forceinline__ explicit TileReads(uint32_t lane)
+    {
+        const uint32_t n = lane & 31u, hh = lane >> 5, L = lane & 15u, grp = lane >> 4;
+        k_lane = 256u * n + 16u * (hh ^ (n & 15u));
+        v_lane = 1024u * (grp >> 1) + 32u * (grp & 1u) + 64u * (L >> 2) + 8u * (L & 3u);
     }
+    // A operand of S^T, j < 16: key block j % 2, d chunk j / 2.
+    __device__ __forceinline__ bf16x8_t k(const char* kt, int j) const
+    {
+        return *reinterpret_cast<const bf16x8_t*>(kt + 8192u * (j & 1) + (k_lane ^ (32u * (j >> 1))));
+    }
+    // A operand of O^T, j < 16: 16-key chunk j / 4, d block j % 4, two transposed reads.
+    __device__ __forceinline__ bf16x8_t v(const char* vt, int j) const
+    {
+        const char* const at = vt + v_lane + 4096u * (j >> 2) + 256u * (j & 3);
+        const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (v4i16 __attribute__((address_space(3)))*)(const_cast<char*>(at)));
+        const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (v4i16 __attribute__((address_space(3)))*)(const_cast<char*>(at) + 2048u));
+        return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
+
+constexpr int kAhead = 8; // fragments read ahead of their MFMAs
+
+// S^T of a tile; frag holds the first kAhead K fragments.
+__device__ __forceinline__ void tile_scores(const WaveRows& w, floatx16 (&s)[2], bf16x8_t (&frag)[kAhead],
+                                            const TileReads& rd, const char* kt)
+{
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            s[b][i] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        s[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag[j % kAhead], w.qf[j >> 1], s[j & 1], 0, 0, 0);
+        if (j + kAhead < 16)
+            frag[j % kAhead] = rd.k(kt, j + kAhead);
+    }
+    __builtin_amdgcn_sched_barrier(0);
 }
 
-// A V fragment with zeros for its infinities and NaN.
-__device__ __forceinline__ bf16x8_t finite_only(const bf16x8_t& f)
-{
-    uint4 t = __builtin_bit_cast(uint4, f);
-    uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        w[e] = (w[e] & 0x7f80u) == 0x7f80u ? w[e] & 0xffff0000u : w[e];
-        w[e] = (w[e] & 0x7f800000u) == 0x7f800000u ? w[e] & 0xffffu : w[e];
+// P^T of a tile: chunk c's words (elements 8 (c % 2) .. + 7 of block c / 2) are 4 c .. 4 c + 3.
+struct TileP {
+    uint32_t w[16];
+    __device__ __forceinline__ bf16x8_t chunk(int c) const
+    {
+        return __builtin_bit_cast(bf16x8_t, uint4{w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]});
     }
-    return __builtin_bit_cast(bf16x8_t, uint4{w[0], w[1], w[2], w[3]});
-}
+};
 
 // s unit - m in two roundings.
 __device__ __forceinline__ float rounded_difference(float s, float unit, float m)
@@ -282,52 +283,17 @@ __device__ __forceinline__ float rounded_difference(float s, float unit, float m
     return x - m;
 }
 
-// One tile of 64 keys at t0 for a wave: scores, softmax and its part of O. kt, vt: the tile in LDS; scratch: 4 KB of LDS
-// of the wave's own.
-template <bool CAP, bool BIAS>
-__device__ __forceinline__ void attend_tile(const DenseParams& p, WaveRows& w, const char* kt, const char* vt, uint32_t t0,
-                                            const int32_t* kp, uint16_t* scratch, uint32_t lane)
+// The softmax of a tile at key t0 (MASKED: not every row attends all of it): P^T, and the rows' maxima, sums and (where a maximum moved) rescaled O.
+template <bool CAP, bool BIAS, bool MASKED>
+__device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, floatx16 (&s)[2], TileP& pt, uint32_t t0,
+                                             const int32_t* kp, uint32_t lane)
 {
-    constexpr int kAhead = 8;
-    const uint32_t n = lane & 31u, hh = lane >> 5, L = lane & 15u, grp = lane >> 4;
-    const uint32_t k_lane = 256u * n + 16u * (hh ^ (n & 15u));
-    const char* const vs = vt + 1024u * (grp >> 1) + 32u * (grp & 1u) + 64u * (L >> 2) + 8u * (L & 3u);
-    auto read_k = [&](int j) { // key block j % 2, d chunk j / 2
-        return *reinterpret_cast<const bf16x8_t*>(kt + 8192u * (j & 1) + (k_lane ^ (32u * (j >> 1))));
-    };
-    auto read_v = [&](int j) { // 16-key chunk j / 4, d block j % 4
-        const uint32_t off = 4096u * (j >> 2) + 256u * (j & 3);
-        const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (v4i16 __attribute__((address_space(3)))*)(const_cast<char*>(vs) + off));
-        const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (v4i16 __attribute__((address_space(3)))*)(const_cast<char*>(vs) + off + 2048u));
-        return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
-    floatx16 s[2];
-    bf16x8_t frag[kAhead];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            s[b][i] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-        frag[j] = read_k(j);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        __builtin_amdgcn_sched_barrier(0);
-        s[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag[j % kAhead], w.qf[j >> 1], s[j & 1], 0, 0, 0);
-        if (j + kAhead < 16)
-            frag[j % kAhead] = read_k(j + kAhead);
-    }
-    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t hh = lane >> 5;
     constexpr bool kShaped = CAP || BIAS;
     if (kShaped)
         shape_scores<CAP, BIAS>(p, w, s, t0, hh, kp);
     const float unit = kShaped ? 1.0f : p.scale_log2;
-    const bool masked = t0 < w.all_lo || t0 + 64u > w.all_hi;
-    if (masked) {
-        asm volatile("" ::: "memory"); // kept a branch
+    if (MASKED) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -365,55 +331,100 @@ __device__ __forceinline__ void attend_tile(const DenseParams& p, WaveRows& w, c
                 s[b][i] = rounded_difference(s[b][i], unit, m_ref);
         m_ref = 0.0f, factor = 1.0f;
     }
-    uint32_t pw[4][4]; // P^T chunk c: elements 8 (c % 2) .. + 7 of block c / 2
     float ps = 0.0f;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int b = c >> 1, i = 8 * (c & 1) + 2 * e;
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b][i], factor, -m_ref));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], factor, -m_ref));
-            ps += p0 + p1;
-            pw[c][e] = pack_bf16(p0, p1);
-        }
-    w.l_run += ps;
-    if (masked && tile_not_finite(vt, lane)) {
-        // Keys 32 b + 8 g + 4 hh + 0 .. 3 of row n: words 2 (g % 2) and + 1 of chunk 2 b + g / 2.
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-                *reinterpret_cast<uint2*>(scratch + n * 64u + 32 * (c >> 1) + 8 * (2 * (c & 1) + g) + 4u * hh) =
-                    uint2{pw[c][2 * g], pw[c][2 * g + 1]};
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int c = j >> 2;
-            const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, uint4{pw[c][0], pw[c][1], pw[c][2], pw[c][3]});
-            w.o[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(finite_only(read_v(j)), pf, w.o[j & 3], 0, 0, 0);
-        }
-        add_not_finite(w, vt, scratch, t0, lane);
-        return;
+    for (int e = 0; e < 16; ++e) {
+        const int b = e >> 3, i = 2 * (e & 7);
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b][i], factor, -m_ref));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], factor, -m_ref));
+        ps += p0 + p1;
+        pt.w[e] = pack_bf16(p0, p1);
     }
+    w.l_run += ps;
+}
+
+// O^T += V^T P^T of a tile.
+__device__ __forceinline__ void tile_output(WaveRows& w, const TileP& pt, bf16x8_t (&frag)[kAhead], const TileReads& rd,
+                                            const char* vt)
+{
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-        frag[j] = read_v(j);
-    __builtin_amdgcn_sched_barrier(0);
+        frag[j] = rd.v(vt, j);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, uint4{pw[c][0], pw[c][1], pw[c][2], pw[c][3]});
-#pragma unroll
-        for (int db = 0; db < 4; ++db) {
-            const int j = 4 * c + db;
-            __builtin_amdgcn_sched_barrier(0);
-            w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag[j % kAhead], pf, w.o[db], 0, 0, 0);
-            if (j + kAhead < 16)
-                frag[j % kAhead] = read_v(j + kAhead);
-        }
+    for (int j = 0; j < 16; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        w.o[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag[j % kAhead], pt.chunk(j >> 2), w.o[j & 3], 0, 0, 0);
+        if (j + kAhead < 16)
+            frag[j % kAhead] = rd.v(vt, j + kAhead);
     }
     __builtin_amdgcn_sched_barrier(0);
+}
+
+// All ones in each half of a bf16 pair that is an infinity or a NaN: the sum carries out of an exponent field of ones.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w)
+{
+    return ((((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu;
+}
+
+// A V fragment with zeros for its infinities and NaN; `any` collects whether it held one.
+__device__ __forceinline__ bf16x8_t finite_only(const bf16x8_t& f, uint32_t& any)
+{
+    const uint4 t = __builtin_bit_cast(uint4, f);
+    uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t m = not_finite(w[e]);
+        any |= m;
+        w[e] &= ~m;
+    }
+    return __builtin_bit_cast(bf16x8_t, uint4{w[0], w[1], w[2], w[3]});
+}
+
+// The same for a masked tile: the matrix cores take zeros for V's infinities and NaN, and where there were any these are
+// added one key at a time to the rows that attend them. scratch: 1 KB of LDS of the wave's own, for the probabilities of
+// 16 keys at a time ([row][key], as they entered the MFMA).
+__device__ __forceinline__ void tile_output_masked(WaveRows& w, const TileP& pt, const TileReads& rd, const char* vt,
+                                                   uint32_t t0, uint16_t* scratch, uint32_t lane)
+{
+    uint32_t any = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        w.o[j & 3] =
+            __builtin_amdgcn_mfma_f32_32x32x16_bf16(finite_only(rd.v(vt, j), any), pt.chunk(j >> 2), w.o[j & 3], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!__ballot(any != 0u))
+        return;
+    const uint32_t n = lane & 31u, hh = lane >> 5;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        // Keys 16 c + 8 g + 4 hh + 0 .. 3 of row n: words 2 g and 2 g + 1 of chunk c.
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+            *reinterpret_cast<uint2*>(scratch + 16u * n + 8 * g + 4u * hh) = uint2{pt.w[4 * c + 2 * g],
+                                                                                 pt.w[4 * c + 2 * g + 1]};
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+        for (uint32_t jj = 0; jj < 16u; ++jj) {
+            const uint32_t j = 16u * c + jj;
+            const float pj = __uint_as_float(uint32_t(scratch[16u * n + jj]) << 16);
+            const uint32_t in = t0 + j >= w.lo && t0 + j < w.hi ? ~0u : 0u;
+            const char* const row = vt + 1024u * (j >> 2) + 64u * (j & 3u) + 8u * hh;
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint2 t = *reinterpret_cast<const uint2*>(row + 256 * db + 16 * g);
+                    t.x &= not_finite(t.x) & in, t.y &= not_finite(t.y) & in; // zeros but for those to be added
+                    const float v[4] = {bf16_lo(t.x), bf16_hi(t.x), bf16_lo(t.y), bf16_hi(t.y)};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w.o[db][4 * g + e] = fmaf(pj, v[e], w.o[db][4 * g + e]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
 }
 
 // Writes the wave's rows: normalized, or with splits the part of this split.
@@ -464,49 +475,217 @@ __device__ __forceinline__ bool block_of(const DenseParams& p, uint32_t& kvh, ui
     return kvh < p.kv_heads;
 }
 
-// W waves of 32 list rows each.
-template <int W, bool CAP, bool BIAS>
-__global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_dense_kernel(DenseParams p)
+// The key tiles [first, last) of a workgroup whose rows' keys lie in [k0, k1), for its split.
+__device__ __forceinline__ void tiles_of(const DenseParams& p, uint32_t k0, uint32_t k1, uint32_t split, uint32_t& first,
+                                         uint32_t& last)
 {
-    extern __shared__ __attribute__((aligned(16))) char lds[]; // K, V, key positions, the waves' scratch, 2 W words
+    const uint32_t tiles = k0 < k1 ? (k1 - k0 + 63u) / 64u : 0u;
+    first = uint32_t(uint64_t(tiles) * split / p.splits);
+    last = uint32_t(uint64_t(tiles) * (split + 1u) / p.splits);
+}
+
+// A turn of attn_few_kernel: the tile at key t0. lds: K, V, the wave's scratch, key positions.
+template <bool CAP, bool BIAS, bool MASKED>
+__device__ __forceinline__ void few_turn(const DenseParams& p, WaveRows& w, const TileLoads<16, false>& load_k,
+                                         const TileLoads<16, true>& load_v, const TileReads& rd, char* lds, uint32_t t0,
+                                         uint32_t lane)
+{
+    uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kTileBytes);
+    int32_t* const kp = reinterpret_cast<int32_t*>(lds + 2u * kTileBytes + 1024u);
+    load_k(lds, t0, p.kv_rows);
+    load_v(lds + kTileBytes, t0, p.kv_rows);
+    if (BIAS && p.k_pos)
+        kp[lane] = p.k_pos[min(t0 + lane, p.kv_rows - 1u)];
+    wait_vm<0>();
+    lds_barrier();
+    floatx16 s[2];
+    bf16x8_t frag[kAhead];
+    TileP pt;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        frag[j] = rd.k(lds, j);
+    tile_scores(w, s, frag, rd, lds);
+    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, p.k_pos ? kp : nullptr, lane);
+    if (MASKED)
+        tile_output_masked(w, pt, rd, lds + kTileBytes, t0, scratch, lane);
+    else
+        tile_output(w, pt, frag, rd, lds + kTileBytes);
+    lds_barrier();
+}
+
+// Few rows: one wave of 32 list rows a workgroup, with a tile of its own in LDS; four or five of them share a CU, and
+// one's loads arrive while the others compute.
+template <bool CAP, bool BIAS>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void attn_few_kernel(DenseParams p)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[]; // K, V, scratch, key positions
+    uint32_t kvh, tile, split;
+    if (!block_of(p, kvh, tile, split))
+        return;
+    const uint32_t lane = threadIdx.x;
+    WaveRows w;
+    load_rows<BIAS>(p, kvh, tile * 32u, lane, w);
+    uint32_t first, last;
+    tiles_of(p, w.any_lo, w.any_hi, split, first, last);
+    const uint16_t* const kh = p.k + uint64_t(kvh) * p.khs;
+    const uint16_t* const vh = p.v + uint64_t(kvh) * p.vhs;
+    const TileLoads<16, false> load_k(kh, p.krs, 0u, lane);
+    const TileLoads<16, true> load_v(vh, p.vrs, 0u, lane);
+    const TileReads rd(lane);
+    // Two loops, the masked tiles' and the whole ones': one body with both forms copies O between them at every tile.
+    for (uint32_t t = first; t < last;) {
+#pragma unroll 1
+        for (; t < last && w.masks(w.any_lo + 64u * t); ++t)
+            few_turn<CAP, BIAS, true>(p, w, load_k, load_v, rd, lds, w.any_lo + 64u * t, lane);
+#pragma unroll 1
+        for (; t < last && !w.masks(w.any_lo + 64u * t); ++t)
+            few_turn<CAP, BIAS, false>(p, w, load_k, load_v, rd, lds, w.any_lo + 64u * t, lane);
+    }
+    store_rows(p, w, kvh, tile * 32u, split, lane);
+}
+
+// Many rows: eight waves of 32 list rows, in two groups of four, one wave of each group on a SIMD. A group's turn at a
+// tile has two phases, the products (S of this tile, and O of the one before) and the softmax, and the groups are a phase
+// apart, held there by the barriers: while one group's wave has the matrix core of a SIMD the other's has its vector unit.
+// K and V lie in rings of four tiles; a tile's loads go out three of its K (two of its V) ahead of its use, each wave an
+// eighth.
+constexpr uint32_t kPairWaves = 8, kRing = 4;
+
+// What a wave loads of a workgroup's tiles: its eighth of each tile's K (with all of the tile's key positions, into the
+// wave's own ring) and V. Past the last tile the last one again, into a slot that no one reads any more, so that every turn
+// has the same count of loads.
+template <bool BIAS>
+struct PairFeed {
+    static constexpr int kLoads = BIAS ? 5 : 4; // of a turn
+    TileLoads<2, false> load_k;
+    TileLoads<2, true> load_v;
+    char* kr;
+    char* vr;
+    int32_t* kp;
+    uint32_t k0, tiles, lane;
+    __device__ __forceinline__ char* k_slot(uint32_t t) const { return kr + (t % kRing) * kTileBytes; }
+    __device__ __forceinline__ char* v_slot(uint32_t t) const { return vr + (t % kRing) * kTileBytes; }
+    __device__ __forceinline__ int32_t* kp_slot(uint32_t t) const { return kp + (t % kRing) * 64u; }
+    __device__ __forceinline__ void k(const DenseParams& p, uint32_t t) const
+    {
+        const uint32_t t0 = k0 + 64u * min(t, tiles - 1u);
+        load_k(k_slot(t), t0, p.kv_rows);
+        if (BIAS) {
+            const __amdgpu_buffer_rsrc_t r =
+                buffer_rsrc(p.k_pos ? p.k_pos + t0 : nullptr, p.k_pos ? (p.kv_rows - t0) * 4u : 0u);
+            load_lds4(r, kp_slot(t), 4u * lane);
+        }
+    }
+    __device__ __forceinline__ void v(const DenseParams& p, uint32_t t) const
+    {
+        load_v(v_slot(t), k0 + 64u * min(t, tiles - 1u), p.kv_rows);
+    }
+};
+
+// A turn of attn_pair_kernel. MASKED: tile t or the one before it is not whole for every row of the workgroup, or there is
+// none before it.
+template <bool CAP, bool BIAS, bool MASKED>
+__device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, const PairFeed<BIAS>& feed,
+                                          const TileReads& rd, floatx16 (&s)[2], bf16x8_t (&frag)[kAhead], TileP& pt,
+                                          uint16_t* scratch, uint32_t t, uint32_t lane)
+{
+    const uint32_t t0 = feed.k0 + 64u * t;
+    // The products. Issued here: K of tile t + 3 into the slot of tile t - 1, which both groups have read, and V of tile
+    // t + 2 into that of tile t - 2.
+    feed.k(p, t + 3u);
+    feed.v(p, t + 2u);
+    __builtin_amdgcn_s_setprio(1);
+    tile_scores(w, s, frag, rd, feed.k_slot(t));
+    if (!MASKED)
+        tile_output(w, pt, frag, rd, feed.v_slot(t - 1u));
+    else if (t > 0)
+        tile_output_masked(w, pt, rd, feed.v_slot(t - 1u), t0 - 64u, scratch, lane);
+    __builtin_amdgcn_s_setprio(0);
+    // K of tile t + 2 and V of tile t + 1 have arrived, all but this turn's loads: both groups have passed the barrier below
+    // by the time that either reads them.
+    wait_vm<PairFeed<BIAS>::kLoads>();
+    lds_barrier();
+    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, p.k_pos ? feed.kp_slot(t) : nullptr, lane);
+    // Past the last tile these are some tile's again, and not used.
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        frag[j] = rd.k(feed.k_slot(t + 1u), j);
+    lds_barrier();
+}
+
+template <bool CAP, bool BIAS>
+__global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_pair_kernel(DenseParams p)
+{
+    // K ring, V ring, then a wave's scratch (1 KB) and ring of key positions (1 KB), and the waves' spans.
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t kvh, tile, split;
     if (!block_of(p, kvh, tile, split))
         return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int32_t* const kp = reinterpret_cast<int32_t*>(lds + 2u * kTileBytes);
-    uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kTileBytes + 256u + 4096u * wave);
-    uint32_t* const span = reinterpret_cast<uint32_t*>(lds + 2u * kTileBytes + 256u + 4096u * W);
-    const uint32_t f0 = (tile * W + wave) * 32u;
+    char* const kr = lds;
+    char* const vr = lds + kRing * kTileBytes;
+    uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kRing * kTileBytes + 2048u * wave);
+    int32_t* const kp = reinterpret_cast<int32_t*>(lds + 2u * kRing * kTileBytes + 2048u * wave + 1024u);
+    uint32_t* const span = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + 2048u * kPairWaves);
+    const uint32_t f0 = (tile * kPairWaves + wave) * 32u;
     WaveRows w;
     load_rows<BIAS>(p, kvh, f0, lane, w);
-    uint32_t k0 = w.any_lo, k1 = w.any_hi;
-    if (W > 1) {
-        if (lane == 0)
-            span[2u * wave] = k0, span[2u * wave + 1u] = k1;
-        lds_barrier();
+    if (lane == 0)
+        *reinterpret_cast<uint4*>(span + 4u * wave) = uint4{w.any_lo, w.any_hi, w.all_lo, w.all_hi};
+    lds_barrier();
+    uint32_t k0 = ~0u, k1 = 0u, all_lo = 0u, all_hi = ~0u; // of the workgroup's rows
 #pragma unroll
-        for (int i = 0; i < W; ++i)
-            k0 = min(k0, span[2 * i]), k1 = max(k1, span[2 * i + 1]);
-        k0 = __builtin_amdgcn_readfirstlane(k0), k1 = __builtin_amdgcn_readfirstlane(k1);
+    for (uint32_t i = 0; i < kPairWaves; ++i) {
+        const uint4 t = *reinterpret_cast<const uint4*>(span + 4u * i);
+        k0 = min(k0, t.x), k1 = max(k1, t.y), all_lo = max(all_lo, t.z), all_hi = min(all_hi, t.w);
     }
-    const uint32_t tiles = k0 < k1 ? (k1 - k0 + 63u) / 64u : 0u;
-    const uint32_t t_first = uint32_t(uint64_t(tiles) * split / p.splits);
-    const uint32_t t_last = uint32_t(uint64_t(tiles) * (split + 1u) / p.splits);
+    k0 = __builtin_amdgcn_readfirstlane(k0), k1 = __builtin_amdgcn_readfirstlane(k1);
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    uint32_t first, last;
+    tiles_of(p, k0, k1, split, first, last);
+    if (first >= last) { // the same for every wave
+        store_rows(p, w, kvh, f0, split, lane);
+        return;
+    }
+    k0 += 64u * first;
+    const uint32_t tiles = last - first;
     const uint16_t* const kh = p.k + uint64_t(kvh) * p.khs;
     const uint16_t* const vh = p.v + uint64_t(kvh) * p.vhs;
-    const TileLoads ld(p, lane);
-    for (uint32_t t = t_first; t < t_last; ++t) {
-        const uint32_t t0 = k0 + 64u * t, live = min(64u, p.kv_rows - t0);
-        ld.k_tile<16 / W>(p, kh, lds, t0, wave * (16u / W), live);
-        ld.v_tile<16 / W>(p, vh, lds + kTileBytes, t0, wave * (16u / W), live);
-        if (BIAS && p.k_pos && tid < 64u)
-            kp[tid] = p.k_pos[min(t0 + tid, p.kv_rows - 1u)];
-        wait_vm<0>();
-        lds_barrier(); // the tile is in LDS for every wave
-        if (t0 < w.any_hi && t0 + 64u > w.any_lo)
-            attend_tile<CAP, BIAS>(p, w, lds, lds + kTileBytes, t0, p.k_pos ? kp : nullptr, scratch, lane);
-        lds_barrier(); // every wave is done with it before it is overwritten
-    }
+    const TileReads rd(lane);
+    const PairFeed<BIAS> feed{{kh, p.krs, 2u * wave, lane}, {vh, p.vrs, 2u * wave, lane}, kr, vr, kp, k0, tiles, lane};
+    feed.k(p, 0);
+    feed.k(p, 1);
+    feed.v(p, 0);
+    feed.k(p, 2);
+    feed.v(p, 1);
+    wait_vm<PairFeed<BIAS>::kLoads>(); // K of tiles 0 and 1, V of tile 0
+    lds_barrier();
+    const bool second = wave >= kPairWaves / 2u;
+    if (second)
+        lds_barrier();
+    floatx16 s[2];
+    bf16x8_t frag[kAhead];
+    TileP pt;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        frag[j] = rd.k(kr, j);
+    // The turns in between, whose own tile and the one before are whole for every row of the workgroup, in a loop of their
+    // own: one body with both forms copies O between them at every tile.
+    uint32_t a = all_lo > k0 ? (all_lo - k0 + 63u) / 64u + 1u : 1u, b = all_hi > k0 ? (all_hi - k0) / 64u : 0u;
+    a = min(a, tiles), b = max(a, min(b, tiles));
+#pragma unroll 1
+    for (uint32_t t = 0; t < a; ++t)
+        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, lane);
+#pragma unroll 1
+    for (uint32_t t = a; t < b; ++t)
+        pair_turn<CAP, BIAS, false>(p, w, feed, rd, s, frag, pt, scratch, t, lane);
+#pragma unroll 1
+    for (uint32_t t = b; t < tiles; ++t)
+        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, lane);
+    tile_output_masked(w, pt, rd, vr + ((tiles - 1u) % kRing) * kTileBytes, k0 + 64u * (tiles - 1u), scratch, lane);
+    if (!second)
+        lds_barrier();
+    wait_vm<0>(); // no load into this workgroup's LDS outlives it
     store_rows(p, w, kvh, f0, split, lane);
 }
 
@@ -594,7 +773,7 @@ Plan plan_of(const MH3DenseAttnArgs& a)
     Plan p{};
     p.list = uint64_t(a.q_rows) * (a.heads / a.kv_heads);
     const uint64_t cus = uint64_t(std::max(host::cu_count(), 1));
-    p.waves = (p.list + 127u) / 128u * a.kv_heads >= cus ? 4u : 1u;
+    p.waves = (p.list + 255u) / 256u * a.kv_heads * 2u >= cus ? kPairWaves : 1u;
     p.tiles = (p.list + 32u * p.waves - 1u) / (32u * p.waves);
     const uint64_t blocks = p.tiles * a.kv_heads, key_tiles = (uint64_t(a.kv_rows) + 63u) / 64u;
     const uint64_t want = blocks >= 2u * cus ? 1u : (4u * cus + blocks - 1u) / blocks;
@@ -632,24 +811,23 @@ int check_args(const MH3DenseAttnArgs* args)
     return MH3_OK;
 }
 
-template <int W, bool CAP, bool BIAS>
-int launch_dense(const DenseParams& p, hipStream_t stream)
+template <typename Kernel>
+int launch_rows(Kernel kernel, size_t lds, const DenseParams& p, uint32_t waves, hipStream_t stream)
 {
-    const auto kernel = &attn_dense_kernel<W, CAP, BIAS>;
-    const size_t lds = 2u * kTileBytes + 256u + 4096u * W + 8u * W;
     if (const hipError_t e = host::allow_dynamic_lds(reinterpret_cast<const void*>(kernel), lds); e != hipSuccess)
         return host::hip_error(e);
     const uint32_t blocks = (p.kv_heads * p.tiles * p.splits + 7u) / 8u * 8u;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(W * 64), lds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(waves * 64u), lds, stream, p);
     return host::check_launch();
 }
 
-template <int W>
-int launch_by_score(const DenseParams& p, bool cap, bool bias, hipStream_t stream)
+template <bool CAP, bool BIAS>
+int launch_dense(const DenseParams& p, uint32_t waves, hipStream_t stream)
 {
-    if (cap)
-        return bias ? launch_dense<W, true, true>(p, stream) : launch_dense<W, true, false>(p, stream);
-    return bias ? launch_dense<W, false, true>(p, stream) : launch_dense<W, false, false>(p, stream);
+    if (waves == kPairWaves)
+        return launch_rows(attn_pair_kernel<CAP, BIAS>, 2u * kRing * kTileBytes + (2048u + 16u) * kPairWaves, p, waves,
+                           stream);
+    return launch_rows(attn_few_kernel<CAP, BIAS>, 2u * kTileBytes + 1024u + 256u, p, waves, stream);
 }
 
 } // namespace
@@ -719,7 +897,9 @@ extern "C" int mh3_flash_attn_128(const MH3DenseAttnArgs* args, const uint16_t* 
         p.cap_in = 2.0f * kLog2e * (scale / p.q_pow) / a.cap, p.cap_out = a.cap * kLog2e;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const bool cap = a.cap > 0.0f, bias = slopes != nullptr;
-    const int rc = plan.waves == 4u ? launch_by_score<4>(p, cap, bias, s) : launch_by_score<1>(p, cap, bias, s);
+    const int rc = cap ? bias ? launch_dense<true, true>(p, plan.waves, s) : launch_dense<true, false>(p, plan.waves, s)
+                   : bias ? launch_dense<false, true>(p, plan.waves, s)
+                          : launch_dense<false, false>(p, plan.waves, s);
     if (rc != MH3_OK || p.splits == 1u)
         return rc;
     const uint64_t items = uint64_t(p.kv_heads) * p.list;
