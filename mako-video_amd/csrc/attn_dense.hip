@@ -30,8 +30,8 @@ namespace {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef short v4i16 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
@@ -75,15 +75,42 @@ __device__ __forceinline__ void lds_barrier()
     asm volatile("" ::: "memory");
 }
 
-// 16 or 4 bytes a lane from a buffer straight into LDS, lane L's at lds + 16 L or 4 L. (Not in templates: the host's pass
-// checks the size again at each instantiation, as of its own target, and leaves the kernel out without a word.)
-__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t offset)
+// A raw buffer of `bytes` at base, as the instructions below take it: reads past its end return zeros.
+__device__ __forceinline__ u32x4_t buffer_words(const void* base, uint32_t bytes)
 {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)lds, 16, offset, 0, 0, 0);
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    return u32x4_t{uint32_t(a), uint32_t(a >> 32) & 0xffffu, bytes, uint32_t(kRsrcFlags)};
 }
-__device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t offset)
+
+// The workgroup's barrier alone, with nothing moved across it: between phases whose LDS reads are used up, or are meant to
+// stay in flight.
+__device__ __forceinline__ void phase_barrier()
 {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)lds, 4, offset, 0, 0, 0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+// 16 or 4 bytes a lane from a buffer straight into LDS, lane L's at lds + 16 L or 4 L. Written as assembly for what the
+// compiler would make of the builtin here: it waits for every such load in flight before each transposed LDS read, as
+// if one might land under it, which cost half of the time (960 x 544: 10.1 ms; the tiles' slots and the waits in
+// pair_turn and few_turn order them). No vector register is written, so nothing is in flight that the compiler has to know
+// of, and M0 is used by nothing else in this file.
+__device__ __forceinline__ void load_lds16(const u32x4_t& buffer, char* lds, uint32_t offset)
+{
+    const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(offset),
+                 "s"(buffer)
+                 : "memory");
+}
+__device__ __forceinline__ void load_lds4(const u32x4_t& buffer, char* lds, uint32_t offset)
+{
+    const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(at), "v"(offset),
+                 "s"(buffer)
+                 : "memory");
 }
 
 // The keys [lo, hi) of list row f, within [0, kv_rows]; none for a row past the list.
@@ -103,25 +130,22 @@ __device__ __forceinline__ void range_of(const DenseParams& p, uint32_t f, uint3
 // aligned 64-byte piece of a row. The descriptor ends behind the last key, so keys past it read zeros.
 template <int N, bool VALUE>
 struct TileLoads {
-    const uint16_t* head;
-    uint64_t stride; // elements between keys
-    uint32_t off[N], i0;
-    __device__ __forceinline__ TileLoads(const uint16_t* h, uint64_t s, uint32_t first, uint32_t lane)
-        : head(h), stride(s), i0(first)
+    uint32_t row, off[N], i0; // row: bytes from a key to the next
+    __device__ __forceinline__ TileLoads(uint64_t stride, uint32_t first, uint32_t lane)
+        : row(uint32_t(stride) * 2u), i0(first)
     {
 #pragma unroll
         for (uint32_t u = 0; u < uint32_t(N); ++u) {
             const uint32_t i = first + u;
             const uint32_t key = VALUE ? (lane >> 2) & 3u : lane >> 4;
             const uint32_t chunk = VALUE ? 4u * (lane >> 4) + (lane & 3u) : (lane & 15u) ^ (4u * (i & 3u) + key);
-            off[u] = (4u * i + key) * uint32_t(s) * 2u + 16u * chunk;
+            off[u] = (4u * i + key) * row + 16u * chunk;
         }
     }
-    // The tile at key t0 < keys.
-    __device__ __forceinline__ void operator()(char* dst, uint32_t t0, uint32_t keys) const
+    // The tile whose first key is at `base`, `keys` >= 1 of whose 64 exist.
+    __device__ __forceinline__ void operator()(char* dst, const uint16_t* base, uint32_t keys) const
     {
-        const uint32_t bytes = (min(64u, keys - t0) - 1u) * uint32_t(stride) * 2u + 256u;
-        const __amdgpu_buffer_rsrc_t r = buffer_rsrc(head + uint64_t(t0) * stride, bytes);
+        const u32x4_t r = buffer_words(base, (min(64u, keys) - 1u) * row + 256u);
 #pragma unroll
         for (uint32_t u = 0; u < uint32_t(N); ++u)
             load_lds16(r, dst + 1024u * (i0 + u), off[u]);
@@ -133,6 +157,7 @@ struct WaveRows {
     bf16x8_t qf[8];  // B operand of S^T: lane (n, hh) holds d 16 dc + 8 hh .. + 7 of row n
     floatx16 o[4];   // O^T: d 32 db + 8 (i / 4) + 4 hh + i % 4 of row n
     float m_run, l_run;
+    bool settled;    // every row has a maximum, of no more than 2^20
     uint32_t lo, hi;            // the lane's row's keys
     uint32_t all_lo, all_hi;    // keys that every row with any attends: [all_lo, all_hi)
     uint32_t any_lo, any_hi;    // keys that some row attends lie in [any_lo, any_hi)
@@ -163,7 +188,7 @@ __device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, ui
 #pragma unroll
         for (int e = 0; e < 16; ++e)
             w.o[b][e] = 0.0f;
-    w.m_run = -kInf, w.l_run = 0.0f;
+    w.m_run = -kInf, w.l_run = 0.0f, w.settled = false;
     range_of(p, f, row, w.lo, w.hi);
     const bool any = w.lo < w.hi;
     w.any_lo = wave_min_u32(any ? w.lo : ~0u);
@@ -247,25 +272,6 @@ struct TileReads {
 
 constexpr int kAhead = 8; // fragments read ahead of their MFMAs
 
-// S^T of a tile; frag holds the first kAhead K fragments.
-__device__ __forceinline__ void tile_scores(const WaveRows& w, floatx16 (&s)[2], bf16x8_t (&frag)[kAhead],
-                                            const TileReads& rd, const char* kt)
-{
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            s[b][i] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        __builtin_amdgcn_sched_barrier(0);
-        s[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag[j % kAhead], w.qf[j >> 1], s[j & 1], 0, 0, 0);
-        if (j + kAhead < 16)
-            frag[j % kAhead] = rd.k(kt, j + kAhead);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-}
-
 // P^T of a tile: chunk c's words (elements 8 (c % 2) .. + 7 of block c / 2) are 4 c .. 4 c + 3.
 struct TileP {
     uint32_t w[16];
@@ -283,7 +289,31 @@ __device__ __forceinline__ float rounded_difference(float s, float unit, float m
     return x - m;
 }
 
-// The softmax of a tile at key t0 (MASKED: not every row attends all of it): P^T, and the rows' maxima, sums and (where a maximum moved) rescaled O.
+// The larger of a lane's value and its lane +- 32 twin's.
+__device__ __forceinline__ float both_halves_max(float v)
+{
+    const uint32_t u = __float_as_uint(v);
+    const auto t = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+// P^T of a tile from its scores, exp2(factor s - m), and a row's sum of them over the lane's keys.
+__device__ __forceinline__ float tile_exponentials(const floatx16 (&s)[2], TileP& pt, float factor, float m)
+{
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int b = e >> 3, i = 2 * (e & 7);
+        const floatx2 t = {__builtin_amdgcn_exp2f(fmaf(s[b][i], factor, -m)),
+                           __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], factor, -m))};
+        sum[0] += t[0], sum[1] += t[1];
+        pt.w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(t, bf16x2_t)); // one conversion for both
+    }
+    return sum[0] + sum[1];
+}
+
+// The softmax of a tile at key t0 (MASKED: not every row attends all of it): P^T, and the rows' maxima, sums and (where a
+// maximum moved) rescaled O.
 template <bool CAP, bool BIAS, bool MASKED>
 __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, floatx16 (&s)[2], TileP& pt, uint32_t t0,
                                              const int32_t* kp, uint32_t lane)
@@ -302,48 +332,81 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
                 s[b][i] = key >= w.lo && key < w.hi ? s[b][i] : -kInf;
             }
     }
-    float mt = -kInf;
+    // Most tiles raise no maximum by much, and the sum over a lane's 32 keys of a row tells: up to 2^10 no key is above
+    // that, and the old maximum serves. That spares the search for the new one in a phase whose vector instructions take 7
+    // clocks each beside the other group's MFMAs. At most one more pass with the maxima brought up to date.
+    float m_ref = w.m_run, factor = unit, sum;
+    bool update = MASKED || !w.settled;
+#pragma unroll 1
+    for (;;) {
+        if (update) {
+            float mt = -kInf;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    mt = fmaxf(mt, s[b][i]);
+            const float m_new = fmaxf(w.m_run, both_halves_max(mt) * unit);
+            const float alpha = w.m_run == -kInf ? 0.0f : __builtin_amdgcn_exp2f(w.m_run - m_new);
+            if (__ballot(m_new > w.m_run)) {
+                w.l_run *= alpha;
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        w.o[b][i] *= m_new > w.m_run ? alpha : 1.0f;
+            }
+            w.m_run = m_new;
+            m_ref = m_new == -kInf ? 0.0f : m_new;
+            w.settled = !__ballot(!(fabsf(m_new) <= 0x1p20f));
+            // s unit - m in one fused operation keeps the rounding of m, 2^-24 of it, in the exponent: common to all of a
+            // row's probabilities and harmless, until it leaves the exponent's range. Scores so large are rounded as m was.
+            if (__ballot(fabsf(m_ref) > 0x1p20f)) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[b][i] = rounded_difference(s[b][i], unit, m_ref);
+                m_ref = 0.0f, factor = 1.0f;
+            }
+        }
+        sum = tile_exponentials(s, pt, factor, m_ref);
+        if (update || !__ballot(!(sum <= 0x1p10f)))
+            break;
+        update = true;
+    }
+    w.l_run += sum;
+}
+
+// S^T of a tile, and then with PV the O^T += V^T P^T of another (the one before it in a walk), in one run of MFMAs: frag
+// holds the first kAhead K fragments, and each MFMA's slot takes the fragment of the MFMA kAhead on, so V's are on their
+// way before the last scores are out.
+template <bool PV>
+__device__ __forceinline__ void tile_products(WaveRows& w, floatx16 (&s)[2], const TileP& pt, bf16x8_t (&frag)[kAhead],
+                                              const TileReads& rd, const char* kt, const char* vt)
+{
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            mt = fmaxf(mt, s[b][i]);
-    mt = fmaxf(mt, __shfl_xor(mt, 32, kWave)) * unit;
-    if (__ballot(mt > w.m_run + 8.0f)) {
-        const float m_new = fmaxf(w.m_run, mt);
-        const float alpha = w.m_run == -kInf ? 0.0f : __builtin_amdgcn_exp2f(w.m_run - m_new);
-        w.m_run = m_new;
-        w.l_run *= alpha;
+            s[b][i] = 0.0f;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                w.o[b][i] *= alpha;
+    for (int j = 0; j < (PV ? 32 : 16); ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8_t& f = frag[j % kAhead];
+        if (j < 16)
+            s[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, w.qf[j >> 1], s[j & 1], 0, 0, 0);
+        else
+            w.o[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, pt.chunk((j - 16) >> 2), w.o[j & 3], 0, 0, 0);
+        if (j + kAhead < 16)
+            f = rd.k(kt, j + kAhead);
+        else if (PV && j + kAhead < 32)
+            f = rd.v(vt, j + kAhead - 16);
     }
-    float m_ref = w.m_run == -kInf ? 0.0f : w.m_run, factor = unit;
-    // s unit - m in one fused operation keeps the rounding of m, 2^-24 of it, in the exponent: common to all of a row's
-    // probabilities and harmless, until it leaves the exponent's range. Scores so large are rounded as m was first.
-    if (__ballot(fabsf(m_ref) > 0x1p20f)) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                s[b][i] = rounded_difference(s[b][i], unit, m_ref);
-        m_ref = 0.0f, factor = 1.0f;
-    }
-    float ps = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const int b = e >> 3, i = 2 * (e & 7);
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b][i], factor, -m_ref));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], factor, -m_ref));
-        ps += p0 + p1;
-        pt.w[e] = pack_bf16(p0, p1);
-    }
-    w.l_run += ps;
+    __builtin_amdgcn_sched_barrier(0);
 }
 
-// O^T += V^T P^T of a tile.
+// O^T += V^T P^T of a tile alone.
 __device__ __forceinline__ void tile_output(WaveRows& w, const TileP& pt, bf16x8_t (&frag)[kAhead], const TileReads& rd,
                                             const char* vt)
 {
@@ -487,13 +550,13 @@ __device__ __forceinline__ void tiles_of(const DenseParams& p, uint32_t k0, uint
 // A turn of attn_few_kernel: the tile at key t0. lds: K, V, the wave's scratch, key positions.
 template <bool CAP, bool BIAS, bool MASKED>
 __device__ __forceinline__ void few_turn(const DenseParams& p, WaveRows& w, const TileLoads<16, false>& load_k,
-                                         const TileLoads<16, true>& load_v, const TileReads& rd, char* lds, uint32_t t0,
-                                         uint32_t lane)
+                                         const TileLoads<16, true>& load_v, const uint16_t* kh, const uint16_t* vh,
+                                         const TileReads& rd, char* lds, uint32_t t0, uint32_t lane)
 {
     uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kTileBytes);
     int32_t* const kp = reinterpret_cast<int32_t*>(lds + 2u * kTileBytes + 1024u);
-    load_k(lds, t0, p.kv_rows);
-    load_v(lds + kTileBytes, t0, p.kv_rows);
+    load_k(lds, kh + uint64_t(t0) * p.krs, p.kv_rows - t0);
+    load_v(lds + kTileBytes, vh + uint64_t(t0) * p.vrs, p.kv_rows - t0);
     if (BIAS && p.k_pos)
         kp[lane] = p.k_pos[min(t0 + lane, p.kv_rows - 1u)];
     wait_vm<0>();
@@ -504,7 +567,7 @@ __device__ __forceinline__ void few_turn(const DenseParams& p, WaveRows& w, cons
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
         frag[j] = rd.k(lds, j);
-    tile_scores(w, s, frag, rd, lds);
+    tile_products<false>(w, s, pt, frag, rd, lds, nullptr);
     tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, p.k_pos ? kp : nullptr, lane);
     if (MASKED)
         tile_output_masked(w, pt, rd, lds + kTileBytes, t0, scratch, lane);
@@ -529,17 +592,17 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void at
     tiles_of(p, w.any_lo, w.any_hi, split, first, last);
     const uint16_t* const kh = p.k + uint64_t(kvh) * p.khs;
     const uint16_t* const vh = p.v + uint64_t(kvh) * p.vhs;
-    const TileLoads<16, false> load_k(kh, p.krs, 0u, lane);
-    const TileLoads<16, true> load_v(vh, p.vrs, 0u, lane);
+    const TileLoads<16, false> load_k(p.krs, 0u, lane);
+    const TileLoads<16, true> load_v(p.vrs, 0u, lane);
     const TileReads rd(lane);
     // Two loops, the masked tiles' and the whole ones': one body with both forms copies O between them at every tile.
     for (uint32_t t = first; t < last;) {
 #pragma unroll 1
         for (; t < last && w.masks(w.any_lo + 64u * t); ++t)
-            few_turn<CAP, BIAS, true>(p, w, load_k, load_v, rd, lds, w.any_lo + 64u * t, lane);
+            few_turn<CAP, BIAS, true>(p, w, load_k, load_v, kh, vh, rd, lds, w.any_lo + 64u * t, lane);
 #pragma unroll 1
         for (; t < last && !w.masks(w.any_lo + 64u * t); ++t)
-            few_turn<CAP, BIAS, false>(p, w, load_k, load_v, rd, lds, w.any_lo + 64u * t, lane);
+            few_turn<CAP, BIAS, false>(p, w, load_k, load_v, kh, vh, rd, lds, w.any_lo + 64u * t, lane);
     }
     store_rows(p, w, kvh, tile * 32u, split, lane);
 }
@@ -551,66 +614,74 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void at
 // eighth.
 constexpr uint32_t kPairWaves = 8, kRing = 4;
 
-// What a wave loads of a workgroup's tiles: its eighth of each tile's K (with all of the tile's key positions, into the
-// wave's own ring) and V. Past the last tile the last one again, into a slot that no one reads any more, so that every turn
-// has the same count of loads.
-template <bool BIAS>
-struct PairFeed {
-    static constexpr int kLoads = BIAS ? 5 : 4; // of a turn
-    TileLoads<2, false> load_k;
-    TileLoads<2, true> load_v;
-    char* kr;
-    char* vr;
-    int32_t* kp;
-    uint32_t k0, tiles, lane;
-    __device__ __forceinline__ char* k_slot(uint32_t t) const { return kr + (t % kRing) * kTileBytes; }
-    __device__ __forceinline__ char* v_slot(uint32_t t) const { return vr + (t % kRing) * kTileBytes; }
-    __device__ __forceinline__ int32_t* kp_slot(uint32_t t) const { return kp + (t % kRing) * 64u; }
-    __device__ __forceinline__ void k(const DenseParams& p, uint32_t t) const
+// What a wave loads of a workgroup's tiles, a call a tile: its eighth of K (with all of the tile's key positions, into the
+// wave's own ring) or of V. Behind the last key the last tile again, so that every turn has the same count of loads; what
+// lies behind the workgroup's last tile is not read. The state is scalar and moves by additions.
+template <bool VALUE, bool POS>
+struct PairStream {
+    TileLoads<2, VALUE> ld;
+    const uint16_t* at; // the next tile's first key
+    uint64_t step;      // elements a tile
+    uint32_t left;      // keys from it on
+    char* ring;
+    uint32_t slot; // byte offset in the ring
+    const int32_t* pos;
+    char* pos_ring;
+    uint32_t lane;
+    __device__ __forceinline__ void operator()()
     {
-        const uint32_t t0 = k0 + 64u * min(t, tiles - 1u);
-        load_k(k_slot(t), t0, p.kv_rows);
-        if (BIAS) {
-            const __amdgpu_buffer_rsrc_t r =
-                buffer_rsrc(p.k_pos ? p.k_pos + t0 : nullptr, p.k_pos ? (p.kv_rows - t0) * 4u : 0u);
-            load_lds4(r, kp_slot(t), 4u * lane);
-        }
-    }
-    __device__ __forceinline__ void v(const DenseParams& p, uint32_t t) const
-    {
-        load_v(v_slot(t), k0 + 64u * min(t, tiles - 1u), p.kv_rows);
+        ld(ring + slot, at, left);
+        if (POS) // no positions: no records, and zeros
+            load_lds4(buffer_words(pos, pos ? left * 4u : 0u), pos_ring + slot / 64u, 4u * lane);
+        slot = (slot + kTileBytes) & (kRing * kTileBytes - 1u);
+        const bool more = left > 64u;
+        at += more ? step : 0u;
+        left -= more ? 64u : 0u;
+        if (POS)
+            pos += more && pos ? 64 : 0;
     }
 };
 
-// A turn of attn_pair_kernel. MASKED: tile t or the one before it is not whole for every row of the workgroup, or there is
-// none before it.
+template <bool BIAS>
+struct PairFeed {
+    static constexpr int kLoads = BIAS ? 5 : 4; // of a turn
+    PairStream<false, BIAS> k;
+    PairStream<true, false> v;
+    __device__ __forceinline__ const char* k_tile(uint32_t t) const { return k.ring + (t % kRing) * kTileBytes; }
+    __device__ __forceinline__ const char* v_tile(uint32_t t) const { return v.ring + (t % kRing) * kTileBytes; }
+    __device__ __forceinline__ const int32_t* positions(uint32_t t) const
+    {
+        return reinterpret_cast<const int32_t*>(k.pos_ring + (t % kRing) * 256u);
+    }
+};
+
+// A turn of attn_pair_kernel, tile t at key t0. MASKED: this tile or the one before it is not whole for every row of the
+// workgroup, or there is none before it.
 template <bool CAP, bool BIAS, bool MASKED>
-__device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, const PairFeed<BIAS>& feed,
-                                          const TileReads& rd, floatx16 (&s)[2], bf16x8_t (&frag)[kAhead], TileP& pt,
-                                          uint16_t* scratch, uint32_t t, uint32_t lane)
+__device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, PairFeed<BIAS>& feed, const TileReads& rd,
+                                          floatx16 (&s)[2], bf16x8_t (&frag)[kAhead], TileP& pt, uint16_t* scratch,
+                                          uint32_t t, uint32_t t0, uint32_t lane)
 {
-    const uint32_t t0 = feed.k0 + 64u * t;
-    // The products. Issued here: K of tile t + 3 into the slot of tile t - 1, which both groups have read, and V of tile
-    // t + 2 into that of tile t - 2.
-    feed.k(p, t + 3u);
-    feed.v(p, t + 2u);
+    // The products.
     __builtin_amdgcn_s_setprio(1);
-    tile_scores(w, s, frag, rd, feed.k_slot(t));
-    if (!MASKED)
-        tile_output(w, pt, frag, rd, feed.v_slot(t - 1u));
-    else if (t > 0)
-        tile_output_masked(w, pt, rd, feed.v_slot(t - 1u), t0 - 64u, scratch, lane);
+    tile_products<!MASKED>(w, s, pt, frag, rd, feed.k_tile(t), feed.v_tile(t - 1u));
+    if (MASKED && t > 0)
+        tile_output_masked(w, pt, rd, feed.v_tile(t - 1u), t0 - 64u, scratch, lane);
     __builtin_amdgcn_s_setprio(0);
-    // K of tile t + 2 and V of tile t + 1 have arrived, all but this turn's loads: both groups have passed the barrier below
-    // by the time that either reads them.
-    wait_vm<PairFeed<BIAS>::kLoads>();
-    lds_barrier();
-    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, p.k_pos ? feed.kp_slot(t) : nullptr, lane);
+    phase_barrier();
+    // The softmax. With it go out K of tile t + 3, into the slot of tile t - 1, which both groups have read, and V of tile
+    // t + 2 into that of tile t - 2 (among the products they cost 10%: this phase is the shorter one).
+    feed.k();
+    feed.v();
+    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, p.k_pos ? feed.positions(t) : nullptr, lane);
     // Past the last tile these are some tile's again, and not used.
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-        frag[j] = rd.k(feed.k_slot(t + 1u), j);
-    lds_barrier();
+        frag[j] = rd.k(feed.k_tile(t + 1u), j);
+    // K of tile t + 2 and V of tile t + 1 have arrived, all but this turn's loads: both groups are past their barriers by
+    // the time that either reads them.
+    wait_vm<PairFeed<BIAS>::kLoads>();
+    phase_barrier();
 }
 
 template <bool CAP, bool BIAS>
@@ -622,10 +693,7 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     if (!block_of(p, kvh, tile, split))
         return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    char* const kr = lds;
-    char* const vr = lds + kRing * kTileBytes;
     uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kRing * kTileBytes + 2048u * wave);
-    int32_t* const kp = reinterpret_cast<int32_t*>(lds + 2u * kRing * kTileBytes + 2048u * wave + 1024u);
     uint32_t* const span = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + 2048u * kPairWaves);
     const uint32_t f0 = (tile * kPairWaves + wave) * 32u;
     WaveRows w;
@@ -649,42 +717,57 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     }
     k0 += 64u * first;
     const uint32_t tiles = last - first;
-    const uint16_t* const kh = p.k + uint64_t(kvh) * p.khs;
-    const uint16_t* const vh = p.v + uint64_t(kvh) * p.vhs;
     const TileReads rd(lane);
-    const PairFeed<BIAS> feed{{kh, p.krs, 2u * wave, lane}, {vh, p.vrs, 2u * wave, lane}, kr, vr, kp, k0, tiles, lane};
-    feed.k(p, 0);
-    feed.k(p, 1);
-    feed.v(p, 0);
-    feed.k(p, 2);
-    feed.v(p, 1);
+    PairFeed<BIAS> feed{{{p.krs, 2u * wave, lane},
+                         p.k + uint64_t(kvh) * p.khs + uint64_t(k0) * p.krs,
+                         64u * p.krs,
+                         p.kv_rows - k0,
+                         lds,
+                         0u,
+                         p.k_pos ? p.k_pos + k0 : nullptr,
+                         reinterpret_cast<char*>(scratch) + 1024,
+                         lane},
+                        {{p.vrs, 2u * wave, lane},
+                         p.v + uint64_t(kvh) * p.vhs + uint64_t(k0) * p.vrs,
+                         64u * p.vrs,
+                         p.kv_rows - k0,
+                         lds + kRing * kTileBytes,
+                         0u,
+                         nullptr,
+                         nullptr,
+                         lane}};
+    feed.k();
+    feed.k();
+    feed.v();
+    feed.k();
+    feed.v();
     wait_vm<PairFeed<BIAS>::kLoads>(); // K of tiles 0 and 1, V of tile 0
     lds_barrier();
     const bool second = wave >= kPairWaves / 2u;
     if (second)
-        lds_barrier();
+        phase_barrier();
     floatx16 s[2];
     bf16x8_t frag[kAhead];
     TileP pt;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-        frag[j] = rd.k(kr, j);
+        frag[j] = rd.k(lds, j);
     // The turns in between, whose own tile and the one before are whole for every row of the workgroup, in a loop of their
     // own: one body with both forms copies O between them at every tile.
     uint32_t a = all_lo > k0 ? (all_lo - k0 + 63u) / 64u + 1u : 1u, b = all_hi > k0 ? (all_hi - k0) / 64u : 0u;
     a = min(a, tiles), b = max(a, min(b, tiles));
 #pragma unroll 1
     for (uint32_t t = 0; t < a; ++t)
-        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, lane);
+        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, k0 + 64u * t, lane);
 #pragma unroll 1
     for (uint32_t t = a; t < b; ++t)
-        pair_turn<CAP, BIAS, false>(p, w, feed, rd, s, frag, pt, scratch, t, lane);
+        pair_turn<CAP, BIAS, false>(p, w, feed, rd, s, frag, pt, scratch, t, k0 + 64u * t, lane);
 #pragma unroll 1
     for (uint32_t t = b; t < tiles; ++t)
-        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, lane);
-    tile_output_masked(w, pt, rd, vr + ((tiles - 1u) % kRing) * kTileBytes, k0 + 64u * (tiles - 1u), scratch, lane);
+        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, k0 + 64u * t, lane);
+    tile_output_masked(w, pt, rd, feed.v_tile(tiles - 1u), k0 + 64u * (tiles - 1u), scratch, lane);
     if (!second)
-        lds_barrier();
+        phase_barrier();
     wait_vm<0>(); // no load into this workgroup's LDS outlives it
     store_rows(p, w, kvh, f0, split, lane);
 }
