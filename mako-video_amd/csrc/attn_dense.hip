@@ -772,29 +772,56 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     store_rows(p, w, kvh, f0, split, lane);
 }
 
-// Joins the splits of a list row: a wave a row, two values of d a lane.
+// Joins the splits of a list row, a workgroup of four waves each: every wave takes every fourth split, two values of d a
+// lane, eight splits in flight, and the four sums meet in LDS in a fixed order.
 __global__ __launch_bounds__(256) void attn_join_kernel(DenseParams p)
 {
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t item = uint64_t(blockIdx.x) * 4u + (threadIdx.x >> 6), items = uint64_t(p.kv_heads) * p.list;
-    if (item >= items)
-        return;
+    __shared__ float part[4][4][64]; // a wave's maximum, sum and two values of O, by lane
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint64_t item = blockIdx.x, items = uint64_t(p.kv_heads) * p.list;
     const uint32_t kvh = uint32_t(item / p.list), f = uint32_t(item - uint64_t(kvh) * p.list);
     const uint32_t row = p.div_group.div(f), head = kvh * p.group + (f - row * p.group);
+    const float2* const ml = reinterpret_cast<const float2*>(p.part + uint64_t(p.splits) * items * 128u);
+    constexpr uint32_t kU = 8;
+    float m = -kInf, l = 0.0f, a = 0.0f, b = 0.0f;
+    for (uint32_t s0 = wave; s0 < p.splits; s0 += 4u * kU) {
+        float2 t[kU], o[kU];
+#pragma unroll
+        for (uint32_t u = 0; u < kU; ++u) {
+            const uint32_t s = s0 + 4u * u;
+            const bool in = s < p.splits;
+            t[u] = in ? ml[s * items + item] : float2{-kInf, 0.0f};
+            o[u] = in ? *reinterpret_cast<const float2*>(p.part + (s * items + item) * 128u + 2u * lane)
+                      : float2{0.0f, 0.0f};
+        }
+        float m_new = m;
+#pragma unroll
+        for (uint32_t u = 0; u < kU; ++u)
+            m_new = fmaxf(m_new, t[u].x);
+        // A split without a key of this row has left zeros and -inf. (A NaN of its scores is in its sum and its O.)
+        const float old = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+        l *= old, a *= old, b *= old, m = m_new;
+#pragma unroll
+        for (uint32_t u = 0; u < kU; ++u) {
+            const float e = t[u].x == -kInf ? 1.0f : __builtin_amdgcn_exp2f(t[u].x - m_new);
+            l = fmaf(t[u].y, e, l), a = fmaf(o[u].x, e, a), b = fmaf(o[u].y, e, b);
+        }
+    }
+    part[wave][0][lane] = m, part[wave][1][lane] = l, part[wave][2][lane] = a, part[wave][3][lane] = b;
+    __syncthreads();
+    if (wave != 0)
+        return;
     uint32_t lo, hi;
     range_of(p, f, row, lo, hi);
-    const float2* const ml = reinterpret_cast<const float2*>(p.part + uint64_t(p.splits) * items * 128u);
-    float m = -kInf;
-    for (uint32_t s = 0; s < p.splits; ++s)
-        m = fmaxf(m, ml[s * items + item].x);
-    const float m_ref = m == -kInf ? 0.0f : m;
-    float l = 0.0f, a = 0.0f, b = 0.0f;
-    for (uint32_t s = 0; s < p.splits; ++s) {
-        const float2 t = ml[s * items + item];
-        const float2 o = *reinterpret_cast<const float2*>(p.part + (s * items + item) * 128u + 2u * lane);
-        // A split without a key of this row has left zeros and -inf. (A NaN of its scores is in its sum and its O.)
-        const float f = t.x == -kInf ? 1.0f : __builtin_amdgcn_exp2f(t.x - m_ref);
-        l = fmaf(t.y, f, l), a = fmaf(o.x, f, a), b = fmaf(o.y, f, b);
+    float mm = m;
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+        mm = fmaxf(mm, part[w][0][lane]);
+    l = a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float e = part[w][0][lane] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(part[w][0][lane] - mm);
+        l = fmaf(part[w][1][lane], e, l), a = fmaf(part[w][2][lane], e, a), b = fmaf(part[w][3][lane], e, b);
     }
     const float inv = lo < hi ? 1.0f / l : 0.0f;
     *reinterpret_cast<uint32_t*>(p.out + uint64_t(head) * p.ohs + uint64_t(row) * p.ors + 2u * lane) =
@@ -850,18 +877,37 @@ struct Plan {
     uint64_t list, tiles;
 };
 
-// The workgroup's waves and the key splits of a call.
+// The workgroup's waves and the key splits of a call: the pair of least estimated time, of the two kernels with no split
+// or as many as give the chip one, two or four workgroups a CU. In us, measured: a workgroup of eight waves takes 14 and
+// 1.5 a key tile (it has a CU to itself), one of a single wave 10 and 1.75 (four share a CU); K and V come from HBM once at
+// 6 TB/s, and for each further row tile from the MALL or L2 at some 16; the join takes 6 and its parts' bytes. Heads, query
+// and key rows, eight waves and one, each at its best splits (us): 56, 945 x 945 45 and 68; 40, 212 x 212 20 and 14; 40,
+// 64 x 20,000 123 and 100; 40 on 8 key heads, 1 x 5000 20 and 15, 3 x 129,536 113 and 98; 7 on 1, 500 x 16,000 53 and 73;
+// 56 on 8, 64 x 100,000 202 and 383. (Ranges that leave most keys out are not known here.)
 Plan plan_of(const MH3DenseAttnArgs& a)
 {
-    Plan p{};
-    p.list = uint64_t(a.q_rows) * (a.heads / a.kv_heads);
+    const uint64_t list = uint64_t(a.q_rows) * (a.heads / a.kv_heads), key_tiles = (uint64_t(a.kv_rows) + 63u) / 64u;
     const uint64_t cus = uint64_t(std::max(host::cu_count(), 1));
-    p.waves = (p.list + 255u) / 256u * a.kv_heads * 2u >= cus ? kPairWaves : 1u;
-    p.tiles = (p.list + 32u * p.waves - 1u) / (32u * p.waves);
-    const uint64_t blocks = p.tiles * a.kv_heads, key_tiles = (uint64_t(a.kv_rows) + 63u) / 64u;
-    const uint64_t want = blocks >= 2u * cus ? 1u : (4u * cus + blocks - 1u) / blocks;
-    p.splits = uint32_t(std::max<uint64_t>(1u, std::min<uint64_t>({want, key_tiles / 4u, 256u})));
-    return p;
+    const double head_us = double(a.kv_heads) * a.kv_rows * 512.0 * 1e-6; // us a pass over K and V at 1 TB/s
+    Plan best{};
+    double best_us = 0.0;
+    for (const uint32_t waves : {kPairWaves, 1u}) {
+        const bool pair = waves == kPairWaves;
+        const uint64_t tiles = (list + 32u * waves - 1u) / (32u * waves), blocks = tiles * a.kv_heads;
+        for (const uint64_t fill : {uint64_t(0), cus, 2u * cus, 4u * cus}) {
+            // At least four key tiles a split.
+            const uint64_t splits = std::max<uint64_t>(1u, std::min<uint64_t>({fill / blocks, key_tiles / 4u, 256u}));
+            const uint64_t rounds = (blocks * splits + (pair ? cus : 4u * cus) - 1u) / (pair ? cus : 4u * cus);
+            const double turns = double((key_tiles + splits - 1u) / splits);
+            double us = std::max(double(rounds) * (pair ? 14.0 + 1.5 * turns : 10.0 + 1.75 * turns),
+                                 head_us * (1.0 / 6.0 + double(tiles - 1u) / 16.0));
+            if (splits > 1u)
+                us += 6.0 + double(splits) * double(a.kv_heads) * double(list) * 1040.0 * 1e-6 / 4.0;
+            if (best.waves == 0u || us < best_us)
+                best = Plan{waves, uint32_t(splits), list, tiles}, best_us = us;
+        }
+    }
+    return best;
 }
 
 uint64_t workspace_bytes(const MH3DenseAttnArgs& a, const Plan& p)
@@ -986,7 +1032,7 @@ extern "C" int mh3_flash_attn_128(const MH3DenseAttnArgs* args, const uint16_t* 
     if (rc != MH3_OK || p.splits == 1u)
         return rc;
     const uint64_t items = uint64_t(p.kv_heads) * p.list;
-    hipLaunchKernelGGL(attn_join_kernel, dim3(uint32_t((items + 3u) / 4u)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(attn_join_kernel, dim3(uint32_t(items)), dim3(256), 0, s, p);
     return host::check_launch();
 }
 

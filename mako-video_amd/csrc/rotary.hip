@@ -46,9 +46,10 @@ int rotary_setup(const MH3AxesArgs* args, const int32_t* pos, uint32_t half, Rot
         if (!(a.theta[x] >= 1.0) || !std::isfinite(a.theta[x]) || !(std::fabs(a.step[x]) <= 1e6) ||
             a.pairs[x] > kMaxRotPairs || at + a.pairs[x] > kMaxRotPairs)
             return MH3_ERR_PARAM;
+        // theta^(-j / pairs) as an exponential (the argument, at most some 700, is within 2^-54: far below the bound).
+        const long double ln = a.pairs[x] ? logl((long double)a.theta[x]) / (long double)a.pairs[x] : 0.0L;
         for (uint32_t j = 0; j < a.pairs[x]; ++j) {
-            const long double f = (long double)a.step[x] *
-                                  powl((long double)a.theta[x], -(long double)j / (long double)a.pairs[x]) /
+            const long double f = (long double)a.step[x] * expl(-(long double)j * ln) /
                                   6.283185307179586476925286766559005768L;
             const long double frac = f - floorl(f); // [0, 1]
             const long double fixed = rintl(ldexpl(frac, 64));

@@ -12,6 +12,7 @@ fallback: if libmako_h3.so is missing, importing this module raises.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import os
 from pathlib import Path
@@ -197,21 +198,22 @@ def _one_device(**tensors: torch.Tensor | None) -> torch.device:
             continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}: expected a tensor")
-        if t.device.type != "cuda":
-            raise ValueError(f"{name}: must be on the GPU")
-        if device is not None and t.device != device:
+        if device is None:
+            device = t.device
+            if device.type != "cuda":
+                raise ValueError(f"{name}: must be on the GPU")
+        elif t.device != device:
             raise ValueError(f"{name}: on {t.device}, other operands on {device}")
-        device = t.device
     return device
 
 
-def _on(device: torch.device, call, what: str) -> None:
-    """call(stream) on `device` as the current one, with its current stream."""
+def _on(device: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, stream) with `device` the current one, on its current stream."""
     if device.index == torch.cuda.current_device():
-        _check(call(_stream()), what)
+        _check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
     else:
         with torch.cuda.device(device):
-            _check(call(_stream()), what)
+            _check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -655,23 +657,31 @@ def heads_partial_pool(qkv, heads, grid, q_w=None, k_w=None, cos_t=None, sin_t=N
 
 # ---- rotary positions with several axes ------------------------------------------------------------------------------
 
-def _axes_args(pos, pairs, theta, step) -> AxesArgs:
+@functools.lru_cache(maxsize=64)
+def _axes(pairs, theta, step) -> AxesArgs:
+    """The argument struct of a set of axes (one a configuration, so its fields are checked and filled once)."""
     axes = len(pairs)
     if not 1 <= axes <= 4:
         raise ValueError("one to four axes")
-    theta = (theta,) * axes if isinstance(theta, (int, float)) else tuple(theta)
-    step = (step,) * axes if isinstance(step, (int, float)) else tuple(step)
+    theta = (theta,) * axes if isinstance(theta, (int, float)) else theta
+    step = (step,) * axes if isinstance(step, (int, float)) else step
     if len(theta) != axes or len(step) != axes:
         raise ValueError("theta and step: one value, or one an axis")
-    if pos.dim() != 2 or pos.shape[1] != axes:
-        raise ValueError(f"pos must be [rows][{axes}]")
     if any(int(n) != n or not 0 <= n <= 64 for n in pairs):
         raise ValueError("pairs: 0 to 64 an axis")
-    _need(pos, "pos", torch.int32, pos.numel())
     a = AxesArgs()
     a.axes = axes
     for i in range(axes):
         a.pairs[i], a.theta[i], a.step[i] = int(pairs[i]), theta[i], step[i]
+    return a
+
+
+def _axes_args(pos, pairs, theta, step) -> AxesArgs:
+    a = _axes(tuple(pairs), theta if isinstance(theta, (int, float)) else tuple(theta),
+              step if isinstance(step, (int, float)) else tuple(step))
+    if pos.dim() != 2 or pos.shape[1] != a.axes:
+        raise ValueError(f"pos must be [rows][{a.axes}]")
+    _need(pos, "pos", torch.int32, pos.numel())
     return a
 
 
@@ -680,13 +690,15 @@ def rotary_axes(pos, pairs, *, theta=10000.0, step=1.0, cos=None, sin=None):
     [rows][axes], the first pairs[0] of a head's pairs turned by axis 0, the next pairs[1] by axis 1, ...; pair j of
     axis a by pos[:, a] step[a] theta[a]^(-j / pairs[a]) radians. Returns (cos, sin), float [rows][sum(pairs)]."""
     a = _axes_args(pos, pairs, theta, step)
-    rows, half = pos.shape[0], sum(int(n) for n in pairs)
-    cos = torch.empty((rows, half), dtype=torch.float32, device=pos.device) if cos is None else cos
-    sin = torch.empty((rows, half), dtype=torch.float32, device=pos.device) if sin is None else sin
-    _need(cos, "cos", torch.float32, rows * half)
-    _need(sin, "sin", torch.float32, rows * half)
-    _on(_one_device(pos=pos, cos=cos, sin=sin),
-        lambda s: lib.mh3_rotary_axes(C.byref(a), rows, _ptr(pos), _ptr(cos), _ptr(sin), s), "rotary_axes")
+    rows, half, device = pos.shape[0], sum(a.pairs), pos.device
+    given = cos is not None or sin is not None
+    cos = torch.empty((rows, half), dtype=torch.float32, device=device) if cos is None else cos
+    sin = torch.empty((rows, half), dtype=torch.float32, device=device) if sin is None else sin
+    if given:
+        _need(cos, "cos", torch.float32, rows * half)
+        _need(sin, "sin", torch.float32, rows * half)
+        _one_device(pos=pos, cos=cos, sin=sin)
+    _on(device, "rotary_axes", lib.mh3_rotary_axes, C.byref(a), rows, pos.data_ptr(), cos.data_ptr(), sin.data_ptr())
     return cos, sin
 
 
@@ -697,12 +709,11 @@ def heads_partial_axes(qkv, heads, pos, pairs, q_w=None, k_w=None, *, theta=1000
     ax = _axes_args(pos, pairs, theta, step)
     if qkv.dim() == 2 and pos.shape[0] != qkv.shape[0]:
         raise ValueError("pos: one row a row of qkv")
-    rot = 2 * sum(int(n) for n in pairs)
     device = _one_device(qkv=qkv, pos=pos, q_w=q_w, k_w=k_w, map=map, q=q, k=k, v=v)
     a, outs, ptrs = _heads_setup(qkv, heads, q_w, k_w, None, None, 0, eps, map, with_v, layout, q, k, v)
-    a.rot = rot
-    _on(device, lambda s: lib.mh3_heads_partial_axes(C.byref(a), C.byref(ax), *ptrs[:3], _ptr(pos), ptrs[5],
-                                                     *(_ptr(t) for t in outs), s), "heads_partial_axes")
+    a.rot = 2 * sum(ax.pairs)
+    _on(device, "heads_partial_axes", lib.mh3_heads_partial_axes, C.byref(a), C.byref(ax), ptrs[0], ptrs[1], ptrs[2],
+        pos.data_ptr(), ptrs[5], _ptr(outs[0]), _ptr(outs[1]), _ptr(outs[2]))
     return tuple(outs)
 
 
@@ -743,32 +754,24 @@ def attn_ranges(q_off, k_off, q_rows, kv_rows, *, prefix=None, causal=False, ran
     _need(ranges, "ranges", torch.int32, 2 * q_rows)
     if docs < 1:
         raise ValueError("q_off: at least one document")
-    a = RangeArgs()
-    a.q_rows, a.kv_rows, a.docs, a.causal = q_rows, kv_rows, docs, int(bool(causal))
-    _on(_one_device(q_off=q_off, k_off=k_off, prefix=prefix, ranges=ranges),
-        lambda s: lib.mh3_attn_ranges(C.byref(a), _ptr(q_off), _ptr(k_off), _ptr(prefix), _ptr(ranges), s),
-        "attn_ranges")
+    a = RangeArgs(q_rows, kv_rows, docs, int(bool(causal)))
+    _on(_one_device(q_off=q_off, k_off=k_off, prefix=prefix, ranges=ranges), "attn_ranges", lib.mh3_attn_ranges,
+        C.byref(a), q_off.data_ptr(), k_off.data_ptr(), _ptr(prefix), ranges.data_ptr())
     return ranges
 
 
-def _dense_args(q, k, v, out, layout, out_layout, scale, cap) -> DenseAttnArgs:
+def _dense_args(q, k, v, layout, scale, cap) -> DenseAttnArgs:
     heads, q_rows, qhs, qrs = _head_rows(q, "q", layout)
     kv_heads, kv_rows, khs, krs = _head_rows(k, "k", layout)
-    if _head_rows(v, "v", layout)[:2] != (kv_heads, kv_rows):
+    v_heads, v_rows, vhs, vrs = _head_rows(v, "v", layout)
+    if v_heads != kv_heads or v_rows != kv_rows:
         raise ValueError("k and v: the same heads and rows")
-    if _head_rows(out, "out", out_layout)[:2] != (heads, q_rows):
-        raise ValueError("out: q's heads and rows")
-    a = DenseAttnArgs()
-    a.heads, a.kv_heads, a.head_dim, a.q_rows, a.kv_rows, a.scale, a.cap = heads, kv_heads, 128, q_rows, kv_rows, scale, cap
-    a.q_head_stride, a.q_row_stride, a.k_head_stride, a.k_row_stride = qhs, qrs, khs, krs
-    a.v_head_stride, a.v_row_stride = _head_rows(v, "v", layout)[2:]
-    a.out_head_stride, a.out_row_stride = _head_rows(out, "out", out_layout)[2:]
-    return a
+    return DenseAttnArgs(heads, kv_heads, 128, q_rows, kv_rows, scale, cap, 0, qhs, qrs, khs, krs, vhs, vrs, 0, 128)
 
 
 def flash_attn_128_workspace_bytes(q, k, v, *, layout="heads") -> int:
     """Bytes of workspace that flash_attn_128 needs for these operands (0 where it needs none)."""
-    n = int(lib.mh3_flash_attn_128_workspace_bytes(C.byref(_dense_args(q, k, v, q, layout, layout, 0.0, 0.0))))
+    n = int(lib.mh3_flash_attn_128_workspace_bytes(C.byref(_dense_args(q, k, v, layout, 0.0, 0.0))))
     _check(min(n, 0), "flash_attn_128_workspace_bytes")
     return n
 
@@ -784,26 +787,35 @@ def flash_attn_128(q, k, v, *, ranges=None, scale=0.0, cap=0.0, slopes=None, q_p
     out_layout = layout if out_layout is None else out_layout
     if layout not in ("heads", "rows") or out_layout not in ("heads", "rows"):
         raise ValueError("layout is 'heads' or 'rows'")
-    heads, q_rows = _head_rows(q, "q", layout)[:2]
+    a = _dense_args(q, k, v, layout, scale, cap)
+    heads, q_rows = a.heads, a.q_rows
     device = _one_device(q=q, k=k, v=v, ranges=ranges, slopes=slopes, q_pos=q_pos, k_pos=k_pos, out=out,
                          workspace=workspace)
     if out is None:
         out = torch.empty((heads, q_rows, 128) if out_layout == "heads" else (q_rows, heads * 128),
                           dtype=torch.bfloat16, device=device)
-    a = _dense_args(q, k, v, out, layout, out_layout, scale, cap)
-    for name, t, dtype, n in (("ranges", ranges, torch.int32, 2 * q_rows), ("slopes", slopes, torch.float32, heads),
-                              ("q_pos", q_pos, torch.int32, q_rows), ("k_pos", k_pos, torch.int32, a.kv_rows)):
-        if t is not None:
-            _need(t, name, dtype, n)
-    nbytes = int(lib.mh3_flash_attn_128_workspace_bytes(C.byref(a)))
-    _check(min(nbytes, 0), "flash_attn_128")
-    if workspace is None and nbytes:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    out_heads, out_rows, a.out_head_stride, a.out_row_stride = _head_rows(out, "out", out_layout)
+    if out_heads != heads or out_rows != q_rows:
+        raise ValueError("out: q's heads and rows")
+    if ranges is not None:
+        _need(ranges, "ranges", torch.int32, 2 * q_rows)
+    if slopes is not None:
+        _need(slopes, "slopes", torch.float32, heads)
+    if q_pos is not None:
+        _need(q_pos, "q_pos", torch.int32, q_rows)
+    if k_pos is not None:
+        _need(k_pos, "k_pos", torch.int32, a.kv_rows)
+    ref = C.byref(a)
+    nbytes = lib.mh3_flash_attn_128_workspace_bytes(ref)
+    if nbytes < 0:
+        _check(nbytes, "flash_attn_128")
     if workspace is not None:
         _need(workspace, "workspace", torch.uint8, nbytes)
-    _on(device, lambda s: lib.mh3_flash_attn_128(
-        C.byref(a), _ptr(q), _ptr(k), _ptr(v), _ptr(ranges), _ptr(slopes), _ptr(q_pos), _ptr(k_pos), _ptr(workspace),
-        0 if workspace is None else workspace.numel(), _ptr(out), s), "flash_attn_128")
+    elif nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _on(device, "flash_attn_128", lib.mh3_flash_attn_128, ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(ranges),
+        _ptr(slopes), _ptr(q_pos), _ptr(k_pos), _ptr(workspace), 0 if workspace is None else workspace.numel(),
+        out.data_ptr())
     return out
 
 
@@ -986,8 +998,8 @@ def quant_rows_mx4(w, *, q=None, scale=None):
     scale = torch.empty((a.cols // 256, a.rows, 8), dtype=torch.uint8, device=w.device) if scale is None else scale
     _need(q, "q", torch.uint8, w.numel() // 2)
     _need(scale, "scale", torch.uint8, w.numel() // 32)
-    _on(_one_device(w=w, q=q, scale=scale),
-        lambda s: lib.mh3_quant_rows_mx4(C.byref(a), _ptr(w), _ptr(q), _ptr(scale), s), "quant_rows_mx4")
+    _on(_one_device(w=w, q=q, scale=scale), "quant_rows_mx4", lib.mh3_quant_rows_mx4, C.byref(a), w.data_ptr(),
+        q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
@@ -1009,8 +1021,8 @@ def gemm_mx4(x, x_scale, w, w_scale, *, out=None):
     a = _mx4_args(x, x_scale, w, w_scale)
     out = torch.empty((a.m, a.n), dtype=torch.bfloat16, device=x.device) if out is None else out
     _need(out, "out", torch.bfloat16, a.m * a.n)
-    _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, out=out),
-        lambda s: lib.mh3_gemm_mx4(C.byref(a), _ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(out), s), "gemm_mx4")
+    _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, out=out), "gemm_mx4", lib.mh3_gemm_mx4, C.byref(a),
+        x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), out.data_ptr())
     return out
 
 
@@ -1022,9 +1034,8 @@ def gemm_mx4_swiglu(x, x_scale, w, w_scale, *, out=None):
     a.n //= 2
     out = torch.empty((a.m, a.n), dtype=torch.bfloat16, device=x.device) if out is None else out
     _need(out, "out", torch.bfloat16, a.m * a.n)
-    _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, out=out),
-        lambda s: lib.mh3_gemm_mx4_swiglu(C.byref(a), _ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(out), s),
-        "gemm_mx4_swiglu")
+    _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, out=out), "gemm_mx4_swiglu", lib.mh3_gemm_mx4_swiglu,
+        C.byref(a), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), out.data_ptr())
     return out
 
 
@@ -1039,6 +1050,6 @@ def gemm_mx4_gate_add(x, x_scale, w, w_scale, residual, gate, *, set_of_row=None
         _need(set_of_row, "set_of_row", torch.uint8, a.m)
     fn = lib.mh3_gemm_mx4_gate_add_f32 if f32 else lib.mh3_gemm_mx4_gate_add
     _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, residual=residual, gate=gate, set_of_row=set_of_row),
-        lambda s: fn(C.byref(a), _ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(gate), _ptr(set_of_row),
-                     _ptr(residual), s), "gemm_mx4_gate_add")
+        "gemm_mx4_gate_add", fn, C.byref(a), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+        gate.data_ptr(), _ptr(set_of_row), residual.data_ptr())
     return residual
