@@ -15,11 +15,24 @@
 #include "gemm.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace mh3 {
 namespace {
 
 typedef int int32x8 __attribute__((ext_vector_type(8)));
+
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ u32x4_t load_b128(__amdgpu_buffer_rsrc_t buffer, uint32_t offset, int soffset)
+{
+    return __builtin_amdgcn_raw_buffer_load_b128(buffer, offset, soffset, 0);
+}
+
+__device__ __forceinline__ u32x2_t load_b64(__amdgpu_buffer_rsrc_t buffer, uint32_t offset, int soffset)
+{
+    return __builtin_amdgcn_raw_buffer_load_b64(buffer, offset, soffset, 0);
+}
 
 constexpr uint32_t kPastEnd = 0x80000000u; // a buffer offset past num_records: the load reads zeros
 
@@ -208,6 +221,147 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx4_kernel(const uint8_t* __
     gemm_epilogue<BM, BN, WM, WN, kBf16, EPI, TM, TN>(acc, smem, M, N, m0, w_lo, w_hi, nullptr, nullptr, out, gg);
 }
 
+// Up to 16 MT rows: the time is w's one pass from memory. A workgroup takes 32 rows of w (SwiGLU: 16 gate rows and their
+// 16 up rows), its eight waves the K-steps in turn, from memory straight into registers; their sums are joined through LDS
+// in the waves' order. The products are w x^T: a lane then holds four consecutive columns of one row of the result.
+constexpr uint32_t kFewWaves = 8, kFewTiles = 2; // tiles of 16 rows of w
+
+template <int MT, int EPI>
+__global__ __launch_bounds__(kFewWaves * 64) void gemm_mx4_few_kernel(const uint8_t* __restrict__ x,
+                                                                      const uint8_t* __restrict__ xs,
+                                                                      const uint8_t* __restrict__ w,
+                                                                      const uint8_t* __restrict__ ws,
+                                                                      uint16_t* __restrict__ out, uint32_t M, uint32_t N,
+                                                                      uint32_t K, GemmGate gg)
+{
+    constexpr uint32_t NT = kFewTiles, kPair = EPI == kSwiGLU ? 1u : NT; // column tiles of the result
+    __shared__ floatx4 part[kFewWaves][MT * NT][64];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t KB = K / 2u, KT = K / 256u, w_rows = EPI == kSwiGLU ? 2u * N : N, n0 = blockIdx.x * 16u * kPair;
+    const uint32_t r = lane % 16u, kq = lane >> 4, shift = kq * 8u;
+
+    // A thread's four results: columns 16 j + 4 kq .. of row 16 i + r, for the wave's tile (i, j). What the epilogue adds
+    // to is on its way while the products are made.
+    const uint32_t ti = wave / kPair, tj = wave % kPair;
+    const uint32_t row = 16u * ti + r, col = n0 + 16u * tj + kq * 4u;
+    const bool stores = wave < MT * kPair && row < M;
+    const uint64_t at = uint64_t(row) * N + col;
+    floatx4 gate{}, res{};
+    if constexpr (EPI == kGateAdd || EPI == kGateAddF32) {
+        if (stores) {
+            const uint32_t set = gg.set_of_row ? min(uint32_t(gg.set_of_row[row]), gg.n_sets - 1u) : 0u;
+            const float* const g = gg.gate + uint64_t(set) * gg.gate_stride + col;
+            gate = floatx4{g[0], g[1], g[2], g[3]};
+            if constexpr (EPI == kGateAddF32) {
+                res = *reinterpret_cast<const floatx4*>(reinterpret_cast<const float*>(out) + at);
+            } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(out + at);
+                res = floatx4{bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y)};
+            }
+        }
+    }
+
+    // A lane's 16 bytes of a K-step's half h are block 4 h + kq of its row. Rows past M repeat the last one.
+    const __amdgpu_buffer_rsrc_t ra = buffer_rsrc(x, M * KB), rb = buffer_rsrc(w, w_rows * KB);
+    const __amdgpu_buffer_rsrc_t rsa = buffer_rsrc(xs, KT * M * 8u), rsb = buffer_rsrc(ws, KT * w_rows * 8u);
+    uint32_t a_row[MT], b_row[NT];
+#pragma unroll
+    for (uint32_t t = 0; t < MT; ++t)
+        a_row[t] = min(16u * t + r, M - 1u);
+#pragma unroll
+    for (uint32_t t = 0; t < NT; ++t)
+        b_row[t] = n0 + r + (EPI == kSwiGLU ? t * N : 16u * t);
+
+    floatx4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < int(NT); ++j)
+            acc[i][j] = floatx4{};
+    auto widen = [](const u32x4_t& v) { return int32x8{int(v[0]), int(v[1]), int(v[2]), int(v[3]), 0, 0, 0, 0}; };
+    struct Step {
+        u32x4_t fa[MT][2], fb[NT][2];
+        u32x2_t sa[MT], sb[NT];
+    };
+    auto load = [&](uint32_t kt, Step& p) {
+#pragma unroll
+        for (int t = 0; t < int(NT); ++t) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+                p.fb[t][h] = load_b128(rb, b_row[t] * KB + kq * 16u + h * 64u, int(kt * 128u));
+            p.sb[t] = load_b64(rsb, b_row[t] * 8u, int(kt * w_rows * 8u));
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+                p.fa[t][h] = load_b128(ra, a_row[t] * KB + kq * 16u + h * 64u, int(kt * 128u));
+            p.sa[t] = load_b64(rsa, a_row[t] * 8u, int(kt * M * 8u));
+        }
+        __builtin_amdgcn_sched_barrier(0); // before the products of the step before
+    };
+    auto multiply = [&](const Step& p) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < int(NT); ++j)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        widen(p.fb[j][h]), widen(p.fa[i][h]), acc[i][j], 4, 4, 0, int(p.sb[j][h] >> shift), 0,
+                        int(p.sa[i][h] >> shift));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // A step's loads go out before the products of the step before it.
+    if (wave < KT) {
+        Step p[2];
+        load(wave, p[0]);
+        uint32_t kt = wave;
+        for (; kt + 2u * kFewWaves < KT; kt += 2u * kFewWaves) {
+            load(kt + kFewWaves, p[1]);
+            multiply(p[0]);
+            load(kt + 2u * kFewWaves, p[0]);
+            multiply(p[1]);
+        }
+        if (kt + kFewWaves < KT)
+            load(kt + kFewWaves, p[1]);
+        multiply(p[0]);
+        if (kt + kFewWaves < KT)
+            multiply(p[1]);
+    }
+
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < int(NT); ++j)
+            part[wave][i * int(NT) + j][lane] = acc[i][j];
+    __syncthreads();
+    if (!stores)
+        return;
+    auto joined = [&](uint32_t tile) {
+        floatx4 y = part[0][tile][lane];
+#pragma unroll
+        for (uint32_t v = 1; v < kFewWaves; ++v)
+            y += part[v][tile][lane];
+        return y;
+    };
+    floatx4 y = joined(ti * NT + tj);
+    if constexpr (EPI == kSwiGLU) {
+        const floatx4 up = joined(ti * NT + 1u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            y[e] = y[e] * __builtin_amdgcn_rcpf(1.0f + __expf(-y[e])) * up[e];
+    }
+    if constexpr (EPI == kGateAdd || EPI == kGateAddF32)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            y[e] = fmaf(gate[e], y[e], res[e]);
+    if constexpr (EPI == kGateAddF32)
+        *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(out) + at) = y;
+    else
+        *reinterpret_cast<uint2*>(out + at) = uint2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+}
+
 // The launch with tiles of BM rows and BN columns (2 BN where the epilogue pairs none).
 template <int BM, int BN, int WM, int WN, int S, int EPI>
 int launch_tile(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* xs, const uint8_t* w, const uint8_t* ws,
@@ -221,6 +375,47 @@ int launch_tile(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* xs, const
     hipLaunchKernelGGL(kernel, dim3(mt * nt), dim3(WM * WN * 64), kLds, static_cast<hipStream_t>(stream), x, xs, w, ws,
                        out, a->m, a->n, a->k, mt, nt, gg);
     return host::check_launch();
+}
+
+template <int MT, int EPI>
+int launch_few(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* xs, const uint8_t* w, const uint8_t* ws,
+               uint16_t* out, const GemmGate& gg, mh3_stream_t stream)
+{
+    hipLaunchKernelGGL((gemm_mx4_few_kernel<MT, EPI>), dim3(a->n / (EPI == kSwiGLU ? 16u : 32u)), dim3(kFewWaves * 64), 0,
+                       static_cast<hipStream_t>(stream), x, xs, w, ws, out, a->m, a->n, a->k, gg);
+    return host::check_launch();
+}
+
+// The kernels by their tiles: rows, and rows of w.
+enum Mx4Tile { kFew, k64x128, k128x128, k192x256, k256x256 };
+
+// The kernel of least estimated time (us), from the sizes alone. A tile kernel: rounds of the 256 CUs, each the K-steps'
+// time in one tile; measured on one round of 21 .. 56 steps, 0.45 .. 0.55, 0.70 .. 0.75, 1.4 .. 1.6 and 1.6 .. 1.9 us a step.
+// The few-row kernel: its bytes, x's from the caches, at the rate that either reads w from memory with.
+// At n 5376, k 14336, rows 1, 32, 128, 512, 1024: few 11.3, 17.0, -; 64 x 128 26, 28, 31, 56, 83; 128 x 128 -, -, 42, 41,
+// 80; 192 x 256 -, -, 84, 86, 84; 256 x 256 -, -, 90, 98, 97. At n 21504, k 5376, rows 1, 64, 192, 945: few 13.1, -; 64 x
+// 128 14.0, 16.6, 27.9; 128 x 128 -, 18.5, 35.4; 192 x 256 -, 33, 38, 77; 256 x 256 -, 36, 39, 87.
+Mx4Tile tile_of_sizes(uint32_t m, uint32_t w_rows, uint32_t k)
+{
+    const float steps = float(k / 256u), kStart = 4.0f, kRate = 6.2e6f; // bytes a us
+    const float w_us = float(w_rows) * float(k) * (0.53125f / kRate);
+    struct Tile {
+        Mx4Tile tile;
+        uint32_t rows, cols;
+        float step_us;
+    };
+    constexpr Tile kTiles[] = {
+        {k256x256, 256, 256, 1.75f}, {k192x256, 192, 256, 1.5f}, {k128x128, 128, 128, 0.73f}, {k64x128, 64, 128, 0.48f}};
+    Mx4Tile best = k256x256;
+    float least = INFINITY;
+    for (const Tile& t : kTiles) {
+        const uint64_t tiles = uint64_t((m + t.rows - 1u) / t.rows) * (w_rows / t.cols);
+        const float us = kStart + std::max(float((tiles + 255u) / 256u) * steps * t.step_us, w_us);
+        if (us < least)
+            least = us, best = t.tile;
+    }
+    const float x_us = float(w_rows / 32u) * float(m) * float(k) * (0.5f * 0.7f / kRate);
+    return m <= 32u && kStart + w_us + x_us <= least ? kFew : best;
 }
 
 // The checks of the four entry points and their launch.
@@ -263,7 +458,20 @@ int launch_mx4(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* xs, const 
     const uint32_t nt = a->n / kCols;
     if (uint64_t((a->m + 63u) / 64u) * nt * 4u >= (uint64_t(1) << 23)) // a launch holds under 2^32 threads
         return MH3_ERR_SHAPE;
-    return launch_tile<256, kBN, 2, 4, 2, EPI>(a, x, xs, w, ws, out, gg, stream);
+    switch (tile_of_sizes(a->m, uint32_t(w_rows), a->k)) {
+    case kFew:
+        return a->m <= 16u ? launch_few<1, EPI>(a, x, xs, w, ws, out, gg, stream)
+                           : launch_few<2, EPI>(a, x, xs, w, ws, out, gg, stream);
+    case k64x128:
+        return launch_tile<64, 64, 2, 4, 4, EPI>(a, x, xs, w, ws, out, gg, stream);
+    case k128x128:
+        return launch_tile<128, 64, 2, 4, 3, EPI>(a, x, xs, w, ws, out, gg, stream);
+    case k192x256:
+        return launch_tile<192, 128, 2, 4, 2, EPI>(a, x, xs, w, ws, out, gg, stream);
+    case k256x256:
+        break;
+    }
+    return launch_tile<256, 128, 2, 4, 2, EPI>(a, x, xs, w, ws, out, gg, stream);
 }
 
 const GemmGate kNoGate{nullptr, nullptr, 0, 0};
