@@ -180,7 +180,7 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name}: must be on the GPU")
     if t.dtype != dtype:
         raise ValueError(f"{name}: dtype {t.dtype}, expected {dtype}")
@@ -190,30 +190,33 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int) -> None:
         raise ValueError(f"{name}: {t.numel()} elements, the call touches {numel}")
 
 
-def _one_device(**tensors: torch.Tensor | None) -> torch.device:
-    """The GPU that all of the tensors (None skipped) are on."""
-    device = None
+def _one_device(**tensors: torch.Tensor | None) -> int:
+    """The index of the GPU that all of the tensors (None skipped) are on."""
+    device = -1
     for name, t in tensors.items():
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}: expected a tensor")
-        if device is None:
-            device = t.device
-            if device.type != "cuda":
+        index = t.get_device()
+        if index != device:
+            if index < 0 or not t.is_cuda:
                 raise ValueError(f"{name}: must be on the GPU")
-        elif t.device != device:
-            raise ValueError(f"{name}: on {t.device}, other operands on {device}")
+            if device >= 0:
+                raise ValueError(f"{name}: on GPU {index}, other operands on GPU {device}")
+            device = index
     return device
 
 
-def _on(device: torch.device, what: str, fn, *args) -> None:
+def _on(device: int, what: str, fn, *args) -> None:
     """fn(*args, stream) with `device` the current one, on its current stream."""
-    if device.index == torch.cuda.current_device():
-        _check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+    if device == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            _check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc != OK:
+        _check(rc, what)
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -673,6 +676,7 @@ def _axes(pairs, theta, step) -> AxesArgs:
     a.axes = axes
     for i in range(axes):
         a.pairs[i], a.theta[i], a.step[i] = int(pairs[i]), theta[i], step[i]
+    a.half = sum(a.pairs)
     return a
 
 
@@ -690,7 +694,7 @@ def rotary_axes(pos, pairs, *, theta=10000.0, step=1.0, cos=None, sin=None):
     [rows][axes], the first pairs[0] of a head's pairs turned by axis 0, the next pairs[1] by axis 1, ...; pair j of
     axis a by pos[:, a] step[a] theta[a]^(-j / pairs[a]) radians. Returns (cos, sin), float [rows][sum(pairs)]."""
     a = _axes_args(pos, pairs, theta, step)
-    rows, half, device = pos.shape[0], sum(a.pairs), pos.device
+    rows, half, device = pos.shape[0], a.half, pos.device
     given = cos is not None or sin is not None
     cos = torch.empty((rows, half), dtype=torch.float32, device=device) if cos is None else cos
     sin = torch.empty((rows, half), dtype=torch.float32, device=device) if sin is None else sin
@@ -698,7 +702,7 @@ def rotary_axes(pos, pairs, *, theta=10000.0, step=1.0, cos=None, sin=None):
         _need(cos, "cos", torch.float32, rows * half)
         _need(sin, "sin", torch.float32, rows * half)
         _one_device(pos=pos, cos=cos, sin=sin)
-    _on(device, "rotary_axes", lib.mh3_rotary_axes, C.byref(a), rows, pos.data_ptr(), cos.data_ptr(), sin.data_ptr())
+    _on(device.index, "rotary_axes", lib.mh3_rotary_axes, C.byref(a), rows, pos.data_ptr(), cos.data_ptr(), sin.data_ptr())
     return cos, sin
 
 
@@ -711,7 +715,7 @@ def heads_partial_axes(qkv, heads, pos, pairs, q_w=None, k_w=None, *, theta=1000
         raise ValueError("pos: one row a row of qkv")
     device = _one_device(qkv=qkv, pos=pos, q_w=q_w, k_w=k_w, map=map, q=q, k=k, v=v)
     a, outs, ptrs = _heads_setup(qkv, heads, q_w, k_w, None, None, 0, eps, map, with_v, layout, q, k, v)
-    a.rot = 2 * sum(ax.pairs)
+    a.rot = 2 * ax.half
     _on(device, "heads_partial_axes", lib.mh3_heads_partial_axes, C.byref(a), C.byref(ax), ptrs[0], ptrs[1], ptrs[2],
         pos.data_ptr(), ptrs[5], _ptr(outs[0]), _ptr(outs[1]), _ptr(outs[2]))
     return tuple(outs)
