@@ -162,11 +162,14 @@ struct WaveRows {
     uint32_t all_lo, all_hi;    // keys that every row with any attends: [all_lo, all_hi)
     uint32_t any_lo, any_hi;    // keys that some row attends lie in [any_lo, any_hi)
     float slope_log2;           // BIAS: the row's head's slope, in base-2 units
-    int32_t q_pos;
-    // Whether the wave has work in the tile at key t0, and whether some row's range does not cover it.
-    __device__ __forceinline__ bool meets(uint32_t t0) const { return t0 < any_hi && t0 + 64u > any_lo; }
+    int32_t q_pos, q_base;      // BIAS: the row's position, the wave's first row's
+    float q_rel;                // BIAS: their difference, if q_near: it is under 2^23 in all of the wave's rows
+    bool q_near;
+    // Whether some row's range does not cover the tile at key t0.
     __device__ __forceinline__ bool masks(uint32_t t0) const { return t0 < all_lo || t0 + 64u > all_hi; }
 };
+
+__device__ __forceinline__ bool is_near(int32_t rel) { return rel > -(1 << 23) && rel < (1 << 23); }
 
 template <bool BIAS>
 __device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, uint32_t f0, uint32_t lane, WaveRows& w)
@@ -198,50 +201,62 @@ __device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, ui
     if (BIAS) {
         w.slope_log2 = p.slopes[head] * kLog2e;
         w.q_pos = p.q_pos ? p.q_pos[row] : int32_t(row);
+        w.q_base = __builtin_amdgcn_readfirstlane(w.q_pos);
+        const int32_t rel = __builtin_elementwise_sub_sat(w.q_pos, w.q_base);
+        w.q_near = !__ballot(!is_near(rel));
+        w.q_rel = float(rel);
     }
 }
 
-// Scores of a tile at key t0 to base-2 units where a cap or a bias needs every one changed; kp: the tile's key positions
-// (LDS, or null: the keys' numbers).
-template <bool CAP, bool BIAS>
-__device__ __forceinline__ void shape_scores(const DenseParams& p, const WaveRows& w, floatx16 (&s)[2], uint32_t t0,
-                                             uint32_t hh, const int32_t* kp)
+// Scores x under a cap, without their factor and but for a constant, which a softmax does not see: tanh(u) =
+// 1 - 2 / (exp(2 u) + 1), so cap tanh(u) log2(e) is cap_out + 2 cap_out times -1 / (exp2(cap_in x) + 1). At either end the
+// exponential gives +-cap, and the error near zero is 2^-23 of the cap, below what bf16 operands leave of the score.
+__device__ __forceinline__ void cap_scores(const DenseParams& p, floatx16 (&s)[2])
 {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const uint32_t key = 32u * b + 8u * g + 4u * hh;
-            int32_t pos[4];
-            if (BIAS) {
-                if (kp) {
-                    const int4 t = *reinterpret_cast<const int4*>(kp + key);
-                    pos[0] = t.x, pos[1] = t.y, pos[2] = t.z, pos[3] = t.w;
-                } else {
+        for (int i = 0; i < 16; ++i)
+            s[b][i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[b][i] * p.cap_in));
+}
+
+// The key positions of a tile at key t0 as floats from the wave's base, into kp (LDS of the wave's own, which holds
+// k_pos's values where there is one), if they and the wave's rows are all under 2^23 from it: float differences of them
+// are then exact, two operations a score. Otherwise kp is left as it was.
+__device__ __forceinline__ bool near_positions(const DenseParams& p, const WaveRows& w, uint32_t t0, int32_t* kp,
+                                               uint32_t lane)
+{
+    const int32_t rel = __builtin_elementwise_sub_sat(p.k_pos ? kp[lane] : int32_t(t0 + lane), w.q_base);
+    if (!w.q_near || __ballot(!is_near(rel)))
+        return false;
+    reinterpret_cast<float*>(kp)[lane] = float(rel);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return true;
+}
+
+// Scores in units of `unit` to base-2 units less the bias. NEAR: kp as near_positions leaves it; otherwise the distances
+// are those of int32 positions (of the tile's key numbers without k_pos), exact before they round to float.
+template <bool NEAR>
+__device__ __forceinline__ void bias_scores(const DenseParams& p, const WaveRows& w, floatx16 (&s)[2], float unit,
+                                            uint32_t t0, const int32_t* kp, uint32_t lane)
+{
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        pos[e] = int32_t(t0 + key) + e;
-                }
-            }
+    for (int g = 0; g < 8; ++g) {
+        const uint32_t key = 8u * uint32_t(g) + 4u * (lane >> 5);
+        const int4 t = NEAR || p.k_pos ? *reinterpret_cast<const int4*>(kp + key)
+                                       : int4{int32_t(t0 + key), int32_t(t0 + key) + 1, int32_t(t0 + key) + 2,
+                                              int32_t(t0 + key) + 3};
+        const int32_t pos[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float x = s[b][4 * g + e];
-                // tanh(u) = 1 - 2 / (exp(2 u) + 1): at either end the exponential gives +-1, and its error near zero is
-                // 2^-23 of the cap, below what bf16 operands leave of the score.
-                if (CAP)
-                    x = fmaf(-2.0f * p.cap_out,
-                             __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * p.cap_in) + 1.0f), p.cap_out);
-                else
-                    x *= p.scale_log2;
-                // The distance of two int32 positions fits 32 bits without a sign.
-                if (BIAS) {
-                    const uint32_t d = w.q_pos > pos[e] ? uint32_t(w.q_pos) - uint32_t(pos[e])
-                                                        : uint32_t(pos[e]) - uint32_t(w.q_pos);
-                    x = fmaf(-w.slope_log2, float(d), x);
-                }
-                s[b][4 * g + e] = x;
-            }
+        for (int e = 0; e < 4; ++e) {
+            const int i = 4 * (g & 3) + e;
+            // The distance of two int32 positions fits 32 bits without a sign.
+            const float d = NEAR ? fabsf(w.q_rel - __int_as_float(pos[e]))
+                                 : float(w.q_pos > pos[e] ? uint32_t(w.q_pos) - uint32_t(pos[e])
+                                                          : uint32_t(pos[e]) - uint32_t(w.q_pos));
+            s[g >> 2][i] = fmaf(s[g >> 2][i], unit, -w.slope_log2 * d);
         }
+    }
 }
 
 // Where a wave's lanes find their operands in a tile's LDS images.
@@ -312,17 +327,44 @@ __device__ __forceinline__ float tile_exponentials(const floatx16 (&s)[2], TileP
     return sum[0] + sum[1];
 }
 
+// The same under a bias, kp as near_positions leaves it.
+__device__ __forceinline__ float tile_exponentials_near(const WaveRows& w, const floatx16 (&s)[2], TileP& pt, float factor,
+                                                        float m, const int32_t* kp, uint32_t lane)
+{
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+        const float4 pos = *reinterpret_cast<const float4*>(kp + 8u * uint32_t(g) + 4u * (lane >> 5));
+        const float at[4] = {pos.x, pos.y, pos.z, pos.w};
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            floatx2 t;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                t[h] = __builtin_amdgcn_exp2f(fmaf(s[g >> 2][4 * (g & 3) + e + h], factor,
+                                                   fmaf(-w.slope_log2, fabsf(w.q_rel - at[e + h]), -m)));
+            sum[0] += t[0], sum[1] += t[1];
+            pt.w[2 * g + e / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(t, bf16x2_t));
+        }
+    }
+    return sum[0] + sum[1];
+}
+
 // The softmax of a tile at key t0 (MASKED: not every row attends all of it): P^T, and the rows' maxima, sums and (where a
 // maximum moved) rescaled O.
 template <bool CAP, bool BIAS, bool MASKED>
 __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, floatx16 (&s)[2], TileP& pt, uint32_t t0,
-                                             const int32_t* kp, uint32_t lane)
+                                             int32_t* kp, uint32_t lane)
 {
     const uint32_t hh = lane >> 5;
-    constexpr bool kShaped = CAP || BIAS;
-    if (kShaped)
-        shape_scores<CAP, BIAS>(p, w, s, t0, hh, kp);
-    const float unit = kShaped ? 1.0f : p.scale_log2;
+    float factor = CAP ? 2.0f * p.cap_out : p.scale_log2; // of the scores as they stand: base-2 units
+    if (CAP)
+        cap_scores(p, s);
+    bool near = BIAS && near_positions(p, w, t0, kp, lane); // the bias is yet to be taken off
+    if (BIAS && !near) {
+        bias_scores<false>(p, w, s, factor, t0, kp, lane);
+        factor = 1.0f;
+    }
     if (MASKED) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -335,18 +377,22 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
     // Most tiles raise no maximum by much, and the sum over a lane's 32 keys of a row tells: up to 2^10 no key is above
     // that, and the old maximum serves. That spares the search for the new one in a phase whose vector instructions take 7
     // clocks each beside the other group's MFMAs. At most one more pass with the maxima brought up to date.
-    float m_ref = w.m_run, factor = unit, sum;
+    float m_ref = w.m_run, sum;
     bool update = MASKED || !w.settled;
 #pragma unroll 1
     for (;;) {
         if (update) {
+            if (BIAS && near) {
+                bias_scores<true>(p, w, s, factor, t0, kp, lane);
+                near = false, factor = 1.0f;
+            }
             float mt = -kInf;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     mt = fmaxf(mt, s[b][i]);
-            const float m_new = fmaxf(w.m_run, both_halves_max(mt) * unit);
+            const float m_new = fmaxf(w.m_run, both_halves_max(mt) * factor);
             const float alpha = w.m_run == -kInf ? 0.0f : __builtin_amdgcn_exp2f(w.m_run - m_new);
             if (__ballot(m_new > w.m_run)) {
                 w.l_run *= alpha;
@@ -359,18 +405,19 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
             w.m_run = m_new;
             m_ref = m_new == -kInf ? 0.0f : m_new;
             w.settled = !__ballot(!(fabsf(m_new) <= 0x1p20f));
-            // s unit - m in one fused operation keeps the rounding of m, 2^-24 of it, in the exponent: common to all of a
+            // factor s - m in one fused operation keeps the rounding of m, 2^-24 of it, in the exponent: common to all of a
             // row's probabilities and harmless, until it leaves the exponent's range. Scores so large are rounded as m was.
             if (__ballot(fabsf(m_ref) > 0x1p20f)) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        s[b][i] = rounded_difference(s[b][i], unit, m_ref);
+                        s[b][i] = rounded_difference(s[b][i], factor, m_ref);
                 m_ref = 0.0f, factor = 1.0f;
             }
         }
-        sum = tile_exponentials(s, pt, factor, m_ref);
+        sum = BIAS && near ? tile_exponentials_near(w, s, pt, factor, m_ref, kp, lane)
+                           : tile_exponentials(s, pt, factor, m_ref);
         if (update || !__ballot(!(sum <= 0x1p10f)))
             break;
         update = true;
@@ -568,7 +615,7 @@ __device__ __forceinline__ void few_turn(const DenseParams& p, WaveRows& w, cons
     for (int j = 0; j < kAhead; ++j)
         frag[j] = rd.k(lds, j);
     tile_products<false>(w, s, pt, frag, rd, lds, nullptr);
-    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, p.k_pos ? kp : nullptr, lane);
+    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, kp, lane);
     if (MASKED)
         tile_output_masked(w, pt, rd, lds + kTileBytes, t0, scratch, lane);
     else
@@ -649,9 +696,9 @@ struct PairFeed {
     PairStream<true, false> v;
     __device__ __forceinline__ const char* k_tile(uint32_t t) const { return k.ring + (t % kRing) * kTileBytes; }
     __device__ __forceinline__ const char* v_tile(uint32_t t) const { return v.ring + (t % kRing) * kTileBytes; }
-    __device__ __forceinline__ const int32_t* positions(uint32_t t) const
+    __device__ __forceinline__ int32_t* positions(uint32_t t) const
     {
-        return reinterpret_cast<const int32_t*>(k.pos_ring + (t % kRing) * 256u);
+        return reinterpret_cast<int32_t*>(k.pos_ring + (t % kRing) * 256u);
     }
 };
 
@@ -673,7 +720,7 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Pai
     // t + 2 into that of tile t - 2 (among the products they cost 10%: this phase is the shorter one).
     feed.k();
     feed.v();
-    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, p.k_pos ? feed.positions(t) : nullptr, lane);
+    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, feed.positions(t), lane);
     // Past the last tile these are some tile's again, and not used.
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
