@@ -10,7 +10,9 @@
 //   once for all of them, and with one new row a stream fills the MFMA's columns with heads.
 // - A wave takes 32 rows. Scores are transposed, S^T = K Q^T: a row's keys lie in one lane and its lane + 32 twin, so the
 //   softmax's maximum and sum need one exchange, and P^T is the B operand of O^T += V^T P^T as it stands.
-// - A workgroup walks the key tiles from its rows' lowest lo to their highest hi. A wave masks a tile only where its own
+// - A workgroup walks the key tiles from its rows' lowest lo to their highest hi, under a bias from the last to the first:
+//   a causal row's scores then fall from its own position on, and the first tile's maximum serves to the end (2 x 4096
+//   causal rows, 40 heads on 8, slopes 2^-1 .. 2^-8: 571 us in rising order). A wave masks a tile only where its own
 //   rows' ranges do not all cover it.
 // - A masked probability is a zero, and zero times an infinite or NaN value of V would still be NaN in the rows that do
 //   not attend it: in a masked tile the wave looks for such values, and where there are any the matrix cores take zeros
@@ -30,6 +32,7 @@ namespace {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4_t __attribute__((ext_vector_type(4)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef short v4i16 __attribute__((ext_vector_type(4)));
 
@@ -164,14 +167,22 @@ struct WaveRows {
     float slope_log2;           // BIAS: the row's head's slope, in base-2 units
     int32_t q_pos, q_base;      // BIAS: the row's position, the wave's first row's
     float q_rel;                // BIAS: their difference, if q_near: it is under 2^23 in all of the wave's rows
-    bool q_near;
+    bool q_near;                // (and the slope in units of a score ordinary)
+    float slope_unit;
     // Whether some row's range does not cover the tile at key t0.
     __device__ __forceinline__ bool masks(uint32_t t0) const { return t0 < all_lo || t0 + 64u > all_hi; }
 };
 
+// What one of a score as the products (and cap_scores) leave it is in base 2.
+template <bool CAP>
+__device__ __forceinline__ float score_unit(const DenseParams& p)
+{
+    return CAP ? 2.0f * p.cap_out : p.scale_log2;
+}
+
 __device__ __forceinline__ bool is_near(int32_t rel) { return rel > -(1 << 23) && rel < (1 << 23); }
 
-template <bool BIAS>
+template <bool CAP, bool BIAS>
 __device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, uint32_t f0, uint32_t lane, WaveRows& w)
 {
     const uint32_t n = lane & 31u, hh = lane >> 5, f = f0 + n;
@@ -203,8 +214,9 @@ __device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, ui
         w.q_pos = p.q_pos ? p.q_pos[row] : int32_t(row);
         w.q_base = __builtin_amdgcn_readfirstlane(w.q_pos);
         const int32_t rel = __builtin_elementwise_sub_sat(w.q_pos, w.q_base);
-        w.q_near = !__ballot(!is_near(rel));
         w.q_rel = float(rel);
+        w.slope_unit = w.slope_log2 / score_unit<CAP>(p);
+        w.q_near = !__ballot(!is_near(rel) || !(fabsf(w.slope_unit) <= 0x1p80f));
     }
 }
 
@@ -220,43 +232,44 @@ __device__ __forceinline__ void cap_scores(const DenseParams& p, floatx16 (&s)[2
             s[b][i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[b][i] * p.cap_in));
 }
 
-// The key positions of a tile at key t0 as floats from the wave's base, into kp (LDS of the wave's own, which holds
-// k_pos's values where there is one), if they and the wave's rows are all under 2^23 from it: float differences of them
-// are then exact, two operations a score. Otherwise kp is left as it was.
-__device__ __forceinline__ bool near_positions(const DenseParams& p, const WaveRows& w, uint32_t t0, int32_t* kp,
-                                               uint32_t lane)
+// The key positions of a tile as floats from the wave's base, if they and the wave's rows are all under 2^23 from it: the
+// float differences are then exact, and the bias takes two operations a score. pos: the position of the tile's key `lane`;
+// near_pos (64 floats of LDS, the wave's own) takes the result, zeros if this is not so.
+__device__ __forceinline__ bool near_positions(const WaveRows& w, int32_t pos, float* near_pos, uint32_t lane)
 {
-    const int32_t rel = __builtin_elementwise_sub_sat(p.k_pos ? kp[lane] : int32_t(t0 + lane), w.q_base);
-    if (!w.q_near || __ballot(!is_near(rel)))
-        return false;
-    reinterpret_cast<float*>(kp)[lane] = float(rel);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    return true;
+    const int32_t rel = __builtin_elementwise_sub_sat(pos, w.q_base);
+    const bool near = w.q_near && !__ballot(!is_near(rel));
+    near_pos[lane] = near ? float(rel) : 0.0f;
+    asm volatile("" ::: "memory"); // a wave's LDS accesses are in order
+    return near;
 }
 
-// Scores in units of `unit` to base-2 units less the bias. NEAR: kp as near_positions leaves it; otherwise the distances
-// are those of int32 positions (of the tile's key numbers without k_pos), exact before they round to float.
-template <bool NEAR>
-__device__ __forceinline__ void bias_scores(const DenseParams& p, const WaveRows& w, floatx16 (&s)[2], float unit,
-                                            uint32_t t0, const int32_t* kp, uint32_t lane)
+// The bias off the scores, from near_positions: key is the first of the four positions that x's belong to.
+__device__ __forceinline__ float less_bias(const WaveRows& w, float x, float slope_unit, float key)
+{
+    return fmaf(-slope_unit, fabsf(w.q_rel - key), x);
+}
+
+__device__ __forceinline__ floatx4_t near_four(const float* near_pos, int g, uint32_t lane)
+{
+    return *reinterpret_cast<const floatx4_t*>(near_pos + 8 * g + 4u * (lane >> 5));
+}
+
+// Scores to base-2 units less the bias, from the distances of int32 positions (kp: the tile's; the keys' numbers without
+// k_pos), which are exact before they round to float.
+__device__ __forceinline__ void bias_scores_far(const DenseParams& p, const WaveRows& w, floatx16 (&s)[2], float unit,
+                                                uint32_t t0, const int32_t* kp, uint32_t lane)
 {
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-        const uint32_t key = 8u * uint32_t(g) + 4u * (lane >> 5);
-        const int4 t = NEAR || p.k_pos ? *reinterpret_cast<const int4*>(kp + key)
-                                       : int4{int32_t(t0 + key), int32_t(t0 + key) + 1, int32_t(t0 + key) + 2,
-                                              int32_t(t0 + key) + 3};
-        const int32_t pos[4] = {t.x, t.y, t.z, t.w};
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = 4 * (g & 3) + e;
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t key = 32u * b + 8u * (i >> 2) + 4u * (lane >> 5) + (i & 3);
+            const int32_t pos = p.k_pos ? kp[key] : int32_t(t0 + key);
             // The distance of two int32 positions fits 32 bits without a sign.
-            const float d = NEAR ? fabsf(w.q_rel - __int_as_float(pos[e]))
-                                 : float(w.q_pos > pos[e] ? uint32_t(w.q_pos) - uint32_t(pos[e])
-                                                          : uint32_t(pos[e]) - uint32_t(w.q_pos));
-            s[g >> 2][i] = fmaf(s[g >> 2][i], unit, -w.slope_log2 * d);
+            const uint32_t d = w.q_pos > pos ? uint32_t(w.q_pos) - uint32_t(pos) : uint32_t(pos) - uint32_t(w.q_pos);
+            s[b][i] = fmaf(s[b][i], unit, -w.slope_log2 * float(d));
         }
-    }
 }
 
 // Where a wave's lanes find their operands in a tile's LDS images.
@@ -327,43 +340,34 @@ __device__ __forceinline__ float tile_exponentials(const floatx16 (&s)[2], TileP
     return sum[0] + sum[1];
 }
 
-// The same under a bias, kp as near_positions leaves it.
-__device__ __forceinline__ float tile_exponentials_near(const WaveRows& w, const floatx16 (&s)[2], TileP& pt, float factor,
-                                                        float m, const int32_t* kp, uint32_t lane)
-{
-    float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int g = 0; g < 8; ++g) {
-        const float4 pos = *reinterpret_cast<const float4*>(kp + 8u * uint32_t(g) + 4u * (lane >> 5));
-        const float at[4] = {pos.x, pos.y, pos.z, pos.w};
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-            floatx2 t;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                t[h] = __builtin_amdgcn_exp2f(fmaf(s[g >> 2][4 * (g & 3) + e + h], factor,
-                                                   fmaf(-w.slope_log2, fabsf(w.q_rel - at[e + h]), -m)));
-            sum[0] += t[0], sum[1] += t[1];
-            pt.w[2 * g + e / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(t, bf16x2_t));
-        }
-    }
-    return sum[0] + sum[1];
-}
-
 // The softmax of a tile at key t0 (MASKED: not every row attends all of it): P^T, and the rows' maxima, sums and (where a
-// maximum moved) rescaled O.
+// maximum moved) rescaled O. BIAS: kp and near_pos are LDS for the tile's positions; sloped: tile_products has taken the
+// bias off, if the positions are near.
 template <bool CAP, bool BIAS, bool MASKED>
 __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, floatx16 (&s)[2], TileP& pt, uint32_t t0,
-                                             int32_t* kp, uint32_t lane)
+                                             const int32_t* kp, float* near_pos, bool sloped, bool near, uint32_t lane)
 {
     const uint32_t hh = lane >> 5;
-    float factor = CAP ? 2.0f * p.cap_out : p.scale_log2; // of the scores as they stand: base-2 units
+    float factor = score_unit<CAP>(p); // of the scores as they stand: base-2 units
     if (CAP)
         cap_scores(p, s);
-    bool near = BIAS && near_positions(p, w, t0, kp, lane); // the bias is yet to be taken off
-    if (BIAS && !near) {
-        bias_scores<false>(p, w, s, factor, t0, kp, lane);
-        factor = 1.0f;
+    if (BIAS) {
+        if (!sloped) {
+            near = near_positions(w, p.k_pos ? kp[lane] : int32_t(t0 + lane), near_pos, lane);
+            if (near) {
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    const floatx4_t key = near_four(near_pos, g, lane);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[g >> 2][4 * (g & 3) + e] = less_bias(w, s[g >> 2][4 * (g & 3) + e], w.slope_unit, key[e]);
+                }
+            }
+        }
+        if (!near) {
+            bias_scores_far(p, w, s, factor, t0, kp, lane);
+            factor = 1.0f;
+        }
     }
     if (MASKED) {
 #pragma unroll
@@ -382,10 +386,6 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
 #pragma unroll 1
     for (;;) {
         if (update) {
-            if (BIAS && near) {
-                bias_scores<true>(p, w, s, factor, t0, kp, lane);
-                near = false, factor = 1.0f;
-            }
             float mt = -kInf;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -416,8 +416,7 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
                 m_ref = 0.0f, factor = 1.0f;
             }
         }
-        sum = BIAS && near ? tile_exponentials_near(w, s, pt, factor, m_ref, kp, lane)
-                           : tile_exponentials(s, pt, factor, m_ref);
+        sum = tile_exponentials(s, pt, factor, m_ref);
         if (update || !__ballot(!(sum <= 0x1p10f)))
             break;
         update = true;
@@ -427,11 +426,17 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
 
 // S^T of a tile, and then with PV the O^T += V^T P^T of another (the one before it in a walk), in one run of MFMAs: frag
 // holds the first kAhead K fragments, and each MFMA's slot takes the fragment of the MFMA kAhead on, so V's are on their
-// way before the last scores are out.
-template <bool PV>
-__device__ __forceinline__ void tile_products(WaveRows& w, floatx16 (&s)[2], const TileP& pt, bf16x8_t (&frag)[kAhead],
-                                              const TileReads& rd, const char* kt, const char* vt)
+// way before the last scores are out. SLOPED: the bias comes off the scores in the slots of the V^T P^T, where the vector
+// unit is idle, if the key positions (pos: that of key `lane`) are near, which is returned.
+template <bool PV, bool SLOPED>
+__device__ __forceinline__ bool tile_products(WaveRows& w, floatx16 (&s)[2], const TileP& pt, bf16x8_t (&frag)[kAhead],
+                                              const TileReads& rd, const char* kt, const char* vt, int32_t pos,
+                                              float* near_pos, uint32_t lane)
 {
+    static_assert(PV || !SLOPED);
+    bool near = false;
+    float slope = 0.0f;
+    floatx4_t key[8];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -449,8 +454,19 @@ __device__ __forceinline__ void tile_products(WaveRows& w, floatx16 (&s)[2], con
             f = rd.k(kt, j + kAhead);
         else if (PV && j + kAhead < 32)
             f = rd.v(vt, j + kAhead - 16);
+        if (SLOPED && j == 5) {
+            near = near_positions(w, pos, near_pos, lane);
+            slope = near ? w.slope_unit : 0.0f;
+        }
+        if (SLOPED && j >= 12 && j % 2 == 0 && j < 28)
+            key[(j - 12) / 2] = near_four(near_pos, (j - 12) / 2, lane);
+        if (SLOPED && j >= 17)
+#pragma unroll
+            for (int e = 2 * (j - 17); e < (j == 31 ? 32 : 2 * (j - 16)); ++e)
+                s[e >> 4][e & 15] = less_bias(w, s[e >> 4][e & 15], slope, key[e >> 2][e & 3]);
     }
     __builtin_amdgcn_sched_barrier(0);
+    return near;
 }
 
 // O^T += V^T P^T of a tile alone.
@@ -614,8 +630,8 @@ __device__ __forceinline__ void few_turn(const DenseParams& p, WaveRows& w, cons
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
         frag[j] = rd.k(lds, j);
-    tile_products<false>(w, s, pt, frag, rd, lds, nullptr);
-    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, kp, lane);
+    tile_products<false, false>(w, s, pt, frag, rd, lds, nullptr, 0, nullptr, lane);
+    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, kp, reinterpret_cast<float*>(scratch), false, false, lane);
     if (MASKED)
         tile_output_masked(w, pt, rd, lds + kTileBytes, t0, scratch, lane);
     else
@@ -634,7 +650,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void at
         return;
     const uint32_t lane = threadIdx.x;
     WaveRows w;
-    load_rows<BIAS>(p, kvh, tile * 32u, lane, w);
+    load_rows<CAP, BIAS>(p, kvh, tile * 32u, lane, w);
     uint32_t first, last;
     tiles_of(p, w.any_lo, w.any_hi, split, first, last);
     const uint16_t* const kh = p.k + uint64_t(kvh) * p.khs;
@@ -643,13 +659,15 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void at
     const TileLoads<16, true> load_v(p.vrs, 0u, lane);
     const TileReads rd(lane);
     // Two loops, the masked tiles' and the whole ones': one body with both forms copies O between them at every tile.
-    for (uint32_t t = first; t < last;) {
+    const uint32_t tiles = last - first;
+    const auto key_of = [&](uint32_t t) { return w.any_lo + 64u * (BIAS ? last - 1u - t : first + t); };
+    for (uint32_t t = 0; t < tiles;) {
 #pragma unroll 1
-        for (; t < last && w.masks(w.any_lo + 64u * t); ++t)
-            few_turn<CAP, BIAS, true>(p, w, load_k, load_v, kh, vh, rd, lds, w.any_lo + 64u * t, lane);
+        for (; t < tiles && w.masks(key_of(t)); ++t)
+            few_turn<CAP, BIAS, true>(p, w, load_k, load_v, kh, vh, rd, lds, key_of(t), lane);
 #pragma unroll 1
-        for (; t < last && !w.masks(w.any_lo + 64u * t); ++t)
-            few_turn<CAP, BIAS, false>(p, w, load_k, load_v, kh, vh, rd, lds, w.any_lo + 64u * t, lane);
+        for (; t < tiles && !w.masks(key_of(t)); ++t)
+            few_turn<CAP, BIAS, false>(p, w, load_k, load_v, kh, vh, rd, lds, key_of(t), lane);
     }
     store_rows(p, w, kvh, tile * 32u, split, lane);
 }
@@ -662,14 +680,15 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void at
 constexpr uint32_t kPairWaves = 8, kRing = 4;
 
 // What a wave loads of a workgroup's tiles, a call a tile: its eighth of K (with all of the tile's key positions, into the
-// wave's own ring) or of V. Behind the last key the last tile again, so that every turn has the same count of loads; what
-// lies behind the workgroup's last tile is not read. The state is scalar and moves by additions.
+// wave's own ring) or of V. After the workgroup's last tile the same again, so that every turn has the same count of loads;
+// these are not read. The state is scalar and moves by additions.
 template <bool VALUE, bool POS>
 struct PairStream {
     TileLoads<2, VALUE> ld;
-    const uint16_t* at; // the next tile's first key
-    uint64_t step;      // elements a tile
-    uint32_t left;      // keys from it on
+    const uint16_t* at;       // the next tile's first key
+    int64_t step;             // elements to the one after it
+    uint32_t left, left_step; // keys from it on
+    uint32_t more;            // tiles after it
     char* ring;
     uint32_t slot; // byte offset in the ring
     const int32_t* pos;
@@ -681,11 +700,11 @@ struct PairStream {
         if (POS) // no positions: no records, and zeros
             load_lds4(buffer_words(pos, pos ? left * 4u : 0u), pos_ring + slot / 64u, 4u * lane);
         slot = (slot + kTileBytes) & (kRing * kTileBytes - 1u);
-        const bool more = left > 64u;
-        at += more ? step : 0u;
-        left -= more ? 64u : 0u;
+        at += more ? step : 0;
+        left += more ? left_step : 0u;
         if (POS)
-            pos += more && pos ? 64 : 0;
+            pos -= more && pos ? int32_t(left_step) : 0;
+        more -= more ? 1u : 0u;
     }
 };
 
@@ -711,16 +730,22 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Pai
 {
     // The products.
     __builtin_amdgcn_s_setprio(1);
-    tile_products<!MASKED>(w, s, pt, frag, rd, feed.k_tile(t), feed.v_tile(t - 1u));
+    constexpr bool kSloped = BIAS && !CAP && !MASKED;
+    float* const near_pos = reinterpret_cast<float*>(scratch);
+    int32_t pos = 0;
+    if (kSloped)
+        pos = feed.positions(t)[lane], pos = p.k_pos ? pos : int32_t(t0 + lane);
+    const bool near = tile_products<!MASKED, kSloped>(w, s, pt, frag, rd, feed.k_tile(t), feed.v_tile(t - 1u), pos,
+                                                      near_pos, lane);
     if (MASKED && t > 0)
-        tile_output_masked(w, pt, rd, feed.v_tile(t - 1u), t0 - 64u, scratch, lane);
+        tile_output_masked(w, pt, rd, feed.v_tile(t - 1u), BIAS ? t0 + 64u : t0 - 64u, scratch, lane);
     __builtin_amdgcn_s_setprio(0);
     phase_barrier();
     // The softmax. With it go out K of tile t + 3, into the slot of tile t - 1, which both groups have read, and V of tile
     // t + 2 into that of tile t - 2 (among the products they cost 10%: this phase is the shorter one).
     feed.k();
     feed.v();
-    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, feed.positions(t), lane);
+    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, feed.positions(t), near_pos, kSloped, near, lane);
     // Past the last tile these are some tile's again, and not used.
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
@@ -744,7 +769,7 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     uint32_t* const span = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + 2048u * kPairWaves);
     const uint32_t f0 = (tile * kPairWaves + wave) * 32u;
     WaveRows w;
-    load_rows<BIAS>(p, kvh, f0, lane, w);
+    load_rows<CAP, BIAS>(p, kvh, f0, lane, w);
     if (lane == 0)
         *reinterpret_cast<uint4*>(span + 4u * wave) = uint4{w.any_lo, w.any_hi, w.all_lo, w.all_hi};
     lds_barrier();
@@ -764,20 +789,28 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     }
     k0 += 64u * first;
     const uint32_t tiles = last - first;
+    // Turn t's tile.
+    const auto key_of = [&](uint32_t t) { return k0 + 64u * (BIAS ? tiles - 1u - t : t); };
     const TileReads rd(lane);
+    const uint32_t from = key_of(0), left_step = BIAS ? 64u : -64u;
+    const auto stride = [](uint64_t row) { return (BIAS ? -64 : 64) * int64_t(row); };
     PairFeed<BIAS> feed{{{p.krs, 2u * wave, lane},
-                         p.k + uint64_t(kvh) * p.khs + uint64_t(k0) * p.krs,
-                         64u * p.krs,
-                         p.kv_rows - k0,
+                         p.k + uint64_t(kvh) * p.khs + uint64_t(from) * p.krs,
+                         stride(p.krs),
+                         p.kv_rows - from,
+                         left_step,
+                         tiles - 1u,
                          lds,
                          0u,
-                         p.k_pos ? p.k_pos + k0 : nullptr,
+                         p.k_pos ? p.k_pos + from : nullptr,
                          reinterpret_cast<char*>(scratch) + 1024,
                          lane},
                         {{p.vrs, 2u * wave, lane},
-                         p.v + uint64_t(kvh) * p.vhs + uint64_t(k0) * p.vrs,
-                         64u * p.vrs,
-                         p.kv_rows - k0,
+                         p.v + uint64_t(kvh) * p.vhs + uint64_t(from) * p.vrs,
+                         stride(p.vrs),
+                         p.kv_rows - from,
+                         left_step,
+                         tiles - 1u,
                          lds + kRing * kTileBytes,
                          0u,
                          nullptr,
@@ -801,18 +834,23 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
         frag[j] = rd.k(lds, j);
     // The turns in between, whose own tile and the one before are whole for every row of the workgroup, in a loop of their
     // own: one body with both forms copies O between them at every tile.
-    uint32_t a = all_lo > k0 ? (all_lo - k0 + 63u) / 64u + 1u : 1u, b = all_hi > k0 ? (all_hi - k0) / 64u : 0u;
-    a = min(a, tiles), b = max(a, min(b, tiles));
+    uint32_t a = min(all_lo > k0 ? (all_lo - k0 + 63u) / 64u : 0u, tiles);
+    uint32_t b = min(all_hi > k0 ? (all_hi - k0) / 64u : 0u, tiles);
+    if (BIAS) {
+        const uint32_t t = tiles - a;
+        a = tiles - b, b = t;
+    }
+    a = min(a + 1u, tiles), b = max(a, b);
 #pragma unroll 1
     for (uint32_t t = 0; t < a; ++t)
-        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, k0 + 64u * t, lane);
+        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, key_of(t), lane);
 #pragma unroll 1
     for (uint32_t t = a; t < b; ++t)
-        pair_turn<CAP, BIAS, false>(p, w, feed, rd, s, frag, pt, scratch, t, k0 + 64u * t, lane);
+        pair_turn<CAP, BIAS, false>(p, w, feed, rd, s, frag, pt, scratch, t, key_of(t), lane);
 #pragma unroll 1
     for (uint32_t t = b; t < tiles; ++t)
-        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, k0 + 64u * t, lane);
-    tile_output_masked(w, pt, rd, feed.v_tile(tiles - 1u), k0 + 64u * (tiles - 1u), scratch, lane);
+        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, key_of(t), lane);
+    tile_output_masked(w, pt, rd, feed.v_tile(tiles - 1u), key_of(tiles - 1u), scratch, lane);
     if (!second)
         phase_barrier();
     wait_vm<0>(); // no load into this workgroup's LDS outlives it
