@@ -721,12 +721,44 @@ struct PairFeed {
     }
 };
 
+// Whether 2 KB of a V tile hold an infinity or a NaN.
+__device__ __forceinline__ bool holds_nonfinite(const char* part, uint32_t lane)
+{
+    uint32_t any = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        const u32x4_t t = *reinterpret_cast<const u32x4_t*>(part + 1024u * i + 16u * lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            any |= ((t[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u; // carries out of an exponent of ones
+    }
+    return __ballot(any != 0u) != 0u;
+}
+
+// tile_output where the tile may have been masked; odd: the eight waves' words from holds_nonfinite for it (null: it was
+// whole).
+__device__ __forceinline__ void masked_output(WaveRows& w, const TileP& pt, bf16x8_t (&frag)[kAhead], const TileReads& rd,
+                                              const char* vt, uint32_t t0, const uint32_t* odd, uint16_t* scratch,
+                                              uint32_t lane)
+{
+    uint32_t any = 0;
+    if (odd) {
+        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(odd), b = *reinterpret_cast<const u32x4_t*>(odd + 4);
+        any = a[0] | a[1] | a[2] | a[3] | b[0] | b[1] | b[2] | b[3];
+    }
+    if (__builtin_amdgcn_readfirstlane(any))
+        tile_output_masked(w, pt, rd, vt, t0, scratch, lane);
+    else
+        tile_output(w, pt, frag, rd, vt);
+}
+
 // A turn of attn_pair_kernel, tile t at key t0. MASKED: this tile or the one before it is not whole for every row of the
-// workgroup, or there is none before it.
+// workgroup, or there is none before it; checked: the turn before was of this form too.
 template <bool CAP, bool BIAS, bool MASKED>
 __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, PairFeed<BIAS>& feed, const TileReads& rd,
                                           floatx16 (&s)[2], bf16x8_t (&frag)[kAhead], TileP& pt, uint16_t* scratch,
-                                          uint32_t t, uint32_t t0, uint32_t lane)
+                                          uint32_t* odd, bool checked, uint32_t wave, uint32_t t, uint32_t t0,
+                                          uint32_t lane)
 {
     // The products.
     __builtin_amdgcn_s_setprio(1);
@@ -737,8 +769,16 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Pai
         pos = feed.positions(t)[lane], pos = p.k_pos ? pos : int32_t(t0 + lane);
     const bool near = tile_products<!MASKED, kSloped>(w, s, pt, frag, rd, feed.k_tile(t), feed.v_tile(t - 1u), pos,
                                                       near_pos, lane);
-    if (MASKED && t > 0)
-        tile_output_masked(w, pt, rd, feed.v_tile(t - 1u), BIAS ? t0 + 64u : t0 - 64u, scratch, lane);
+    if (MASKED) {
+        if (t > 0)
+            masked_output(w, pt, frag, rd, feed.v_tile(t - 1u), BIAS ? t0 + 64u : t0 - 64u,
+                          checked ? odd + kPairWaves * ((t - 1u) % 2u) : nullptr, scratch, lane);
+        // The part of V that this wave loaded: every wave's word is read at the next products, a barrier on.
+        const bool any = holds_nonfinite(feed.v_tile(t) + 2048u * wave, lane);
+        if (lane == 0)
+            odd[kPairWaves * (t % 2u) + wave] = any;
+        __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0)
+    }
     __builtin_amdgcn_s_setprio(0);
     phase_barrier();
     // The softmax. With it go out K of tile t + 3, into the slot of tile t - 1, which both groups have read, and V of tile
@@ -773,6 +813,7 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     if (lane == 0)
         *reinterpret_cast<uint4*>(span + 4u * wave) = uint4{w.any_lo, w.any_hi, w.all_lo, w.all_hi};
     lds_barrier();
+    uint32_t* const odd = span + 4u * kPairWaves; // [2][kPairWaves]: a masked tile's V holds an infinity or a NaN
     uint32_t k0 = ~0u, k1 = 0u, all_lo = 0u, all_hi = ~0u; // of the workgroup's rows
 #pragma unroll
     for (uint32_t i = 0; i < kPairWaves; ++i) {
@@ -843,14 +884,19 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     a = min(a + 1u, tiles), b = max(a, b);
 #pragma unroll 1
     for (uint32_t t = 0; t < a; ++t)
-        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, key_of(t), lane);
+        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, odd, true, wave, t, key_of(t), lane);
 #pragma unroll 1
     for (uint32_t t = a; t < b; ++t)
-        pair_turn<CAP, BIAS, false>(p, w, feed, rd, s, frag, pt, scratch, t, key_of(t), lane);
+        pair_turn<CAP, BIAS, false>(p, w, feed, rd, s, frag, pt, scratch, odd, true, wave, t, key_of(t), lane);
 #pragma unroll 1
     for (uint32_t t = b; t < tiles; ++t)
-        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, t, key_of(t), lane);
-    tile_output_masked(w, pt, rd, feed.v_tile(tiles - 1u), key_of(tiles - 1u), scratch, lane);
+        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, odd, t > b || a == b, wave, t, key_of(t),
+                                    lane);
+    const uint32_t end = tiles - 1u;
+    if (b < tiles || a == tiles) // the last turn was of the masked form
+        masked_output(w, pt, frag, rd, feed.v_tile(end), key_of(end), odd + kPairWaves * (end % 2u), scratch, lane);
+    else
+        tile_output(w, pt, frag, rd, feed.v_tile(end));
     if (!second)
         phase_barrier();
     wait_vm<0>(); // no load into this workgroup's LDS outlives it
@@ -1039,7 +1085,7 @@ template <bool CAP, bool BIAS>
 int launch_dense(const DenseParams& p, uint32_t waves, hipStream_t stream)
 {
     if (waves == kPairWaves)
-        return launch_rows(attn_pair_kernel<CAP, BIAS>, 2u * kRing * kTileBytes + (2048u + 16u) * kPairWaves, p, waves,
+        return launch_rows(attn_pair_kernel<CAP, BIAS>, 2u * kRing * kTileBytes + (2048u + 16u + 8u) * kPairWaves, p, waves,
                            stream);
     return launch_rows(attn_few_kernel<CAP, BIAS>, 2u * kTileBytes + 1024u + 256u, p, waves, stream);
 }
