@@ -78,6 +78,14 @@ __device__ __forceinline__ void lds_barrier()
     asm volatile("" ::: "memory");
 }
 
+// A wave's LDS reads done, with no memory access moved across it.
+__device__ __forceinline__ void wait_lds()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0)
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // A raw buffer of `bytes` at base, as the instructions below take it: reads past its end return zeros.
 __device__ __forceinline__ u32x4_t buffer_words(const void* base, uint32_t bytes)
 {
@@ -133,12 +141,14 @@ __device__ __forceinline__ void range_of(const DenseParams& p, uint32_t f, uint3
 // aligned 64-byte piece of a row. The descriptor ends behind the last key, so keys past it read zeros.
 template <int N, bool VALUE>
 struct TileLoads {
-    uint32_t row, off[N], i0; // row: bytes from a key to the next
+    // Instructions i and i + 4 of K, any two of V, differ by a multiple of the row stride.
+    static constexpr int kOff = VALUE ? 1 : N < 4 ? N : 4;
+    uint32_t row, off[kOff], i0; // row: bytes from a key to the next
     __device__ __forceinline__ TileLoads(uint64_t stride, uint32_t first, uint32_t lane)
         : row(uint32_t(stride) * 2u), i0(first)
     {
 #pragma unroll
-        for (uint32_t u = 0; u < uint32_t(N); ++u) {
+        for (uint32_t u = 0; u < uint32_t(kOff); ++u) {
             const uint32_t i = first + u;
             const uint32_t key = VALUE ? (lane >> 2) & 3u : lane >> 4;
             const uint32_t chunk = VALUE ? 4u * (lane >> 4) + (lane & 3u) : (lane & 15u) ^ (4u * (i & 3u) + key);
@@ -149,9 +159,11 @@ struct TileLoads {
     __device__ __forceinline__ void operator()(char* dst, const uint16_t* base, uint32_t keys) const
     {
         const u32x4_t r = buffer_words(base, (min(64u, keys) - 1u) * row + 256u);
+        uint32_t step = 4u * row;
+        asm volatile("" : "+s"(step)); // an addition a load, not registers kept through the products
 #pragma unroll
         for (uint32_t u = 0; u < uint32_t(N); ++u)
-            load_lds16(r, dst + 1024u * (i0 + u), off[u]);
+            load_lds16(r, dst + 1024u * (i0 + u), off[u % uint32_t(kOff)] + u / uint32_t(kOff) * uint32_t(kOff) * step);
     }
 };
 
@@ -610,41 +622,89 @@ __device__ __forceinline__ void tiles_of(const DenseParams& p, uint32_t k0, uint
     last = uint32_t(uint64_t(tiles) * (split + 1u) / p.splits);
 }
 
-// A turn of attn_few_kernel: the tile at key t0. lds: K, V, the wave's scratch, key positions.
-template <bool CAP, bool BIAS, bool MASKED>
-__device__ __forceinline__ void few_turn(const DenseParams& p, WaveRows& w, const TileLoads<16, false>& load_k,
-                                         const TileLoads<16, true>& load_v, const uint16_t* kh, const uint16_t* vh,
-                                         const TileReads& rd, char* lds, uint32_t t0, uint32_t lane)
+// Whether N KB of a V tile hold an infinity or a NaN.
+template <int N>
+__device__ __forceinline__ bool holds_nonfinite(const char* part, uint32_t lane)
 {
-    uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kTileBytes);
-    int32_t* const kp = reinterpret_cast<int32_t*>(lds + 2u * kTileBytes + 1024u);
-    load_k(lds, kh + uint64_t(t0) * p.krs, p.kv_rows - t0);
-    load_v(lds + kTileBytes, vh + uint64_t(t0) * p.vrs, p.kv_rows - t0);
-    if (BIAS && p.k_pos)
-        kp[lane] = p.k_pos[min(t0 + lane, p.kv_rows - 1u)];
-    wait_vm<0>();
-    lds_barrier();
+    uint32_t any = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < uint32_t(N); ++i) {
+        const u32x4_t t = *reinterpret_cast<const u32x4_t*>(part + 1024u * i + 16u * lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            any |= (t[e] & 0x7f807f80u) + 0x00800080u; // carries out of an exponent of ones
+    }
+    return __ballot((any & 0x80008000u) != 0u) != 0u;
+}
+
+// What attn_few_kernel loads of a tile: K and, in the slot of its turn, the key positions; or V.
+template <bool BIAS>
+struct FewLoads {
+    TileLoads<16, false> load_k;
+    TileLoads<16, true> load_v;
+    const uint16_t* kh;
+    const uint16_t* vh;
+    char* lds; // K, V, the wave's scratch (1 KB), two tiles' key positions
+    __device__ __forceinline__ int32_t* positions(uint32_t t) const
+    {
+        return reinterpret_cast<int32_t*>(lds + 2u * kTileBytes + 1024u + 256u * (t & 1u));
+    }
+    __device__ __forceinline__ void k(const DenseParams& p, uint32_t t, uint32_t t0, uint32_t lane) const
+    {
+        load_k(lds, kh + uint64_t(t0) * p.krs, p.kv_rows - t0);
+        if (BIAS) // no positions: no records, and zeros
+            load_lds4(buffer_words(p.k_pos ? p.k_pos + t0 : nullptr, p.k_pos ? (p.kv_rows - t0) * 4u : 0u),
+                      reinterpret_cast<char*>(positions(t)), 4u * lane);
+    }
+    __device__ __forceinline__ void v(const DenseParams& p, uint32_t t0) const
+    {
+        load_v(lds + kTileBytes, vh + uint64_t(t0) * p.vrs, p.kv_rows - t0);
+    }
+};
+
+// A turn of attn_few_kernel, tile t at key t0; next: the next tile's key, if there is one (more). A tile's K is on its way
+// from the products before it to its own, its V from the output before.
+template <bool CAP, bool BIAS, bool MASKED>
+__device__ __forceinline__ void few_turn(const DenseParams& p, WaveRows& w, const FewLoads<BIAS>& feed,
+                                         const TileReads& rd, uint32_t t, uint32_t t0, bool more, uint32_t next,
+                                         uint32_t lane)
+{
+    uint16_t* const scratch = reinterpret_cast<uint16_t*>(feed.lds + 2u * kTileBytes);
+    const char* const vt = feed.lds + kTileBytes;
     floatx16 s[2];
     bf16x8_t frag[kAhead];
     TileP pt;
+    wait_vm<16>(); // K and the positions; V may still be in flight
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-        frag[j] = rd.k(lds, j);
-    tile_products<false, false>(w, s, pt, frag, rd, lds, nullptr, 0, nullptr, lane);
-    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, kp, reinterpret_cast<float*>(scratch), false, false, lane);
-    if (MASKED)
-        tile_output_masked(w, pt, rd, lds + kTileBytes, t0, scratch, lane);
+        frag[j] = rd.k(feed.lds, j);
+    tile_products<false, false>(w, s, pt, frag, rd, feed.lds, nullptr, 0, nullptr, lane);
+    wait_lds();
+    if (more) {
+        feed.k(p, t + 1u, next, lane);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, feed.positions(t), reinterpret_cast<float*>(scratch), false, false,
+                                    lane);
+    if (more)
+        wait_vm<BIAS ? 17 : 16>(); // V, but not the next K
     else
-        tile_output(w, pt, frag, rd, lds + kTileBytes);
-    lds_barrier();
+        wait_vm<0>();
+    if (MASKED && holds_nonfinite<16>(vt, lane))
+        tile_output_masked(w, pt, rd, vt, t0, scratch, lane);
+    else
+        tile_output(w, pt, frag, rd, vt);
+    wait_lds();
+    if (more)
+        feed.v(p, next);
 }
 
 // Few rows: one wave of 32 list rows a workgroup, with a tile of its own in LDS; four or five of them share a CU, and
 // one's loads arrive while the others compute.
 template <bool CAP, bool BIAS>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void attn_few_kernel(DenseParams p)
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void attn_few_kernel(DenseParams p)
 {
-    extern __shared__ __attribute__((aligned(16))) char lds[]; // K, V, scratch, key positions
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t kvh, tile, split;
     if (!block_of(p, kvh, tile, split))
         return;
@@ -653,21 +713,26 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void at
     load_rows<CAP, BIAS>(p, kvh, tile * 32u, lane, w);
     uint32_t first, last;
     tiles_of(p, w.any_lo, w.any_hi, split, first, last);
-    const uint16_t* const kh = p.k + uint64_t(kvh) * p.khs;
-    const uint16_t* const vh = p.v + uint64_t(kvh) * p.vhs;
-    const TileLoads<16, false> load_k(p.krs, 0u, lane);
-    const TileLoads<16, true> load_v(p.vrs, 0u, lane);
+    const FewLoads<BIAS> feed{{p.krs, 0u, lane},
+                              {p.vrs, 0u, lane},
+                              p.k + uint64_t(kvh) * p.khs,
+                              p.v + uint64_t(kvh) * p.vhs,
+                              lds};
     const TileReads rd(lane);
-    // Two loops, the masked tiles' and the whole ones': one body with both forms copies O between them at every tile.
     const uint32_t tiles = last - first;
     const auto key_of = [&](uint32_t t) { return w.any_lo + 64u * (BIAS ? last - 1u - t : first + t); };
+    if (tiles) {
+        feed.k(p, 0u, key_of(0u), lane);
+        feed.v(p, key_of(0u));
+    }
+    // Two loops, the masked tiles' and the whole ones': one body with both forms copies O between them at every tile.
     for (uint32_t t = 0; t < tiles;) {
 #pragma unroll 1
         for (; t < tiles && w.masks(key_of(t)); ++t)
-            few_turn<CAP, BIAS, true>(p, w, load_k, load_v, kh, vh, rd, lds, key_of(t), lane);
+            few_turn<CAP, BIAS, true>(p, w, feed, rd, t, key_of(t), t + 1u < tiles, key_of(t + 1u), lane);
 #pragma unroll 1
         for (; t < tiles && !w.masks(key_of(t)); ++t)
-            few_turn<CAP, BIAS, false>(p, w, load_k, load_v, kh, vh, rd, lds, key_of(t), lane);
+            few_turn<CAP, BIAS, false>(p, w, feed, rd, t, key_of(t), t + 1u < tiles, key_of(t + 1u), lane);
     }
     store_rows(p, w, kvh, tile * 32u, split, lane);
 }
@@ -721,20 +786,6 @@ struct PairFeed {
     }
 };
 
-// Whether 2 KB of a V tile hold an infinity or a NaN.
-__device__ __forceinline__ bool holds_nonfinite(const char* part, uint32_t lane)
-{
-    uint32_t any = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        const u32x4_t t = *reinterpret_cast<const u32x4_t*>(part + 1024u * i + 16u * lane);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            any |= ((t[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u; // carries out of an exponent of ones
-    }
-    return __ballot(any != 0u) != 0u;
-}
-
 // tile_output where the tile may have been masked; odd: the eight waves' words from holds_nonfinite for it (null: it was
 // whole).
 __device__ __forceinline__ void masked_output(WaveRows& w, const TileP& pt, bf16x8_t (&frag)[kAhead], const TileReads& rd,
@@ -774,10 +825,10 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Pai
             masked_output(w, pt, frag, rd, feed.v_tile(t - 1u), BIAS ? t0 + 64u : t0 - 64u,
                           checked ? odd + kPairWaves * ((t - 1u) % 2u) : nullptr, scratch, lane);
         // The part of V that this wave loaded: every wave's word is read at the next products, a barrier on.
-        const bool any = holds_nonfinite(feed.v_tile(t) + 2048u * wave, lane);
+        const bool any = holds_nonfinite<2>(feed.v_tile(t) + 2048u * wave, lane);
         if (lane == 0)
             odd[kPairWaves * (t % 2u) + wave] = any;
-        __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0)
+        wait_lds();
     }
     __builtin_amdgcn_s_setprio(0);
     phase_barrier();
@@ -1087,7 +1138,7 @@ int launch_dense(const DenseParams& p, uint32_t waves, hipStream_t stream)
     if (waves == kPairWaves)
         return launch_rows(attn_pair_kernel<CAP, BIAS>, 2u * kRing * kTileBytes + (2048u + 16u + 8u) * kPairWaves, p, waves,
                            stream);
-    return launch_rows(attn_few_kernel<CAP, BIAS>, 2u * kTileBytes + 1024u + 256u, p, waves, stream);
+    return launch_rows(attn_few_kernel<CAP, BIAS>, 2u * kTileBytes + 1024u + 512u, p, waves, stream);
 }
 
 } // namespace
