@@ -348,7 +348,8 @@ int mh3_flash_attn_sparse_128_ordered(const MH3AttnArgs* args, const uint16_t* q
  *           the pointer NULL; MH3_ERR_SHAPE if smaller). The call overwrites it, so calls that overlap in time, two
  *           captured graphs among them, need their own.
  * out may not overlap q, k, v, ranges, slopes, the positions or the workspace (each taken as the span from its start to
- * the last row of its last head), else MH3_ERR_PARAM. */
+ * the last row of its last head), nor its rows each other: heads lie one behind the other or side by side in wider rows
+ * (MH3_ERR_PARAM otherwise). */
 typedef struct MH3DenseAttnArgs {
     uint32_t heads;    /* query heads, a multiple of kv_heads */
     uint32_t kv_heads;

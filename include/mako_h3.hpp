@@ -142,6 +142,67 @@ struct Heads {
                             qkv_stride ? qkv_stride : 3ull * heads * 128,
                             out_head_stride ? out_head_stride : uint64_t(rows) * 128,
                             out_row_stride ? out_row_stride : 128};
+
+// The axes of rotary positions (a video's time, height and width): one to four, a head's pairs in their order.
+struct Axes {
+    struct Axis {
+        uint32_t pairs = 0;
+        double theta = 10000.0, step = 1.0;
+    };
+    std::vector<Axis> axes;
+
+    MH3AxesArgs args() const
+    {
+        MH3AxesArgs a{};
+        if (axes.empty() || axes.size() > 4)
+            throw error("rotary_axes", MH3_ERR_PARAM);
+        a.axes = uint32_t(axes.size());
+        for (size_t i = 0; i < axes.size(); ++i)
+            a.pairs[i] = axes[i].pairs, a.theta[i] = axes[i].theta, a.step[i] = axes[i].step;
+        return a;
+    }
+};
+
+// The shape of a flash_attn_128 call. Zero kv_heads: as many as heads; zero strides: [heads][rows][128].
+struct Dense {
+    struct Strides {
+        uint64_t head = 0, row = 0;
+    };
+    uint32_t heads = 0, kv_heads = 0, q_rows = 0, kv_rows = 0;
+    float scale = 0.0f, cap = 0.0f; // 0: 1 / sqrt(128); no cap
+    Strides q, k, v, out;
+
+    MH3DenseAttnArgs args() const
+    {
+        const auto head = [](const Strides& s, uint32_t rows) { return s.head || s.row ? s.head : uint64_t(rows) * 128; };
+        const auto row = [](const Strides& s) { return s.row ? s.row : 128u; };
+        return MH3DenseAttnArgs{heads,
+                                kv_heads ? kv_heads : heads,
+                                128,
+                                q_rows,
+                                kv_rows,
+                                scale,
+                                cap,
+                                0,
+                                head(q, q_rows),
+                                row(q),
+                                head(k, kv_rows),
+                                row(k),
+                                head(v, kv_rows),
+                                row(v),
+                                head(out, q_rows),
+                                row(out)};
+    }
+};
+
+// What changes a row's scores in flash_attn_128, all on the device and all optional: each query row's keys [lo, hi)
+// (attn_ranges), each head's slope of the distance bias, and the positions its distances are of (rows' numbers without).
+struct Scores {
+    const int32_t* ranges = nullptr;
+    const float* slopes = nullptr;
+    const int32_t* q_pos = nullptr;
+    const int32_t* k_pos = nullptr;
+};
     }
 };
 
@@ -310,6 +371,46 @@ public:
         check(mh3_heads_partial_pool(&a, &ca, qkv, q_w, k_w, cos_t, sin_t, map, q, k, v, qc, kc, counts, s_),
               "heads_partial_pool");
     }
+    // The tables of heads_partial (float [rows][pairs in all]) from positions, int32 [rows][axes].
+    void rotary_axes(const Axes& ax, uint32_t rows, const int32_t* pos, float* cos_t, float* sin_t) const
+    {
+        const MH3AxesArgs a = ax.args();
+        check(mh3_rotary_axes(&a, rows, pos, cos_t, sin_t, s_), "rotary_axes");
+    }
+    // heads_partial with those made on the way (hd.rot twice the axes' pairs; pos int32 [model_rows][axes]).
+    void heads_partial_axes(const Heads& hd, const Axes& ax, const uint16_t* qkv, const float* q_w, const float* k_w,
+                            const int32_t* pos, const int32_t* map, uint16_t* q, uint16_t* k, uint16_t* v) const
+    {
+        const MH3HeadsArgs a = hd.args();
+        const MH3AxesArgs axes = ax.args();
+        check(mh3_heads_partial_axes(&a, &axes, qkv, q_w, k_w, pos, map, q, k, v, s_), "heads_partial_axes");
+    }
+    // Attention over whole rows, with `workspace` of at least flash_attn_128_workspace_bytes() bytes (none where that is
+    // 0; overwritten by every call).
+    static uint64_t flash_attn_128_workspace_bytes(const Dense& d)
+    {
+        const MH3DenseAttnArgs a = d.args();
+        const int64_t n = mh3_flash_attn_128_workspace_bytes(&a);
+        if (n < 0)
+            throw error("flash_attn_128", int(n));
+        return uint64_t(n);
+    }
+    void flash_attn_128(const Dense& d, const uint16_t* q, const uint16_t* k, const uint16_t* v, const Scores& sc,
+                        void* workspace, uint64_t workspace_bytes, uint16_t* out) const
+    {
+        const MH3DenseAttnArgs a = d.args();
+        check(mh3_flash_attn_128(&a, q, k, v, sc.ranges, sc.slopes, sc.q_pos, sc.k_pos, workspace, workspace_bytes, out,
+                                 s_),
+              "flash_attn_128");
+    }
+    // Each query row's keys for documents packed into one batch, int32 [q_rows][2]: rows q_off[d] .. q_off[d + 1] - 1
+    // attend keys k_off[d] .. k_off[d + 1] - 1; causal: those up to their own, and the first prefix[d] (may be null).
+    void attn_ranges(uint32_t q_rows, uint32_t kv_rows, uint32_t docs, bool causal, const int32_t* q_off,
+                     const int32_t* k_off, const int32_t* prefix, int32_t* ranges) const
+    {
+        const MH3RangeArgs a{q_rows, kv_rows, docs, causal ? 1u : 0u};
+        check(mh3_attn_ranges(&a, q_off, k_off, prefix, ranges, s_), "attn_ranges");
+    }
     // Flash attention over the pass lists idx / cnt of cube_select (or cube_topk) and the dense rows
     // [dense_row0, dense_row0 + n_dense); q, k, v and out in c's cube geometry. scale 0: 1 / sqrt(128).
     void flash_attn_sparse_128(const Cubes& c, const uint16_t* q, const uint16_t* k, const uint16_t* v,
@@ -381,6 +482,43 @@ public:
         const MH3GemmArgs a{rows, n, k, m.n_sets, m.set_stride, 0};
         check(mh3_gemm_gate_add_f32(&a, form, x, x_scale, w, w_scale, m.gate, m.set_of_row, residual, s_),
               form == MH3_GEMM_BF16 ? "Gemm::encode+gate_add_rows" : "gemm_i8+gate_add_rows");
+    }
+
+    // Rows to 4-bit microscaled values (blocks of 32 that share a power of two): q [rows][cols / 2] bytes, scale
+    // [cols / 256][rows][8], for weights at load and for activations on the way.
+    void quant_rows_mx4(uint32_t rows, uint32_t cols, uint32_t dtype, const void* w, uint8_t* q, uint8_t* scale) const
+    {
+        const MH3QuantArgs a{rows, cols, dtype, 0};
+        check(mh3_quant_rows_mx4(&a, w, q, scale, s_), "quant_rows_mx4");
+    }
+    // The block's products on such operands: the qkv projection (w [n][k]), ...
+    void gemm_mx4(uint32_t m, uint32_t n, uint32_t k, const uint8_t* x, const uint8_t* x_scale, const uint8_t* w,
+                  const uint8_t* w_scale, uint16_t* out) const
+    {
+        const MH3GemmArgs a{m, n, k, 0, 0, 0};
+        check(mh3_gemm_mx4(&a, x, x_scale, w, w_scale, out, s_), "gemm_mx4");
+    }
+    // ... fc1 with SwiGLU (w [2 ffn][dim]), ...
+    void fc1_swiglu_mx4(uint32_t m, uint32_t ffn, uint32_t dim, const uint8_t* x, const uint8_t* x_scale,
+                        const uint8_t* w, const uint8_t* w_scale, uint16_t* out) const
+    {
+        const MH3GemmArgs a{m, ffn, dim, 0, 0, 0};
+        check(mh3_gemm_mx4_swiglu(&a, x, x_scale, w, w_scale, out, s_), "gemm_mx4+swiglu_rows");
+    }
+    // ... and the out projection and fc2 into the residual, bf16 or float (m as for gemm_gate_add).
+    void gemm_mx4_gate_add(uint32_t rows, uint32_t n, uint32_t k, const uint8_t* x, const uint8_t* x_scale,
+                           const uint8_t* w, const uint8_t* w_scale, const Modulation& m, uint16_t* residual) const
+    {
+        const MH3GemmArgs a{rows, n, k, m.n_sets, m.set_stride, 0};
+        check(mh3_gemm_mx4_gate_add(&a, x, x_scale, w, w_scale, m.gate, m.set_of_row, residual, s_),
+              "gemm_mx4+gate_add_rows");
+    }
+    void gemm_mx4_gate_add(uint32_t rows, uint32_t n, uint32_t k, const uint8_t* x, const uint8_t* x_scale,
+                           const uint8_t* w, const uint8_t* w_scale, const Modulation& m, float* residual) const
+    {
+        const MH3GemmArgs a{rows, n, k, m.n_sets, m.set_stride, 0};
+        check(mh3_gemm_mx4_gate_add_f32(&a, x, x_scale, w, w_scale, m.gate, m.set_of_row, residual, s_),
+              "gemm_mx4+gate_add_rows");
     }
 
 private:

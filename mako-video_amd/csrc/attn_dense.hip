@@ -1061,11 +1061,11 @@ struct Plan {
 
 // The workgroup's waves and the key splits of a call: the pair of least estimated time, of the two kernels with no split
 // or as many as give the chip one, two or four workgroups a CU. In us, measured: a workgroup of eight waves takes 14 and
-// 1.5 a key tile (it has a CU to itself), one of a single wave 10 and 1.75 (four share a CU); K and V come from HBM once at
+// 1.5 a key tile (it has a CU to itself), one of a single wave 10 and 1.5 (four share a CU); K and V come from HBM once at
 // 6 TB/s, and for each further row tile from the MALL or L2 at some 16; the join takes 6 and its parts' bytes. Heads, query
-// and key rows, eight waves and one, each at its best splits (us): 56, 945 x 945 45 and 68; 40, 212 x 212 20 and 14; 40,
-// 64 x 20,000 123 and 100; 40 on 8 key heads, 1 x 5000 20 and 15, 3 x 129,536 113 and 98; 7 on 1, 500 x 16,000 53 and 73;
-// 56 on 8, 64 x 100,000 202 and 383. (Ranges that leave most keys out are not known here.)
+// and key rows, eight waves and one, each at its best splits (us): 56, 945 x 945 44 and 68; 40, 212 x 212 20 and 15; 7,
+// 700 x 700 30 and 24; 40, 64 x 20,000 125 and 93; 40 on 8 key heads, 1 x 5000 18 and 15, 3 x 129,536 108 and 94; 7 on 1,
+// 500 x 16,000 52 and 71; 56 on 8, 64 x 100,000 198 and 324. (Ranges that leave most keys out are not known here.)
 Plan plan_of(const MH3DenseAttnArgs& a)
 {
     const uint64_t list = uint64_t(a.q_rows) * (a.heads / a.kv_heads), key_tiles = (uint64_t(a.kv_rows) + 63u) / 64u;
@@ -1081,7 +1081,7 @@ Plan plan_of(const MH3DenseAttnArgs& a)
             const uint64_t splits = std::max<uint64_t>(1u, std::min<uint64_t>({fill / blocks, key_tiles / 4u, 256u}));
             const uint64_t rounds = (blocks * splits + (pair ? cus : 4u * cus) - 1u) / (pair ? cus : 4u * cus);
             const double turns = double((key_tiles + splits - 1u) / splits);
-            double us = std::max(double(rounds) * (pair ? 14.0 + 1.5 * turns : 10.0 + 1.75 * turns),
+            double us = std::max(double(rounds) * (pair ? 14.0 + 1.5 * turns : 10.0 + 1.5 * turns),
                                  head_us * (1.0 / 6.0 + double(tiles - 1u) / 16.0));
             if (splits > 1u)
                 us += 6.0 + double(splits) * double(a.kv_heads) * double(list) * 1040.0 * 1e-6 / 4.0;
@@ -1175,6 +1175,12 @@ extern "C" int mh3_flash_attn_128(const MH3DenseAttnArgs* args, const uint16_t* 
                 4u !=
             0u)
         return MH3_ERR_ALIGN;
+    // out's rows apart from each other: heads one behind the other, or side by side in a row.
+    const bool behind = a.heads == 1u || a.out_head_stride >= (a.q_rows - 1u) * a.out_row_stride + 128u;
+    const bool beside = a.out_head_stride >= 128u &&
+                        (a.q_rows == 1u || a.out_row_stride >= (a.heads - 1u) * a.out_head_stride + 128u);
+    if (!behind && !beside)
+        return MH3_ERR_PARAM;
     const auto span = [](uint64_t heads, uint64_t hs, uint64_t rows, uint64_t rs) {
         return rows ? ((heads - 1u) * hs + (rows - 1u) * rs + 128u) * 2u : 0u;
     };

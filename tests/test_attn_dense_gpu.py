@@ -271,3 +271,60 @@ def test_replayed_from_graphs(dev):
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(outs[i], run(i))
+
+
+@pytest.mark.parametrize("rows,keys", [(700, 1000), (6, 900), (130, 70)])
+@pytest.mark.parametrize("cap", [0.0, 15.0])
+def test_positions_near_and_far(dev, rows, keys, cap):
+    """Positions whose differences a float holds, ones that it does not, both in one call (key tiles of either kind,
+    query rows of either kind), and both ends of int32."""
+    g = torch.Generator(device=dev).manual_seed(rows + keys)
+    q, k, v = make(g, 6, rows, dev), make(g, 2, keys, dev), make(g, 2, keys, dev)
+    near_q = torch.randint(0, 100, (rows,), generator=g, device=dev, dtype=torch.int32)
+    near_k = torch.randint(0, 100, (keys,), generator=g, device=dev, dtype=torch.int32)
+    far_q = torch.randint(-(1 << 31), 1 << 31, (rows,), generator=g, device=dev).int()
+    far_k = torch.randint(-(1 << 31), 1 << 31, (keys,), generator=g, device=dev).int()
+    far_k[:2] = torch.tensor([-(1 << 31), (1 << 31) - 1], device=dev).int()
+    far_q[0] = -(1 << 31)
+    mixed_k = torch.where(torch.arange(keys, device=dev) // 64 % 3 == 1, far_k, near_k)
+    mixed_q = torch.where(torch.arange(rows, device=dev) // 40 % 2 == 1, far_q, near_q)
+    shifted = 1 << 30
+    for slope, qp, kp in ((0.1, near_q, near_k), (0.1, near_q + shifted, near_k + shifted), (3e-9, far_q, far_k),
+                          (3e-9, near_q, mixed_k), (3e-9, mixed_q, near_k), (3e-9, mixed_q, mixed_k),
+                          (2e-6, near_q * 300000, near_k * 300000), (0.0, far_q, near_k), (-0.05, near_q, near_k)):
+        slopes = slope * (1 + torch.rand(6, generator=g, device=dev))
+        kw = {"slopes": slopes, "q_pos": qp.contiguous(), "k_pos": kp.contiguous(), "cap": cap,
+              "ranges": random_ranges(g, rows, keys, dev)}
+        check(mh.flash_attn_128(q, k, v, **kw), *attention64(q, k, v, **kw), f"slope {slope}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,rows", [(40, 8, 900), (8, 8, 600), (8, 1, 40)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_steep_slopes(dev, heads, kv_heads, rows, causal):
+    """Scores that rise or fall by tens a key tile: a bias of up to 450, whose 2^-24 is inside the bound's 2^-11."""
+    g = torch.Generator(device=dev).manual_seed(heads * rows)
+    q, k, v = make(g, heads, rows, dev), make(g, kv_heads, rows, dev), make(g, kv_heads, rows, dev)
+    off = torch.tensor([0, rows], dtype=torch.int32, device=dev)
+    ranges = mh.attn_ranges(off, off, rows, rows, causal=causal)
+    for sign in (1.0, -1.0):
+        slopes = sign * 0.5 ** torch.linspace(1.0, 8.0, heads, device=dev)
+        check(mh.flash_attn_128(q, k, v, ranges=ranges, slopes=slopes), *attention64(q, k, v, ranges=ranges, slopes=slopes))
+
+
+@pytest.mark.parametrize("lengths", [[300, 64, 500, 129], [700, 5], [64, 64, 64, 512, 256]])
+@pytest.mark.parametrize("causal,bias,cap", [(False, False, 0.0), (True, False, 0.0), (True, True, 0.0), (False, True, 9.0)])
+def test_infinite_values_in_masked_and_whole_tiles(dev, lengths, causal, bias, cap):
+    """Infinities and NaN in the values of some keys of every document: they reach the rows that attend them, and no
+    others, whether their tile is masked, whole, or between the two."""
+    g = torch.Generator(device=dev).manual_seed(sum(lengths))
+    n = sum(lengths)
+    q, k, v = make(g, 4, n, dev), make(g, 2, n, dev), make(g, 2, n, dev)
+    off = torch.tensor([0, *torch.tensor(lengths).cumsum(0).tolist()], dtype=torch.int32, device=dev)
+    for i, (start, length) in enumerate(zip(off.tolist(), lengths)):
+        v[i % 2, start + length // 2, 3 * i] = float("inf")
+        v[(i + 1) % 2, start + length - 1, 40 + i] = float("-inf") if i % 2 else float("nan")
+    ranges = mh.attn_ranges(off, off, n, n, causal=causal)
+    kw = {"ranges": ranges, "cap": cap}
+    if bias:
+        kw["slopes"] = torch.rand(4, generator=g, device=dev) * 0.02
+    check(mh.flash_attn_128(q, k, v, **kw), *attention64(q, k, v, **kw))

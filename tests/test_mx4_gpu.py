@@ -143,6 +143,31 @@ def test_gemm_gate_add(dev, m, n, k, sets, dtype):
     assert bool(((got.double() - want).abs() <= unit * want.abs() + gate.abs() * (tol + 2.0 ** -24 * y.abs())).all())
 
 
+@pytest.mark.parametrize("m,n", [(1, 20480), (32, 16384), (33, 16384), (63, 512), (300, 10240), (383, 10240), (577, 16384),
+                                 (769, 16384), (1024, 16384), (1025, 512)])
+def test_every_kernel_with_every_epilogue(dev, m, n):
+    """Sizes that take each of the kernels (few rows, tiles of 64, 128, 192 and 256 rows), with whole and cut tiles."""
+    g = torch.Generator(device=dev).manual_seed(m + n)
+    for k in (256, 768):
+        x, w = operand(g, m, k, dev), operand(g, n, k, dev, 1.5 / k ** 0.5)
+        y, tol = products(x, w, k)
+        out = mh.gemm_mx4(*x, *w)
+        assert bool(((out.double() - y).abs() <= 2.0 ** -8 * y.abs() + tol).all())
+        res = torch.randn((m, n), generator=g, device=dev)
+        gate = torch.randn(n, generator=g, device=dev)
+        want = res.double() + gate.double() * y
+        got = mh.gemm_mx4_gate_add(*x, *w, res, gate[None])
+        assert got is res
+        slack = gate.double().abs() * (tol + 2.0 ** -24 * y.abs())
+        assert bool(((got.double() - want).abs() <= 2.0 ** -23 * want.abs() + slack).all())
+        h = n // 2
+        out = mh.gemm_mx4_swiglu(*x, *w)
+        a, u, ta, tu = y[:, :h], y[:, h:], tol[:, :h], tol[:, h:]
+        want = a * torch.sigmoid(a) * u
+        slack = 1.1 * ta * (u.abs() + tu) + (a * torch.sigmoid(a)).abs() * tu + 2.0 ** -21 * (1 + a.abs()) * want.abs()
+        assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + slack).all())
+
+
 def test_nan_scales_stay_in_their_rows_and_columns(dev):
     """A block of scale 255 makes its row of x (its row of w) NaN and nothing else."""
     g = torch.Generator(device=dev).manual_seed(5)
