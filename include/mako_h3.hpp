@@ -142,6 +142,8 @@ struct Heads {
                             qkv_stride ? qkv_stride : 3ull * heads * 128,
                             out_head_stride ? out_head_stride : uint64_t(rows) * 128,
                             out_row_stride ? out_row_stride : 128};
+    }
+};
 
 // The axes of rotary positions (a video's time, height and width): one to four, a head's pairs in their order.
 struct Axes {
@@ -202,8 +204,6 @@ struct Scores {
     const float* slopes = nullptr;
     const int32_t* q_pos = nullptr;
     const int32_t* k_pos = nullptr;
-};
-    }
 };
 
 inline std::optional<uint32_t> parse_int8(const std::string& text)
