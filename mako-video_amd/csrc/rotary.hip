@@ -40,19 +40,29 @@ int rotary_setup(const MH3AxesArgs* args, const int32_t* pos, uint32_t half, Rot
     p = RotaryParams{};
     p.pos = pos, p.axes = a.axes;
     uint64_t at = 0;
+    long double power[kMaxRotPairs + 3];
     for (uint32_t x = 0; x < a.axes; ++x) {
         // Frequencies at most |step| (theta >= 1), so a position is below 2^18 turns and F keeps 46 bits of fraction
         // at the extreme, all 64 for steps of a turn or less.
         if (!(a.theta[x] >= 1.0) || !std::isfinite(a.theta[x]) || !(std::fabs(a.step[x]) <= 1e6) ||
             a.pairs[x] > kMaxRotPairs || at + a.pairs[x] > kMaxRotPairs)
             return MH3_ERR_PARAM;
-        // theta^(-j / pairs) as an exponential (the argument, at most some 700, is within 2^-54: far below the bound).
-        const long double ln = a.pairs[x] ? logl((long double)a.theta[x]) / (long double)a.pairs[x] : 0.0L;
+        // theta^(-j / pairs) as exponentials (their argument, at most some 700, is within 2^-54: far below the bound): every
+        // fourth, times the first four. Axes alike take the same.
+        if (x == 0 || a.pairs[x] != a.pairs[x - 1] || a.theta[x] != a.theta[x - 1]) {
+            const long double ln = a.pairs[x] ? logl((long double)a.theta[x]) / (long double)a.pairs[x] : 0.0L;
+            long double low[4] = {1.0L, expl(-ln), expl(-2.0L * ln), expl(-3.0L * ln)};
+            for (uint32_t j = 0; j < a.pairs[x]; j += 4) {
+                const long double high = j ? expl(-(long double)j * ln) : 1.0L;
+                for (uint32_t i = 0; i < 4; ++i)
+                    power[j + i] = high * low[i];
+            }
+        }
         for (uint32_t j = 0; j < a.pairs[x]; ++j) {
-            const long double f = (long double)a.step[x] * expl(-(long double)j * ln) /
-                                  6.283185307179586476925286766559005768L;
-            const long double frac = f - floorl(f); // [0, 1]
-            const long double fixed = rintl(ldexpl(frac, 64));
+            const long double f = (long double)a.step[x] * power[j] / 6.283185307179586476925286766559005768L;
+            long double frac = f - (long double)int64_t(f); // |f| < 2^18
+            frac += frac < 0.0L ? 1.0L : 0.0L;
+            const long double fixed = frac * 0x1p64L + 0.5L;
             p.turn[at + j] = fixed >= 0x1p64L ? 0u : uint64_t(fixed);
         }
         at += a.pairs[x];

@@ -208,9 +208,29 @@ def _one_device(**tensors: torch.Tensor | None) -> int:
     return device
 
 
+def _operands(*operands) -> int:
+    """_need for each (tensor, name, dtype, elements), the tensors that are None skipped, and _one_device of them all."""
+    device = -1
+    for t, name, dtype, numel in operands:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a tensor")
+        index = t.get_device()
+        if index != device:
+            if index < 0 or not t.is_cuda:
+                raise ValueError(f"{name}: must be on the GPU")
+            if device >= 0:
+                raise ValueError(f"{name}: on GPU {index}, other operands on GPU {device}")
+            device = index
+        if t.dtype != dtype or t.numel() < numel or not t.is_contiguous():
+            _need(t, name, dtype, numel)
+    return device
+
+
 def _on(device: int, what: str, fn, *args) -> None:
     """fn(*args, stream) with `device` the current one, on its current stream."""
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
@@ -685,7 +705,6 @@ def _axes_args(pos, pairs, theta, step) -> AxesArgs:
               step if isinstance(step, (int, float)) else tuple(step))
     if pos.dim() != 2 or pos.shape[1] != a.axes:
         raise ValueError(f"pos must be [rows][{a.axes}]")
-    _need(pos, "pos", torch.int32, pos.numel())
     return a
 
 
@@ -695,14 +714,11 @@ def rotary_axes(pos, pairs, *, theta=10000.0, step=1.0, cos=None, sin=None):
     axis a by pos[:, a] step[a] theta[a]^(-j / pairs[a]) radians. Returns (cos, sin), float [rows][sum(pairs)]."""
     a = _axes_args(pos, pairs, theta, step)
     rows, half, device = pos.shape[0], a.half, pos.device
-    given = cos is not None or sin is not None
     cos = torch.empty((rows, half), dtype=torch.float32, device=device) if cos is None else cos
     sin = torch.empty((rows, half), dtype=torch.float32, device=device) if sin is None else sin
-    if given:
-        _need(cos, "cos", torch.float32, rows * half)
-        _need(sin, "sin", torch.float32, rows * half)
-        _one_device(pos=pos, cos=cos, sin=sin)
-    _on(device.index, "rotary_axes", lib.mh3_rotary_axes, C.byref(a), rows, pos.data_ptr(), cos.data_ptr(), sin.data_ptr())
+    index = _operands((pos, "pos", torch.int32, rows * a.axes), (cos, "cos", torch.float32, rows * half),
+                      (sin, "sin", torch.float32, rows * half))
+    _on(index, "rotary_axes", lib.mh3_rotary_axes, C.byref(a), rows, pos.data_ptr(), cos.data_ptr(), sin.data_ptr())
     return cos, sin
 
 
@@ -713,6 +729,7 @@ def heads_partial_axes(qkv, heads, pos, pairs, q_w=None, k_w=None, *, theta=1000
     ax = _axes_args(pos, pairs, theta, step)
     if qkv.dim() == 2 and pos.shape[0] != qkv.shape[0]:
         raise ValueError("pos: one row a row of qkv")
+    _need(pos, "pos", torch.int32, pos.numel())
     device = _one_device(qkv=qkv, pos=pos, q_w=q_w, k_w=k_w, map=map, q=q, k=k, v=v)
     a, outs, ptrs = _heads_setup(qkv, heads, q_w, k_w, None, None, 0, eps, map, with_v, layout, q, k, v)
     a.rot = 2 * ax.half
@@ -987,73 +1004,84 @@ def gemm_gate_add(x, w, residual, gate, *, x_scale=None, w_scale=None, set_of_ro
 
 # ---- 4-bit microscaled operands --------------------------------------------------------------------------------------
 
+@functools.lru_cache(maxsize=256)
+def _quant_ref(rows, cols, dtype):
+    """An argument struct by reference: one a shape, as the library only reads it."""
+    if cols == 0 or cols % 256:
+        raise ValueError("cols must be a multiple of 256")
+    a = QuantArgs()
+    a.rows, a.cols, a.dtype = rows, cols, dtype
+    return C.byref(a)
+
+
+@functools.lru_cache(maxsize=256)
+def _gemm_ref(m, n, k, n_sets=0, gate_stride=0):
+    a = GemmArgs()
+    a.m, a.n, a.k, a.n_sets, a.gate_stride = m, n, k, n_sets, gate_stride
+    return C.byref(a)
+
+
 def quant_rows_mx4(w, *, q=None, scale=None):
     """Each row to 4-bit floats in blocks of 32 columns that share a power of two (OCP MX: e2m1, E8M0): w f32 or bf16
     [rows][cols], cols % 256 == 0 -> (q uint8 [rows][cols / 2], the lower column in a byte's low half; scale uint8
     [cols / 256][rows][8], byte (c / 8, r, c % 8) scaling columns 32 c .. of row r by 2^(byte - 127))."""
     if w.dim() != 2:
         raise ValueError("w must be [rows][cols]")
-    a = QuantArgs()
-    a.rows, a.cols, a.dtype = w.shape[0], w.shape[1], _dt(w)
-    if a.cols == 0 or a.cols % 256:
-        raise ValueError("cols must be a multiple of 256")
-    _need(w, "w", w.dtype, w.numel())
-    q = torch.empty((a.rows, a.cols // 2), dtype=torch.uint8, device=w.device) if q is None else q
-    scale = torch.empty((a.cols // 256, a.rows, 8), dtype=torch.uint8, device=w.device) if scale is None else scale
-    _need(q, "q", torch.uint8, w.numel() // 2)
-    _need(scale, "scale", torch.uint8, w.numel() // 32)
-    _on(_one_device(w=w, q=q, scale=scale), "quant_rows_mx4", lib.mh3_quant_rows_mx4, C.byref(a), w.data_ptr(),
-        q.data_ptr(), scale.data_ptr())
+    rows, cols = w.shape
+    ref = _quant_ref(rows, cols, _dt(w))
+    q = torch.empty((rows, cols // 2), dtype=torch.uint8, device=w.device) if q is None else q
+    scale = torch.empty((cols // 256, rows, 8), dtype=torch.uint8, device=w.device) if scale is None else scale
+    n = rows * cols
+    device = _operands((w, "w", w.dtype, n), (q, "q", torch.uint8, n // 2), (scale, "scale", torch.uint8, n // 32))
+    _on(device, "quant_rows_mx4", lib.mh3_quant_rows_mx4, ref, w.data_ptr(), q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
-def _mx4_args(x, x_scale, w, w_scale) -> GemmArgs:
+def _mx4(x, x_scale, w, w_scale):
+    """(m, rows of w, k, operands) of a product of 4-bit matrices."""
     if x.dim() != 2 or w.dim() != 2 or w.shape[1] != x.shape[1]:
         raise ValueError("x must be [m][k / 2] and w [n][k / 2]")
     m, half = x.shape
     n = w.shape[0]
-    for name, t, numel in (("x", x, m * half), ("x_scale", x_scale, m * half // 16), ("w", w, n * half),
-                           ("w_scale", w_scale, n * half // 16)):
-        _need(t, name, torch.uint8, numel)
-    a = GemmArgs()
-    a.m, a.n, a.k = m, n, 2 * half
-    return a
+    u8 = torch.uint8
+    return m, n, 2 * half, ((x, "x", u8, m * half), (x_scale, "x_scale", u8, m * half // 16), (w, "w", u8, n * half),
+                            (w_scale, "w_scale", u8, n * half // 16))
 
 
 def gemm_mx4(x, x_scale, w, w_scale, *, out=None):
     """out = x w^T of two matrices as quant_rows_mx4 leaves them (x [m][k], w [n][k]), bf16 [m][n]."""
-    a = _mx4_args(x, x_scale, w, w_scale)
-    out = torch.empty((a.m, a.n), dtype=torch.bfloat16, device=x.device) if out is None else out
-    _need(out, "out", torch.bfloat16, a.m * a.n)
-    _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, out=out), "gemm_mx4", lib.mh3_gemm_mx4, C.byref(a),
-        x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), out.data_ptr())
+    m, n, k, operands = _mx4(x, x_scale, w, w_scale)
+    out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device) if out is None else out
+    device = _operands(*operands, (out, "out", torch.bfloat16, m * n))
+    _on(device, "gemm_mx4", lib.mh3_gemm_mx4, _gemm_ref(m, n, k), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(),
+        w_scale.data_ptr(), out.data_ptr())
     return out
 
 
 def gemm_mx4_swiglu(x, x_scale, w, w_scale, *, out=None):
     """fc1 + SwiGLU: w [2n][k] (gate rows then up rows), out = silu(x Wg^T) * (x Wu^T), bf16 [m][n]."""
-    a = _mx4_args(x, x_scale, w, w_scale)
-    if a.n % 2:
+    m, n, k, operands = _mx4(x, x_scale, w, w_scale)
+    if n % 2:
         raise ValueError("w must be [2n][k / 2]")
-    a.n //= 2
-    out = torch.empty((a.m, a.n), dtype=torch.bfloat16, device=x.device) if out is None else out
-    _need(out, "out", torch.bfloat16, a.m * a.n)
-    _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, out=out), "gemm_mx4_swiglu", lib.mh3_gemm_mx4_swiglu,
-        C.byref(a), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), out.data_ptr())
+    n //= 2
+    out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device) if out is None else out
+    device = _operands(*operands, (out, "out", torch.bfloat16, m * n))
+    _on(device, "gemm_mx4_swiglu", lib.mh3_gemm_mx4_swiglu, _gemm_ref(m, n, k), x.data_ptr(), x_scale.data_ptr(),
+        w.data_ptr(), w_scale.data_ptr(), out.data_ptr())
     return out
 
 
 def gemm_mx4_gate_add(x, x_scale, w, w_scale, residual, gate, *, set_of_row=None, n_sets=1):
     """The out projection and fc2 with gate_add_rows folded in: residual += gate[s] * (x w^T), [m][n] in place, bf16 or
     float; gate and set_of_row as gemm_gate_add takes them. Returns residual."""
-    a = _mx4_args(x, x_scale, w, w_scale)
+    m, n, k, operands = _mx4(x, x_scale, w, w_scale)
     f32 = residual.dtype == torch.float32
-    _need(residual, "residual", torch.float32 if f32 else torch.bfloat16, a.m * a.n)
-    a.n_sets, a.gate_stride = n_sets, _set_stride(gate, "gate", a.n, n_sets)
-    if set_of_row is not None:
-        _need(set_of_row, "set_of_row", torch.uint8, a.m)
+    device = _operands(*operands, (residual, "residual", torch.float32 if f32 else torch.bfloat16, m * n),
+                       (set_of_row, "set_of_row", torch.uint8, m))
+    stride = _set_stride(gate, "gate", n, n_sets)
+    if gate.get_device() != device:
+        raise ValueError(f"gate: on GPU {gate.get_device()}, other operands on GPU {device}")
     fn = lib.mh3_gemm_mx4_gate_add_f32 if f32 else lib.mh3_gemm_mx4_gate_add
-    _on(_one_device(x=x, x_scale=x_scale, w=w, w_scale=w_scale, residual=residual, gate=gate, set_of_row=set_of_row),
-        "gemm_mx4_gate_add", fn, C.byref(a), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
-        gate.data_ptr(), _ptr(set_of_row), residual.data_ptr())
+    _on(device, "gemm_mx4_gate_add", fn, _gemm_ref(m, n, k, n_sets, stride), x.data_ptr(), x_scale.data_ptr(),
+        w.data_ptr(), w_scale.data_ptr(), gate.data_ptr(), _ptr(set_of_row), residual.data_ptr())
     return residual
