@@ -2,7 +2,9 @@
  * mako_h3.h — C-ABI of the MI355X (gfx950) kernels for the per-block hot path of mako-video's MiniMax-H3
  * transformer: the adaLN-modulated RMS norm and the gated residual (`rms_mod_rows`, `gate_add_rows`, fused),
  * `swiglu_rows`, the `--sparse` cube selector (`cube_pool`, `cube_scores`, `cube_topk`, fused `cube_select`),
- * the `--int8` weight quantizer (`quant_rows_i8`) and the int8 weight-only fc1 GEMM with its SwiGLU epilogue.
+ * the `--int8` weight quantizer (`quant_rows_i8`) and the int8 weight-only fc1 GEMM with its SwiGLU epilogue; and of
+ * the dense path beside it: rotary positions on several axes (`rotary_axes`), attention over whole rows
+ * (`flash_attn_128`) and 4-bit microscaled products (`gemm_mx4`).
  *
  * The reference runs these as Metal kernels looked up by name in mako-common's TransformerRuntime
  * (`dispatch(enc, name, {buffers}, &args, sizeof args, grid, tg)`, the in-repo instance being

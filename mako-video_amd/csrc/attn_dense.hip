@@ -15,13 +15,18 @@
 //   causal rows, 40 heads on 8, slopes 2^-1 .. 2^-8: 571 us in rising order). A wave masks a tile only where its own
 //   rows' ranges do not all cover it.
 // - A masked probability is a zero, and zero times an infinite or NaN value of V would still be NaN in the rows that do
-//   not attend it: in a masked tile the wave looks for such values, and where there are any the matrix cores take zeros
-//   for them, and they are added one key at a time to the rows that attend it.
-// - Softmax in base 2. A row's running maximum moves only when a tile raises it by more than 8, so P stays below 2^8 and
-//   most tiles skip the rescale of O. P rounds to bf16 for the matrix cores (2^-9 of each probability, below the output's
-//   own rounding); maxima, sums and O are float.
+//   not attend it: masked tiles are searched for such values, and where there are any the matrix cores take zeros for
+//   them, and they are added one key at a time to the rows that attend it. (All tiles masked, 40 heads, 14,080 rows on
+//   11,264 keys: 4.25 ms, and 2.81 ms with none masked.)
+// - Softmax in base 2. A row's running maximum is brought up to date only when a tile's probabilities sum up to more than
+//   2^10 in a lane, so P stays below 2^10 and most tiles neither search a maximum nor rescale O. P rounds to bf16 for the
+//   matrix cores (2^-9 of each probability, below the output's own rounding); maxima, sums and O are float.
 // - Few rows leave the chip idle: their keys are then split over workgroups, each leaves its part of O, the maximum and the
 //   sum in the workspace, and a second kernel joins them in a fixed order.
+// What bounds it: many rows, the chip's power (960 x 544, 56 heads, 19,305 rows: 9.1 .. 9.3 ms, 1150 .. 1180 TFLOP/s, the
+// clock at 1.7 GHz and the matrix cores busy 68% of it); under a cap the vector unit (five more operations a score, two
+// of them transcendental: 14,925 rows of 40 heads 5.0 ms, without one 4.1); few rows, the one pass over K and V (129,536
+// keys of 8 heads in 105 us, 5.0 TB/s).
 #include "mh3_common.hpp"
 
 #include <algorithm>
@@ -106,8 +111,8 @@ __device__ __forceinline__ void phase_barrier()
 
 // 16 or 4 bytes a lane from a buffer straight into LDS, lane L's at lds + 16 L or 4 L. Written as assembly for what the
 // compiler would make of the builtin here: it waits for every such load in flight before each transposed LDS read, as
-// if one might land under it, which cost half of the time (960 x 544: 10.1 ms; the tiles' slots and the waits in
-// pair_turn and few_turn order them). No vector register is written, so nothing is in flight that the compiler has to know
+// if one might land under it, which made a turn half as long again (the tiles' slots and the waits in pair_turn and
+// few_turn order them). No vector register is written, so nothing is in flight that the compiler has to know
 // of, and M0 is used by nothing else in this file.
 __device__ __forceinline__ void load_lds16(const u32x4_t& buffer, char* lds, uint32_t offset)
 {

@@ -3,15 +3,19 @@
 // int8 and bf16 forms (gemm.hip) with the same epilogues: a plain store (qkv), SwiGLU (fc1), gate_add_rows (out, fc2).
 //   y[r][c] = sum over the blocks b of 2^(sx[r][b] + sw[c][b] - 254) sum_{i in b} x[r][i] w[c][i], in float.
 //
-// Design (gfx950):
-// - The tile, the wave layout, the LDS swizzle and the XCD map are gemm_kernel's: a row of an LDS stage is 128 bytes of
-//   k, here 256 values, and one MFMA operand is 16 bytes a lane, here the 32 values of one block. So each lane has one
-//   scale byte an operand, and a K-step of 256 k is 64 MFMAs a wave with four times the bf16 kernel's products.
+// Design (gfx950), the tile kernels:
+// - The wave layout, the LDS swizzle and the XCD map are gemm_kernel's: a row of an LDS stage is 128 bytes of k, here 256
+//   values, and one MFMA operand is 16 bytes a lane, here the 32 values of one block. So each lane has one scale byte an
+//   operand, and a K-step of 256 k is 64 MFMAs a wave (256 x 256 tiles) with four times the bf16 kernel's products.
 // - The scale bytes come eight blocks (a K-step) of all rows at a time, [k / 256][rows][8]: a tile's are then one
 //   contiguous run a K-step, 4 bytes a lane of one DMA instruction a wave, and an operand's byte is one ds_read_u8.
 // - Both operands and their scales go out together, into a ring of stages each of which holds a whole K-step; the
 //   loads of tile kt + kStages start as soon as every wave has read tile kt, behind the barrier that publishes
 //   tile kt + 1.
+// What bounds them: large products, the chip's power (19,305 x 5376 -> 2 x 14,336: 1.45 ms, 4.1 PFLOP/s, the clock at 1.6 to
+// 1.9 GHz; the bare MFMA in a loop reaches 6.0 at 1.5 GHz, this kernel without its loads 4.75, and loads a tile ahead with
+// stores straight from registers, or four waves of 128 x 128, no more than it does now); middle ones the rounds of tiles;
+// few rows the weights' bytes (3 rows, 5376 x 14,336: 11.3 us, 41 MB at 3.6 TB/s with the launch in it).
 #include "gemm.hpp"
 
 #include <algorithm>
@@ -224,6 +228,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx4_kernel(const uint8_t* __
 // Up to 16 MT rows: the time is w's one pass from memory. A workgroup takes 32 rows of w (SwiGLU: 16 gate rows and their
 // 16 up rows), its eight waves the K-steps in turn, from memory straight into registers; their sums are joined through LDS
 // in the waves' order. The products are w x^T: a lane then holds four consecutive columns of one row of the result.
+// (3 rows, 5376 x 14,336: 11.3 us. With 16 rows of w a workgroup 15.0, with 64 21.8; sixteen waves 13.2; two steps ahead
+// 14.1, where the loads past the end cost as much as others; non-temporal loads 15.1; the 64 x 128 tiles 26.)
 constexpr uint32_t kFewWaves = 8, kFewTiles = 2; // tiles of 16 rows of w
 
 template <int MT, int EPI>

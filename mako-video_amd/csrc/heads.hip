@@ -204,6 +204,8 @@ __global__ __launch_bounds__(kHeadsThreads) void heads_kernel(HeadsParams p)
     heads_rows(p, r0, min(p.rows_per_block, p.rows - r0), lds);
 }
 
+// The same with the cosines and sines of its rows made in LDS, where heads_kernel keeps those it reads. HBM-bound (19,305
+// rows of 56 heads: 310 us, 5.35 TB/s, and with tables in memory as much again and a call to make them).
 __global__ __launch_bounds__(kHeadsThreads) void heads_axes_kernel(HeadsParams p, RotaryParams axes)
 {
     extern __shared__ float lds[];

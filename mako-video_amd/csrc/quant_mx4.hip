@@ -5,7 +5,7 @@
 //
 // HBM-bound: 2 bytes read (bf16) and 17/32 of a byte written a value. Four lanes take a block, 8 values each, so a
 // wave's 16-byte loads cover 1 KB without gaps; the block's maximum is two DPP steps within the quad, and a quad's codes
-// go out as one 16-byte run.
+// go out as one 16-byte run. 19,305 x 5376 in 51 us, 5.2 TB/s.
 #include "mh3_common.hpp"
 
 namespace mh3 {

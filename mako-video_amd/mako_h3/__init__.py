@@ -2,7 +2,8 @@
 
 The op names are the reference's kernel names (mako-common's `rms_mod_rows`, `gate_add_rows`, `swiglu_rows`,
 `cube_pool`, `cube_scores`, `cube_topk`, `quant_rows_i8`; fc1's `gemm_i8` + `swiglu_rows` as `gemm_w8a16_swiglu`),
-and errors raise RuntimeError as the reference's host code throws std::runtime_error on a bad call
+with the dense path beside them (`rotary_axes`, `heads_partial_axes`, `flash_attn_128`, `attn_ranges`, `quant_rows_mx4`,
+`gemm_mx4*`, which also run on the GPU that their tensors are on where it is not the current one), and errors raise RuntimeError as the reference's host code throws std::runtime_error on a bad call
 (src/video/audio_vae.cpp:231-232). Every call checks the tensors against the sizes the kernel will touch before it
 reaches the library, launches on torch's current stream, and returns without synchronizing.
 
