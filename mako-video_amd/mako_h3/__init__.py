@@ -792,7 +792,7 @@ def _dense_args(q, k, v, layout, scale, cap) -> DenseAttnArgs:
 
 
 def flash_attn_128_workspace_bytes(q, k, v, *, layout="heads") -> int:
-    """Bytes of workspace that flash_attn_128 needs for these operands (0 where it needs none)."""
+    """Bytes of workspace that flash_attn_128 needs for these operands on the current device (0 where it needs none)."""
     n = int(lib.mh3_flash_attn_128_workspace_bytes(C.byref(_dense_args(q, k, v, layout, 0.0, 0.0))))
     _check(min(n, 0), "flash_attn_128_workspace_bytes")
     return n
@@ -813,6 +813,10 @@ def flash_attn_128(q, k, v, *, ranges=None, scale=0.0, cap=0.0, slopes=None, q_p
     heads, q_rows = a.heads, a.q_rows
     device = _one_device(q=q, k=k, v=v, ranges=ranges, slopes=slopes, q_pos=q_pos, k_pos=k_pos, out=out,
                          workspace=workspace)
+    if device != torch._C._cuda_getDevice():  # the workspace's size is of the current device
+        with torch.cuda.device(device):
+            return flash_attn_128(q, k, v, ranges=ranges, scale=scale, cap=cap, slopes=slopes, q_pos=q_pos, k_pos=k_pos,
+                                  layout=layout, out=out, out_layout=out_layout, workspace=workspace)
     if out is None:
         out = torch.empty((heads, q_rows, 128) if out_layout == "heads" else (q_rows, heads * 128),
                           dtype=torch.bfloat16, device=device)
