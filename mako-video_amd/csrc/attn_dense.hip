@@ -39,11 +39,20 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4_t __attribute__((ext_vector_type(4)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
 typedef short v4i16 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
 constexpr uint32_t kTileBytes = 16384; // 64 keys of K, or of V
+
+// Ranges that the host has not seen: both kernels are launched, and each of their workgroups finds out from the ranges
+// which of the two has less to do. The other ends at once.
+struct Contest {
+    uint32_t pair_splits, few_splits; // 0: no contest
+    uint32_t cus;
+    uint32_t* winner; // its splits, for the join
+};
 
 struct DenseParams {
     const uint16_t* q;
@@ -59,6 +68,7 @@ struct DenseParams {
     uint32_t kv_heads, group, q_rows, kv_rows, list; // list = q_rows group
     uint32_t tiles, splits;                          // row tiles a key head, key splits
     FastDiv div_group, div_tiles, div_splits;
+    Contest contest;
     // A score comes from the matrix cores of q times a power of two, q_pow (exact), which leaves the rest of the scale: so
     // a dot product overflows only where the scaled score nearly would.
     float q_pow;
@@ -138,6 +148,48 @@ __device__ __forceinline__ void range_of(const DenseParams& p, uint32_t f, uint3
         lo = uint32_t(min(max(r.x, 0), int32_t(p.kv_rows)));
         hi = uint32_t(min(max(r.y, int32_t(lo)), int32_t(p.kv_rows)));
     }
+}
+
+// Whether attn_few_kernel has less to do than attn_pair_kernel, from the key tiles that the rows of each one's workgroups
+// span: in tenths of a us, a workgroup's start and its turns (plan_of's figures, and 2.3 and 2.8 us a turn of eight waves
+// and of one whose rows do not attend the same keys), of the longest workgroup or of all of them over the CUs. Integers, so that both
+// kernels find the same. A lane takes a tile of 32 rows, eight of them are a tile of 256.
+__device__ __forceinline__ bool few_has_less(const DenseParams& p, uint32_t lane)
+{
+    uint32_t few_max = 0, pair_max = 0;
+    uint64_t few_sum = 0, pair_sum = 0;
+    for (uint32_t t0 = 0; t0 * 32u < p.list; t0 += 64u) {
+        const uint32_t f0 = (t0 + lane) * 32u;
+        uint32_t lo = ~0u, hi = 0u, all_lo = 0u, all_hi = ~0u;
+        if (f0 < p.list) {
+            const uint32_t r1 = p.div_group.div(min(f0 + 32u, p.list) - 1u);
+            for (uint32_t r = p.div_group.div(f0); r <= r1; ++r) {
+                uint32_t a, b;
+                range_of(p, f0, r, a, b);
+                if (a < b)
+                    lo = min(lo, a), hi = max(hi, b);
+                all_lo = max(all_lo, a), all_hi = min(all_hi, b);
+            }
+        }
+        const auto alike = [&] { return all_lo < all_hi && uint64_t(all_hi - all_lo) * 8u >= uint64_t(hi - lo) * 7u; };
+        const uint32_t few = lo < hi ? (hi - lo + 63u) / 64u * (alike() ? 15u : 28u) : 0u;
+#pragma unroll
+        for (int d = 1; d < 8; d *= 2) {
+            lo = min(lo, uint32_t(__shfl_xor(int(lo), d, kWave))), hi = max(hi, uint32_t(__shfl_xor(int(hi), d, kWave)));
+            all_lo = max(all_lo, uint32_t(__shfl_xor(int(all_lo), d, kWave)));
+            all_hi = min(all_hi, uint32_t(__shfl_xor(int(all_hi), d, kWave)));
+        }
+        const uint32_t pair = (lane & 7u) == 0u && lo < hi ? (hi - lo + 63u) / 64u * (alike() ? 15u : 23u) : 0u;
+        few_max = max(few_max, wave_max_u32(few)), pair_max = max(pair_max, wave_max_u32(pair));
+        for (uint32_t i = 0; i < 64u; ++i)
+            few_sum += uint32_t(__builtin_amdgcn_readlane(int(few), int(i)));
+        for (uint32_t i = 0; i < 64u; i += 8u)
+            pair_sum += uint32_t(__builtin_amdgcn_readlane(int(pair), int(i)));
+    }
+    const Contest& c = p.contest;
+    const uint64_t few = 100u + max(uint64_t(few_max / c.few_splits), few_sum * p.kv_heads / (4u * c.cus));
+    const uint64_t pair = 140u + max(uint64_t(pair_max / c.pair_splits), pair_sum * p.kv_heads / c.cus);
+    return few < pair;
 }
 
 // N of a tile's 16 DMA instructions of K (VALUE false) or V, the ones from i0 on. Instruction i fills the LDS kilobyte
@@ -387,13 +439,12 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
         }
     }
     if (MASKED) {
+        const uint32_t from_lo = t0 + 4u * hh - w.lo, keys = w.hi - w.lo; // modulo 2^32: below lo is past every count
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint32_t key = t0 + 32u * b + 8u * (i >> 2) + 4u * hh + (i & 3);
-                s[b][i] = key >= w.lo && key < w.hi ? s[b][i] : -kInf;
-            }
+            for (int i = 0; i < 16; ++i)
+                s[b][i] = from_lo + (32u * b + 8u * (i >> 2) + (i & 3)) < keys ? s[b][i] : -kInf;
     }
     // Most tiles raise no maximum by much, and the sum over a lane's 32 keys of a row tells: up to 2^10 no key is above
     // that, and the old maximum serves. That spares the search for the new one in a phase whose vector instructions take 7
@@ -631,15 +682,15 @@ __device__ __forceinline__ void tiles_of(const DenseParams& p, uint32_t k0, uint
 template <int N>
 __device__ __forceinline__ bool holds_nonfinite(const char* part, uint32_t lane)
 {
-    uint32_t any = 0;
+    ushortx2 top{0, 0}; // the largest magnitudes: an exponent of ones is above every other
 #pragma unroll
     for (uint32_t i = 0; i < uint32_t(N); ++i) {
         const u32x4_t t = *reinterpret_cast<const u32x4_t*>(part + 1024u * i + 16u * lane);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            any |= (t[e] & 0x7f807f80u) + 0x00800080u; // carries out of an exponent of ones
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(ushortx2, t[e] & 0x7fff7fffu));
     }
-    return __ballot((any & 0x80008000u) != 0u) != 0u;
+    return __ballot(top[0] >= 0x7f80u || top[1] >= 0x7f80u) != 0u;
 }
 
 // What attn_few_kernel loads of a tile: K and, in the slot of its turn, the key positions; or V.
@@ -714,6 +765,12 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     if (!block_of(p, kvh, tile, split))
         return;
     const uint32_t lane = threadIdx.x;
+    if (p.contest.few_splits) {
+        if (!few_has_less(p, lane))
+            return;
+        if (blockIdx.x == 0 && lane == 0)
+            *p.contest.winner = p.splits;
+    }
     WaveRows w;
     load_rows<CAP, BIAS>(p, kvh, tile * 32u, lane, w);
     uint32_t first, last;
@@ -861,6 +918,12 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     if (!block_of(p, kvh, tile, split))
         return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (p.contest.few_splits) {
+        if (few_has_less(p, lane))
+            return; // every wave finds the same
+        if (blockIdx.x == 0 && tid == 0)
+            *p.contest.winner = p.splits;
+    }
     uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kRing * kTileBytes + 2048u * wave);
     uint32_t* const span = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + 2048u * kPairWaves);
     const uint32_t f0 = (tile * kPairWaves + wave) * 32u;
@@ -964,6 +1027,11 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
 __global__ __launch_bounds__(256) void attn_join_kernel(DenseParams p)
 {
     __shared__ float part[4][4][64]; // a wave's maximum, sum and two values of O, by lane
+    if (p.contest.few_splits) {
+        p.splits = *p.contest.winner;
+        if (p.splits == 1u)
+            return; // the rows are written
+    }
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint64_t item = blockIdx.x, items = uint64_t(p.kv_heads) * p.list;
     const uint32_t kvh = uint32_t(item / p.list), f = uint32_t(item - uint64_t(kvh) * p.list);
@@ -1061,45 +1129,74 @@ using namespace mh3;
 
 struct Plan {
     uint32_t waves, splits;
-    uint64_t list, tiles;
+    uint64_t tiles;
+    double us; // estimated
 };
 
-// The workgroup's waves and the key splits of a call: the pair of least estimated time, of the two kernels with no split
-// or as many as give the chip one, two or four workgroups a CU. In us, measured: a workgroup of eight waves takes 14 and
-// 1.5 a key tile (it has a CU to itself), one of a single wave 10 and 1.5 (four share a CU); K and V come from HBM once at
-// 6 TB/s, and for each further row tile from the MALL or L2 at some 16; the join takes 6 and its parts' bytes. Heads, query
-// and key rows, eight waves and one, each at its best splits (us): 56, 945 x 945 44 and 68; 40, 212 x 212 20 and 15; 7,
+// The key splits of a call for the kernel of `waves` waves a workgroup: those of least estimated time, of none and as many
+// as give the chip one, two or four workgroups a CU. In us, measured: a workgroup of eight waves takes 14 and 1.5 a key
+// tile (it has a CU to itself), one of a single wave 10 and 1.5 (four share a CU); K and V come from HBM once at 6 TB/s,
+// and for each further row tile from the MALL or L2 at some 16; the join takes 6 and its parts' bytes. Heads, query and
+// key rows, eight waves and one, each at its best splits (us): 56, 945 x 945 44 and 68; 40, 212 x 212 20 and 15; 7,
 // 700 x 700 30 and 24; 40, 64 x 20,000 125 and 93; 40 on 8 key heads, 1 x 5000 18 and 15, 3 x 129,536 108 and 94; 7 on 1,
-// 500 x 16,000 52 and 71; 56 on 8, 64 x 100,000 198 and 324. (Ranges that leave most keys out are not known here.)
-Plan plan_of(const MH3DenseAttnArgs& a)
+// 500 x 16,000 52 and 71; 56 on 8, 64 x 100,000 198 and 324.
+Plan plan_of(const MH3DenseAttnArgs& a, uint32_t waves)
 {
     const uint64_t list = uint64_t(a.q_rows) * (a.heads / a.kv_heads), key_tiles = (uint64_t(a.kv_rows) + 63u) / 64u;
     const uint64_t cus = uint64_t(std::max(host::cu_count(), 1));
     const double head_us = double(a.kv_heads) * a.kv_rows * 512.0 * 1e-6; // us a pass over K and V at 1 TB/s
+    const bool pair = waves == kPairWaves;
+    const uint64_t tiles = (list + 32u * waves - 1u) / (32u * waves), blocks = tiles * a.kv_heads;
     Plan best{};
-    double best_us = 0.0;
-    for (const uint32_t waves : {kPairWaves, 1u}) {
-        const bool pair = waves == kPairWaves;
-        const uint64_t tiles = (list + 32u * waves - 1u) / (32u * waves), blocks = tiles * a.kv_heads;
-        for (const uint64_t fill : {uint64_t(0), cus, 2u * cus, 4u * cus}) {
-            // At least four key tiles a split.
-            const uint64_t splits = std::max<uint64_t>(1u, std::min<uint64_t>({fill / blocks, key_tiles / 4u, 256u}));
-            const uint64_t rounds = (blocks * splits + (pair ? cus : 4u * cus) - 1u) / (pair ? cus : 4u * cus);
-            const double turns = double((key_tiles + splits - 1u) / splits);
-            double us = std::max(double(rounds) * (pair ? 14.0 + 1.5 * turns : 10.0 + 1.5 * turns),
-                                 head_us * (1.0 / 6.0 + double(tiles - 1u) / 16.0));
-            if (splits > 1u)
-                us += 6.0 + double(splits) * double(a.kv_heads) * double(list) * 1040.0 * 1e-6 / 4.0;
-            if (best.waves == 0u || us < best_us)
-                best = Plan{waves, uint32_t(splits), list, tiles}, best_us = us;
-        }
+    for (const uint64_t fill : {uint64_t(0), cus, 2u * cus, 4u * cus}) {
+        // At least four key tiles a split.
+        const uint64_t splits = std::max<uint64_t>(1u, std::min<uint64_t>({fill / blocks, key_tiles / 4u, 256u}));
+        const uint64_t rounds = (blocks * splits + (pair ? cus : 4u * cus) - 1u) / (pair ? cus : 4u * cus);
+        const double turns = double((key_tiles + splits - 1u) / splits);
+        double us = std::max(double(rounds) * (pair ? 14.0 + 1.5 * turns : 10.0 + 1.5 * turns),
+                             head_us * (1.0 / 6.0 + double(tiles - 1u) / 16.0));
+        if (splits > 1u)
+            us += 6.0 + double(splits) * double(a.kv_heads) * double(list) * 1040.0 * 1e-6 / 4.0;
+        if (best.waves == 0u || us < best.us)
+            best = Plan{waves, uint32_t(splits), tiles, us};
     }
     return best;
 }
 
-uint64_t workspace_bytes(const MH3DenseAttnArgs& a, const Plan& p)
+// Both kernels' plans, the one to run first. With ranges, few rows against many keys may be of many documents, of which a
+// workgroup of eight waves spans several and walks all of their keys with most of its waves idle; or of one, where it
+// reads K and V once for more rows. So that is decided on the device (few_has_less; contest), where a call is long
+// enough for the second launch and the look at the ranges, some 6 us. One-wave workgroups then take more splits, as those
+// that span two documents are longer than the others, where there are many (4 x 28 rows below: 7 splits 422, 14 300). Heads, documents, query rows of each, keys in all,
+// eight waves and one at their best splits (us): 40 on 8, 64 x 1, 129,536 207 and 112; 3 x 4, 129,536 184 and 105; 1 x 28,
+// 116,105 118 and 150; 56 on 8, 1 x 64, 100,000 212 and 329; 2 x 64, 100,000 348 and 337; 40, 4 x 64, 20,000 183 and 105.
+struct Plans {
+    Plan first, second;
+    uint64_t list;
+    bool contest;
+};
+
+Plans plans_of(const MH3DenseAttnArgs& a)
 {
-    return p.splits > 1u ? uint64_t(p.splits) * a.kv_heads * p.list * 130u * 4u : 0u;
+    const Plan pair = plan_of(a, kPairWaves);
+    Plan few = plan_of(a, 1u);
+    const uint64_t list = uint64_t(a.q_rows) * (a.heads / a.kv_heads);
+    const bool contest = list > 32u && list <= 8192u && uint64_t(a.q_rows) * 4u <= a.kv_rows &&
+                         (pair.splits > 1u || few.splits > 1u) && std::min(pair.us, few.us) >= 60.0;
+    if (!contest)
+        return pair.us < few.us ? Plans{pair, few, list, false} : Plans{few, pair, list, false};
+    const uint64_t fill = (few.tiles > 8u ? 8u : 4u) * uint64_t(std::max(host::cu_count(), 1));
+    few.splits = uint32_t(std::max<uint64_t>(
+        1u, std::min<uint64_t>({fill / (few.tiles * a.kv_heads), (uint64_t(a.kv_rows) + 255u) / 256u, 256u})));
+    return pair.us < few.us ? Plans{pair, few, list, true} : Plans{few, pair, list, true};
+}
+
+constexpr uint64_t kHeader = 16u; // bytes before the parts: the contest's winner
+
+uint64_t workspace_bytes(const MH3DenseAttnArgs& a, const Plans& p)
+{
+    const uint32_t splits = p.contest ? std::max(p.first.splits, p.second.splits) : p.first.splits;
+    return splits > 1u ? kHeader + uint64_t(splits) * a.kv_heads * p.list * 130u * 4u : 0u;
 }
 
 int check_args(const MH3DenseAttnArgs* args)
@@ -1154,7 +1251,7 @@ extern "C" int64_t mh3_flash_attn_128_workspace_bytes(const MH3DenseAttnArgs* ar
         return rc;
     if (args->q_rows == 0)
         return 0;
-    return int64_t(workspace_bytes(*args, plan_of(*args)));
+    return int64_t(workspace_bytes(*args, plans_of(*args)));
 }
 
 extern "C" int mh3_flash_attn_128(const MH3DenseAttnArgs* args, const uint16_t* q, const uint16_t* k, const uint16_t* v,
@@ -1166,8 +1263,8 @@ extern "C" int mh3_flash_attn_128(const MH3DenseAttnArgs* args, const uint16_t* 
     const MH3DenseAttnArgs& a = *args;
     if (a.q_rows == 0)
         return MH3_OK;
-    const Plan plan = plan_of(a);
-    const uint64_t need = workspace_bytes(a, plan);
+    const Plans plans = plans_of(a);
+    const uint64_t need = workspace_bytes(a, plans);
     if (!q || !out || (a.kv_rows && (!k || !v)) || (need && !workspace))
         return MH3_ERR_POINTER;
     if (!q_pos != !k_pos || (q_pos && !slopes))
@@ -1199,16 +1296,17 @@ extern "C" int mh3_flash_attn_128(const MH3DenseAttnArgs* args, const uint16_t* 
     const host::Span o[] = {{out, span(a.heads, a.out_head_stride, a.q_rows, a.out_row_stride)}, {workspace, need}};
     if (host::any_overlap(in, o))
         return MH3_ERR_PARAM;
-    if (plan.tiles * a.kv_heads * plan.splits * plan.waves * 64u >= (1ull << 31))
-        return MH3_ERR_SHAPE;
+    for (const Plan& plan : {plans.first, plans.second})
+        if (plan.tiles * a.kv_heads * plan.splits * plan.waves * 64u >= (1ull << 31))
+            return MH3_ERR_SHAPE;
     DenseParams p{};
     p.q = q, p.k = k, p.v = v, p.out = out, p.ranges = ranges, p.slopes = slopes, p.q_pos = q_pos, p.k_pos = k_pos;
-    p.part = static_cast<float*>(workspace);
+    p.part = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kHeader) : nullptr;
     p.qhs = a.q_head_stride, p.qrs = a.q_row_stride, p.khs = a.k_head_stride, p.krs = a.k_row_stride;
     p.vhs = a.v_head_stride, p.vrs = a.v_row_stride, p.ohs = a.out_head_stride, p.ors = a.out_row_stride;
     p.kv_heads = a.kv_heads, p.group = a.heads / a.kv_heads, p.q_rows = a.q_rows, p.kv_rows = a.kv_rows;
-    p.list = uint32_t(plan.list), p.tiles = uint32_t(plan.tiles), p.splits = plan.splits;
-    p.div_group = FastDiv::make(p.group), p.div_tiles = FastDiv::make(p.tiles), p.div_splits = FastDiv::make(p.splits);
+    p.list = uint32_t(plans.list);
+    p.div_group = FastDiv::make(p.group);
     const float scale = a.scale > 0.0f ? a.scale : 0.08838834764831845f; // 1 / sqrt(128)
     int pow = 0;
     std::frexp(scale, &pow);
@@ -1217,12 +1315,25 @@ extern "C" int mh3_flash_attn_128(const MH3DenseAttnArgs* args, const uint16_t* 
     p.scale_log2 = scale / p.q_pow * kLog2e;
     if (a.cap > 0.0f)
         p.cap_in = 2.0f * kLog2e * (scale / p.q_pow) / a.cap, p.cap_out = a.cap * kLog2e;
+    const bool contest = plans.contest && ranges;
+    if (contest) {
+        const bool pair_first = plans.first.waves == kPairWaves;
+        p.contest = Contest{(pair_first ? plans.first : plans.second).splits, (pair_first ? plans.second : plans.first).splits,
+                            uint32_t(std::max(host::cu_count(), 1)), static_cast<uint32_t*>(workspace)};
+    }
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const bool cap = a.cap > 0.0f, bias = slopes != nullptr;
-    const int rc = cap ? bias ? launch_dense<true, true>(p, plan.waves, s) : launch_dense<true, false>(p, plan.waves, s)
+    const auto run = [&](const Plan& plan) {
+        p.tiles = uint32_t(plan.tiles), p.splits = plan.splits;
+        p.div_tiles = FastDiv::make(p.tiles), p.div_splits = FastDiv::make(p.splits);
+        return cap ? bias ? launch_dense<true, true>(p, plan.waves, s) : launch_dense<true, false>(p, plan.waves, s)
                    : bias ? launch_dense<false, true>(p, plan.waves, s)
                           : launch_dense<false, false>(p, plan.waves, s);
-    if (rc != MH3_OK || p.splits == 1u)
+    };
+    int rc = run(plans.first);
+    if (rc == MH3_OK && contest)
+        rc = run(plans.second);
+    if (rc != MH3_OK || (!contest && p.splits == 1u))
         return rc;
     const uint64_t items = uint64_t(p.kv_heads) * p.list;
     hipLaunchKernelGGL(attn_join_kernel, dim3(uint32_t(items)), dim3(256), 0, s, p);

@@ -328,3 +328,57 @@ def test_infinite_values_in_masked_and_whole_tiles(dev, lengths, causal, bias, c
     if bias:
         kw["slopes"] = torch.rand(4, generator=g, device=dev) * 0.02
     check(mh.flash_attn_128(q, k, v, **kw), *attention64(q, k, v, **kw))
+
+
+@pytest.mark.parametrize("heads,kv_heads,keys,news", [
+    (16, 16, [60000], [40]), (16, 16, [20000, 20001, 19999], [12, 12, 12]), (16, 16, [1, 30000, 63, 0, 30000], [1, 30, 5, 0, 20]),
+    (40, 8, [100000], [28]), (40, 8, [30000, 40000, 30000], [4, 4, 4]), (40, 8, [2000] * 50, [1] * 50),
+    (40, 8, [50000, 50000], [28, 28])])
+@pytest.mark.parametrize("causal,cap,bias", [(True, 0.0, False), (False, 30.0, False), (True, 0.0, True)])
+def test_a_batch_of_streams_with_new_rows(dev, heads, kv_heads, keys, news, causal, cap, bias):
+    """New rows of one or many streams against long kept keys: the sizes where the ranges decide which of the two kernels
+    runs, with one, few or many rows a stream, empty streams, and rows of none in front."""
+    g = torch.Generator(device=dev).manual_seed(sum(keys) + sum(news))
+    rows, n = 3 + sum(news), sum(keys)
+    q, k, v = make(g, heads, rows, dev), make(g, kv_heads, n, dev), make(g, kv_heads, n, dev)
+    cut = lambda a, at: torch.tensor([at, *(torch.tensor(a).cumsum(0) + at).tolist()], dtype=torch.int32, device=dev)  # noqa: E731
+    kw = {"ranges": mh.attn_ranges(cut(news, 3), cut(keys, 0), rows, n, causal=causal), "cap": cap}
+    if bias:
+        kw["slopes"] = 0.5 ** torch.linspace(4.0, 12.0, heads, device=dev)
+        kw["q_pos"] = torch.randint(0, 40, (rows,), generator=g, device=dev, dtype=torch.int32)
+        kw["k_pos"] = torch.arange(n, device=dev, dtype=torch.int32) // 510
+    ws = torch.full((mh.flash_attn_128_workspace_bytes(q, k, v),), 0xff, dtype=torch.uint8, device=dev)
+    out = mh.flash_attn_128(q, k, v, workspace=ws, **kw)
+    ws.fill_(0xff)
+    assert torch.equal(mh.flash_attn_128(q, k, v, workspace=ws, **kw), out)
+    for h in range(0, heads, heads // 4):
+        j = h // (heads // kv_heads)
+        part = {**kw, **({"slopes": kw["slopes"][h:h + 1]} if bias else {})}
+        check(out[h:h + 1], *attention64(q[h:h + 1], k[j:j + 1], v[j:j + 1], **part), f"head {h}")
+
+
+def test_streams_that_change_under_a_graph(dev):
+    """One captured call, replayed for one stream and for many: each replay takes the kernel of its own ranges."""
+    g = torch.Generator(device=dev).manual_seed(77)
+    rows, n = 28, 100000
+    q, k, v = make(g, 40, rows, dev), make(g, 8, n, dev), make(g, 8, n, dev)
+    ranges = torch.zeros((rows, 2), dtype=torch.int32, device=dev)
+    run = lambda: mh.flash_attn_128(q, k, v, ranges=ranges)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for docs in (1, 28, 2, 0, 7):
+        ranges.zero_()
+        if docs:
+            lo = torch.arange(rows, device=dev) * docs // rows * (n // docs)
+            ranges.copy_(torch.stack([lo, lo + n // docs], 1))
+        graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        check(out[:1], *attention64(q[:1], k[:1], v[:1], ranges=ranges), f"{docs} streams")
