@@ -238,7 +238,8 @@ struct WaveRows {
     float q_rel;                // BIAS: their difference, if q_near: it is under 2^23 in all of the wave's rows
     bool q_near;                // (and the slope in units of a score ordinary)
     float slope_unit;
-    // Whether some row's range does not cover the tile at key t0.
+    // Whether the wave has work in the tile at key t0, and whether some row's range does not cover it.
+    __device__ __forceinline__ bool meets(uint32_t t0) const { return t0 < any_hi && t0 + 64u > any_lo; }
     __device__ __forceinline__ bool masks(uint32_t t0) const { return t0 < all_lo || t0 + 64u > all_hi; }
 };
 
@@ -329,15 +330,18 @@ __device__ __forceinline__ floatx4_t near_four(const float* near_pos, int g, uin
 __device__ __forceinline__ void bias_scores_far(const DenseParams& p, const WaveRows& w, floatx16 (&s)[2], float unit,
                                                 uint32_t t0, const int32_t* kp, uint32_t lane)
 {
+    const uint32_t given = p.k_pos ? ~0u : 0u; // no branch a score
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const uint32_t key = 32u * b + 8u * (i >> 2) + 4u * (lane >> 5) + (i & 3);
-            const int32_t pos = p.k_pos ? kp[key] : int32_t(t0 + key);
+            const int32_t pos = int32_t((uint32_t(kp[key]) & given) | ((t0 + key) & ~given));
             // The distance of two int32 positions fits 32 bits without a sign.
             const uint32_t d = w.q_pos > pos ? uint32_t(w.q_pos) - uint32_t(pos) : uint32_t(pos) - uint32_t(w.q_pos);
             s[b][i] = fmaf(s[b][i], unit, -w.slope_log2 * float(d));
+            if (i % 4 == 3)
+                __builtin_amdgcn_sched_barrier(0); // four positions' registers at a time
         }
 }
 
@@ -430,6 +434,8 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         s[g >> 2][4 * (g & 3) + e] = less_bias(w, s[g >> 2][4 * (g & 3) + e], w.slope_unit, key[e]);
+                    if (g % 2)
+                        __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
@@ -450,7 +456,7 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
     // that, and the old maximum serves. That spares the search for the new one in a phase whose vector instructions take 7
     // clocks each beside the other group's MFMAs. At most one more pass with the maxima brought up to date.
     float m_ref = w.m_run, sum;
-    bool update = MASKED || !w.settled;
+    bool update = !w.settled;
 #pragma unroll 1
     for (;;) {
         if (update) {
@@ -880,10 +886,11 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Pai
     int32_t pos = 0;
     if (kSloped)
         pos = feed.positions(t)[lane], pos = p.k_pos ? pos : int32_t(t0 + lane);
-    const bool near = tile_products<!MASKED, kSloped>(w, s, pt, frag, rd, feed.k_tile(t), feed.v_tile(t - 1u), pos,
-                                                      near_pos, lane);
+    bool near = false;
+    if (!MASKED || w.meets(t0))
+        near = tile_products<!MASKED, kSloped>(w, s, pt, frag, rd, feed.k_tile(t), feed.v_tile(t - 1u), pos, near_pos, lane);
     if (MASKED) {
-        if (t > 0)
+        if (t > 0 && w.meets(BIAS ? t0 + 64u : t0 - 64u))
             masked_output(w, pt, frag, rd, feed.v_tile(t - 1u), BIAS ? t0 + 64u : t0 - 64u,
                           checked ? odd + kPairWaves * ((t - 1u) % 2u) : nullptr, scratch, lane);
         // The part of V that this wave loaded: every wave's word is read at the next products, a barrier on.
@@ -898,7 +905,8 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Pai
     // t + 2 into that of tile t - 2 (among the products they cost 10%: this phase is the shorter one).
     feed.k();
     feed.v();
-    tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, feed.positions(t), near_pos, kSloped, near, lane);
+    if (!MASKED || w.meets(t0))
+        tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, feed.positions(t), near_pos, kSloped, near, lane);
     // Past the last tile these are some tile's again, and not used.
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
@@ -1012,7 +1020,9 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
         pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, odd, t > b || a == b, wave, t, key_of(t),
                                     lane);
     const uint32_t end = tiles - 1u;
-    if (b < tiles || a == tiles) // the last turn was of the masked form
+    if (!w.meets(key_of(end)))
+        ; // nothing of it is this wave's
+    else if (b < tiles || a == tiles) // the last turn was of the masked form
         masked_output(w, pt, frag, rd, feed.v_tile(end), key_of(end), odd + kPairWaves * (end % 2u), scratch, lane);
     else
         tile_output(w, pt, frag, rd, feed.v_tile(end));
