@@ -17,16 +17,16 @@
 // - A masked probability is a zero, and zero times an infinite or NaN value of V would still be NaN in the rows that do
 //   not attend it: masked tiles are searched for such values, and where there are any the matrix cores take zeros for
 //   them, and they are added one key at a time to the rows that attend it. (All tiles masked, 40 heads, 14,080 rows on
-//   11,264 keys: 4.25 ms, and 2.81 ms with none masked.)
+//   11,264 keys: 3.73 ms, and 2.73 ms with none masked.)
 // - Softmax in base 2. A row's running maximum is brought up to date only when a tile's probabilities sum up to more than
 //   2^10 in a lane, so P stays below 2^10 and most tiles neither search a maximum nor rescale O. P rounds to bf16 for the
 //   matrix cores (2^-9 of each probability, below the output's own rounding); maxima, sums and O are float.
 // - Few rows leave the chip idle: their keys are then split over workgroups, each leaves its part of O, the maximum and the
 //   sum in the workspace, and a second kernel joins them in a fixed order.
-// What bounds it: many rows, the chip's power (960 x 544, 56 heads, 19,305 rows: 9.1 .. 9.3 ms, 1150 .. 1180 TFLOP/s, the
-// clock at 1.7 GHz and the matrix cores busy 68% of it); under a cap the vector unit (five more operations a score, two
+// What bounds it: many rows, the chip's power (960 x 544, 56 heads, 19,305 rows: 8.9 .. 9.3 ms, 1150 .. 1200 TFLOP/s, the
+// clock at 1.7 GHz and the matrix cores busy 69% of it); under a cap the vector unit (five more operations a score, two
 // of them transcendental: 14,925 rows of 40 heads 5.0 ms, without one 4.1); few rows, the one pass over K and V (129,536
-// keys of 8 heads in 105 us, 5.0 TB/s).
+// keys of 8 heads in 95 us, 5.5 TB/s).
 #include "mh3_common.hpp"
 
 #include <algorithm>
@@ -151,7 +151,7 @@ __device__ __forceinline__ void range_of(const DenseParams& p, uint32_t f, uint3
 }
 
 // Whether attn_few_kernel has less to do than attn_pair_kernel, from the key tiles that the rows of each one's workgroups
-// span: in tenths of a us, a workgroup's start and its turns (plan_of's figures, and 2.3 and 2.8 us a turn of eight waves
+// span: in tenths of a us, a workgroup's start and its turns (plan_of's figures, and 2.0 and 2.8 us a turn of eight waves
 // and of one whose rows do not attend the same keys), of the longest workgroup or of all of them over the CUs. Integers, so that both
 // kernels find the same. A lane takes a tile of 32 rows, eight of them are a tile of 256.
 __device__ __forceinline__ bool few_has_less(const DenseParams& p, uint32_t lane)
@@ -179,7 +179,7 @@ __device__ __forceinline__ bool few_has_less(const DenseParams& p, uint32_t lane
             all_lo = max(all_lo, uint32_t(__shfl_xor(int(all_lo), d, kWave)));
             all_hi = min(all_hi, uint32_t(__shfl_xor(int(all_hi), d, kWave)));
         }
-        const uint32_t pair = (lane & 7u) == 0u && lo < hi ? (hi - lo + 63u) / 64u * (alike() ? 15u : 23u) : 0u;
+        const uint32_t pair = (lane & 7u) == 0u && lo < hi ? (hi - lo + 63u) / 64u * (alike() ? 15u : 20u) : 0u;
         few_max = max(few_max, wave_max_u32(few)), pair_max = max(pair_max, wave_max_u32(pair));
         for (uint32_t i = 0; i < 64u; ++i)
             few_sum += uint32_t(__builtin_amdgcn_readlane(int(few), int(i)));
@@ -1177,9 +1177,10 @@ Plan plan_of(const MH3DenseAttnArgs& a, uint32_t waves)
 // workgroup of eight waves spans several and walks all of their keys with most of its waves idle; or of one, where it
 // reads K and V once for more rows. So that is decided on the device (few_has_less; contest), where a call is long
 // enough for the second launch and the look at the ranges, some 6 us. One-wave workgroups then take more splits, as those
-// that span two documents are longer than the others, where there are many (4 x 28 rows below: 7 splits 422, 14 300). Heads, documents, query rows of each, keys in all,
-// eight waves and one at their best splits (us): 40 on 8, 64 x 1, 129,536 207 and 112; 3 x 4, 129,536 184 and 105; 1 x 28,
-// 116,105 118 and 150; 56 on 8, 1 x 64, 100,000 212 and 329; 2 x 64, 100,000 348 and 337; 40, 4 x 64, 20,000 183 and 105.
+// that span two documents are longer than the others, where there are many (4 x 28 rows below: 7 splits 422, 14 282). Heads, documents, query rows of each, keys in all,
+// eight waves and one at their best splits (us): 40 on 8, 64 x 1, 129,536 162 and 107; 3 x 4, 129,536 139 and 99; 1 x 28,
+// 116,105 118 and 152; 4 x 28 227 and 267; 56 on 8, 1 x 64, 100,000 198 and 335; 2 x 64 314 and 341; 40, 4 x 64, 20,000
+// 136 and 102; 56, 5 x 18, 63,257 484 and 429.
 struct Plans {
     Plan first, second;
     uint64_t list;
