@@ -393,14 +393,16 @@ int launch_few(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* xs, const 
 }
 
 // The kernels by their tiles: rows, and rows of w.
-enum Mx4Tile { kFew, k64x128, k128x128, k192x256, k256x256 };
+enum Mx4Tile { kFew, k64x64, k64x128, k128x128, k192x256, k256x256 };
 
 // The kernel of least estimated time (us), from the sizes alone. A tile kernel: rounds of the 256 CUs, each the K-steps'
-// time in one tile; measured on one round of 21 .. 56 steps, 0.45 .. 0.55, 0.70 .. 0.75, 1.4 .. 1.6 and 1.6 .. 1.9 us a step.
+// time in one tile; measured on one round of 21 .. 56 steps, 0.34, 0.45 .. 0.55, 0.70 .. 0.75, 1.4 .. 1.6 and 1.6 .. 1.9 us
+// a step (64 x 64 to 256 x 256).
 // The few-row kernel: its bytes, x's from the caches, at the rate that either reads w from memory with.
-// At n 5376, k 14336, rows 1, 32, 128, 512, 1024: few 11.3, 17.0, -; 64 x 128 26, 28, 31, 56, 83; 128 x 128 -, -, 42, 41,
-// 80; 192 x 256 -, -, 84, 86, 84; 256 x 256 -, -, 90, 98, 97. At n 21504, k 5376, rows 1, 64, 192, 945: few 13.1, -; 64 x
-// 128 14.0, 16.6, 27.9; 128 x 128 -, 18.5, 35.4; 192 x 256 -, 33, 38, 77; 256 x 256 -, 36, 39, 87.
+// At n 5376, k 14336, rows 1, 32, 128, 512, 1024: few 11.3, 17.0, -; 64 x 64 -, 21.7, 22.6, 51, -; 64 x 128 26, 28, 31, 56,
+// 83; 128 x 128 -, -, 42, 41, 80; 192 x 256 -, -, 84, 86, 84; 256 x 256 -, -, 90, 98, 97. At n 21504, k 5376, rows 1, 64,
+// 192, 945: few 13.1, -; 64 x 64 -, 19.1, 30.5; 64 x 128 14.0, 16.6, 27.9; 128 x 128 -, 18.5, 35.4; 192 x 256 -, 33, 38,
+// 77; 256 x 256 -, 36, 39, 87. (A tile's K-steps split over two groups of waves: 43 for 31 at 128 rows of the first.)
 Mx4Tile tile_of_sizes(uint32_t m, uint32_t w_rows, uint32_t k)
 {
     const float steps = float(k / 256u), kStart = 4.0f, kRate = 6.2e6f; // bytes a us
@@ -411,7 +413,8 @@ Mx4Tile tile_of_sizes(uint32_t m, uint32_t w_rows, uint32_t k)
         float step_us;
     };
     constexpr Tile kTiles[] = {
-        {k256x256, 256, 256, 1.75f}, {k192x256, 192, 256, 1.5f}, {k128x128, 128, 128, 0.73f}, {k64x128, 64, 128, 0.48f}};
+        {k256x256, 256, 256, 1.75f}, {k192x256, 192, 256, 1.5f}, {k128x128, 128, 128, 0.73f}, {k64x128, 64, 128, 0.48f},
+        {k64x64, 64, 64, 0.35f}};
     Mx4Tile best = k256x256;
     float least = INFINITY;
     for (const Tile& t : kTiles) {
@@ -468,6 +471,8 @@ int launch_mx4(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* xs, const 
     case kFew:
         return a->m <= 16u ? launch_few<1, EPI>(a, x, xs, w, ws, out, gg, stream)
                            : launch_few<2, EPI>(a, x, xs, w, ws, out, gg, stream);
+    case k64x64:
+        return launch_tile<64, 32, 2, 2, 4, EPI>(a, x, xs, w, ws, out, gg, stream);
     case k64x128:
         return launch_tile<64, 64, 2, 4, 4, EPI>(a, x, xs, w, ws, out, gg, stream);
     case k128x128:

@@ -143,7 +143,7 @@ def test_gemm_gate_add(dev, m, n, k, sets, dtype):
     assert bool(((got.double() - want).abs() <= unit * want.abs() + gate.abs() * (tol + 2.0 ** -24 * y.abs())).all())
 
 
-@pytest.mark.parametrize("m,n", [(1, 20480), (32, 16384), (33, 16384), (63, 512), (300, 10240), (383, 10240), (577, 16384),
+@pytest.mark.parametrize("m,n", [(1, 20480), (32, 16384), (33, 16384), (33, 20480), (63, 512), (300, 10240), (383, 10240), (577, 16384),
                                  (769, 16384), (1024, 16384), (1025, 512)])
 def test_every_kernel_with_every_epilogue(dev, m, n):
     """Sizes that take each of the kernels (few rows, tiles of 64, 128, 192 and 256 rows), with whole and cut tiles."""
