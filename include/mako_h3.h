@@ -358,8 +358,8 @@ typedef struct MH3DenseAttnArgs {
     uint32_t head_dim; /* 128 */
     uint32_t q_rows;   /* 0: nothing is done */
     uint32_t kv_rows;  /* 0: every row is zero */
-    float scale;       /* score scale; 0 means 1 / sqrt(128) */
-    float cap;         /* tanh cap; 0: none */
+    float scale;       /* score scale, up to 2^100; 0 means 1 / sqrt(128) */
+    float cap;         /* tanh cap, 2^-60 .. 1024; 0: none */
     uint32_t reserved;
     uint64_t q_head_stride, q_row_stride, k_head_stride, k_row_stride;
     uint64_t v_head_stride, v_row_stride, out_head_stride, out_row_stride;

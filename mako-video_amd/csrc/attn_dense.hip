@@ -152,8 +152,8 @@ __device__ __forceinline__ void range_of(const DenseParams& p, uint32_t f, uint3
 
 // Whether attn_few_kernel has less to do than attn_pair_kernel, from the key tiles that the rows of each one's workgroups
 // span: in tenths of a us, a workgroup's start and its turns (plan_of's figures, and 2.0 and 2.8 us a turn of eight waves
-// and of one whose rows do not attend the same keys), of the longest workgroup or of all of them over the CUs. Integers, so that both
-// kernels find the same. A lane takes a tile of 32 rows, eight of them are a tile of 256.
+// and of one whose rows do not attend the same keys), of the longest workgroup or of all of them over the CUs. Integers,
+// so that both kernels find the same. A lane takes a tile of 32 rows, eight of them are a tile of 256.
 __device__ __forceinline__ bool few_has_less(const DenseParams& p, uint32_t lane)
 {
     uint32_t few_max = 0, pair_max = 0;
@@ -314,7 +314,7 @@ __device__ __forceinline__ bool near_positions(const WaveRows& w, int32_t pos, f
     return near;
 }
 
-// The bias off the scores, from near_positions: key is the first of the four positions that x's belong to.
+// The bias off a score, from its key's position as near_positions leaves it.
 __device__ __forceinline__ float less_bias(const WaveRows& w, float x, float slope_unit, float key)
 {
     return fmaf(-slope_unit, fabsf(w.q_rel - key), x);
@@ -1219,7 +1219,8 @@ int check_args(const MH3DenseAttnArgs* args)
         return MH3_ERR_SHAPE;
     if (a.head_dim != 128)
         return MH3_ERR_UNSUPPORTED;
-    if (!(a.scale >= 0.0f) || a.scale == __builtin_inff() || !(a.cap >= 0.0f) || a.cap == __builtin_inff())
+    // The factors made of them stay ordinary floats, and the capped scores' error (2^-23 of the cap) below bf16's.
+    if (!(a.scale >= 0.0f && a.scale <= 0x1p100f) || !(a.cap == 0.0f || (a.cap >= 0x1p-60f && a.cap <= 1024.0f)))
         return MH3_ERR_PARAM;
     if (a.heads > 4096u || a.q_rows >= (1u << 30) || a.kv_rows >= (1u << 30) ||
         uint64_t(a.q_rows) * (a.heads / a.kv_heads) >= (1u << 30))

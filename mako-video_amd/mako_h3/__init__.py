@@ -801,7 +801,7 @@ def flash_attn_128_workspace_bytes(q, k, v, *, layout="heads") -> int:
 def flash_attn_128(q, k, v, *, ranges=None, scale=0.0, cap=0.0, slopes=None, q_pos=None, k_pos=None, layout="heads",
                    out=None, out_layout=None, workspace=None):
     """Attention over whole rows, head_dim 128, bf16: out_i = softmax_j(s_ij) v over the keys of ranges[i] (int32
-    [q_rows][2], [lo, hi); None: all), s = scale q k, under a cap cap tanh(s / cap), less slopes[h] |q_pos_i - k_pos_j|
+    [q_rows][2], [lo, hi); None: all), s = scale q k, under a cap (up to 1024) cap tanh(s / cap), less slopes[h] |q_pos_i - k_pos_j|
     (float [heads], int32 [q_rows] and [kv_rows], None: the rows' numbers). Fewer key heads than query heads are shared
     in order; scale 0 is 1 / sqrt(128); a row without keys is zero. layout "heads": [heads][rows][128], "rows":
     [rows][heads * 128] (slices of wider rows too); out_layout: out's, the same by default. `workspace` (uint8, at least

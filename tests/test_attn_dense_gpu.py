@@ -382,3 +382,15 @@ def test_streams_that_change_under_a_graph(dev):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         check(out[:1], *attention64(q[:1], k[:1], v[:1], ranges=ranges), f"{docs} streams")
+
+
+@pytest.mark.parametrize("cap,scale", [(2.0 ** -60, None), (1e-6, None), (1024.0, None), (1024.0, 3.0), (30.0, 1e-30), (0.0, 1e-40),
+                                       (0.0, 0.5)])
+def test_ends_of_the_caps_and_scales(dev, cap, scale):
+    """The whole domain of both: a cap of 1024 is off by 2^-23 of it, inside the bound's 2^-11."""
+    g = torch.Generator(device=dev).manual_seed(3)
+    q, k, v = make(g, 2, 300, dev), make(g, 2, 200, dev), make(g, 2, 200, dev)
+    q[0, 7], k[1, 5] = 0.0, 0.0
+    for rows in (300, 5):
+        kw = {"cap": cap, **({"scale": scale} if scale else {})}
+        check(mh.flash_attn_128(q[:, :rows], k, v, **kw), *attention64(q[:, :rows], k, v, **kw), f"{rows} rows")

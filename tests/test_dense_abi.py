@@ -104,7 +104,8 @@ DENSE_BAD = [({"heads": 0}, mh.ERR_SHAPE), ({"kv_heads": 0}, mh.ERR_SHAPE), ({"k
              ({"kv_heads": 16}, mh.ERR_SHAPE), ({"head_dim": 0}, mh.ERR_SHAPE), ({"head_dim": 64}, mh.ERR_UNSUPPORTED),
              ({"scale": -1.0}, mh.ERR_PARAM), ({"scale": float("nan")}, mh.ERR_PARAM),
              ({"scale": float("inf")}, mh.ERR_PARAM), ({"cap": -1.0}, mh.ERR_PARAM), ({"cap": float("nan")}, mh.ERR_PARAM),
-             ({"cap": float("inf")}, mh.ERR_PARAM), ({"heads": 8192, "kv_heads": 8192}, mh.ERR_SHAPE),
+             ({"cap": float("inf")}, mh.ERR_PARAM), ({"cap": 1025.0}, mh.ERR_PARAM), ({"cap": 1e-19}, mh.ERR_PARAM),
+             ({"scale": 2e30}, mh.ERR_PARAM), ({"heads": 8192, "kv_heads": 8192}, mh.ERR_SHAPE),
              ({"q_rows": 1 << 30}, mh.ERR_SHAPE), ({"kv_rows": 1 << 30}, mh.ERR_SHAPE),
              ({"q_rows": 1 << 28}, mh.ERR_SHAPE),  # 2^28 rows of four heads a key head
              ({"q_row_stride": 132}, mh.ERR_ALIGN), ({"k_row_stride": 120}, mh.ERR_SHAPE),
