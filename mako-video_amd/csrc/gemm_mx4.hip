@@ -9,10 +9,10 @@
 //   operand, and a K-step of 256 k is 64 MFMAs a wave (256 x 256 tiles) with four times the bf16 kernel's products.
 // - The scale bytes come eight blocks (a K-step) of all rows at a time, [k / 256][rows][8]: a tile's are then one
 //   contiguous run a K-step, 4 bytes a lane of one DMA instruction a wave, and an operand's byte is one ds_read_u8.
-// - Both operands and their scales go out together, into a ring of stages each of which holds a whole K-step; the
-//   loads of tile kt + kStages start as soon as every wave has read tile kt, behind the barrier that publishes
-//   tile kt + 1.
-// What bounds them: large products, the chip's power (19,305 x 5376 -> 2 x 14,336: 1.45 ms, 4.1 PFLOP/s, the clock at 1.6 to
+// - A ring of stages holds a whole K-step each. x's loads of tile kt + kStages start as soon as every wave has read tile
+//   kt, behind the barrier that publishes tile kt + 1; w's and the scales' with the next step's first products, since all at
+//   once held the products up behind them (256 x 256 tiles, 2985 x 5376 x 7168: 68 us, now 63 to 65).
+// What bounds them: large products, the chip's power (19,305 x 5376 -> 2 x 14,336: 1.42 ms, 4.2 PFLOP/s, the clock at 1.6 to
 // 1.9 GHz; the bare MFMA in a loop reaches 6.0 at 1.5 GHz, this kernel without its loads 4.75, and loads a tile ahead with
 // stores straight from registers, or four waves of 128 x 128, no more than it does now); middle ones the rounds of tiles;
 // few rows the weights' bytes (3 rows, 5376 x 14,336: 11.3 us, 41 MB at 3.6 TB/s with the launch in it).
@@ -105,11 +105,15 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx4_kernel(const uint8_t* __
         sb_off = row < 2u * BN ? wrow * 8u + (d & 1u) * 4u : kPastEnd;
     }
     constexpr int kLoads = AI + BI + 2; // a wave's loads of one K-step
-    auto issue = [&](uint32_t kt) {
+    auto issue_x = [&](uint32_t kt) {
         char* const stage = lds + (kt % S) * Ring::kStage;
 #pragma unroll
         for (int i = 0; i < AI; ++i)
             lds_dma16(ra, stage + (wave * AI + uint32_t(i)) * 1024u, a_off[i], int(kt * 128u));
+        __builtin_amdgcn_sched_barrier(0); // the waits count these loads
+    };
+    auto issue_rest = [&](uint32_t kt) {
+        char* const stage = lds + (kt % S) * Ring::kStage;
 #pragma unroll
         for (int i = 0; i < BI; ++i)
             lds_dma16(rb, stage + Ring::kA + (wave * BI + uint32_t(i)) * 1024u, b_off[i], int(kt * 128u));
@@ -117,7 +121,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx4_kernel(const uint8_t* __
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr_t)sc, 4, sa_off, int(kt * M * 8u), 0, 0);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb, (lds_ptr_t)(sc + Ring::kScale), 4, sb_off, int(kt * w_rows * 8u), 0,
                                                  0);
-        __builtin_amdgcn_sched_barrier(0); // the waits count these loads
+        __builtin_amdgcn_sched_barrier(0);
     };
 
     // Operands of sub-step ks (k-half h = ks / 2, the wave's row tiles (ks % 2) FA ..): 16 bytes a lane, row
@@ -177,22 +181,27 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx4_kernel(const uint8_t* __
     };
 
     for (uint32_t t = 0; t < uint32_t(S); ++t)
-        if (t < KT)
-            issue(t);
+        if (t < KT) {
+            issue_x(t);
+            if (t + 1u < uint32_t(S))
+                issue_rest(t); // the last stage's goes out with the first step
+        }
     if (KT >= uint32_t(S))
-        __builtin_amdgcn_s_waitcnt(waitcnt_vm((S - 1) * kLoads));
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm((S - 2) * kLoads + AI));
     else
         __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     asm volatile("" ::"s"(out), "s"(gg.gate), "s"(gg.set_of_row)); // no scalar load in flight in the loop
     lds_barrier();
     frags_a(0, 0, fa[0], sa[0]);
     frags_b(0, 0, fb[0], sb[0]);
-    // One K-step of tile kt; more: tile kt + S exists; last: there is no tile kt + 1. No branch lies between the MFMAs (the
+    // One K-step of tile kt; more: tile kt + S exists; rest: tile kt + S - 1 does; last: there is no tile kt + 1. No branch lies between the MFMAs (the
     // compiler sinks them past one, to the step's end, and then spills the operands that all wait for it).
-    auto kstep = [&](uint32_t kt, auto more, auto last) {
-        constexpr bool kMore = decltype(more)::value, kLast = decltype(last)::value;
+    auto kstep = [&](uint32_t kt, auto more, auto rest, auto last) {
+        constexpr bool kMore = decltype(more)::value, kRest = decltype(rest)::value, kLast = decltype(last)::value;
         frags_a(kt, 1, fa[1], sa[1]);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kRest)
+            issue_rest(kt + uint32_t(S) - 1u);
         mfmas(0, fa[0], sa[0], fb[0], sb[0]);
         frags_a(kt, 2, fa[0], sa[0]);
         frags_b(kt, 2, fb[1], sb[1]);
@@ -210,17 +219,21 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx4_kernel(const uint8_t* __
             frags_b(kt + 1, 0, fb[0], sb[0]);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (kMore)
-                issue(kt + uint32_t(S)); // into the stage that every wave has read
+                issue_x(kt + uint32_t(S)); // into the stage that every wave has read
         }
         __builtin_amdgcn_sched_barrier(0);
         mfmas(3, fa[1], sa[1], fb[1], sb[1]);
     };
+    using Yes = std::true_type;
+    using No = std::false_type;
     uint32_t kt = 0;
     for (; kt + uint32_t(S) < KT; ++kt)
-        kstep(kt, std::true_type{}, std::false_type{});
+        kstep(kt, Yes{}, Yes{}, No{});
+    if (KT >= uint32_t(S)) // S >= 2, so this step is not the last
+        kstep(kt++, No{}, Yes{}, No{});
     for (; kt + 1u < KT; ++kt)
-        kstep(kt, std::false_type{}, std::false_type{});
-    kstep(kt, std::false_type{}, std::true_type{});
+        kstep(kt, No{}, No{}, No{});
+    kstep(kt, No{}, No{}, Yes{});
 
     gemm_epilogue<BM, BN, WM, WN, kBf16, EPI, TM, TN>(acc, smem, M, N, m0, w_lo, w_hi, nullptr, nullptr, out, gg);
 }
