@@ -13,7 +13,7 @@
 //   kt, behind the barrier that publishes tile kt + 1; w's and the scales' with the next step's first products, since all at
 //   once held the products up behind them (256 x 256 tiles, 2985 x 5376 x 7168: 68 us, now 63 to 65).
 // What bounds them: large products, the chip's power (19,305 x 5376 -> 2 x 14,336: 1.42 ms, 4.2 PFLOP/s, the clock at 1.6 to
-// 1.9 GHz; the bare MFMA in a loop reaches 6.0 at 1.5 GHz, this kernel without its loads 4.75, and loads a tile ahead with
+// 1.8 GHz and the matrix cores busy 58% of it; the bare MFMA in a loop reaches 6.0 at 1.5 GHz, this kernel without its loads 4.75, and loads a tile ahead with
 // stores straight from registers, or four waves of 128 x 128, no more than it does now); middle ones the rounds of tiles;
 // few rows the weights' bytes (3 rows, 5376 x 14,336: 11.3 us, 41 MB at 3.6 TB/s with the launch in it).
 #include "gemm.hpp"
@@ -409,13 +409,14 @@ int launch_few(const MH3GemmArgs* a, const uint8_t* x, const uint8_t* xs, const 
 enum Mx4Tile { kFew, k64x64, k64x128, k128x128, k192x256, k256x256 };
 
 // The kernel of least estimated time (us), from the sizes alone. A tile kernel: rounds of the 256 CUs, each the K-steps'
-// time in one tile; measured on one round of 21 .. 56 steps, 0.34, 0.45 .. 0.55, 0.70 .. 0.75, 1.4 .. 1.6 and 1.6 .. 1.9 us
-// a step (64 x 64 to 256 x 256).
-// The few-row kernel: its bytes, x's from the caches, at the rate that either reads w from memory with.
-// At n 5376, k 14336, rows 1, 32, 128, 512, 1024: few 11.3, 17.0, -; 64 x 64 -, 21.7, 22.6, 51, -; 64 x 128 26, 28, 31, 56,
-// 83; 128 x 128 -, -, 42, 41, 80; 192 x 256 -, -, 84, 86, 84; 256 x 256 -, -, 90, 98, 97. At n 21504, k 5376, rows 1, 64,
-// 192, 945: few 13.1, -; 64 x 64 -, 19.1, 30.5; 64 x 128 14.0, 16.6, 27.9; 128 x 128 -, 18.5, 35.4; 192 x 256 -, 33, 38,
-// 77; 256 x 256 -, 36, 39, 87. (A tile's K-steps split over two groups of waves: 43 for 31 at 128 rows of the first.)
+// time in one tile; measured on one round of 21 .. 56 steps, 0.34, 0.45 .. 0.55, 0.68 .. 0.75, 1.4 .. 1.6 and 1.55 .. 1.8
+// us a step (64 x 64 to 256 x 256). The few-row kernel: its bytes, x's from the caches, at the rate that either reads w
+// from memory with.
+// At n 5376, k 14336, rows 1, 32, 128, 512, 1024: few 11.3, 17.1, -; 64 x 64 22.5, 22.3, 23.3, 52, 90; 64 x 128 25.8, 27.8,
+// 31, 57, 84; 128 x 128 -, -, 41, 40, 79; 192 x 256 -, -, 85, 84, 84; 256 x 256 -, -, 88, 91, 90. At n 21504, k 5376, rows
+// 1, 64, 192, 945: few 13.1, -; 64 x 64 15.8, 19.4, 31, 116; 64 x 128 14.1, 16.4, 27.6, 104; 128 x 128 -, 17.8, 33, 96;
+// 192 x 256 -, 35, 37, 80; 256 x 256 -, 37, 39, 79. (A tile's K-steps split over two groups of waves: 43 for 31 at 128 rows
+// of the first.)
 Mx4Tile tile_of_sizes(uint32_t m, uint32_t w_rows, uint32_t k)
 {
     const float steps = float(k / 256u), kStart = 4.0f, kRate = 6.2e6f; // bytes a us
@@ -426,7 +427,7 @@ Mx4Tile tile_of_sizes(uint32_t m, uint32_t w_rows, uint32_t k)
         float step_us;
     };
     constexpr Tile kTiles[] = {
-        {k256x256, 256, 256, 1.75f}, {k192x256, 192, 256, 1.5f}, {k128x128, 128, 128, 0.73f}, {k64x128, 64, 128, 0.48f},
+        {k256x256, 256, 256, 1.65f}, {k192x256, 192, 256, 1.5f}, {k128x128, 128, 128, 0.71f}, {k64x128, 64, 128, 0.48f},
         {k64x64, 64, 64, 0.35f}};
     Mx4Tile best = k256x256;
     float least = INFINITY;
