@@ -14,9 +14,9 @@
 //   kt, behind the barrier that publishes tile kt + 1; w's and the scales' with the next step's first products, since all at
 //   once held the products up behind them (256 x 256 tiles, 2985 x 5376 x 7168: 68 us, now 63 to 65).
 // What bounds them: large products, the chip's power (19,305 x 5376 -> 2 x 14,336: 1.42 ms, 4.2 PFLOP/s, the clock at 1.6 to
-// 1.8 GHz and the matrix cores busy 58% of it; the bare MFMA in a loop reaches 6.0 at 1.5 GHz, this kernel without its loads 4.75, and loads a tile ahead with
-// stores straight from registers, or four waves of 128 x 128, no more than it does now); middle ones the rounds of tiles;
-// few rows the weights' bytes (3 rows, 5376 x 14,336: 11.3 us, 41 MB at 3.6 TB/s with the launch in it).
+// 1.8 GHz and the matrix cores busy 58% of it; the bare MFMA in a loop reaches 6.0 at 1.5 GHz, this kernel without its
+// loads 4.75; loads a tile ahead with stores straight from registers, or four waves of 128 x 128, were slower); middle ones
+// the rounds of tiles; few rows the weights' bytes (3 rows, 5376 x 14,336: 11.3 us, 41 MB at 3.6 TB/s with the launch in it).
 #include "gemm.hpp"
 
 #include <algorithm>
