@@ -200,7 +200,7 @@ def _one_device(**tensors: torch.Tensor | None) -> int:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}: expected a tensor")
         index = t.get_device()
-        if index != device:
+        if index != device or index < 0:  # a host tensor's index is -1, as no device's here
             if index < 0 or not t.is_cuda:
                 raise ValueError(f"{name}: must be on the GPU")
             if device >= 0:
@@ -218,7 +218,7 @@ def _operands(*operands) -> int:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}: expected a tensor")
         index = t.get_device()
-        if index != device:
+        if index != device or index < 0:  # a host tensor's index is -1, as no device's here
             if index < 0 or not t.is_cuda:
                 raise ValueError(f"{name}: must be on the GPU")
             if device >= 0:

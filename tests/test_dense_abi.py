@@ -286,3 +286,39 @@ def test_binding_refuses_host_tensors_and_shapes():
     for call in calls:
         with pytest.raises((ValueError, RuntimeError)):
             call()
+
+
+class OnGpu(torch.Tensor):
+    """A host tensor that says that it is on a GPU."""
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+
+@pytest.mark.parametrize("place", [0, 1, 2])
+def test_a_host_tensor_among_the_operands_is_refused(place):
+    """Wherever it stands, the first included: the kernel would take its host address."""
+    host = torch.zeros(4)
+    ts = [host if i == place else torch.zeros(4).as_subclass(OnGpu) for i in range(3)]
+    with pytest.raises(ValueError, match=f"t{place}: must be on the GPU"):
+        mh._operands(*((t, f"t{i}", torch.float32, 4) for i, t in enumerate(ts)))
+    with pytest.raises(ValueError, match=f"t{place}: must be on the GPU"):
+        mh._one_device(**{f"t{i}": t for i, t in enumerate(ts)})
+    assert mh._operands(*((t, "t", torch.float32, 4) for i, t in enumerate(ts) if i != place)) == 0
+    assert mh._one_device(none=None, **{f"t{i}": t for i, t in enumerate(ts) if i != place}) == 0
+
+
+def test_host_tensors_alone_are_refused():
+    """Every operand on the host: refused by name before the library or the GPU's runtime is called."""
+    bf, i32, u8 = torch.bfloat16, torch.int32, torch.uint8
+    q, pos, off = torch.zeros((2, 5, 128), dtype=bf), torch.zeros((5, 3), dtype=i32), torch.zeros(3, dtype=i32)
+    x, xs = torch.zeros((3, 128), dtype=u8), torch.zeros((1, 3, 8), dtype=u8)
+    w, ws = torch.zeros((256, 128), dtype=u8), torch.zeros((1, 256, 8), dtype=u8)
+    for call in (lambda: mh.rotary_axes(pos, (16, 16, 16)), lambda: mh.attn_ranges(off, off, 4, 4),
+                 lambda: mh.heads_partial_axes(torch.zeros((5, 768), dtype=bf), 2, pos, (16, 16, 16)),
+                 lambda: mh.flash_attn_128(q, q, q), lambda: mh.quant_rows_mx4(torch.zeros((2, 256))),
+                 lambda: mh.gemm_mx4(x, xs, w, ws), lambda: mh.gemm_mx4_swiglu(x, xs, w, ws),
+                 lambda: mh.gemm_mx4_gate_add(x, xs, w, ws, torch.zeros((3, 256), dtype=bf), torch.zeros(256))):
+        with pytest.raises(ValueError, match="must be on the GPU"):
+            call()
