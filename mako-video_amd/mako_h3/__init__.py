@@ -300,6 +300,8 @@ def _set_stride(t: torch.Tensor, name: str, dim: int, n_sets: int) -> int:
         sets *= n
     if sets < n_sets:
         raise ValueError(f"{name}: {sets} sets, the call uses {n_sets}")
+    if n_sets > 1 and lead[-1][1] == 0:  # a broadcast vector; a stride of 0 means dim to the library
+        raise ValueError(f"{name}: its sets lie over each other")
     return lead[-1][1] if lead else dim
 
 

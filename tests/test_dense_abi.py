@@ -322,3 +322,19 @@ def test_host_tensors_alone_are_refused():
                  lambda: mh.gemm_mx4_gate_add(x, xs, w, ws, torch.zeros((3, 256), dtype=bf), torch.zeros(256))):
         with pytest.raises(ValueError, match="must be on the GPU"):
             call()
+
+
+class OnGpuTable(OnGpu):
+    device = torch.device("cuda", 0)
+
+
+def test_sets_that_are_one_vector_expanded_are_refused():
+    """A broadcast gate has a stride of zero, which to the library means the sets lie one behind the other: it would read
+    past the one vector that there is. A call of one set reads that vector alone."""
+    one = torch.zeros((1, 256)).as_subclass(OnGpuTable)
+    for gate in (one.expand(3, 256), one[0].expand(3, 256), one.expand(2, 3, 256)):
+        with pytest.raises(ValueError, match="gate: its sets lie over each other"):
+            mh._set_stride(gate, "gate", 256, 3)
+        assert mh._set_stride(gate, "gate", 256, 1) in (0, 256)
+    table = torch.zeros((3, 6, 256)).as_subclass(OnGpuTable)
+    assert mh._set_stride(table[:, 2], "gate", 256, 3) == 6 * 256
