@@ -465,7 +465,7 @@ int mh3_gemm_gate_add_f32(const MH3GemmArgs* args, uint32_t form, const void* x,
  *   q:     uint8 [rows][cols / 2], two values a byte, the lower column in the low half: bit 3 of a value its sign, bits
  *          2..0 the magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6;
  *   scale: uint8 [cols / 256][rows][8]: byte (c / 8, r, c % 8) scales columns 32 c .. 32 c + 31 of row r by
- *          2^(byte - 127); 255 makes them NaN.
+ *          2^(byte - 127); 255 makes them NaN. `rows` is the matrix's own: a slice of its rows is no prefix of the scales.
  * mh3_quant_rows_mx4: w (float or bf16, `dtype`) to that form. A block's exponent is floor(log2(max |block|)) - 2, at
  * least -127 (an all-zero block: -127), its values are rounded to nearest, ties to the even code, and saturate at 6; a
  * block with an infinity or a NaN gets scale 255. cols % 256 == 0; 16-byte aligned pointers; q and scale may not overlap

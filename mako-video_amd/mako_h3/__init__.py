@@ -1028,6 +1028,15 @@ def _gemm_ref(m, n, k, n_sets=0, gate_stride=0):
     return C.byref(a)
 
 
+def _scale_bytes(t, name, rows, cols) -> None:
+    """A matrix's scales lie [cols / 256][rows][8], so those of more or fewer rows are others from the second 256 columns
+    on: the tensor has that shape, or (not of three dimensions) just as many bytes."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor")
+    if t.shape != (cols // 256, rows, 8) and (t.dim() == 3 or t.numel() != rows * cols // 32):
+        raise ValueError(f"{name}: {tuple(t.shape)}, the scales of {rows} rows of {cols} are {(cols // 256, rows, 8)}")
+
+
 def quant_rows_mx4(w, *, q=None, scale=None):
     """Each row to 4-bit floats in blocks of 32 columns that share a power of two (OCP MX: e2m1, E8M0): w f32 or bf16
     [rows][cols], cols % 256 == 0 -> (q uint8 [rows][cols / 2], the lower column in a byte's low half; scale uint8
@@ -1037,7 +1046,10 @@ def quant_rows_mx4(w, *, q=None, scale=None):
     rows, cols = w.shape
     ref = _quant_ref(rows, cols, _dt(w))
     q = torch.empty((rows, cols // 2), dtype=torch.uint8, device=w.device) if q is None else q
-    scale = torch.empty((cols // 256, rows, 8), dtype=torch.uint8, device=w.device) if scale is None else scale
+    if scale is None:
+        scale = torch.empty((cols // 256, rows, 8), dtype=torch.uint8, device=w.device)
+    else:
+        _scale_bytes(scale, "scale", rows, cols)
     n = rows * cols
     device = _operands((w, "w", w.dtype, n), (q, "q", torch.uint8, n // 2), (scale, "scale", torch.uint8, n // 32))
     _on(device, "quant_rows_mx4", lib.mh3_quant_rows_mx4, ref, w.data_ptr(), q.data_ptr(), scale.data_ptr())
@@ -1045,18 +1057,21 @@ def quant_rows_mx4(w, *, q=None, scale=None):
 
 
 def _mx4(x, x_scale, w, w_scale):
-    """(m, rows of w, k, operands) of a product of 4-bit matrices."""
+    """(m, rows of w, k, operands) of a product of 4-bit matrices, each with scales of its own rows."""
     if x.dim() != 2 or w.dim() != 2 or w.shape[1] != x.shape[1]:
         raise ValueError("x must be [m][k / 2] and w [n][k / 2]")
     m, half = x.shape
     n = w.shape[0]
+    _scale_bytes(x_scale, "x_scale", m, 2 * half)
+    _scale_bytes(w_scale, "w_scale", n, 2 * half)
     u8 = torch.uint8
     return m, n, 2 * half, ((x, "x", u8, m * half), (x_scale, "x_scale", u8, m * half // 16), (w, "w", u8, n * half),
                             (w_scale, "w_scale", u8, n * half // 16))
 
 
 def gemm_mx4(x, x_scale, w, w_scale, *, out=None):
-    """out = x w^T of two matrices as quant_rows_mx4 leaves them (x [m][k], w [n][k]), bf16 [m][n]."""
+    """out = x w^T of two matrices as quant_rows_mx4 leaves them (x [m][k], w [n][k]), bf16 [m][n]. A slice of rows takes
+    its own scales, x_scale[:, a:b].contiguous(): those of all rows are refused."""
     m, n, k, operands = _mx4(x, x_scale, w, w_scale)
     out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device) if out is None else out
     device = _operands(*operands, (out, "out", torch.bfloat16, m * n))

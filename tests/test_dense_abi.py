@@ -338,3 +338,32 @@ def test_sets_that_are_one_vector_expanded_are_refused():
         assert mh._set_stride(gate, "gate", 256, 1) in (0, 256)
     table = torch.zeros((3, 6, 256)).as_subclass(OnGpuTable)
     assert mh._set_stride(table[:, 2], "gate", 256, 3) == 6 * 256
+
+def test_scales_of_other_rows_are_refused():
+    """A scale buffer of more rows than its matrix holds other blocks' bytes from the second 256 columns on. The shapes are
+    looked at before the device, so host tensors show it."""
+    u8 = torch.uint8
+    m, n, k = 3, 256, 512
+    x, w = torch.zeros((m, k // 2), dtype=u8), torch.zeros((n, k // 2), dtype=u8)
+    xs, ws = torch.zeros((k // 256, m, 8), dtype=u8), torch.zeros((k // 256, n, 8), dtype=u8)
+    more_x, more_w = torch.zeros((k // 256, m + 1, 8), dtype=u8), torch.zeros((k // 256, 2 * n, 8), dtype=u8)
+    res, gate = torch.zeros((m, n), dtype=torch.bfloat16), torch.zeros((1, n))
+    ops = [lambda a, b: mh.gemm_mx4(x, a, w, b), lambda a, b: mh.gemm_mx4_swiglu(x, a, w, b),
+           lambda a, b: mh.gemm_mx4_gate_add(x, a, w, b, res, gate)]
+    for op in ops:
+        for bad in (more_x, more_x.flatten(), xs.flatten()[:-8], xs.view(m, k // 256, 8), torch.zeros((1, 2 * m, 8), dtype=u8)):
+            with pytest.raises(ValueError, match="x_scale: .*the scales of 3 rows of 512"):
+                op(bad, ws)
+        for bad in (more_w, more_w.flatten(), ws[:, :-1]):
+            with pytest.raises(ValueError, match="w_scale: .*the scales of 256 rows of 512"):
+                op(xs, bad)
+        for good in ((xs, ws), (xs.flatten(), ws.flatten())):
+            with pytest.raises(ValueError, match="must be on the GPU"):
+                op(*good)
+    v = torch.zeros((m, k))
+    for bad in (more_x, more_x.flatten(), xs[:, :2]):
+        with pytest.raises(ValueError, match="scale: .*the scales of 3 rows of 512"):
+            mh.quant_rows_mx4(v, scale=bad)
+    for good in (xs, xs.flatten()):
+        with pytest.raises(ValueError, match="must be on the GPU"):
+            mh.quant_rows_mx4(v, scale=good)
