@@ -31,6 +31,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 namespace mh3 {
 namespace {
@@ -1219,7 +1220,8 @@ int check_args(const MH3DenseAttnArgs* args)
         return MH3_ERR_SHAPE;
     if (a.head_dim != 128)
         return MH3_ERR_UNSUPPORTED;
-    // The factors made of them stay ordinary floats, and the capped scores' error (2^-23 of the cap) below bf16's.
+    // The factors made of them stay ordinary floats (cap_in where it is made), and the capped scores' error (2^-23 of the
+    // cap) below bf16's.
     if (!(a.scale >= 0.0f && a.scale <= 0x1p100f) || !(a.cap == 0.0f || (a.cap >= 0x1p-60f && a.cap <= 1024.0f)))
         return MH3_ERR_PARAM;
     if (a.heads > 4096u || a.q_rows >= (1u << 30) || a.kv_rows >= (1u << 30) ||
@@ -1325,8 +1327,11 @@ extern "C" int mh3_flash_attn_128(const MH3DenseAttnArgs* args, const uint16_t* 
     pow = std::min(std::max(pow, -16), 0);
     p.q_pow = std::ldexp(1.0f, pow);
     p.scale_log2 = scale / p.q_pow * kLog2e;
+    // cap_in stays finite, for scores of zero to stay that. It leaves a float's range only where the cap is below 2^-26: no
+    // score is then more than that from zero, whatever its product, and the probabilities are equal in float.
     if (a.cap > 0.0f)
-        p.cap_in = 2.0f * kLog2e * (scale / p.q_pow) / a.cap, p.cap_out = a.cap * kLog2e;
+        p.cap_in = std::min(2.0f * kLog2e * (scale / p.q_pow) / a.cap, std::numeric_limits<float>::max()),
+        p.cap_out = a.cap * kLog2e;
     const bool contest = plans.contest && ranges;
     if (contest) {
         const bool pair_first = plans.first.waves == kPairWaves;

@@ -394,3 +394,17 @@ def test_ends_of_the_caps_and_scales(dev, cap, scale):
     for rows in (300, 5):
         kw = {"cap": cap, **({"scale": scale} if scale else {})}
         check(mh.flash_attn_128(q[:, :rows], k, v, **kw), *attention64(q[:, :rows], k, v, **kw), f"{rows} rows")
+
+
+@pytest.mark.parametrize("rows", [300, 5])
+@pytest.mark.parametrize("cap,scale", [(2.0 ** -60, 2.0 ** 100), (2.0 ** -60, 2.0 ** 67), (1e-9, 2.0 ** 100), (1024.0, 2.0 ** 100),
+                                       (0.0, 2.0 ** 100)])
+def test_the_largest_scales_under_caps(dev, rows, cap, scale):
+    """scale / cap beyond what a float holds: a dot product of zero is still a score of zero, others are at the cap."""
+    g = torch.Generator(device=dev).manual_seed(4)
+    q, k, v = make(g, 2, rows, dev), make(g, 2, 200, dev), make(g, 2, 200, dev)
+    q[0, 3], q[1], k[:, 7], k[1, 150:] = 0.0, 0.0, 0.0, 0.0
+    kw = {"cap": cap, "scale": scale}
+    check(mh.flash_attn_128(q, k, v, **kw), *attention64(q, k, v, **kw))
+    kw["ranges"] = random_ranges(g, rows, 200, dev)
+    check(mh.flash_attn_128(q, k, v, **kw), *attention64(q, k, v, **kw))
