@@ -372,10 +372,11 @@ int mh3_flash_attn_128(const MH3DenseAttnArgs* args, const uint16_t* q, const ui
  * first query and key rows and their ends: query rows q_off[d] .. q_off[d + 1] - 1 attend keys k_off[d] .. k_off[d + 1]
  * - 1; rows of no document attend none. With causal 1 a document's last query row sits on its last key row and a row
  * attends the keys up to its own, and the first prefix[d] of its document in any case (prefix int32 [docs], or NULL: no
- * prefix; only with causal). ranges is int32 [q_rows][2], 8-byte aligned; it may not overlap an input (MH3_ERR_PARAM). */
+ * prefix; only with causal). Offsets may lie before the first key and past the last: of the ranges that they give, what
+ * lies in [0, kv_rows) remains. ranges is int32 [q_rows][2], 8-byte aligned; it may not overlap an input (MH3_ERR_PARAM). */
 typedef struct MH3RangeArgs {
     uint32_t q_rows;
-    uint32_t kv_rows; /* the ranges are clamped to [0, kv_rows] */
+    uint32_t kv_rows; /* the ranges are cut off at 0 and kv_rows */
     uint32_t docs;    /* >= 1 */
     uint32_t causal;  /* 0 or 1 */
 } MH3RangeArgs;

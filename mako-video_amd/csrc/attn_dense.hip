@@ -1118,15 +1118,16 @@ __global__ __launch_bounds__(256) void attn_ranges_kernel(RangeParams p)
     }
     int2 r{0, 0};
     if (a < p.docs && p.q_off[a] <= int32_t(i)) {
-        const int32_t n = int32_t(p.kv_rows);
-        const int32_t lo = min(max(p.k_off[a], 0), n), end = min(max(p.k_off[a + 1u], lo), n);
-        int32_t hi = end;
+        // Diagonal and prefix lie where the offsets say, wherever the keys end: the result is what is cut off.
+        const int64_t start = p.k_off[a], end = p.k_off[a + 1u], n = p.kv_rows;
+        int64_t hi = end;
         if (p.causal) {
-            const int64_t own = int64_t(end) - p.q_off[a + 1u] + i; // the last query row sits on the last key row
-            const int64_t seen = int64_t(lo) + (p.prefix ? max(p.prefix[a], 0) : 0);
-            hi = int32_t(max(int64_t(lo), min(int64_t(end), max(own + 1, seen))));
+            const int64_t own = end - p.q_off[a + 1u] + i; // the last query row sits on the last key row
+            const int64_t seen = start + (p.prefix ? max(p.prefix[a], 0) : 0);
+            hi = min(end, max(own + 1, seen));
         }
-        r = int2{lo, hi};
+        const int64_t lo = min(max(start, int64_t(0)), n);
+        r = int2{int32_t(lo), int32_t(min(max(hi, lo), n))};
     }
     p.ranges[i] = r;
 }

@@ -408,3 +408,25 @@ def test_the_largest_scales_under_caps(dev, rows, cap, scale):
     check(mh.flash_attn_128(q, k, v, **kw), *attention64(q, k, v, **kw))
     kw["ranges"] = random_ranges(g, rows, 200, dev)
     check(mh.flash_attn_128(q, k, v, **kw), *attention64(q, k, v, **kw))
+
+
+@pytest.mark.parametrize("causal,prefix", [(False, None), (True, None), (True, [30, 0]), (True, [-5, 1 << 30])])
+@pytest.mark.parametrize("k_cuts,keys", [([0, 100, 180], 90), ([-20, 40, 130], 90), ([-50, -10, 20], 200), ([5, 300, 310], 100),
+                                         ([120, 150, 200], 100), ([-(1 << 31), 0, (1 << 31) - 1], 50), ([0, 60, 130], 130)])
+def test_documents_that_the_keys_cut_off(dev, k_cuts, keys, causal, prefix):
+    """Offsets before the first key and past the last: the documents' rows, diagonals and prefixes lie where the offsets say,
+    and of the resulting ranges what the keys hold remains."""
+    q_cuts = [4, 64, 131]
+    rows = 140
+    off = lambda c: torch.tensor(c, dtype=torch.int64, device=dev).int()  # noqa: E731
+    got = mh.attn_ranges(off(q_cuts), off(k_cuts), rows, keys, causal=causal, prefix=None if prefix is None else off(prefix))
+    want = torch.zeros((rows, 2), dtype=torch.int64)
+    for d in range(2):
+        start, end = k_cuts[d], k_cuts[d + 1]
+        for i in range(q_cuts[d], q_cuts[d + 1]):
+            hi = end
+            if causal:
+                hi = min(end, max(end - q_cuts[d + 1] + i + 1, start + max(prefix[d] if prefix else 0, 0)))
+            lo = min(max(start, 0), keys)
+            want[i] = torch.tensor([lo, min(max(hi, lo), keys)])
+    assert torch.equal(got.cpu().long(), want)
