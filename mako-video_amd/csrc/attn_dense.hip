@@ -1179,10 +1179,14 @@ Plan plan_of(const MH3DenseAttnArgs& a, uint32_t waves)
 // workgroup of eight waves spans several and walks all of their keys with most of its waves idle; or of one, where it
 // reads K and V once for more rows. So that is decided on the device (few_has_less; contest), where a call is long
 // enough for the second launch and the look at the ranges, some 6 us. One-wave workgroups then take more splits, as those
-// that span two documents are longer than the others, where there are many (4 x 28 rows below: 7 splits 422, 14 282). Heads, documents, query rows of each, keys in all,
-// eight waves and one at their best splits (us): 40 on 8, 64 x 1, 129,536 162 and 107; 3 x 4, 129,536 139 and 99; 1 x 28,
-// 116,105 118 and 152; 4 x 28 227 and 267; 56 on 8, 1 x 64, 100,000 198 and 335; 2 x 64 314 and 341; 40, 4 x 64, 20,000
-// 136 and 102; 56, 5 x 18, 63,257 484 and 429.
+// that span two documents are longer than the others, where there are many (4 x 28 rows below: 7 splits 422, 14 282).
+// Heads, documents, query rows of each, keys in all, eight waves and one at their best splits (us): 40 on 8, 64 x 1,
+// 129,536 162 and 107; 3 x 4, 129,536 139 and 99; 1 x 28, 116,105 118 and 152; 4 x 28 227 and 267; 56 on 8, 1 x 64,
+// 100,000 198 and 335; 2 x 64 314 and 341; 40, 4 x 64, 20,000 136 and 102; 56, 5 x 18, 63,257 484 and 429.
+// Calls of these sizes without ranges hold no contest, but take the same splits where one-wave workgroups are the first
+// plan: more of them than plan_of's is faster there too, or costs little (us, plan_of's splits and these: 56, 51 x 14,922 4
+// 100 and 9 90; 16, 39 x 29,920 16 54 and 32 45; 392 on 56, 9 x 11,066 4 79 and 9 70; 35 on 7, 11 x 69,694 36 67 and
+// 73 70; 7, 34 x 75,312 36 72 and 73 74).
 struct Plans {
     Plan first, second;
     uint64_t list;

@@ -430,3 +430,17 @@ def test_documents_that_the_keys_cut_off(dev, k_cuts, keys, causal, prefix):
             lo = min(max(start, 0), keys)
             want[i] = torch.tensor([lo, min(max(hi, lo), keys)])
     assert torch.equal(got.cpu().long(), want)
+
+
+@pytest.mark.parametrize("heads,kv_heads,rows,keys", [(56, 56, 51, 14922), (40, 40, 57, 18626), (35, 7, 11, 69694),
+                                                      (16, 16, 39, 29920), (40, 8, 28, 116105)])
+def test_few_rows_without_ranges(dev, heads, kv_heads, rows, keys):
+    """Sizes at which ranges would decide the kernel, and a call that has none: the splits of a call with ranges, in a
+    workspace that holds garbage."""
+    g = torch.Generator(device=dev).manual_seed(rows)
+    q, k, v = make(g, heads, rows, dev), make(g, kv_heads, keys, dev), make(g, kv_heads, keys, dev)
+    ws = torch.full((mh.flash_attn_128_workspace_bytes(q, k, v),), 0xff, dtype=torch.uint8, device=dev)
+    out = mh.flash_attn_128(q, k, v, workspace=ws)
+    for h in (0, heads - 1):
+        j = h // (heads // kv_heads)
+        check(out[h:h + 1], *attention64(q[h:h + 1], k[j:j + 1], v[j:j + 1]), f"head {h}")
