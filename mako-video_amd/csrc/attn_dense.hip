@@ -230,7 +230,7 @@ struct WaveRows {
     bf16x8_t qf[8];  // B operand of S^T: lane (n, hh) holds d 16 dc + 8 hh .. + 7 of row n
     floatx16 o[4];   // O^T: d 32 db + 8 (i / 4) + 4 hh + i % 4 of row n
     float m_run, l_run;
-    bool settled;    // every row has a maximum, of no more than 2^20
+    bool settled;    // every row has a maximum, of no more than 2^20 (0 stands for one in rows without keys)
     uint32_t lo, hi;            // the lane's row's keys
     uint32_t all_lo, all_hi;    // keys that every row with any attends: [all_lo, all_hi)
     uint32_t any_lo, any_hi;    // keys that some row attends lie in [any_lo, any_hi)
@@ -273,9 +273,9 @@ __device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, ui
 #pragma unroll
         for (int e = 0; e < 16; ++e)
             w.o[b][e] = 0.0f;
-    w.m_run = -kInf, w.l_run = 0.0f, w.settled = false;
     range_of(p, f, row, w.lo, w.hi);
     const bool any = w.lo < w.hi;
+    w.m_run = any ? -kInf : 0.0f, w.l_run = 0.0f, w.settled = false;
     w.any_lo = wave_min_u32(any ? w.lo : ~0u);
     w.any_hi = wave_max_u32(any ? w.hi : 0u);
     w.all_lo = wave_max_u32(w.lo); // a row of the list without keys masks every tile, one past it none
@@ -455,46 +455,62 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
     }
     // Most tiles raise no maximum by much, and the sum over a lane's 32 keys of a row tells: up to 2^10 no key is above
     // that, and the old maximum serves. That spares the search for the new one in a phase whose vector instructions take 7
-    // clocks each beside the other group's MFMAs. At most one more pass with the maxima brought up to date.
+    // clocks each beside the other group's MFMAs. Rows without a maximum or with a large one take the tile's without the
+    // look at their sums, and so do all rows in a tile where the range of one of the wave's begins. Each row thus goes by its
+    // own scores and by the ranges: none of its bits depends on the scores of the rows beside it.
+    const auto known = [&] { return fabsf(w.m_run) <= 0x1p20f; };
     float m_ref = w.m_run, sum;
-    bool update = !w.settled;
-#pragma unroll 1
-    for (;;) {
-        if (update) {
-            float mt = -kInf;
+    bool asks = false, looks = true; // the row asks for its maximum; some row of the wave goes by its sum
+    uint64_t asking = 0, over = 0;   // rows that ask, and lanes whose row asks by its sum
+    if (MASKED) {
+        const uint32_t end = t0 + 64u;
+        const bool here = max(w.lo, t0) < min(w.hi, end);
+        const bool begins = __ballot(here && (BIAS ? w.hi <= end : w.lo >= t0)) != 0; // with its last key under a bias
+        m_ref = known() ? m_ref : 0.0f; // a row without a key here has zeros for probabilities
+        asks = here && (begins || !known());
+        asking = __ballot(asks), looks = asking == 0 || __ballot(here && !asks) != 0;
+    } else if (__builtin_expect(!w.settled, false)) {
+        asks = !known();
+        asking = __ballot(asks), looks = ~asking != 0;
+    }
+    if (__builtin_expect(looks, !MASKED)) {
+        sum = tile_exponentials(s, pt, factor, m_ref);
+        over = __ballot(!(sum <= 0x1p10f));
+    }
+    if (__builtin_expect((asking | over) != 0, MASKED)) {
+        asks |= ((over | over >> 32 | over << 32) >> lane & 1u) != 0;
+        float mt = -kInf;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                mt = fmaxf(mt, s[b][i]);
+        mt = both_halves_max(mt) * factor;
+        const float m_new = asks ? fmaxf(w.m_run, mt) : w.m_run;
+        const float alpha = w.m_run == -kInf ? 0.0f : __builtin_amdgcn_exp2f(w.m_run - m_new);
+        if (__ballot(m_new > w.m_run)) {
+            w.l_run *= alpha;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    w.o[b][i] *= m_new > w.m_run ? alpha : 1.0f;
+        }
+        w.m_run = m_new;
+        w.settled = !__ballot(!known());
+        m_ref = m_new == -kInf ? 0.0f : m_new;
+        // factor s - m in one fused operation keeps the rounding of m, 2^-24 of it, in the exponent: common to all of a
+        // row's probabilities and harmless, until it leaves the exponent's range. Scores so large are rounded as m was.
+        const bool large = fabsf(m_ref) > 0x1p20f;
+        if (__ballot(large)) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    mt = fmaxf(mt, s[b][i]);
-            const float m_new = fmaxf(w.m_run, both_halves_max(mt) * factor);
-            const float alpha = w.m_run == -kInf ? 0.0f : __builtin_amdgcn_exp2f(w.m_run - m_new);
-            if (__ballot(m_new > w.m_run)) {
-                w.l_run *= alpha;
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        w.o[b][i] *= m_new > w.m_run ? alpha : 1.0f;
-            }
-            w.m_run = m_new;
-            m_ref = m_new == -kInf ? 0.0f : m_new;
-            w.settled = !__ballot(!(fabsf(m_new) <= 0x1p20f));
-            // factor s - m in one fused operation keeps the rounding of m, 2^-24 of it, in the exponent: common to all of a
-            // row's probabilities and harmless, until it leaves the exponent's range. Scores so large are rounded as m was.
-            if (__ballot(fabsf(m_ref) > 0x1p20f)) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[b][i] = rounded_difference(s[b][i], factor, m_ref);
-                m_ref = 0.0f, factor = 1.0f;
-            }
+                    s[b][i] = large ? rounded_difference(s[b][i], factor, m_ref) : fmaf(s[b][i], factor, -m_ref);
+            m_ref = 0.0f, factor = 1.0f;
         }
         sum = tile_exponentials(s, pt, factor, m_ref);
-        if (update || !__ballot(!(sum <= 0x1p10f)))
-            break;
-        update = true;
     }
     w.l_run += sum;
 }

@@ -444,3 +444,63 @@ def test_few_rows_without_ranges(dev, heads, kv_heads, rows, keys):
     for h in (0, heads - 1):
         j = h // (heads // kv_heads)
         check(out[h:h + 1], *attention64(q[h:h + 1], k[j:j + 1], v[j:j + 1]), f"head {h}")
+
+
+def causal_ranges(rows, keys, dev):
+    """The last row on the last key."""
+    hi = torch.arange(rows, device=dev) + keys - rows + 1
+    return torch.stack([torch.zeros_like(hi), hi], 1).int().contiguous()
+
+
+@pytest.mark.parametrize("heads,kv_heads,rows,keys", [(2, 2, 100, 100), (8, 2, 30, 300), (1, 1, 20, 9000), (6, 6, 700, 700),
+                                                     (40, 8, 300, 333), (16, 16, 40, 30000)])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (5.0, False), (0.0, True), (20.0, True)])
+def test_no_bit_of_a_row_comes_from_keys_that_its_neighbours_attend(dev, heads, kv_heads, rows, keys, cap, bias):
+    """Causal rows, one key poisoned at a time (NaN, infinite, scores past 2^20 and 2^10, values): the rows
+    before it attend the rest of its tile, and are the same bits. Then one query row."""
+    g = torch.Generator(device=dev).manual_seed(rows + keys + heads)
+    q, k, v = make(g, heads, rows, dev), make(g, kv_heads, keys, dev), make(g, kv_heads, keys, dev)
+    kw = {"ranges": causal_ranges(rows, keys, dev), "cap": cap}
+    if bias:
+        kw["slopes"] = torch.rand(heads, generator=g, device=dev) * 0.2
+        kw["q_pos"] = torch.randint(-50, 50, (rows,), generator=g, device=dev, dtype=torch.int32)
+        kw["k_pos"] = torch.randint(-50, 50, (keys,), generator=g, device=dev, dtype=torch.int32)
+    clean = mh.flash_attn_128(q, k, v, **kw)
+    first = keys - rows
+    check(clean[:1], *attention64(q[:1], k[:1], v[:1], **{**kw, **({"slopes": kw["slopes"][:1]} if bias else {})}))
+    for row in {1, 5, rows // 3, rows // 2 + 3, rows - 1}:
+        for what in (float("nan"), float("inf"), 1e6, 300.0):
+            bad = k.clone()
+            bad[:, first + row] = torch.where(bad[:, first + row] > 0, what, -what)
+            assert torch.equal(mh.flash_attn_128(q, bad, v, **kw)[:, :row], clean[:, :row]), f"key of row {row}: {what}"
+        bad = v.clone()
+        bad[:, first + row] = float("inf")
+        assert torch.equal(mh.flash_attn_128(q, k, bad, **kw)[:, :row], clean[:, :row]), f"value of row {row}"
+        others = torch.arange(rows, device=dev) != row
+        for what in (float("nan"), 1e6, 300.0):
+            bad = q.clone()
+            bad[:, row] = what
+            assert torch.equal(mh.flash_attn_128(bad, k, v, **kw)[:, others], clean[:, others]), f"row {row}: {what}"
+            no_ranges = {**kw, "ranges": None}
+            assert torch.equal(mh.flash_attn_128(bad, k, v, **no_ranges)[:, others],
+                               mh.flash_attn_128(q, k, v, **no_ranges)[:, others]), f"row {row}: {what}, all keys"
+
+
+def test_scores_far_beyond_and_ordinary_ones_in_a_wave(dev):
+    """Rows of the first tiles' large scores (past 2^20) beside ordinary rows, in rising and falling order, each against
+    float64 and against itself alone."""
+    g = torch.Generator(device=dev).manual_seed(5)
+    rows, keys = 64, 500
+    q, k, v = make(g, 2, rows, dev), make(g, 2, keys, dev), make(g, 2, keys, dev)
+    q[:, 1::3] *= 2.0 ** 18
+    q[:, 2::3] *= 2.0 ** 9
+    for kw in ({}, {"ranges": causal_ranges(rows, keys, dev)}, {"ranges": random_ranges(g, rows, keys, dev)}):
+        out = mh.flash_attn_128(q, k, v, **kw)
+        for part in (slice(0, None, 3), slice(1, None, 3), slice(2, None, 3)):
+            pw = {n: t[part].contiguous() for n, t in kw.items()}
+            alone = q.clone()
+            alone[:] = q[:, part][:, :1].expand_as(q)   # a call of the same sizes, all rows of one kind
+            alone[:, part] = q[:, part]
+            assert torch.equal(mh.flash_attn_128(alone, k, v, **kw)[:, part], out[:, part])
+            if part.start == 0:
+                check(out[:, part], *attention64(q[:, part], k, v, **pw))
