@@ -237,7 +237,8 @@ struct WaveRows {
     float slope_log2;           // BIAS: the row's head's slope, in base-2 units
     int32_t q_pos, q_base;      // BIAS: the row's position, the wave's first row's
     float q_rel;                // BIAS: their difference, if q_near: it is under 2^23 in all of the wave's rows
-    bool q_near;                // (and the slope in units of a score ordinary)
+    bool q_near;                // (and none of them is steep)
+    bool steep;                 // a slope of the wave's rows is beyond 2^80 units of a score
     float slope_unit;
     // Whether the wave has work in the tile at key t0, and whether some row's range does not cover it.
     __device__ __forceinline__ bool meets(uint32_t t0) const { return t0 < any_hi && t0 + 64u > any_lo; }
@@ -287,7 +288,8 @@ __device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, ui
         const int32_t rel = __builtin_elementwise_sub_sat(w.q_pos, w.q_base);
         w.q_rel = float(rel);
         w.slope_unit = w.slope_log2 / score_unit<CAP>(p);
-        w.q_near = !__ballot(!is_near(rel) || !(fabsf(w.slope_unit) <= 0x1p80f));
+        w.steep = __ballot(!(fabsf(w.slope_unit) <= 0x1p80f)) != 0;
+        w.q_near = !w.steep && !__ballot(!is_near(rel));
     }
 }
 
@@ -326,12 +328,15 @@ __device__ __forceinline__ floatx4_t near_four(const float* near_pos, int g, uin
     return *reinterpret_cast<const floatx4_t*>(near_pos + 8 * g + 4u * (lane >> 5));
 }
 
-// Scores to base-2 units less the bias, from the distances of int32 positions (kp: the tile's; the keys' numbers without
-// k_pos), which are exact before they round to float.
-__device__ __forceinline__ void bias_scores_far(const DenseParams& p, const WaveRows& w, floatx16 (&s)[2], float unit,
-                                                uint32_t t0, const int32_t* kp, uint32_t lane)
+// The bias off the scores, from the distances of int32 positions (kp: the tile's; the keys' numbers without k_pos), which
+// are exact before they round to float. That is less_bias' own operation, so a row's bits do not depend on the positions that
+// made its wave come here; or with a steep slope in the wave in base-2 units, as what is returned, the factor of the scores
+// as they then stand, says.
+__device__ __forceinline__ float bias_scores_far(const DenseParams& p, const WaveRows& w, floatx16 (&s)[2], float unit,
+                                                 uint32_t t0, const int32_t* kp, uint32_t lane)
 {
     const uint32_t given = p.k_pos ? ~0u : 0u; // no branch a score
+    const float scale = w.steep ? unit : 1.0f, slope = w.steep ? w.slope_log2 : w.slope_unit;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -340,10 +345,11 @@ __device__ __forceinline__ void bias_scores_far(const DenseParams& p, const Wave
             const int32_t pos = int32_t((uint32_t(kp[key]) & given) | ((t0 + key) & ~given));
             // The distance of two int32 positions fits 32 bits without a sign.
             const uint32_t d = w.q_pos > pos ? uint32_t(w.q_pos) - uint32_t(pos) : uint32_t(pos) - uint32_t(w.q_pos);
-            s[b][i] = fmaf(s[b][i], unit, -w.slope_log2 * float(d));
+            s[b][i] = fmaf(-slope, float(d), s[b][i] * scale);
             if (i % 4 == 3)
                 __builtin_amdgcn_sched_barrier(0); // four positions' registers at a time
         }
+    return w.steep ? 1.0f : unit;
 }
 
 // Where a wave's lanes find their operands in a tile's LDS images.
@@ -440,10 +446,8 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
                 }
             }
         }
-        if (!near) {
-            bias_scores_far(p, w, s, factor, t0, kp, lane);
-            factor = 1.0f;
-        }
+        if (!near)
+            factor = bias_scores_far(p, w, s, factor, t0, kp, lane);
     }
     if (MASKED) {
         const uint32_t from_lo = t0 + 4u * hh - w.lo, keys = w.hi - w.lo; // modulo 2^32: below lo is past every count

@@ -456,8 +456,8 @@ def causal_ranges(rows, keys, dev):
                                                      (40, 8, 300, 333), (16, 16, 40, 30000)])
 @pytest.mark.parametrize("cap,bias", [(0.0, False), (5.0, False), (0.0, True), (20.0, True)])
 def test_no_bit_of_a_row_comes_from_keys_that_its_neighbours_attend(dev, heads, kv_heads, rows, keys, cap, bias):
-    """Causal rows, one key poisoned at a time (NaN, infinite, scores past 2^20 and 2^10, values): the rows
-    before it attend the rest of its tile, and are the same bits. Then one query row."""
+    """Causal rows, one key poisoned at a time (NaN, infinite, scores past 2^20 and 2^10, values, a far position): the rows
+    before it attend the rest of its tile, and are the same bits. Then one query row, and its position."""
     g = torch.Generator(device=dev).manual_seed(rows + keys + heads)
     q, k, v = make(g, heads, rows, dev), make(g, kv_heads, keys, dev), make(g, kv_heads, keys, dev)
     kw = {"ranges": causal_ranges(rows, keys, dev), "cap": cap}
@@ -484,6 +484,15 @@ def test_no_bit_of_a_row_comes_from_keys_that_its_neighbours_attend(dev, heads, 
             no_ranges = {**kw, "ranges": None}
             assert torch.equal(mh.flash_attn_128(bad, k, v, **no_ranges)[:, others],
                                mh.flash_attn_128(q, k, v, **no_ranges)[:, others]), f"row {row}: {what}, all keys"
+        if bias:
+            for what in (1 << 30, -(1 << 31)):
+                bad = kw["k_pos"].clone()
+                bad[first + row] = what
+                assert torch.equal(mh.flash_attn_128(q, k, v, **{**kw, "k_pos": bad})[:, :row], clean[:, :row])
+                bad = kw["q_pos"].clone()
+                bad[row - 1] = what
+                others = torch.arange(rows, device=dev) != row - 1
+                assert torch.equal(mh.flash_attn_128(q, k, v, **{**kw, "q_pos": bad})[:, others], clean[:, others])
 
 
 def test_scores_far_beyond_and_ordinary_ones_in_a_wave(dev):
