@@ -229,3 +229,69 @@ def test_replayed_from_a_graph(dev):
         want = run()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def tile_of_sizes(m, w_rows, k):
+    """The kernel that a product's sizes take (the rule of gemm_mx4.hip, in float as there)."""
+    f = np.float32
+    tiles = (("256x256", 256, 256, 1.65), ("192x256", 192, 256, 1.5), ("128x128", 128, 128, 0.71), ("64x128", 64, 128, 0.48),
+             ("64x64", 64, 64, 0.35))
+    w_us, best, least = f(w_rows) * f(k) * f(0.53125 / 6.2e6), None, f(np.inf)
+    for name, rows, cols, step in tiles:
+        rounds = (-(-m // rows) * (w_rows // cols) + 255) // 256
+        us = f(4) + max(f(rounds) * f(k // 256) * f(step), w_us)
+        if us < least:
+            best, least = name, us
+    few = f(4) + w_us + f(w_rows // 32) * f(m) * f(k) * f(0.35 / 6.2e6)
+    return ("few 16" if m <= 16 else "few 32") if m <= 32 and few <= least else best
+
+
+LONG = [("few 16", 5, 512), ("few 16", 16, 1024), ("few 32", 17, 512), ("few 32", 32, 2048), ("64x64", 65, 512),
+        ("64x64", 129, 512), ("64x128", 129, 8192), ("64x128", 300, 4096), ("128x128", 385, 5120), ("128x128", 700, 3328),
+        ("192x256", 769, 10240), ("192x256", 2100, 4096), ("256x256", 769, 16384), ("256x256", 3000, 5120)]
+
+
+@pytest.mark.parametrize("k", [2560, 2816])
+@pytest.mark.parametrize("kernel,m,n", LONG)
+def test_every_kernel_over_many_steps_with_every_epilogue(dev, kernel, m, n, k):
+    """Ten and eleven K-steps of 256, several times round every kernel's ring of stages, with cut row tiles and all four
+    epilogues."""
+    assert tile_of_sizes(m, n, k) == kernel
+    g = torch.Generator(device=dev).manual_seed(m + n + k)
+    x, w = operand(g, m, k, dev), operand(g, n, k, dev, 1.5 / k ** 0.5)
+    y, tol = products(x, w, k)
+    out = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device=dev)
+    mh.gemm_mx4(*x, *w, out=out)
+    assert bool(((out.double() - y).abs() <= 2.0 ** -8 * y.abs() + tol).all())
+    table, which = 0.5 * torch.randn((3, n), generator=g, device=dev), torch.randint(0, 3, (m,), generator=g, device=dev).byte()
+    gate = table[which.long()].double()
+    slack = gate.abs() * (tol + 2.0 ** -24 * y.abs())
+    for dtype, unit in ((torch.bfloat16, 2.0 ** -8), (torch.float32, 2.0 ** -23)):
+        res = torch.randn((m, n), generator=g, device=dev).to(dtype)
+        want = res.double() + gate * y
+        got = mh.gemm_mx4_gate_add(*x, *w, res, table, set_of_row=which, n_sets=3)
+        assert bool(((got.double() - want).abs() <= unit * want.abs() + slack).all())
+    h = n // 2
+    out = torch.full((m, h), float("nan"), dtype=torch.bfloat16, device=dev)
+    mh.gemm_mx4_swiglu(*x, *w, out=out)
+    a, u, ta, tu = y[:, :h], y[:, h:], tol[:, :h], tol[:, h:]
+    want = a * torch.sigmoid(a) * u
+    slack = 1.1 * ta * (u.abs() + tu) + (a * torch.sigmoid(a)).abs() * tu + 2.0 ** -21 * (1 + a.abs()) * want.abs()
+    assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + slack).all())
+
+
+@pytest.mark.parametrize("kernel,n,sizes", [("few 16", 512, (16, 1, 7)), ("few 32", 512, (32, 17)), ("64x64", 512, (130, 33, 65)),
+                                            ("64x128", 10240, (129, 65)), ("128x128", 5120, (500, 385)),
+                                            ("192x256", 4096, (3000, 2100)), ("256x256", 16384, (900, 769))])
+def test_a_row_is_the_same_bits_in_any_batch_of_its_kernel(dev, kernel, n, sizes):
+    """Of fewer rows, and at another place among them."""
+    k = 2304
+    g = torch.Generator(device=dev).manual_seed(n)
+    x, w = operand(g, sizes[0], k, dev), operand(g, n, k, dev, 0.02)
+    full = mh.gemm_mx4(*x, *w)
+    for m in sizes:
+        assert tile_of_sizes(m, n, k) == kernel
+        assert torch.equal(mh.gemm_mx4(x[0][:m], x[1][:, :m].contiguous(), *w), full[:m])
+        for by in (1, m // 2):
+            got = mh.gemm_mx4(x[0][:m].roll(by, 0), x[1][:, :m].contiguous().roll(by, 1), *w)
+            assert torch.equal(got.roll(-by, 0), full[:m])
