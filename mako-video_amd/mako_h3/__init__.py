@@ -1062,8 +1062,10 @@ def _mx4(x, x_scale, w, w_scale):
         raise ValueError("x must be [m][k / 2] and w [n][k / 2]")
     m, half = x.shape
     n = w.shape[0]
-    _scale_bytes(x_scale, "x_scale", m, 2 * half)
-    _scale_bytes(w_scale, "w_scale", n, 2 * half)
+    if getattr(x_scale, "shape", None) != (half // 128, m, 8):
+        _scale_bytes(x_scale, "x_scale", m, 2 * half)
+    if getattr(w_scale, "shape", None) != (half // 128, n, 8):
+        _scale_bytes(w_scale, "w_scale", n, 2 * half)
     u8 = torch.uint8
     return m, n, 2 * half, ((x, "x", u8, m * half), (x_scale, "x_scale", u8, m * half // 16), (w, "w", u8, n * half),
                             (w_scale, "w_scale", u8, n * half // 16))
