@@ -337,11 +337,13 @@ int mh3_flash_attn_sparse_128_ordered(const MH3AttnArgs* args, const uint16_t* q
  * in it. For query head h (key head h / (heads / kv_heads)) and query row i over the keys j in [lo_i, hi_i):
  *   s[j] = scale q_i . k_j, under a cap (cap > 0) cap tanh(scale q_i . k_j / cap),
  *          with slopes less slopes[h] |q_pos[i] - k_pos[j]|;
- *   out_i = sum_j softmax(s)[j] v_j, float accumulation, rounded to bf16 once.
- * A row without keys is zero. What lies in keys that a row does not attend has no effect on it, infinities and NaN
- * included. Element (head, row, d) of q, k, v and out lies at head * head_stride + row * row_stride + d of each (strides
- * in elements, multiples of 8, rows of 128 .. 2^23 - 1 elements apart), so head tiles, the model's [rows][heads * 128]
- * order and slices of wider rows are all taken as they are.
+ *   out_i = sum_j softmax(s)[j] v_j.
+ * Scores, maxima, sums and outputs are accumulated in float. Two things round to bf16: each unnormalized probability for
+ * its product with v_j (the sum that divides takes it unrounded), and the result.
+ * A row without keys is zero. What lies in keys that a row does not attend has no effect on any of its bits, infinities,
+ * NaN and their positions included, nor do other rows' q and positions. Element (head, row, d) of q, k, v and out lies at
+ * head * head_stride + row * row_stride + d of each (strides in elements, multiples of 8, rows of 128 .. 2^23 - 1 elements
+ * apart), so head tiles, the model's [rows][heads * 128] order and slices of wider rows are all taken as they are.
  *   ranges: int32 [q_rows][2], lo and hi of each query row, clamped to [0, kv_rows] (hi at least lo); 8-byte aligned;
  *           NULL: every row attends all kv_rows. mh3_attn_ranges makes those of documents, prefixes and causal rows.
  *   slopes: float [heads], or NULL: no bias. q_pos int32 [q_rows] and k_pos int32 [kv_rows]: both, or both NULL (the rows'

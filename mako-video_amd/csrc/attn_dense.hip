@@ -17,16 +17,21 @@
 // - A masked probability is a zero, and zero times an infinite or NaN value of V would still be NaN in the rows that do
 //   not attend it: masked tiles are searched for such values, and where there are any the matrix cores take zeros for
 //   them, and they are added one key at a time to the rows that attend it. (All tiles masked, 40 heads, 14,080 rows on
-//   11,264 keys: 3.73 ms, and 2.73 ms with none masked.)
+//   11,264 keys: 3.75 ms, and 2.65 ms with none masked.)
 // - Softmax in base 2. A row's running maximum is brought up to date only when a tile's probabilities sum up to more than
 //   2^10 in a lane, so P stays below 2^10 and most tiles neither search a maximum nor rescale O. P rounds to bf16 for the
-//   matrix cores (2^-9 of each probability, below the output's own rounding); maxima, sums and O are float.
+//   matrix cores (by up to 2^-8 of each probability, the sum takes them unrounded); maxima, sums and O are float.
+// - A row's bits come from its own scores, its keys' values and the ranges. Waves and workgroups decide together what to
+//   skip, never how a row rounds: that a neighbour attends an infinity or a far position leaves no trace. (One decision for
+//   the wave's 32 rows instead: the same time within 2%.)
 // - Few rows leave the chip idle: their keys are then split over workgroups, each leaves its part of O, the maximum and the
 //   sum in the workspace, and a second kernel joins them in a fixed order.
-// What bounds it: many rows, the chip's power (960 x 544, 56 heads, 19,305 rows: 8.9 .. 9.3 ms, 1150 .. 1200 TFLOP/s, the
-// clock at 1.7 GHz and the matrix cores busy 69% of it); under a cap the vector unit (five more operations a score, two
-// of them transcendental: 14,925 rows of 40 heads 5.0 ms, without one 4.1); few rows, the one pass over K and V (129,536
-// keys of 8 heads in 95 us, 5.5 TB/s).
+// What bounds it: many rows, the chip's power (960 x 544, 56 heads, 19,305 rows: 8.65 .. 8.9 ms, 1200 .. 1230 TFLOP/s, the
+// clock at 1.65 to 1.7 GHz and the matrix cores busy 72% of it); under a cap also the vector unit's transcendentals (five
+// clips packed into 14,925 rows of 40 heads 1490 us, without a cap 1230, with a multiplication in the place of the cap's
+// exponential and reciprocal 1260); few rows, the one pass over K and V (129,536 keys of 8 heads in 95 us, 5.5 TB/s).
+// Under a bias the eight-wave kernels hold five or six registers in scratch, read between the loops, in masked turns and in
+// rare paths, never in the loop of whole tiles.
 #include "mh3_common.hpp"
 
 #include <algorithm>
