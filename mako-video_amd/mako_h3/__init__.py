@@ -1029,11 +1029,13 @@ def _gemm_ref(m, n, k, n_sets=0, gate_stride=0):
 
 
 def _scale_bytes(t, name, rows, cols) -> None:
-    """A matrix's scales lie [cols / 256][rows][8], so those of more or fewer rows are others from the second 256 columns
-    on: the tensor has that shape, or (not of three dimensions) just as many bytes."""
+    """A matrix's scales lie [cols / 256][rows][8], so those of more rows are others from the second 256 columns on: the
+    tensor has that shape, or (not of three dimensions) just as many bytes. Of 256 columns the first rows' lead."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
-    if t.shape != (cols // 256, rows, 8) and (t.dim() == 3 or t.numel() != rows * cols // 32):
+    if t.shape == (cols // 256, rows, 8) or (cols == 256 and t.numel() >= rows * 8):
+        return
+    if t.dim() == 3 or t.numel() != rows * cols // 32:
         raise ValueError(f"{name}: {tuple(t.shape)}, the scales of {rows} rows of {cols} are {(cols // 256, rows, 8)}")
 
 

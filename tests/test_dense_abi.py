@@ -367,3 +367,6 @@ def test_scales_of_other_rows_are_refused():
     for good in (xs, xs.flatten()):
         with pytest.raises(ValueError, match="must be on the GPU"):
             mh.quant_rows_mx4(v, scale=good)
+    # Of 256 columns there is one run of rows, and the first rows' scales lead it.
+    with pytest.raises(ValueError, match="must be on the GPU"):
+        mh.gemm_mx4(x[:, :128].contiguous(), torch.zeros((1, m + 4, 8), dtype=u8), w[:, :128].contiguous(), ws[:1])

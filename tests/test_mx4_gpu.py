@@ -295,3 +295,15 @@ def test_a_row_is_the_same_bits_in_any_batch_of_its_kernel(dev, kernel, n, sizes
         for by in (1, m // 2):
             got = mh.gemm_mx4(x[0][:m].roll(by, 0), x[1][:, :m].contiguous().roll(by, 1), *w)
             assert torch.equal(got.roll(-by, 0), full[:m])
+
+
+def test_first_rows_with_all_rows_scales_of_256_columns(dev):
+    """One run of scales a matrix: the first rows' lead it. Of more columns the binding refuses the same call."""
+    g = torch.Generator(device=dev).manual_seed(12)
+    for k in (256, 512):
+        x, w = operand(g, 90, k, dev), operand(g, 512, k, dev)
+        if k == 256:
+            assert torch.equal(mh.gemm_mx4(x[0][:70], x[1], *w), mh.gemm_mx4(x[0][:70], x[1][:, :70].contiguous(), *w))
+        else:
+            with pytest.raises(ValueError, match="x_scale"):
+                mh.gemm_mx4(x[0][:70], x[1], *w)
