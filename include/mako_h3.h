@@ -385,6 +385,84 @@ typedef struct MH3RangeArgs {
 int mh3_attn_ranges(const MH3RangeArgs* args, const int32_t* q_off, const int32_t* k_off, const int32_t* prefix,
                     int32_t* ranges, mh3_stream_t stream);
 
+/* ---- kept rows in pages ----------------------------------------------------------------------------------------------
+ * Streams that go on row after row keep their keys and values in pages of a pool that all of them share; the reference has
+ * no counterpart. A stream's kept row j lies at row j % page_rows of page table[stream][j / page_rows]. The table is int32
+ * [streams][cols], table_stride ints from a stream's first entry to the next one's; an entry of -1 is no page, and every
+ * call takes other numbers outside [0, pages) for none too. refs is int32 [pages]: how many of the table's entries name
+ * each page; a page is free if that is zero, and nothing else is kept of it. Streams may share pages (fork). The results of
+ * every call follow from its inputs: nothing depends on the order in which the GPU gets to it.
+ * A pool is `pages` pages of page_bytes, each in one piece, page_stride bytes apart (multiples of 16, the base 16-byte
+ * aligned): of whatever a program keeps by rows, say a layer's keys, or all layers' keys and values. Calls take up to
+ * MH3_MAX_POOLS pools (a host array), which may not overlap each other, the table, refs or another list (MH3_ERR_PARAM;
+ * so for all in- and outputs below). int32 lists and tables are 4-byte aligned, workspaces 16; a call that overlaps
+ * another in time needs its own workspace. */
+enum { MH3_MAX_POOLS = 64, MH3_MAX_STREAMS = 4096, MH3_MAX_PAIRS = 16384 };
+typedef struct MH3PagesArgs {
+    uint32_t streams;      /* 1 .. MH3_MAX_STREAMS */
+    uint32_t cols;         /* entries a stream */
+    uint32_t pages;        /* of the pool, below 2^24 */
+    uint32_t page_rows;    /* fork, write and attention */
+    uint64_t table_stride; /* at least cols; streams * cols below 2^30 */
+} MH3PagesArgs;
+typedef struct MH3Pool {
+    void* base;
+    uint64_t page_bytes;
+    uint64_t page_stride;
+} MH3Pool;
+/* Gives the entries first[s] .. last[s] - 1 of each stream s that are negative a page each, the lowest free ones in the
+ * order (stream, entry), and counts them (refs 1). Entries that find no page stay; *missing (NULL: not wanted) says how
+ * many. first and last: int32 [streams], clamped to [0, cols]. */
+int mh3_pages_take(const MH3PagesArgs* args, int32_t* table, int32_t* refs, const int32_t* first, const int32_t* last,
+                   int32_t* missing, mh3_stream_t stream);
+/* Clears the entries first[s] .. last[s] - 1 of each stream: their pages' counts fall, so that those of no other stream
+ * become free, and the entries become -1. A stream that ends frees all of them, one that takes drafted rows back the last
+ * ones, one under a window those that it has left behind. */
+int mh3_pages_free(const MH3PagesArgs* args, int32_t* table, int32_t* refs, const int32_t* first, const int32_t* last,
+                   mh3_stream_t stream);
+/* Streams that go on from another's rows: row s of new_table (laid out as table, apart from it) holds the first rows[s]
+ * kept rows of stream parents[s] as `table` has it. Their full pages are shared, a page that they have only begun is copied
+ * to the lowest page that was free before the call, in the order of the streams, in all of the pools; what follows is -1.
+ * parents[s] == s leaves row s as it is, whatever rows[s]; a parent outside [0, streams) leaves it empty. refs counts
+ * new_table's entries in place of table's. A begun page that finds no free one is -1 in new_table, and *missing (may be
+ * NULL) says how many did. workspace: mh3_pages_fork_workspace_bytes(args) bytes. */
+int64_t mh3_pages_fork_workspace_bytes(const MH3PagesArgs* args);
+int mh3_pages_fork(const MH3PagesArgs* args, const MH3Pool* pools, uint32_t n_pools, const int32_t* table, int32_t* refs,
+                   const int32_t* parents, const int32_t* rows, int32_t* new_table, int32_t* missing, void* workspace,
+                   uint64_t workspace_bytes, mh3_stream_t stream);
+/* Copies page src[i] to page dst[i], i < n <= MH3_MAX_PAIRS, in all of the pools. A page may be copied to several. A pair
+ * is passed over if either page is none of the pool's, if the call also copies from its dst, or if an earlier pair has the
+ * same dst. */
+int mh3_pages_copy(const MH3Pool* pools, uint32_t n_pools, uint32_t pages, const int32_t* src, const int32_t* dst,
+                   uint32_t n, mh3_stream_t stream);
+/* Moves the pages in use together: if there are u of them, the i-th in use that lies at u or past it goes to the i-th free
+ * one below u, in all of the pools, and the table and refs follow. map (int32 [pages]) takes each page's new number, -1 for
+ * those that were free; *used (may be NULL) takes u. A table entry that is no page, or whose page has no count, becomes
+ * -1. workspace: mh3_pages_compact_workspace_bytes(args) bytes. */
+int64_t mh3_pages_compact_workspace_bytes(const MH3PagesArgs* args);
+int mh3_pages_compact(const MH3PagesArgs* args, const MH3Pool* pools, uint32_t n_pools, int32_t* table, int32_t* refs,
+                      int32_t* map, int32_t* used, void* workspace, uint64_t workspace_bytes, mh3_stream_t stream);
+/* New rows into their places: of the n rows j, those of stream s are off[s] .. off[s + 1] - 1 (int32 [streams + 1],
+ * ascending), and row j goes to kept row starts[s] + j - off[s]. rows (int32 [n], or NULL: the row j itself) says which of
+ * the n_rows rows of k and v that is, for the accepted ones of drafted rows. k and v are bf16 heads as in
+ * mh3_flash_attn_128; element (page, head, row, d) of the pools k_pages and v_pages lies at page * page_stride + head *
+ * page_head_stride + row * page_row_stride + d of each (elements, multiples of 8; rows 128 .. 2^23 - 1 apart), so pages of
+ * head tiles, of [page_rows][kv_heads * 128] rows, and one layer's slices of pages that hold several, are all taken. A row
+ * whose place or page does not exist is passed over. Two streams that write the same row of a shared page leave either's. */
+typedef struct MH3PagesWriteArgs {
+    MH3PagesArgs table;
+    uint32_t kv_heads;
+    uint32_t head_dim; /* 128 */
+    uint32_t n_rows;
+    uint32_t n;
+    uint64_t k_head_stride, k_row_stride, v_head_stride, v_row_stride;
+    uint64_t k_page_stride, k_page_head_stride, k_page_row_stride;
+    uint64_t v_page_stride, v_page_head_stride, v_page_row_stride;
+} MH3PagesWriteArgs;
+int mh3_pages_write(const MH3PagesWriteArgs* args, const uint16_t* k, const uint16_t* v, uint16_t* k_pages,
+                    uint16_t* v_pages, const int32_t* table, const int32_t* starts, const int32_t* off,
+                    const int32_t* rows, mh3_stream_t stream);
+
 /* ---- int8 weights: quant_rows_i8 (weight side) ---------------------------------------------------------------------
  * Reference kernel `quant_rows_i8` (mako-common; docs/performance.md:122-123, docs/architecture.md:54-56): each row
  * of a [rows][cols] matrix (the weight's [out][in] rows) to symmetric int8 with one float scale:

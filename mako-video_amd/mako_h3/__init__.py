@@ -73,6 +73,22 @@ class RangeArgs(C.Structure):
     _fields_ = [("q_rows", C.c_uint32), ("kv_rows", C.c_uint32), ("docs", C.c_uint32), ("causal", C.c_uint32)]
 
 
+class PagesArgs(C.Structure):
+    _fields_ = [("streams", C.c_uint32), ("cols", C.c_uint32), ("pages", C.c_uint32), ("page_rows", C.c_uint32),
+                ("table_stride", C.c_uint64)]
+
+
+class Pool(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("page_bytes", C.c_uint64), ("page_stride", C.c_uint64)]
+
+
+class PagesWriteArgs(C.Structure):
+    _fields_ = [("table", PagesArgs), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("n_rows", C.c_uint32),
+                ("n", C.c_uint32)] + \
+               [(f"{t}_{d}_stride", C.c_uint64) for t in ("k", "v") for d in ("head", "row")] + \
+               [(f"{t}_{d}_stride", C.c_uint64) for t in ("k", "v") for d in ("page", "page_head", "page_row")]
+
+
 class CubeMapArgs(C.Structure):
     _fields_ = [("grid_t", C.c_uint32), ("grid_h", C.c_uint32), ("grid_w", C.c_uint32), ("n_dense", C.c_uint32),
                 ("video_row0", C.c_uint64), ("dense_row0", C.c_uint64)]
@@ -135,6 +151,14 @@ def _load() -> C.CDLL:
         "mh3_flash_attn_128_workspace_bytes": (I64, [C.POINTER(DenseAttnArgs)]),
         "mh3_flash_attn_128": (I32, [C.POINTER(DenseAttnArgs)] + [P] * 8 + [C.c_uint64, P, P]),
         "mh3_attn_ranges": (I32, [C.POINTER(RangeArgs), P, P, P, P, P]),
+        "mh3_pages_take": (I32, [C.POINTER(PagesArgs), P, P, P, P, P, P]),
+        "mh3_pages_free": (I32, [C.POINTER(PagesArgs), P, P, P, P, P]),
+        "mh3_pages_fork_workspace_bytes": (I64, [C.POINTER(PagesArgs)]),
+        "mh3_pages_fork": (I32, [C.POINTER(PagesArgs), C.POINTER(Pool), U32] + [P] * 7 + [C.c_uint64, P]),
+        "mh3_pages_copy": (I32, [C.POINTER(Pool), U32, U32, P, P, U32, P]),
+        "mh3_pages_compact_workspace_bytes": (I64, [C.POINTER(PagesArgs)]),
+        "mh3_pages_compact": (I32, [C.POINTER(PagesArgs), C.POINTER(Pool), U32] + [P] * 5 + [C.c_uint64, P]),
+        "mh3_pages_write": (I32, [C.POINTER(PagesWriteArgs)] + [P] * 9),
         "mh3_quant_rows_mx4": (I32, [C.POINTER(QuantArgs), P, P, P, P]),
         "mh3_gemm_mx4": (I32, [C.POINTER(GemmArgs), P, P, P, P, P, P]),
         "mh3_gemm_mx4_swiglu": (I32, [C.POINTER(GemmArgs), P, P, P, P, P, P]),
@@ -845,6 +869,211 @@ def flash_attn_128(q, k, v, *, ranges=None, scale=0.0, cap=0.0, slopes=None, q_p
         _ptr(slopes), _ptr(q_pos), _ptr(k_pos), _ptr(workspace), 0 if workspace is None else workspace.numel(),
         out.data_ptr())
     return out
+
+
+# ---- kept rows in pages ----------------------------------------------------------------------------------------------
+
+MAX_POOLS, MAX_STREAMS, MAX_PAIRS = 64, 4096, 16384
+
+
+def _page_table(table, pages, page_rows=0, name="table") -> PagesArgs:
+    if not isinstance(table, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor")
+    if table.dtype != torch.int32 or table.dim() != 2:
+        raise ValueError(f"{name}: int32 [streams][entries]")
+    streams, cols = table.shape
+    if cols > 1 and table.stride(1) != 1:
+        raise ValueError(f"{name}: a stream's entries must be contiguous")
+    stride = table.stride(0) if streams > 1 else max(cols, 1)
+    if stride < cols:
+        raise ValueError(f"{name}: its rows lie over each other")
+    return PagesArgs(streams, cols, pages, page_rows, stride)
+
+
+def _counts(refs) -> int:
+    if not isinstance(refs, torch.Tensor):
+        raise TypeError("refs: expected a tensor")
+    if refs.dtype != torch.int32 or refs.dim() != 1 or not refs.is_contiguous():
+        raise ValueError("refs: contiguous int32 [pages]")
+    return refs.shape[0]
+
+
+def _pools(pools, pages=None):
+    """(Pool array, how many, pages, their tensors) of a tensor [pages, ...] or a list of such with as many pages each, a
+    page's contents in one piece."""
+    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    if len(pools) > MAX_POOLS:
+        raise ValueError(f"pools: {len(pools)}, at most {MAX_POOLS} in a call")
+    held = (Pool * len(pools))()
+    for i, t in enumerate(pools):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("pools: expected tensors")
+        if t.dim() < 2:
+            raise ValueError("pools: [pages, ...]")
+        pages = t.shape[0] if pages is None else pages
+        if t.shape[0] != pages:
+            raise ValueError(f"pools: {t.shape[0]} pages, others (or refs) have {pages}")
+        if not t.is_contiguous() and not (pages and t[0].is_contiguous()):
+            raise ValueError("pools: a page's contents must be contiguous")
+        size = t.element_size() * (t.numel() // pages if pages else 0)
+        held[i] = Pool(t.data_ptr(), size, t.stride(0) * t.element_size() if pages > 1 else size)
+    return held, len(pools), pages, pools
+
+
+def _one_device_of(pools, **tensors) -> int:
+    return _one_device(**tensors, **{f"pools[{i}]": t for i, t in enumerate(pools)})
+
+
+def _missing(missing, device):
+    if missing is None:
+        return torch.empty(1, dtype=torch.int32, device=torch.device("cuda", device))
+    _need(missing, "missing", torch.int32, 1)
+    return missing
+
+
+def pages_take(table, refs, first, last, *, missing=None):
+    """Gives the entries first[s] .. last[s] - 1 (int32 [streams]) of each stream's row of `table` (int32
+    [streams][entries], -1: no page) that are -1 a page each, the lowest free ones (refs int32 [pages], 0: free) in the
+    order (stream, entry), and counts them. Returns `missing`, int32 [1]: how many found none and stay -1."""
+    a = _page_table(table, _counts(refs))
+    _need(first, "first", torch.int32, a.streams)
+    _need(last, "last", torch.int32, a.streams)
+    device = _one_device(table=table, refs=refs, first=first, last=last, missing=missing)
+    missing = _missing(missing, device)
+    _on(device, "pages_take", lib.mh3_pages_take, C.byref(a), table.data_ptr(), refs.data_ptr(), first.data_ptr(),
+        last.data_ptr(), missing.data_ptr())
+    return missing
+
+
+def pages_free(table, refs, first, last):
+    """Clears the entries first[s] .. last[s] - 1 of each stream to -1; their pages' counts fall."""
+    a = _page_table(table, _counts(refs))
+    _need(first, "first", torch.int32, a.streams)
+    _need(last, "last", torch.int32, a.streams)
+    _on(_one_device(table=table, refs=refs, first=first, last=last), "pages_free", lib.mh3_pages_free, C.byref(a),
+        table.data_ptr(), refs.data_ptr(), first.data_ptr(), last.data_ptr())
+
+
+def pages_fork(pools, table, refs, parents, rows, page_rows, *, new_table=None, missing=None, workspace=None):
+    """Streams that go on from others: row s of the new table holds the first rows[s] kept rows of stream parents[s] (int32
+    [streams], both), full pages shared, a page begun copied to the lowest one free before the call in all of `pools`
+    (tensors [pages, ...], or one). parents[s] == s leaves row s as it is, one outside the table leaves it empty. refs
+    then counts the new table's entries. Returns (new table, missing): int32 [1], how many pages begun found no free one
+    (their entries are -1)."""
+    held, n_pools, pages, pools = _pools(pools, _counts(refs))
+    a = _page_table(table, pages, page_rows)
+    new_table = torch.empty_strided(table.shape, (a.table_stride, 1), dtype=torch.int32, device=table.device) \
+        if new_table is None else new_table
+    b = _page_table(new_table, pages, page_rows, "new_table")
+    if (b.streams, b.cols, b.table_stride) != (a.streams, a.cols, a.table_stride):
+        raise ValueError("new_table: laid out as table")
+    _need(parents, "parents", torch.int32, a.streams)
+    _need(rows, "rows", torch.int32, a.streams)
+    device = _one_device_of(pools, table=table, refs=refs, parents=parents, rows=rows, new_table=new_table,
+                            missing=missing, workspace=workspace)
+    missing = _missing(missing, device)
+    ref = C.byref(a)
+    nbytes = lib.mh3_pages_fork_workspace_bytes(ref)
+    if nbytes < 0:
+        _check(nbytes, "pages_fork")
+    if workspace is None:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=table.device)
+    _need(workspace, "workspace", torch.uint8, nbytes)
+    _on(device, "pages_fork", lib.mh3_pages_fork, ref, held, n_pools, table.data_ptr(), refs.data_ptr(),
+        parents.data_ptr(), rows.data_ptr(), new_table.data_ptr(), missing.data_ptr(), workspace.data_ptr(),
+        workspace.numel())
+    return new_table, missing
+
+
+def pages_copy(pools, src, dst):
+    """Copies page src[i] to page dst[i] (int32, contiguous, of one length up to 16,384) in all of `pools` (tensors [pages,
+    ...], or one). A pair is passed over if either is no page, if the call also copies from its dst, or if an earlier pair
+    has the same dst."""
+    held, n_pools, pages, pools = _pools(pools)
+    n = src.numel()
+    _need(src, "src", torch.int32, n)
+    _need(dst, "dst", torch.int32, n)
+    if dst.numel() != n:
+        raise ValueError("src and dst: as many pages")
+    if not n_pools:
+        raise ValueError("pools: at least one")
+    _on(_one_device_of(pools, src=src, dst=dst), "pages_copy", lib.mh3_pages_copy, held, n_pools, pages, src.data_ptr(),
+        dst.data_ptr(), n)
+
+
+def pages_compact(pools, table, refs, *, map=None, used=None, workspace=None):
+    """Moves the pages in use to the lowest numbers in all of `pools` (tensors [pages, ...], or one), the i-th of those past
+    where they will end to the i-th free one; table and refs follow. Returns (map, used): int32 [pages], each page's new
+    number (-1: it was free), and int32 [1], how many are in use."""
+    held, n_pools, pages, pools = _pools(pools, _counts(refs))
+    a = _page_table(table, pages)
+    dev = table.device
+    map = torch.empty(pages, dtype=torch.int32, device=dev) if map is None else map
+    used = torch.empty(1, dtype=torch.int32, device=dev) if used is None else used
+    _need(map, "map", torch.int32, pages)
+    _need(used, "used", torch.int32, 1)
+    ref = C.byref(a)
+    nbytes = lib.mh3_pages_compact_workspace_bytes(ref)
+    if nbytes < 0:
+        _check(nbytes, "pages_compact")
+    if workspace is None:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _need(workspace, "workspace", torch.uint8, nbytes)
+    _on(_one_device_of(pools, table=table, refs=refs, map=map, used=used, workspace=workspace), "pages_compact",
+        lib.mh3_pages_compact, ref, held, n_pools, table.data_ptr(), refs.data_ptr(), map.data_ptr(), used.data_ptr(),
+        workspace.data_ptr(), workspace.numel())
+    return map, used
+
+
+def _page_rows(t, name, layout):
+    """(pages, heads, rows a page, page stride, head stride, row stride) of a bf16 pool: "heads" [pages][heads][rows][128],
+    "rows" [pages][rows][heads * 128], either with strides of multiples of 8 elements and the last dimension contiguous."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor")
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected {torch.bfloat16}")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != (4 if layout == "heads" else 3):
+        raise ValueError(f"{name}: [pages][heads][rows][128] for layout 'heads', [pages][rows][heads * 128] for 'rows'")
+    if stride[-1] != 1 and shape[-1]:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    # A dimension of one element may carry any stride: it is never stepped over.
+    page = stride[0] if shape[0] > 1 else 0
+    if layout == "heads":
+        if shape[3] != 128:
+            raise ValueError(f"{name}: rows of 128 values")
+        return (shape[0], shape[1], shape[2], page, stride[1] if shape[1] > 1 else 0, stride[2] if shape[2] > 1 else 128)
+    if shape[2] == 0 or shape[2] % 128:
+        raise ValueError(f"{name}: rows of heads * 128 values")
+    return shape[0], shape[2] // 128, shape[1], page, 128, stride[1] if shape[1] > 1 else shape[2]
+
+
+def pages_write(k, v, k_pages, v_pages, table, starts, off, *, rows=None, layout="heads", page_layout="heads"):
+    """New rows into their pages: of the rows j, those of stream s are off[s] .. off[s + 1] - 1 (int32 [streams + 1]), and
+    row j goes to kept row starts[s] + j - off[s] (int32 [streams]) of its stream. rows (int32 [n]): which row of k and v
+    row j is (None: j itself). k, v bf16 heads as flash_attn_128 takes them (`layout`); the pools bf16
+    [pages][heads][page rows][128] ("heads") or [pages][page rows][heads * 128] ("rows"), slices of wider pages too. A row
+    whose page is missing is passed over."""
+    if layout not in ("heads", "rows") or page_layout not in ("heads", "rows"):
+        raise ValueError("layout is 'heads' or 'rows'")
+    kv_heads, n_rows, khs, krs = _head_rows(k, "k", layout)
+    v_heads, v_rows, vhs, vrs = _head_rows(v, "v", layout)
+    if v_heads != kv_heads or v_rows != n_rows:
+        raise ValueError("k and v: the same heads and rows")
+    pages, heads, page_rows, *k_strides = _page_rows(k_pages, "k_pages", page_layout)
+    shape = _page_rows(v_pages, "v_pages", page_layout)
+    if heads != kv_heads or shape[:3] != (pages, heads, page_rows):
+        raise ValueError("k_pages and v_pages: the heads of k and v, the same pages and rows")
+    a = PagesWriteArgs(_page_table(table, pages, page_rows), kv_heads, 128, n_rows, n_rows, khs, krs, vhs, vrs, *k_strides,
+                       *shape[3:])
+    if rows is not None:
+        a.n = rows.numel()
+        _need(rows, "rows", torch.int32, a.n)
+    _need(starts, "starts", torch.int32, a.table.streams)
+    _need(off, "off", torch.int32, a.table.streams + 1)
+    device = _one_device(k=k, v=v, k_pages=k_pages, v_pages=v_pages, table=table, starts=starts, off=off, rows=rows)
+    _on(device, "pages_write", lib.mh3_pages_write, C.byref(a), k.data_ptr(), v.data_ptr(), k_pages.data_ptr(),
+        v_pages.data_ptr(), table.data_ptr(), starts.data_ptr(), off.data_ptr(), _ptr(rows))
 
 
 # ---- flash_attn_sparse_128 -------------------------------------------------------------------------------------------
