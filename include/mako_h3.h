@@ -385,6 +385,32 @@ typedef struct MH3RangeArgs {
 int mh3_attn_ranges(const MH3RangeArgs* args, const int32_t* q_off, const int32_t* k_off, const int32_t* prefix,
                     int32_t* ranges, mh3_stream_t stream);
 
+/* flash_attn_128 where each row attends a second range of keys too: what a window has left behind and still keeps in sight,
+ * a document's first rows (its text). Row i attends the keys of ranges[i] and those of sinks[i], each key once. ranges (not
+ * NULL) and sinks are int32 [q_rows][2], 8-byte aligned, each clamped as above, in any order and overlapping or not; with
+ * sinks NULL this is mh3_flash_attn_128. Everything else, the workspace included, is mh3_flash_attn_128's. */
+int mh3_flash_attn_128_sinks(const MH3DenseAttnArgs* args, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                             const int32_t* ranges, const int32_t* sinks, const float* slopes, const int32_t* q_pos,
+                             const int32_t* k_pos, void* workspace, uint64_t workspace_bytes, uint16_t* out,
+                             mh3_stream_t stream);
+/* Both for documents under a window. As in mh3_attn_ranges the last query row of a document sits on its last key row, so
+ * row i has key place own = k_off[d + 1] - q_off[d + 1] + i. It attends the document's keys in (own - window, own] with
+ * causal 1, in (own - window, own + window) with causal 0, and of the document's first sinks[d] keys (int32 [docs], or
+ * NULL: none) those up to own with causal 1, all of them with causal 0. ranges takes the window's part, first those of
+ * the first keys that lie before the window (all of them, if it ends among them; 0 and 0 where it covers them); both int32 [q_rows][2], 8-byte
+ * aligned. Rows of no document have two empty ranges. Neither output may overlap an input or the other
+ * (MH3_ERR_PARAM). */
+typedef struct MH3WindowArgs {
+    uint32_t q_rows;
+    uint32_t kv_rows; /* the ranges are cut off at 0 and kv_rows */
+    uint32_t docs;    /* >= 1 */
+    uint32_t causal;  /* 0 or 1 */
+    uint32_t window;  /* >= 1 */
+    uint32_t reserved;
+} MH3WindowArgs;
+int mh3_attn_window_ranges(const MH3WindowArgs* args, const int32_t* q_off, const int32_t* k_off, const int32_t* sinks,
+                           int32_t* ranges, int32_t* first, mh3_stream_t stream);
+
 /* ---- kept rows in pages ----------------------------------------------------------------------------------------------
  * Streams that go on row after row keep their keys and values in pages of a pool that all of them share; the reference has
  * no counterpart. A stream's kept row j lies at row j % page_rows of page table[stream][j / page_rows]. The table is int32

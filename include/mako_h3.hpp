@@ -204,6 +204,7 @@ struct Scores {
     const float* slopes = nullptr;
     const int32_t* q_pos = nullptr;
     const int32_t* k_pos = nullptr;
+    const int32_t* sinks = nullptr; // a second range of each row's, with ranges (attn_window_ranges)
 };
 
 inline std::optional<uint32_t> parse_int8(const std::string& text)
@@ -399,8 +400,8 @@ public:
                         void* workspace, uint64_t workspace_bytes, uint16_t* out) const
     {
         const MH3DenseAttnArgs a = d.args();
-        check(mh3_flash_attn_128(&a, q, k, v, sc.ranges, sc.slopes, sc.q_pos, sc.k_pos, workspace, workspace_bytes, out,
-                                 s_),
+        check(mh3_flash_attn_128_sinks(&a, q, k, v, sc.ranges, sc.sinks, sc.slopes, sc.q_pos, sc.k_pos, workspace,
+                                       workspace_bytes, out, s_),
               "flash_attn_128");
     }
     // Each query row's keys for documents packed into one batch, int32 [q_rows][2]: rows q_off[d] .. q_off[d + 1] - 1

@@ -73,6 +73,11 @@ class RangeArgs(C.Structure):
     _fields_ = [("q_rows", C.c_uint32), ("kv_rows", C.c_uint32), ("docs", C.c_uint32), ("causal", C.c_uint32)]
 
 
+class WindowArgs(C.Structure):
+    _fields_ = [("q_rows", C.c_uint32), ("kv_rows", C.c_uint32), ("docs", C.c_uint32), ("causal", C.c_uint32),
+                ("window", C.c_uint32), ("reserved", C.c_uint32)]
+
+
 class PagesArgs(C.Structure):
     _fields_ = [("streams", C.c_uint32), ("cols", C.c_uint32), ("pages", C.c_uint32), ("page_rows", C.c_uint32),
                 ("table_stride", C.c_uint64)]
@@ -151,6 +156,8 @@ def _load() -> C.CDLL:
         "mh3_flash_attn_128_workspace_bytes": (I64, [C.POINTER(DenseAttnArgs)]),
         "mh3_flash_attn_128": (I32, [C.POINTER(DenseAttnArgs)] + [P] * 8 + [C.c_uint64, P, P]),
         "mh3_attn_ranges": (I32, [C.POINTER(RangeArgs), P, P, P, P, P]),
+        "mh3_flash_attn_128_sinks": (I32, [C.POINTER(DenseAttnArgs)] + [P] * 9 + [C.c_uint64, P, P]),
+        "mh3_attn_window_ranges": (I32, [C.POINTER(WindowArgs), P, P, P, P, P, P]),
         "mh3_pages_take": (I32, [C.POINTER(PagesArgs), P, P, P, P, P, P]),
         "mh3_pages_free": (I32, [C.POINTER(PagesArgs), P, P, P, P, P]),
         "mh3_pages_fork_workspace_bytes": (I64, [C.POINTER(PagesArgs)]),
@@ -808,6 +815,36 @@ def attn_ranges(q_off, k_off, q_rows, kv_rows, *, prefix=None, causal=False, ran
     return ranges
 
 
+def attn_window_ranges(q_off, k_off, q_rows, kv_rows, window, *, sinks=None, causal=True, ranges=None, first=None):
+    """flash_attn_128's `ranges` and `sinks` for documents packed into one batch whose rows attend a window: (ranges,
+    first), int32 [q_rows][2] each. q_off and k_off int32 [docs + 1] as in attn_ranges, a document's last query row on its
+    last key row: a row attends the keys less than `window` before its own (it is one of them), and after it too unless
+    causal, and its document's first sinks[d] keys (int32 [docs], None: none), if causal those up to its own."""
+    if not isinstance(q_off, torch.Tensor):
+        raise TypeError("q_off: expected a tensor")
+    docs = q_off.numel() - 1
+    if docs < 1:
+        raise ValueError("q_off: at least one document")
+    if not 1 <= window <= 0xffffffff:
+        raise ValueError("window: at least one key, the row's own")
+    _need(q_off, "q_off", torch.int32, docs + 1)
+    _need(k_off, "k_off", torch.int32, docs + 1)
+    if sinks is not None:
+        _need(sinks, "sinks", torch.int32, docs)
+    both = torch.empty((2, q_rows, 2), dtype=torch.int32, device=q_off.device) if ranges is None and first is None else None
+    ranges = (both[0] if both is not None else torch.empty((q_rows, 2), dtype=torch.int32, device=q_off.device)) \
+        if ranges is None else ranges
+    first = (both[1] if both is not None else torch.empty((q_rows, 2), dtype=torch.int32, device=q_off.device)) \
+        if first is None else first
+    _need(ranges, "ranges", torch.int32, 2 * q_rows)
+    _need(first, "first", torch.int32, 2 * q_rows)
+    a = WindowArgs(q_rows, kv_rows, docs, int(bool(causal)), window, 0)
+    _on(_one_device(q_off=q_off, k_off=k_off, sinks=sinks, ranges=ranges, first=first), "attn_window_ranges",
+        lib.mh3_attn_window_ranges, C.byref(a), q_off.data_ptr(), k_off.data_ptr(), _ptr(sinks), ranges.data_ptr(),
+        first.data_ptr())
+    return ranges, first
+
+
 def _dense_args(q, k, v, layout, scale, cap) -> DenseAttnArgs:
     heads, q_rows, qhs, qrs = _head_rows(q, "q", layout)
     kv_heads, kv_rows, khs, krs = _head_rows(k, "k", layout)
@@ -824,11 +861,12 @@ def flash_attn_128_workspace_bytes(q, k, v, *, layout="heads") -> int:
     return n
 
 
-def flash_attn_128(q, k, v, *, ranges=None, scale=0.0, cap=0.0, slopes=None, q_pos=None, k_pos=None, layout="heads",
-                   out=None, out_layout=None, workspace=None):
+def flash_attn_128(q, k, v, *, ranges=None, sinks=None, scale=0.0, cap=0.0, slopes=None, q_pos=None, k_pos=None,
+                   layout="heads", out=None, out_layout=None, workspace=None):
     """Attention over whole rows, head_dim 128, bf16: out_i = softmax_j(s_ij) v over the keys of ranges[i] (int32
     [q_rows][2], [lo, hi); None: all), s = scale q k, under a cap (up to 1024) cap tanh(s / cap), less slopes[h] |q_pos_i - k_pos_j|
-    (float [heads], int32 [q_rows] and [kv_rows], None: the rows' numbers). Fewer key heads than query heads are shared
+    (float [heads], int32 [q_rows] and [kv_rows], None: the rows' numbers). sinks: a second range of keys for each row, as
+    `ranges` and with it (attn_window_ranges makes both); a key in both counts once. Fewer key heads than query heads are shared
     in order; scale 0 is 1 / sqrt(128); a row without keys is zero. layout "heads": [heads][rows][128], "rows":
     [rows][heads * 128] (slices of wider rows too); out_layout: out's, the same by default. `workspace` (uint8, at least
     flash_attn_128_workspace_bytes) is allocated here when None. Returns out."""
@@ -837,12 +875,12 @@ def flash_attn_128(q, k, v, *, ranges=None, scale=0.0, cap=0.0, slopes=None, q_p
         raise ValueError("layout is 'heads' or 'rows'")
     a = _dense_args(q, k, v, layout, scale, cap)
     heads, q_rows = a.heads, a.q_rows
-    device = _one_device(q=q, k=k, v=v, ranges=ranges, slopes=slopes, q_pos=q_pos, k_pos=k_pos, out=out,
+    device = _one_device(q=q, k=k, v=v, ranges=ranges, sinks=sinks, slopes=slopes, q_pos=q_pos, k_pos=k_pos, out=out,
                          workspace=workspace)
     if device != torch._C._cuda_getDevice():  # the workspace's size is of the current device
         with torch.cuda.device(device):
-            return flash_attn_128(q, k, v, ranges=ranges, scale=scale, cap=cap, slopes=slopes, q_pos=q_pos, k_pos=k_pos,
-                                  layout=layout, out=out, out_layout=out_layout, workspace=workspace)
+            return flash_attn_128(q, k, v, ranges=ranges, sinks=sinks, scale=scale, cap=cap, slopes=slopes, q_pos=q_pos,
+                                  k_pos=k_pos, layout=layout, out=out, out_layout=out_layout, workspace=workspace)
     if out is None:
         out = torch.empty((heads, q_rows, 128) if out_layout == "heads" else (q_rows, heads * 128),
                           dtype=torch.bfloat16, device=device)
@@ -851,6 +889,10 @@ def flash_attn_128(q, k, v, *, ranges=None, scale=0.0, cap=0.0, slopes=None, q_p
         raise ValueError("out: q's heads and rows")
     if ranges is not None:
         _need(ranges, "ranges", torch.int32, 2 * q_rows)
+    if sinks is not None:
+        if ranges is None:
+            raise ValueError("sinks: only with ranges")
+        _need(sinks, "sinks", torch.int32, 2 * q_rows)
     if slopes is not None:
         _need(slopes, "slopes", torch.float32, heads)
     if q_pos is not None:
@@ -865,9 +907,9 @@ def flash_attn_128(q, k, v, *, ranges=None, scale=0.0, cap=0.0, slopes=None, q_p
         _need(workspace, "workspace", torch.uint8, nbytes)
     elif nbytes:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _on(device, "flash_attn_128", lib.mh3_flash_attn_128, ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(ranges),
-        _ptr(slopes), _ptr(q_pos), _ptr(k_pos), _ptr(workspace), 0 if workspace is None else workspace.numel(),
-        out.data_ptr())
+    _on(device, "flash_attn_128", lib.mh3_flash_attn_128_sinks, ref, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        _ptr(ranges), _ptr(sinks), _ptr(slopes), _ptr(q_pos), _ptr(k_pos), _ptr(workspace),
+        0 if workspace is None else workspace.numel(), out.data_ptr())
     return out
 
 
