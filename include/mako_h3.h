@@ -488,6 +488,42 @@ typedef struct MH3PagesWriteArgs {
 int mh3_pages_write(const MH3PagesWriteArgs* args, const uint16_t* k, const uint16_t* v, uint16_t* k_pages,
                     uint16_t* v_pages, const int32_t* table, const int32_t* starts, const int32_t* off,
                     const int32_t* rows, mh3_stream_t stream);
+/* Attention of the streams' new rows over their kept rows in pages and over themselves, bf16, head_dim 128: mh3_flash_attn_128
+ * where the keys lie in pages. Query rows q_off[s] .. q_off[s + 1] - 1 (int32 [streams + 1], ascending) are the new rows of
+ * stream s; k and v hold the same rows' keys and values (in their pages or not: these are not read for them). Row i of a
+ * stream with L = lengths[s] kept rows (int32 [streams], clamped to [0, cols * page_rows]) has place L + depth(i) and attends
+ *   kept row j     if j < L and (j < sinks[s] or j > place(i) - window);
+ *   new row i'     if i' is i or an ancestor of i and (place(i') < sinks[s] or place(i') > place(i) - window).
+ *   parents: int32 [q_rows], a new row's parent among its stream's (0: the first), for trees of drafted rows. A parent lies
+ *            before its row: any other number makes the row a root. NULL: rows follow each other, i' attended if i' <= i.
+ *            depth(i) is the number of i's ancestors.
+ *   window:  0: none. sinks: int32 [streams], how many first rows stay in sight (NULL: none).
+ * A kept row whose entry is no page is not attended. scale, cap, the strides and rounding are mh3_flash_attn_128's, the pools'
+ * strides mh3_pages_write's; page_rows is a multiple of 16. What lies in rows that a row does not attend, in pages past a
+ * stream's length among them, has no effect on any of its bits. Rows of no stream keep what out holds.
+ *   workspace: mh3_flash_attn_pages_128_workspace_bytes(args) bytes; the call overwrites it, so calls that overlap in time,
+ *            two captured graphs among them, need their own.
+ * out may not overlap an input, the pools or the workspace (MH3_ERR_PARAM). */
+typedef struct MH3PagesAttnArgs {
+    MH3PagesArgs table;
+    uint32_t heads; /* query heads, a multiple of kv_heads */
+    uint32_t kv_heads;
+    uint32_t head_dim; /* 128 */
+    uint32_t q_rows;   /* 0: nothing is done */
+    uint32_t window;
+    float scale; /* score scale, up to 2^100; 0 means 1 / sqrt(128) */
+    float cap;   /* tanh cap, 2^-60 .. 1024; 0: none */
+    uint32_t reserved;
+    uint64_t q_head_stride, q_row_stride, k_head_stride, k_row_stride;
+    uint64_t v_head_stride, v_row_stride, out_head_stride, out_row_stride;
+    uint64_t k_page_stride, k_page_head_stride, k_page_row_stride;
+    uint64_t v_page_stride, v_page_head_stride, v_page_row_stride;
+} MH3PagesAttnArgs;
+int64_t mh3_flash_attn_pages_128_workspace_bytes(const MH3PagesAttnArgs* args); /* a negative code for invalid args */
+int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                             const uint16_t* k_pages, const uint16_t* v_pages, const int32_t* table,
+                             const int32_t* lengths, const int32_t* q_off, const int32_t* parents, const int32_t* sinks,
+                             void* workspace, uint64_t workspace_bytes, uint16_t* out, mh3_stream_t stream);
 
 /* ---- int8 weights: quant_rows_i8 (weight side) ---------------------------------------------------------------------
  * Reference kernel `quant_rows_i8` (mako-common; docs/performance.md:122-123, docs/architecture.md:54-56): each row

@@ -34,9 +34,6 @@
 // rare paths, never in the loop of whole tiles.
 #include "attn_tiles.hpp"
 
-#include <algorithm>
-#include <cmath>
-#include <limits>
 #include <type_traits>
 
 namespace mh3 {
@@ -940,17 +937,7 @@ extern "C" int mh3_flash_attn_128_sinks(const MH3DenseAttnArgs* args, const uint
     p.kv_heads = a.kv_heads, p.group = a.heads / a.kv_heads, p.q_rows = a.q_rows, p.kv_rows = a.kv_rows;
     p.list = uint32_t(plans.list);
     p.div_group = FastDiv::make(p.group);
-    const float scale = a.scale > 0.0f ? a.scale : 0.08838834764831845f; // 1 / sqrt(128)
-    int pow = 0;
-    std::frexp(scale, &pow);
-    pow = std::min(std::max(pow, -16), 0);
-    p.q_pow = std::ldexp(1.0f, pow);
-    p.scale_log2 = scale / p.q_pow * kLog2e;
-    // cap_in stays finite, for scores of zero to stay that. It leaves a float's range only where the cap is below 2^-26: no
-    // score is then more than that from zero, whatever its product, and the probabilities are equal in float.
-    if (a.cap > 0.0f)
-        p.cap_in = std::min(2.0f * kLog2e * (scale / p.q_pow) / a.cap, std::numeric_limits<float>::max()),
-        p.cap_out = a.cap * kLog2e;
+    score_factors(a.scale, a.cap, p);
     const bool contest = plans.contest && ranges && !sinks;
     if (contest) {
         const bool pair_first = plans.first.waves == kPairWaves;

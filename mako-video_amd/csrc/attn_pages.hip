@@ -1,0 +1,638 @@
+// `flash_attn_pages_128`: attention of streams' new rows (a single one each, a tree of drafted ones, a chunk) over their kept
+// rows in pages and over themselves, head_dim 128, bf16 in and out, with a window and first rows that stay in sight.
+//   row i of a stream with L kept rows has place L + depth(i), depth the number of its ancestors (without parents: i);
+//   it attends kept row j if j < L and (j < sinks or j > place_i - window), and new row i' if that is i or one of its
+//   ancestors (without parents: i' <= i) and (place_i' < sinks or place_i' > place_i - window);
+//   s = scale q.k, under a cap cap tanh(s / cap); out_i = sum softmax(s)[j] v_j.
+//
+// Design (the tiles, rows and softmax of attn_tiles.hpp, as attn_dense.hip describes them):
+// - A stream's query heads that share a key head are rows of one list, f = row group + g; an item is 32 of them, a key head
+//   and the tiles of 64 keys that they attend: those of the first rows, those of the window, those of the new rows, these
+//   from the last to the first.
+// - A tile is four groups of 16 rows, each in one page: four descriptors, of as many rows as there are and none where the
+//   entry is no page, so that nothing else is read and what is missing is zeros. The page numbers of 16 tiles lie in the
+//   lanes of one register, 16 entries read at once, and come out of it by readlane.
+// - What a row attends of a tile that is not whole is 64 bits: of ranges, or of the row's line of ancestors. Along it the
+//   rows' numbers fall, and so do the tiles', so a row walks its line once, as far as each tile reaches.
+// - Streams are of any lengths, which the host does not know. All items' tiles are one list, and each of as many workgroups
+//   as the chip holds takes an equal run of it, whichever items that cuts: it writes the items that are its own and leaves
+//   parts (O, the maximum, the sum) of the two at its ends. A second kernel joins those in the order of the tiles. Where the
+//   cuts lie follows from the lengths alone.
+#include "attn_tiles.hpp"
+
+namespace mh3 {
+namespace {
+
+struct PagesParams : DenseParams {
+    const uint16_t* k_pages;
+    const uint16_t* v_pages;
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* q_off;
+    const int32_t* parents;
+    const int32_t* first_rows;
+    uint64_t kps, kphs, kprs, vps, vphs, vprs, table_stride; // elements
+    uint32_t streams, cols, pages, page_rows, window, workers, slot_rows;
+    FastDiv div_page;
+};
+
+constexpr uint32_t kLeastTiles = 3; // of a workgroup: below it the join costs more than the tiles
+
+// A stream: its new rows q0 .. q0 + rows - 1, kept rows, and the tiles of its items.
+struct Stream {
+    uint32_t q0, rows, kept, sinks;
+    uint32_t front, near0, near; // tiles of the first rows; the first tile that the window reaches, and how many from it on
+    uint32_t tiles, row_tiles;
+    __device__ __forceinline__ Stream(const PagesParams& p, uint32_t first_q, uint32_t n, uint32_t kept_rows, uint32_t first)
+        : q0(first_q), rows(n), kept(kept_rows), sinks(first)
+    {
+        const uint32_t all = (kept + 63u) / 64u;
+        const uint32_t reach = p.window && p.window - 1u < kept ? kept - (p.window - 1u) : 0u; // of the first new rows
+        near0 = reach < kept ? reach / 64u : all;
+        near = all - near0;
+        front = min((sinks + 63u) / 64u, near0);
+        tiles = front + near + (rows + 63u) / 64u;
+        row_tiles = (rows * p.group + 31u) / 32u;
+    }
+    // The first key of kept tile u.
+    __device__ __forceinline__ uint32_t key(uint32_t u) const { return 64u * (u < front ? u : near0 + u - front); }
+    __device__ __forceinline__ bool is_kept(uint32_t u) const { return u < front + near; }
+    // The first row of the tile of new rows u.
+    __device__ __forceinline__ uint32_t fresh(uint32_t u) const { return 64u * (tiles - 1u - u); }
+};
+
+// A 64-bit value of one lane, for all of them.
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, uint32_t lane)
+{
+    return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), int(lane)))) |
+           uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), int(lane)))) << 32;
+}
+
+// The sum of v over the lanes up to this one.
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, uint32_t lane)
+{
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const uint64_t o = __shfl_up(static_cast<unsigned long long>(v), d, kWave);
+        v += lane >= uint32_t(d) ? o : 0u;
+    }
+    return v;
+}
+
+// The streams 64 at a time, one a lane, and the sums of their items' tiles.
+struct Streams {
+    uint32_t s0, q0, rows, kept, sinks;
+    uint64_t before, units, end; // the lane's stream's; end: of the 64
+    __device__ __forceinline__ void load(const PagesParams& p, uint32_t from, uint64_t base, uint32_t lane)
+    {
+        s0 = from, q0 = rows = kept = sinks = 0, units = 0;
+        const uint32_t s = from + lane;
+        if (s < p.streams) {
+            const uint32_t a = uint32_t(min(max(p.q_off[s], 0), int32_t(p.q_rows)));
+            q0 = a, rows = uint32_t(min(max(p.q_off[s + 1u], int32_t(a)), int32_t(p.q_rows))) - a;
+            kept = uint32_t(min(max(p.lengths[s], 0), int32_t(p.cols * p.page_rows)));
+            sinks = p.first_rows ? min(uint32_t(max(p.first_rows[s], 0)), 1u << 30) : 0u;
+            const Stream t(p, q0, rows, kept, min(sinks, kept));
+            units = uint64_t(t.row_tiles) * p.kv_heads * t.tiles;
+        }
+        const uint64_t sum = wave_scan_u64(units, lane);
+        before = base + sum - units;
+        end = base + lane_u64(sum, kWave - 1);
+    }
+    __device__ __forceinline__ Stream get(const PagesParams& p, uint32_t lane, uint32_t& sinks_of) const
+    {
+        const auto of = [&](uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), int(lane))); };
+        sinks_of = of(sinks);
+        return Stream(p, of(q0), of(rows), of(kept), min(sinks_of, of(kept)));
+    }
+};
+
+// All items' tiles, and a workgroup's share of them.
+__device__ __forceinline__ uint64_t all_units(const PagesParams& p, Streams& st, uint32_t lane)
+{
+    st.load(p, 0u, 0u, lane);
+    while (st.s0 + kWave < p.streams)
+        st.load(p, st.s0 + kWave, st.end, lane);
+    return st.end;
+}
+__device__ __forceinline__ uint64_t share_of(const PagesParams& p, uint64_t units)
+{
+    return max((units + p.workers - 1u) / p.workers, uint64_t(kLeastTiles));
+}
+
+// The offsets of the four instructions that load 16 rows of a K (VALUE false) or V tile, as TileLoads has them.
+template <bool VALUE>
+struct GroupLoads {
+    static constexpr int kOff = VALUE ? 1 : 4;
+    uint32_t row, off[kOff];
+    __device__ __forceinline__ GroupLoads(uint64_t stride, uint32_t lane) : row(uint32_t(stride) * 2u)
+    {
+#pragma unroll
+        for (uint32_t u = 0; u < uint32_t(kOff); ++u) {
+            const uint32_t key = VALUE ? (lane >> 2) & 3u : lane >> 4;
+            const uint32_t chunk = VALUE ? 4u * (lane >> 4) + (lane & 3u) : (lane & 15u) ^ (4u * u + key);
+            off[u] = (4u * u + key) * row + 16u * chunk;
+        }
+    }
+    // Rows 16 g .. of the tile at dst, `rows` of which (the first) lie at `base`; the others are zeros.
+    __device__ __forceinline__ void operator()(char* dst, uint32_t g, const uint16_t* base, uint32_t rows) const
+    {
+        const u32x4_t r = buffer_words(base, rows ? (rows - 1u) * row + 256u : 0u);
+#pragma unroll
+        for (uint32_t u = 0; u < 4u; ++u)
+            load_lds16(r, dst + 4096u * g + 1024u * u, VALUE ? off[0] + 4u * u * row : off[u % uint32_t(kOff)]);
+    }
+};
+
+// A workgroup's item, and what a lane has of it.
+struct Item {
+    Stream st;
+    uint32_t stream, kvh, list, f0;
+    uint32_t sinks;   // as given: new rows may be among the first ones too
+    uint32_t row, up; // the lane's row's number among the new ones; the row of its line that the walk is at (~0: at its end)
+    uint32_t place;   // the row's
+    uint32_t up_place; // that of `up`
+    uint32_t lo;      // kept rows from it on are under the window
+    uint32_t all_lo;  // of every row
+};
+
+// The row's parent, ~0 for none: a parent lies before its row.
+__device__ __forceinline__ uint32_t parent_of(const PagesParams& p, const Item& it, uint32_t row)
+{
+    const uint32_t up = row < it.st.rows ? uint32_t(p.parents[it.st.q0 + row]) : ~0u;
+    return up < row ? up : ~0u;
+}
+
+__device__ __forceinline__ void load_item(const PagesParams& p, Item& it, uint32_t lane, WaveRows& w)
+{
+    const uint32_t n = lane & 31u, hh = lane >> 5, f = it.f0 + n;
+    const uint32_t fc = min(f, it.list - 1u);
+    it.row = p.div_group.div(fc);
+    const uint32_t head = it.kvh * p.group + (fc - it.row * p.group);
+    const uint16_t* const src = p.q + uint64_t(head) * p.qhs + uint64_t(it.st.q0 + it.row) * p.qrs;
+#pragma unroll
+    for (int dc = 0; dc < 8; ++dc) {
+        const uint4 t = f < it.list ? *reinterpret_cast<const uint4*>(src + 16 * dc + 8u * hh) : uint4{0u, 0u, 0u, 0u};
+        uint32_t x[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            x[e] = pack_bf16(bf16_lo(x[e]) * p.q_pow, bf16_hi(x[e]) * p.q_pow);
+        w.qf[dc] = __builtin_bit_cast(bf16x8_t, uint4{x[0], x[1], x[2], x[3]});
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            w.o[b][e] = 0.0f;
+    uint32_t depth = it.row;
+    if (p.parents && p.window) { // only a window asks for the rows' places
+        depth = 0;
+        for (uint32_t up = parent_of(p, it, it.row); up != ~0u; up = parent_of(p, it, up))
+            ++depth;
+    }
+    it.place = it.st.kept + depth;
+    it.up = it.row, it.up_place = it.place;
+    it.lo = p.window && p.window - 1u < it.place ? it.place - (p.window - 1u) : 0u;
+    it.all_lo = wave_max_u32(it.lo);
+    w.m_run = -kInf, w.l_run = 0.0f, w.settled = false, w.begun = false;
+}
+
+// The bits of the lane's row's keys among the 64 new rows from n0 on. Of a tree the tiles are asked for from the last to
+// the first, each once, but need not begin with the last.
+__device__ __forceinline__ uint64_t fresh_bits(const PagesParams& p, Item& it, uint32_t n0)
+{
+    const uint32_t none = it.st.kept < it.sinks ? it.sinks - it.st.kept : 0u; // new rows that are among the first ones
+    if (!p.parents) {
+        const uint32_t lo = it.lo > it.st.kept ? it.lo - it.st.kept : 0u;
+        return key_bits(lo, it.row + 1u, n0) | key_bits(0u, min(none, it.row + 1u), n0);
+    }
+    uint64_t bits = 0;
+    while (it.up != ~0u && it.up >= n0) {
+        if (it.up < n0 + 64u && (!p.window || it.up_place >= it.lo || it.up_place < it.sinks))
+            bits |= uint64_t(1) << (it.up - n0);
+        it.up = parent_of(p, it, it.up), --it.up_place;
+    }
+    return bits;
+}
+
+// What the workgroup loads, tile by tile.
+struct PageFeed {
+    GroupLoads<false> k_page, k_new;
+    GroupLoads<true> v_page, v_new;
+    char* lds; // K, V, the wave's scratch (1 KB)
+    int32_t ids;   // lane 4 (u % 16) + g: the page of group g of tile u, -1 where there is none
+    __device__ __forceinline__ void numbers(const PagesParams& p, const Item& it, uint32_t u16, uint32_t lane)
+    {
+        const uint32_t u = u16 + lane / 4u;
+        ids = -1;
+        if (it.st.is_kept(u)) {
+            const uint32_t key = it.st.key(u) + 16u * (lane % 4u);
+            if (key < it.st.kept) {
+                const int32_t page = p.table[uint64_t(it.stream) * p.table_stride + p.div_page.div(key)];
+                ids = uint32_t(page) < p.pages ? page : -1;
+            }
+        }
+    }
+    __device__ __forceinline__ int32_t number(uint32_t u, uint32_t g) const
+    {
+        return __builtin_amdgcn_readlane(ids, int(4u * (u % 16u) + g));
+    }
+    // The bits of the tile's keys whose page is there.
+    __device__ __forceinline__ uint64_t there(uint32_t u) const
+    {
+        uint64_t bits = 0;
+#pragma unroll
+        for (uint32_t g = 0; g < 4u; ++g)
+            bits |= number(u, g) >= 0 ? uint64_t(0xffff) << (16u * g) : 0u;
+        return bits;
+    }
+    template <bool VALUE>
+    __device__ __forceinline__ void load(const PagesParams& p, const Item& it, uint32_t u) const
+    {
+        char* const dst = lds + (VALUE ? kTileBytes : 0u);
+        if (it.st.is_kept(u)) {
+            const uint32_t t0 = it.st.key(u);
+#pragma unroll
+            for (uint32_t g = 0; g < 4u; ++g) {
+                const int32_t page = number(u, g);
+                const uint32_t key = t0 + 16u * g, r = key - p.div_page.div(key) * p.page_rows;
+                const uint64_t at = VALUE ? uint32_t(max(page, 0)) * p.vps + it.kvh * p.vphs + r * p.vprs
+                                          : uint32_t(max(page, 0)) * p.kps + it.kvh * p.kphs + r * p.kprs;
+                const uint32_t rows = page >= 0 ? min(16u, it.st.kept - key) : 0u;
+                if (VALUE)
+                    v_page(dst, g, p.v_pages + at, rows);
+                else
+                    k_page(dst, g, p.k_pages + at, rows);
+            }
+        } else {
+            const uint32_t n0 = it.st.fresh(u);
+#pragma unroll
+            for (uint32_t g = 0; g < 4u; ++g) {
+                const uint32_t r = n0 + 16u * g, rows = r < it.st.rows ? min(16u, it.st.rows - r) : 0u;
+                const uint64_t row = it.st.q0 + (rows ? r : 0u);
+                if (VALUE)
+                    v_new(dst, g, p.v + it.kvh * p.vhs + row * p.vrs, rows);
+                else
+                    k_new(dst, g, p.k + it.kvh * p.khs + row * p.krs, rows);
+            }
+        }
+    }
+};
+
+// The keys of tile u that the lane's row attends.
+__device__ __forceinline__ uint64_t bits_of(const PagesParams& p, Item& it, const PageFeed& feed, uint32_t u)
+{
+    if (!it.st.is_kept(u))
+        return fresh_bits(p, it, it.st.fresh(u));
+    const uint32_t t0 = it.st.key(u);
+    return (key_bits(it.lo, it.st.kept, t0) | key_bits(0u, it.st.sinks, t0)) & feed.there(u);
+}
+
+// Whether every row attends all of tile u.
+__device__ __forceinline__ bool is_whole(const Item& it, const PageFeed& feed, uint32_t u)
+{
+    if (!it.st.is_kept(u))
+        return false;
+    const uint32_t t0 = it.st.key(u);
+    return t0 + 64u <= it.st.kept && (t0 >= it.all_lo || t0 + 64u <= it.st.sinks) && feed.there(u) == ~uint64_t(0);
+}
+
+// A turn of attn_pages_kernel, tile u, as few_turn of attn_dense.hip: a tile's K is on its way from the products before it
+// to its own, its V from the output before. The page numbers of tile u + 1 are in the feed by its end.
+template <bool CAP, bool MASKED>
+__device__ __forceinline__ void pages_turn(const PagesParams& p, Item& it, WaveRows& w, PageFeed& feed, const TileReads& rd,
+                                           uint32_t u, uint32_t last, uint32_t lane)
+{
+    uint16_t* const scratch = reinterpret_cast<uint16_t*>(feed.lds + 2u * kTileBytes);
+    const char* const vt = feed.lds + kTileBytes;
+    const bool more = u + 1u < last;
+    const BitsSeen seen(MASKED ? bits_of(p, it, feed, u) : 0u, lane);
+    floatx16 s[2];
+    bf16x8_t frag[kAhead];
+    TileP pt;
+    wait_vm<16>(); // K; V may still be in flight
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        frag[j] = rd.k(feed.lds, j);
+    tile_products<false, false>(w, s, pt, frag, rd, feed.lds, nullptr, 0, nullptr, lane);
+    wait_lds();
+    if (more) {
+        if ((u + 1u) % 16u == 0u)
+            feed.numbers(p, it, u + 1u, lane);
+        feed.load<false>(p, it, u + 1u);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    tile_softmax<CAP, false, MASKED>(p, w, s, pt, 0u, seen, nullptr, nullptr, false, false, lane);
+    if (more)
+        wait_vm<16>(); // V, but not the next K
+    else
+        wait_vm<0>();
+    if (MASKED && holds_nonfinite<16>(vt, lane))
+        tile_output_masked(w, pt, rd, vt, seen, scratch, lane);
+    else
+        tile_output(w, pt, frag, rd, vt);
+    wait_lds();
+    if (more)
+        feed.load<true>(p, it, u + 1u);
+}
+
+// Writes an item's rows, or with `slot` a part of them: O [slot][row][128], behind all slots' the maxima and sums.
+__device__ __forceinline__ void store_item(const PagesParams& p, const Item& it, const WaveRows& w, uint32_t slot,
+                                           uint32_t lane)
+{
+    const uint32_t n = lane & 31u, hh = lane >> 5, f = it.f0 + n;
+    const float l = w.l_run + __shfl_xor(w.l_run, 32, kWave);
+    if (f >= it.list)
+        return;
+    if (slot != ~0u) {
+        const uint64_t at = uint64_t(slot) * p.slot_rows + n;
+        float* const dst = p.part + at * 128u;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<float4*>(dst + 32 * db + 8 * g + 4u * hh) =
+                    float4{w.o[db][4 * g], w.o[db][4 * g + 1], w.o[db][4 * g + 2], w.o[db][4 * g + 3]};
+        if (hh == 0)
+            *reinterpret_cast<float2*>(p.part + 2ull * p.workers * p.slot_rows * 128u + at * 2u) = float2{w.m_run, l};
+        return;
+    }
+    const uint32_t head = it.kvh * p.group + (f - it.row * p.group);
+    const float inv = 1.0f / l; // a row attends itself
+    uint16_t* const dst = p.out + uint64_t(head) * p.ohs + uint64_t(it.st.q0 + it.row) * p.ors;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint2*>(dst + 32 * db + 8 * g + 4u * hh) =
+                uint2{pack_bf16(w.o[db][4 * g] * inv, w.o[db][4 * g + 1] * inv),
+                      pack_bf16(w.o[db][4 * g + 2] * inv, w.o[db][4 * g + 3] * inv)};
+}
+
+// One wave a workgroup, with a tile of its own in LDS; four of them share a CU.
+template <bool CAP>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void attn_pages_kernel(PagesParams p)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t lane = threadIdx.x;
+    // Blocks go to the 8 XCDs round-robin; each takes a contiguous part of the list, key head by key head.
+    const uint32_t worker = (blockIdx.x % 8u) * (gridDim.x / 8u) + blockIdx.x / 8u;
+    Streams streams;
+    const uint64_t units = all_units(p, streams, lane), share = share_of(p, units);
+    uint64_t x = share * worker;
+    const uint64_t end = min(units, x + share);
+    if (x >= end)
+        return;
+    if (streams.s0 != 0u)
+        streams.load(p, 0u, 0u, lane);
+    const TileReads rd(lane);
+    PageFeed feed{{p.kprs, lane}, {p.krs, lane}, {p.vprs, lane}, {p.vrs, lane}, lds, -1};
+    while (x < end) {
+        while (x >= streams.end)
+            streams.load(p, streams.s0 + kWave, streams.end, lane);
+        // The last stream that begins at x or before it and has tiles.
+        const uint32_t at = 63u - uint32_t(__builtin_clzll(__ballot(streams.before <= x && streams.units != 0u)));
+        uint32_t sinks;
+        const Stream st = streams.get(p, at, sinks);
+        const uint64_t local = x - lane_u64(streams.before, at), number = local / st.tiles;
+        const uint32_t first = uint32_t(local - number * st.tiles);
+        const uint32_t last = uint32_t(min(uint64_t(st.tiles), first + (end - x)));
+        Item it{st, streams.s0 + at, uint32_t(number / st.row_tiles), st.rows * p.group, 0u, sinks, 0u, 0u, 0u, 0u, 0u, 0u};
+        it.f0 = 32u * uint32_t(number - uint64_t(it.kvh) * st.row_tiles);
+        WaveRows w;
+        feed.numbers(p, it, first & ~15u, lane);
+        feed.load<false>(p, it, first);
+        feed.load<true>(p, it, first);
+        load_item(p, it, lane, w);
+        for (uint32_t u = first; u < last;) {
+#pragma unroll 1
+            for (; u < last && !is_whole(it, feed, u); ++u)
+                pages_turn<CAP, true>(p, it, w, feed, rd, u, last, lane);
+#pragma unroll 1
+            for (; u < last && is_whole(it, feed, u); ++u)
+                pages_turn<CAP, false>(p, it, w, feed, rd, u, last, lane);
+        }
+        // The item that the share begins with, unless with its first tile, is the first of the worker's two parts.
+        const bool cut = first > 0u || last < st.tiles;
+        store_item(p, it, w, cut ? 2u * worker + (first > 0u ? 0u : 1u) : ~0u, lane);
+        x += last - first;
+    }
+}
+
+// Joins the parts of eight list rows of an item, 32 lanes a row, four values of d each, in the order of the tiles.
+__global__ __launch_bounds__(256) void attn_pages_join_kernel(PagesParams p)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    Streams streams;
+    const uint64_t units = all_units(p, streams, lane), share = share_of(p, units);
+    // The stream of this block's rows: kv_heads ceil(list / 8) blocks each.
+    uint64_t block = blockIdx.x, base = 0;
+    uint32_t at = 64u, per = 0;
+    for (uint32_t s0 = 0; s0 < p.streams; s0 += kWave) {
+        streams.load(p, s0, base, lane);
+        base = streams.end;
+        const uint32_t eights = (streams.rows * p.group + 7u) / 8u;
+        const uint64_t mine = uint64_t(eights) * p.kv_heads, sum = wave_scan_u64(mine, lane);
+        const uint64_t all = lane_u64(sum, kWave - 1);
+        if (block < all) {
+            at = uint32_t(__builtin_ctzll(__ballot(block < sum)));
+            block -= lane_u64(sum - mine, at);
+            per = uint32_t(__builtin_amdgcn_readlane(int(eights), int(at)));
+            break;
+        }
+        block -= all;
+    }
+    if (at == 64u)
+        return;
+    uint32_t sinks;
+    const Stream st = streams.get(p, at, sinks);
+    const uint32_t kvh = uint32_t(block / per), f = 8u * uint32_t(block - uint64_t(kvh) * per) + threadIdx.x / 32u;
+    const uint64_t x0 = lane_u64(streams.before, at) + (uint64_t(kvh) * st.row_tiles + f / 32u) * st.tiles, x1 = x0 + st.tiles;
+    const uint32_t w0 = uint32_t(x0 / share), w1 = uint32_t((x1 - 1u) / share);
+    if (f >= st.rows * p.group || w0 == w1)
+        return;
+    const float2* const ml = reinterpret_cast<const float2*>(p.part + 2ull * p.workers * p.slot_rows * 128u);
+    const uint32_t n = f % 32u, d = 4u * (threadIdx.x & 31u);
+    constexpr uint32_t kU = 8;
+    float m = -kInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t i0 = w0; i0 <= w1; i0 += kU) {
+        float2 t[kU];
+        float4 v[kU];
+#pragma unroll
+        for (uint32_t u = 0; u < kU; ++u) {
+            const uint32_t i = i0 + u;
+            t[u] = float2{-kInf, 0.0f}, v[u] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (i <= w1) {
+                const uint64_t slot = (2ull * i + (share * i <= x0 ? 1u : 0u)) * p.slot_rows + n;
+                t[u] = ml[slot], v[u] = *reinterpret_cast<const float4*>(p.part + slot * 128u + d);
+            }
+        }
+        float m_new = m;
+#pragma unroll
+        for (uint32_t u = 0; u < kU; ++u)
+            m_new = fmaxf(m_new, t[u].x);
+        // A part without a key of this row has left zeros and -inf. (A NaN of its scores is in its sum and its O.)
+        const float old = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+        l *= old, m = m_new;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            o[c] *= old;
+#pragma unroll
+        for (uint32_t u = 0; u < kU; ++u) {
+            const float e = t[u].x == -kInf ? 1.0f : __builtin_amdgcn_exp2f(t[u].x - m_new);
+            l = fmaf(t[u].y, e, l);
+            o[0] = fmaf(v[u].x, e, o[0]), o[1] = fmaf(v[u].y, e, o[1]);
+            o[2] = fmaf(v[u].z, e, o[2]), o[3] = fmaf(v[u].w, e, o[3]);
+        }
+    }
+    const float inv = 1.0f / l;
+    const uint32_t row = p.div_group.div(f), head = kvh * p.group + (f - row * p.group);
+    *reinterpret_cast<uint2*>(p.out + uint64_t(head) * p.ohs + uint64_t(st.q0 + row) * p.ors + d) =
+        uint2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+}
+
+} // namespace
+} // namespace mh3
+
+namespace {
+
+using namespace mh3;
+
+constexpr size_t kPagesLds = 2u * kTileBytes + 1024u;
+
+uint32_t workers_of() { return (4u * uint32_t(std::max(host::cu_count(), 1)) + 7u) / 8u * 8u; }
+
+// Rows of a part: an item's, or all of the call's where they are fewer.
+uint32_t slot_rows_of(const MH3PagesAttnArgs& a)
+{
+    return uint32_t(std::min<uint64_t>(32u, uint64_t(a.q_rows) * (a.heads / a.kv_heads)));
+}
+
+uint64_t pages_workspace(const MH3PagesAttnArgs& a) { return 2ull * workers_of() * slot_rows_of(a) * 130u * 4u; }
+
+int check_pages_args(const MH3PagesAttnArgs* args)
+{
+    if (!args)
+        return MH3_ERR_POINTER;
+    const MH3PagesAttnArgs& a = *args;
+    const MH3PagesArgs& t = a.table;
+    if (a.heads == 0 || a.kv_heads == 0 || a.head_dim == 0 || a.heads % a.kv_heads != 0)
+        return MH3_ERR_SHAPE;
+    if (a.head_dim != 128u)
+        return MH3_ERR_UNSUPPORTED;
+    if (!(a.scale >= 0.0f && a.scale <= 0x1p100f) || !(a.cap == 0.0f || (a.cap >= 0x1p-60f && a.cap <= 1024.0f)))
+        return MH3_ERR_PARAM;
+    if (t.streams == 0 || t.streams > MH3_MAX_STREAMS || t.cols == 0 || t.cols >= (1u << 24) || t.pages == 0 ||
+        t.pages >= (1u << 24) || t.table_stride < t.cols || t.table_stride >= (1ull << 32) || t.page_rows == 0 ||
+        t.page_rows % 16u != 0 || uint64_t(t.cols) * t.page_rows >= (1ull << 30))
+        return MH3_ERR_SHAPE;
+    if (a.heads > 4096u || uint64_t(a.q_rows) * (a.heads / a.kv_heads) >= (1u << 30) || a.q_rows >= (1u << 30))
+        return MH3_ERR_SHAPE;
+    for (const uint64_t s : {a.q_row_stride, a.k_row_stride, a.v_row_stride, a.out_row_stride, a.k_page_row_stride,
+                             a.v_page_row_stride}) {
+        if (s % 8u != 0)
+            return MH3_ERR_ALIGN;
+        if (s < 128u || s >= (1ull << 23)) // 64 rows of a tile in 32-bit byte offsets
+            return MH3_ERR_SHAPE;
+    }
+    for (const uint64_t s : {a.q_head_stride, a.k_head_stride, a.v_head_stride, a.out_head_stride, a.k_page_stride,
+                             a.k_page_head_stride, a.v_page_stride, a.v_page_head_stride}) {
+        if (s % 8u != 0)
+            return MH3_ERR_ALIGN;
+        if (s >= (1ull << 36))
+            return MH3_ERR_SHAPE;
+    }
+    return MH3_OK;
+}
+
+template <bool CAP>
+int launch_pages(const PagesParams& p, hipStream_t stream)
+{
+    const auto kernel = attn_pages_kernel<CAP>;
+    if (const hipError_t e = host::allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kPagesLds); e != hipSuccess)
+        return host::hip_error(e);
+    hipLaunchKernelGGL(kernel, dim3(p.workers), dim3(64), kPagesLds, stream, p);
+    return host::check_launch();
+}
+
+} // namespace
+
+extern "C" int64_t mh3_flash_attn_pages_128_workspace_bytes(const MH3PagesAttnArgs* args)
+{
+    if (const int rc = check_pages_args(args); rc != MH3_OK)
+        return rc;
+    return int64_t(pages_workspace(*args));
+}
+
+extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint16_t* q, const uint16_t* k,
+                                        const uint16_t* v, const uint16_t* k_pages, const uint16_t* v_pages,
+                                        const int32_t* table, const int32_t* lengths, const int32_t* q_off,
+                                        const int32_t* parents, const int32_t* sinks, void* workspace,
+                                        uint64_t workspace_bytes, uint16_t* out, mh3_stream_t stream)
+{
+    if (const int rc = check_pages_args(args); rc != MH3_OK)
+        return rc;
+    const MH3PagesAttnArgs& a = *args;
+    const MH3PagesArgs& t = a.table;
+    if (a.q_rows == 0)
+        return MH3_OK;
+    const uint64_t need = pages_workspace(a);
+    if (!q || !k || !v || !k_pages || !v_pages || !table || !lengths || !q_off || !workspace || !out)
+        return MH3_ERR_POINTER;
+    if (workspace_bytes < need)
+        return MH3_ERR_SHAPE;
+    if (!host::aligned16(q) || !host::aligned16(k) || !host::aligned16(v) || !host::aligned16(k_pages) ||
+        !host::aligned16(v_pages) || !host::aligned16(workspace) || !host::aligned16(out) ||
+        (reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(q_off) |
+         reinterpret_cast<uintptr_t>(parents) | reinterpret_cast<uintptr_t>(sinks)) %
+                4u !=
+            0u)
+        return MH3_ERR_ALIGN;
+    // out's rows apart from each other: heads one behind the other, or side by side in a row.
+    const bool behind = a.heads == 1u || a.out_head_stride >= (a.q_rows - 1u) * a.out_row_stride + 128u;
+    const bool beside = a.out_head_stride >= 128u &&
+                        (a.q_rows == 1u || a.out_row_stride >= (a.heads - 1u) * a.out_head_stride + 128u);
+    if (!behind && !beside)
+        return MH3_ERR_PARAM;
+    const auto span = [&](uint64_t heads, uint64_t hs, uint64_t rs) {
+        return ((heads - 1u) * hs + (a.q_rows - 1ull) * rs + 128u) * 2u;
+    };
+    const auto pool = [&](uint64_t ps, uint64_t hs, uint64_t rs) {
+        return ((t.pages - 1ull) * ps + (a.kv_heads - 1ull) * hs + (t.page_rows - 1ull) * rs + 128u) * 2u;
+    };
+    const host::Span in[] = {{q, span(a.heads, a.q_head_stride, a.q_row_stride)},
+                             {k, span(a.kv_heads, a.k_head_stride, a.k_row_stride)},
+                             {v, span(a.kv_heads, a.v_head_stride, a.v_row_stride)},
+                             {k_pages, pool(a.k_page_stride, a.k_page_head_stride, a.k_page_row_stride)},
+                             {v_pages, pool(a.v_page_stride, a.v_page_head_stride, a.v_page_row_stride)},
+                             {table, ((t.streams - 1ull) * t.table_stride + t.cols) * 4u},
+                             {lengths, t.streams * 4ull},
+                             {q_off, (t.streams + 1ull) * 4u},
+                             {parents, a.q_rows * 4ull},
+                             {sinks, t.streams * 4ull}};
+    const host::Span o[] = {{out, span(a.heads, a.out_head_stride, a.out_row_stride)}, {workspace, need}};
+    if (host::any_overlap(in, o))
+        return MH3_ERR_PARAM;
+    // A block of the join for every eight list rows of a key head, and one more a stream for what is left of eight.
+    const uint64_t blocks = uint64_t(a.kv_heads) * (uint64_t(a.q_rows) * (a.heads / a.kv_heads) / 8u + t.streams);
+    if (blocks >= (1ull << 31))
+        return MH3_ERR_SHAPE;
+    PagesParams p{};
+    p.q = q, p.k = k, p.v = v, p.out = out, p.k_pages = k_pages, p.v_pages = v_pages;
+    p.table = table, p.lengths = lengths, p.q_off = q_off, p.parents = parents, p.first_rows = sinks;
+    p.part = static_cast<float*>(workspace);
+    p.qhs = a.q_head_stride, p.qrs = a.q_row_stride, p.khs = a.k_head_stride, p.krs = a.k_row_stride;
+    p.vhs = a.v_head_stride, p.vrs = a.v_row_stride, p.ohs = a.out_head_stride, p.ors = a.out_row_stride;
+    p.kps = a.k_page_stride, p.kphs = a.k_page_head_stride, p.kprs = a.k_page_row_stride;
+    p.vps = a.v_page_stride, p.vphs = a.v_page_head_stride, p.vprs = a.v_page_row_stride;
+    p.table_stride = t.table_stride, p.streams = t.streams, p.cols = t.cols, p.pages = t.pages;
+    p.page_rows = t.page_rows, p.window = a.window, p.div_page = FastDiv::make(t.page_rows);
+    p.kv_heads = a.kv_heads, p.group = a.heads / a.kv_heads, p.q_rows = a.q_rows, p.div_group = FastDiv::make(p.group);
+    p.workers = workers_of(), p.slot_rows = slot_rows_of(a);
+    score_factors(a.scale, a.cap, p);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (const int rc = a.cap > 0.0f ? launch_pages<true>(p, s) : launch_pages<false>(p, s); rc != MH3_OK)
+        return rc;
+    hipLaunchKernelGGL(attn_pages_join_kernel, dim3(uint32_t(blocks)), dim3(256), 0, s, p);
+    return host::check_launch();
+}

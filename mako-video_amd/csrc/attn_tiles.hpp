@@ -4,6 +4,10 @@
 
 #include "mh3_common.hpp"
 
+#include <algorithm>
+#include <cmath>
+#include <limits>
+
 namespace mh3 {
 namespace {
 
@@ -676,6 +680,22 @@ __device__ __forceinline__ bool holds_nonfinite(const char* part, uint32_t lane)
             top = __builtin_elementwise_max(top, __builtin_bit_cast(ushortx2, t[e] & 0x7fff7fffu));
     }
     return __ballot(top[0] >= 0x7f80u || top[1] >= 0x7f80u) != 0u;
+}
+
+// The factors of the scores from `scale` (0: 1 / sqrt(128)) and `cap` (0: none).
+inline void score_factors(float scale_given, float cap, DenseParams& p)
+{
+    const float scale = scale_given > 0.0f ? scale_given : 0.08838834764831845f; // 1 / sqrt(128)
+    int pow = 0;
+    std::frexp(scale, &pow);
+    pow = std::min(std::max(pow, -16), 0);
+    p.q_pow = std::ldexp(1.0f, pow);
+    p.scale_log2 = scale / p.q_pow * kLog2e;
+    // cap_in stays finite, for scores of zero to stay that. It leaves a float's range only where the cap is below 2^-26: no
+    // score is then more than that from zero, whatever its product, and the probabilities are equal in float.
+    if (cap > 0.0f)
+        p.cap_in = std::min(2.0f * kLog2e * (scale / p.q_pow) / cap, std::numeric_limits<float>::max()),
+        p.cap_out = cap * kLog2e;
 }
 
 } // namespace

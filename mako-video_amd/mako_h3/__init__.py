@@ -94,6 +94,14 @@ class PagesWriteArgs(C.Structure):
                [(f"{t}_{d}_stride", C.c_uint64) for t in ("k", "v") for d in ("page", "page_head", "page_row")]
 
 
+class PagesAttnArgs(C.Structure):
+    _fields_ = [("table", PagesArgs), ("heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("q_rows", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float), ("cap", C.c_float),
+                ("reserved", C.c_uint32)] + \
+               [(f"{t}_{d}_stride", C.c_uint64) for t in ("q", "k", "v", "out") for d in ("head", "row")] + \
+               [(f"{t}_{d}_stride", C.c_uint64) for t in ("k", "v") for d in ("page", "page_head", "page_row")]
+
+
 class CubeMapArgs(C.Structure):
     _fields_ = [("grid_t", C.c_uint32), ("grid_h", C.c_uint32), ("grid_w", C.c_uint32), ("n_dense", C.c_uint32),
                 ("video_row0", C.c_uint64), ("dense_row0", C.c_uint64)]
@@ -166,6 +174,8 @@ def _load() -> C.CDLL:
         "mh3_pages_compact_workspace_bytes": (I64, [C.POINTER(PagesArgs)]),
         "mh3_pages_compact": (I32, [C.POINTER(PagesArgs), C.POINTER(Pool), U32] + [P] * 5 + [C.c_uint64, P]),
         "mh3_pages_write": (I32, [C.POINTER(PagesWriteArgs)] + [P] * 9),
+        "mh3_flash_attn_pages_128_workspace_bytes": (I64, [C.POINTER(PagesAttnArgs)]),
+        "mh3_flash_attn_pages_128": (I32, [C.POINTER(PagesAttnArgs)] + [P] * 11 + [C.c_uint64, P, P]),
         "mh3_quant_rows_mx4": (I32, [C.POINTER(QuantArgs), P, P, P, P]),
         "mh3_gemm_mx4": (I32, [C.POINTER(GemmArgs), P, P, P, P, P, P]),
         "mh3_gemm_mx4_swiglu": (I32, [C.POINTER(GemmArgs), P, P, P, P, P, P]),
@@ -1116,6 +1126,80 @@ def pages_write(k, v, k_pages, v_pages, table, starts, off, *, rows=None, layout
     device = _one_device(k=k, v=v, k_pages=k_pages, v_pages=v_pages, table=table, starts=starts, off=off, rows=rows)
     _on(device, "pages_write", lib.mh3_pages_write, C.byref(a), k.data_ptr(), v.data_ptr(), k_pages.data_ptr(),
         v_pages.data_ptr(), table.data_ptr(), starts.data_ptr(), off.data_ptr(), _ptr(rows))
+
+
+def _pages_attn_args(q, k, v, k_pages, v_pages, table, window, scale, cap, layout, page_layout) -> PagesAttnArgs:
+    if layout not in ("heads", "rows") or page_layout not in ("heads", "rows"):
+        raise ValueError("layout is 'heads' or 'rows'")
+    heads, q_rows, qhs, qrs = _head_rows(q, "q", layout)
+    kv_heads, k_rows, khs, krs = _head_rows(k, "k", layout)
+    v_heads, v_rows, vhs, vrs = _head_rows(v, "v", layout)
+    if k_rows != q_rows or v_rows != q_rows or v_heads != kv_heads:
+        raise ValueError("k and v: q's rows, and the same heads")
+    pages, pool_heads, page_rows, *k_strides = _page_rows(k_pages, "k_pages", page_layout)
+    shape = _page_rows(v_pages, "v_pages", page_layout)
+    if pool_heads != kv_heads or shape[:3] != (pages, kv_heads, page_rows):
+        raise ValueError("k_pages and v_pages: the heads of k and v, the same pages and rows")
+    if not 0 <= window <= 0xffffffff:
+        raise ValueError("window: 0 (none) or the keys that a row sees, its own among them")
+    return PagesAttnArgs(_page_table(table, pages, page_rows), heads, kv_heads, 128, q_rows, window, scale, cap, 0, qhs,
+                         qrs, khs, krs, vhs, vrs, 0, 128, *k_strides, *shape[3:])
+
+
+def flash_attn_pages_128_workspace_bytes(q, k, v, k_pages, v_pages, table, *, layout="heads", page_layout="heads") -> int:
+    """Bytes of workspace that flash_attn_pages_128 needs for these operands on the current device."""
+    a = _pages_attn_args(q, k, v, k_pages, v_pages, table, 0, 0.0, 0.0, layout, page_layout)
+    n = int(lib.mh3_flash_attn_pages_128_workspace_bytes(C.byref(a)))
+    _check(min(n, 0), "flash_attn_pages_128_workspace_bytes")
+    return n
+
+
+def flash_attn_pages_128(q, k, v, k_pages, v_pages, table, lengths, q_off, *, parents=None, window=0, sinks=None,
+                         scale=0.0, cap=0.0, layout="heads", page_layout="heads", out=None, out_layout=None,
+                         workspace=None):
+    """Attention of streams' new rows over their kept rows in pages and over themselves, head_dim 128, bf16. Rows q_off[s]
+    .. q_off[s + 1] - 1 (int32 [streams + 1]) of q, k and v are stream s's; row i of a stream with lengths[s] kept rows
+    (int32 [streams]) has place lengths[s] + depth(i). It attends the kept rows and, of the new ones, itself and those
+    before it, or with `parents` (int32 [q_rows], numbers within the stream, -1: none) itself and its ancestors, of which
+    depth(i) is the number. window (0: none): only those less than `window` places back, and the stream's first sinks[s]
+    rows (int32 [streams]). Table and pools as in pages_write; scale, cap and the layouts as in flash_attn_128. Rows of no
+    stream keep what `out` holds (zeros when it is None). `workspace` (uint8, at least
+    flash_attn_pages_128_workspace_bytes) is allocated here when None. Returns out."""
+    out_layout = layout if out_layout is None else out_layout
+    if out_layout not in ("heads", "rows"):
+        raise ValueError("layout is 'heads' or 'rows'")
+    a = _pages_attn_args(q, k, v, k_pages, v_pages, table, window, scale, cap, layout, page_layout)
+    heads, q_rows, streams = a.heads, a.q_rows, a.table.streams
+    device = _one_device(q=q, k=k, v=v, k_pages=k_pages, v_pages=v_pages, table=table, lengths=lengths, q_off=q_off,
+                         parents=parents, sinks=sinks, out=out, workspace=workspace)
+    if device != torch._C._cuda_getDevice():  # the workspace's size is of the current device
+        with torch.cuda.device(device):
+            return flash_attn_pages_128(q, k, v, k_pages, v_pages, table, lengths, q_off, parents=parents, window=window,
+                                        sinks=sinks, scale=scale, cap=cap, layout=layout, page_layout=page_layout, out=out,
+                                        out_layout=out_layout, workspace=workspace)
+    if out is None:
+        out = torch.zeros((heads, q_rows, 128) if out_layout == "heads" else (q_rows, heads * 128),
+                          dtype=torch.bfloat16, device=device)
+    out_heads, out_rows, a.out_head_stride, a.out_row_stride = _head_rows(out, "out", out_layout)
+    if out_heads != heads or out_rows != q_rows:
+        raise ValueError("out: q's heads and rows")
+    _need(lengths, "lengths", torch.int32, streams)
+    _need(q_off, "q_off", torch.int32, streams + 1)
+    if parents is not None:
+        _need(parents, "parents", torch.int32, q_rows)
+    if sinks is not None:
+        _need(sinks, "sinks", torch.int32, streams)
+    ref = C.byref(a)
+    nbytes = lib.mh3_flash_attn_pages_128_workspace_bytes(ref)
+    if nbytes < 0:
+        _check(nbytes, "flash_attn_pages_128")
+    if workspace is None:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _need(workspace, "workspace", torch.uint8, nbytes)
+    _on(device, "flash_attn_pages_128", lib.mh3_flash_attn_pages_128, ref, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), q_off.data_ptr(), _ptr(parents),
+        _ptr(sinks), workspace.data_ptr(), workspace.numel(), out.data_ptr())
+    return out
 
 
 # ---- flash_attn_sparse_128 -------------------------------------------------------------------------------------------
