@@ -283,13 +283,6 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     store_rows(p, w, kvh, tile * 32u, split, lane);
 }
 
-// Many rows: eight waves of 32 list rows, in two groups of four, one wave of each group on a SIMD. A group's turn at a
-// tile has two phases, the products (S of this tile, and O of the one before) and the softmax, and the groups are a phase
-// apart, held there by the barriers: while one group's wave has the matrix core of a SIMD the other's has its vector unit.
-// K and V lie in rings of four tiles; a tile's loads go out three of its K (two of its V) ahead of its use, each wave an
-// eighth.
-constexpr uint32_t kPairWaves = 8, kRing = 4;
-
 // What a wave loads of a workgroup's tiles, a call a tile: its eighth of K (with all of the tile's key positions, into the
 // wave's own ring) or of V. After the workgroup's last tile the same again, so that every turn has the same count of loads;
 // these are not read. The state is scalar and moves by additions.
@@ -342,77 +335,27 @@ struct PairFeed {
     }
 };
 
-// tile_output where the tile may have been masked; odd: the eight waves' words from holds_nonfinite for it (null: it was
-// whole).
-template <class Seen>
-__device__ __forceinline__ void masked_output(WaveRows& w, const TileP& pt, bf16x8_t (&frag)[kAhead], const TileReads& rd,
-                                              const char* vt, const Seen& seen, const uint32_t* odd, uint16_t* scratch,
-                                              uint32_t lane)
-{
-    uint32_t any = 0;
-    if (odd) {
-        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(odd), b = *reinterpret_cast<const u32x4_t*>(odd + 4);
-        any = a[0] | a[1] | a[2] | a[3] | b[0] | b[1] | b[2] | b[3];
+// The tiles of a workgroup's walk over two parts.
+template <bool BIAS>
+struct PairWalk {
+    const Walk& walk;
+    uint32_t first, last;
+    uint32_t all_lo, all_hi, all_s_lo, all_s_hi;
+    const uint4* rows; // the wave's rows' ranges
+    uint32_t lane;
+    __device__ __forceinline__ uint32_t key(uint32_t t) const { return walk.key(BIAS ? last - 1u - t : first + t); }
+    __device__ __forceinline__ bool whole(uint32_t t) const
+    {
+        const uint32_t t0 = key(t);
+        return (t0 >= all_lo && t0 + 64u <= all_hi) || (t0 >= all_s_lo && t0 + 64u <= all_s_hi);
     }
-    if (__builtin_amdgcn_readfirstlane(any))
-        tile_output_masked(w, pt, rd, vt, seen, scratch, lane);
-    else
-        tile_output(w, pt, frag, rd, vt);
-}
-
-// Whether the wave has work in the tile at key t0.
-template <bool SINKS>
-__device__ __forceinline__ bool meets(const WaveRows& w, uint32_t t0, uint32_t lane)
-{
-    return SINKS ? __ballot(BitsSeen(w, t0, lane).any()) != 0 : w.meets(t0);
-}
-
-// A turn of attn_pair_kernel, tile t at key t0, the one before it at `before`. MASKED: this tile or the one before it is not whole for every row of the
-// workgroup, or there is none before it; checked: the turn before was of this form too.
-template <bool CAP, bool BIAS, bool SINKS, bool MASKED>
-__device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, PairFeed<BIAS, SINKS>& feed,
-                                          const TileReads& rd, floatx16 (&s)[2], bf16x8_t (&frag)[kAhead], TileP& pt,
-                                          uint16_t* scratch, uint32_t* odd, bool checked, uint32_t wave, uint32_t t,
-                                          uint32_t t0, uint32_t before, uint32_t lane)
-{
-    // The products.
-    __builtin_amdgcn_s_setprio(1);
-    constexpr bool kSloped = BIAS && !CAP && !MASKED;
-    float* const near_pos = reinterpret_cast<float*>(scratch);
-    int32_t pos = 0;
-    if (kSloped)
-        pos = feed.positions(t)[lane], pos = p.k_pos ? pos : int32_t(t0 + lane);
-    bool near = false;
-    if (!MASKED || meets<SINKS>(w, t0, lane))
-        near = tile_products<!MASKED, kSloped>(w, s, pt, frag, rd, feed.k_tile(t), feed.v_tile(t - 1u), pos, near_pos, lane);
-    if (MASKED) {
-        if (t > 0 && meets<SINKS>(w, before, lane))
-            masked_output(w, pt, frag, rd, feed.v_tile(t - 1u), Seen<SINKS>(w, before, lane),
-                          checked ? odd + kPairWaves * ((t - 1u) % 2u) : nullptr, scratch, lane);
-        // The part of V that this wave loaded: every wave's word is read at the next products, a barrier on.
-        const bool any = holds_nonfinite<2>(feed.v_tile(t) + 2048u * wave, lane);
-        if (lane == 0)
-            odd[kPairWaves * (t % 2u) + wave] = any;
-        wait_lds();
+    __device__ __forceinline__ BitsSeen seen(uint32_t t) const
+    {
+        const uint4 r = rows[lane & 31u];
+        const uint32_t t0 = key(t);
+        return BitsSeen(key_bits(r.x, r.y, t0) | key_bits(r.z, r.w, t0), lane);
     }
-    __builtin_amdgcn_s_setprio(0);
-    phase_barrier();
-    // The softmax. With it go out K of tile t + 3, into the slot of tile t - 1, which both groups have read, and V of tile
-    // t + 2 into that of tile t - 2 (among the products they cost 10%: this phase is the shorter one).
-    feed.k();
-    feed.v();
-    if (!MASKED || meets<SINKS>(w, t0, lane))
-        tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, Seen<SINKS>(w, t0, lane), feed.positions(t), near_pos, kSloped,
-                                        near, lane);
-    // Past the last tile these are some tile's again, and not used.
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-        frag[j] = rd.k(feed.k_tile(t + 1u), j);
-    // K of tile t + 2 and V of tile t + 1 have arrived, all but this turn's loads: both groups are past their barriers by
-    // the time that either reads them.
-    wait_vm<PairFeed<BIAS, SINKS>::kLoads>();
-    phase_barrier();
-}
+};
 
 template <bool CAP, bool BIAS, bool SINKS>
 __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_pair_kernel(DenseParams p)
@@ -429,13 +372,18 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
         if (blockIdx.x == 0 && tid == 0)
             *p.contest.winner = p.splits;
     }
-    uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kRing * kTileBytes + 2048u * wave);
-    uint32_t* const span = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + 2048u * kPairWaves);
+    constexpr uint32_t kWaveBytes = SINKS ? 2048u + 512u : 2048u;
+    uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kRing * kTileBytes + kWaveBytes * wave);
+    uint32_t* const span = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + kWaveBytes * kPairWaves);
     const uint32_t f0 = (tile * kPairWaves + wave) * 32u;
     WaveRows w;
     load_rows<CAP, BIAS, SINKS>(p, kvh, f0, lane, w);
     uint32_t* const odd = span + 4u * kPairWaves; // [2][kPairWaves]: a masked tile's V holds an infinity or a NaN
     uint32_t* const s_span = odd + 2u * kPairWaves; // SINKS
+    // SINKS: the rows' ranges, out of the registers: only masked turns ask for them.
+    uint4* const rows = reinterpret_cast<uint4*>(scratch + 1024u);
+    if (SINKS && lane < 32u)
+        rows[lane] = uint4{w.lo, w.hi, w.s_lo, w.s_hi};
     if (lane == 0) {
         *reinterpret_cast<uint4*>(span + 4u * wave) = uint4{w.any_lo, w.any_hi, w.all_lo, w.all_hi};
         if (SINKS)
@@ -516,6 +464,14 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     feed.v();
     feed.k();
     feed.v();
+    if (SINKS) {
+        PairWalk<BIAS> turns{walk, first, last, all_lo, all_hi, all_s_lo, all_s_hi, rows, lane};
+        pair_walk<CAP, BIAS>(p, w, feed, turns, rd, scratch, odd, wave, tiles, lane);
+        const uint4 r = rows[lane & 31u];
+        w.lo = r.x, w.hi = r.y;
+        store_rows(p, w, kvh, f0, split, lane);
+        return;
+    }
     wait_vm<PairFeed<BIAS, SINKS>::kLoads>(); // K of tiles 0 and 1, V of tile 0
     lds_barrier();
     const bool second = wave >= kPairWaves / 2u;
@@ -527,56 +483,33 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
         frag[j] = rd.k(lds, j);
-    bool masked = true; // the last turn's form
-    if (SINKS) {
-        const auto whole = [&](uint32_t t) {
-            const uint32_t t0 = key_of(t);
-            return (t0 >= all_lo && t0 + 64u <= all_hi) || (t0 >= all_s_lo && t0 + 64u <= all_s_hi);
-        };
-        for (uint32_t t = 0; t < tiles;) {
-#pragma unroll 1
-            do {
-                pair_turn<CAP, BIAS, SINKS, true>(p, w, feed, rd, s, frag, pt, scratch, odd, masked, wave, t, key_of(t),
-                                                  key_of(t - 1u), lane);
-                masked = true, ++t;
-            } while (t < tiles && !(whole(t) && whole(t - 1u)));
-#pragma unroll 1
-            for (; t < tiles && whole(t); ++t) {
-                pair_turn<CAP, BIAS, SINKS, false>(p, w, feed, rd, s, frag, pt, scratch, odd, true, wave, t, key_of(t),
-                                                   0u, lane);
-                masked = false;
-            }
-        }
-    } else {
-        // The turns in between, whose own tile and the one before are whole for every row of the workgroup, in a loop of
-        // their own: one body with both forms copies O between them at every tile.
-        uint32_t a = min(all_lo > k0 ? (all_lo - k0 + 63u) / 64u : 0u, tiles);
-        uint32_t b = min(all_hi > k0 ? (all_hi - k0) / 64u : 0u, tiles);
-        if (BIAS) {
-            const uint32_t t = tiles - a;
-            a = tiles - b, b = t;
-        }
-        a = min(a + 1u, tiles), b = max(a, b);
-#pragma unroll 1
-        for (uint32_t t = 0; t < a; ++t)
-            pair_turn<CAP, BIAS, SINKS, true>(p, w, feed, rd, s, frag, pt, scratch, odd, true, wave, t, key_of(t),
-                                              key_of(t - 1u), lane);
-#pragma unroll 1
-        for (uint32_t t = a; t < b; ++t)
-            pair_turn<CAP, BIAS, SINKS, false>(p, w, feed, rd, s, frag, pt, scratch, odd, true, wave, t, key_of(t), 0u,
-                                               lane);
-#pragma unroll 1
-        for (uint32_t t = b; t < tiles; ++t)
-            pair_turn<CAP, BIAS, SINKS, true>(p, w, feed, rd, s, frag, pt, scratch, odd, t > b || a == b, wave, t,
-                                              key_of(t), key_of(t - 1u), lane);
-        masked = b < tiles || a == tiles;
+    // The turns in between, whose own tile and the one before are whole for every row of the workgroup, in a loop of their
+    // own: one body with both forms copies O between them at every tile.
+    uint32_t a = min(all_lo > k0 ? (all_lo - k0 + 63u) / 64u : 0u, tiles);
+    uint32_t b = min(all_hi > k0 ? (all_hi - k0) / 64u : 0u, tiles);
+    if (BIAS) {
+        const uint32_t t = tiles - a;
+        a = tiles - b, b = t;
     }
+    a = min(a + 1u, tiles), b = max(a, b);
+    const auto seen = [&](uint32_t t) { return RangeSeen(w, key_of(t), lane); };
+#pragma unroll 1
+    for (uint32_t t = 0; t < a; ++t)
+        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, odd, true, wave, t, key_of(t), seen(t),
+                                   seen(t - 1u), lane);
+#pragma unroll 1
+    for (uint32_t t = a; t < b; ++t)
+        pair_turn<CAP, BIAS, false>(p, w, feed, rd, s, frag, pt, scratch, odd, true, wave, t, key_of(t), seen(t), seen(t),
+                                    lane);
+#pragma unroll 1
+    for (uint32_t t = b; t < tiles; ++t)
+        pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, odd, t > b || a == b, wave, t, key_of(t), seen(t),
+                                   seen(t - 1u), lane);
     const uint32_t end = tiles - 1u;
-    if (!meets<SINKS>(w, key_of(end), lane))
+    if (!w.meets(key_of(end)))
         ; // nothing of it is this wave's
-    else if (masked)
-        masked_output(w, pt, frag, rd, feed.v_tile(end), Seen<SINKS>(w, key_of(end), lane),
-                      odd + kPairWaves * (end % 2u), scratch, lane);
+    else if (b < tiles || a == tiles) // the last turn was of the masked form
+        masked_output(w, pt, frag, rd, feed.v_tile(end), seen(end), odd + kPairWaves * (end % 2u), scratch, lane);
     else
         tile_output(w, pt, frag, rd, feed.v_tile(end));
     if (!second)
@@ -852,7 +785,7 @@ int launch_form(const DenseParams& p, uint32_t waves, hipStream_t stream)
 {
     if (waves == kPairWaves)
         return launch_rows(attn_pair_kernel<CAP, BIAS, SINKS>,
-                           2u * kRing * kTileBytes + (2048u + 16u + 8u + (SINKS ? 16u : 0u)) * kPairWaves, p, waves, stream);
+                           2u * kRing * kTileBytes + (2048u + 16u + 8u + (SINKS ? 512u + 16u : 0u)) * kPairWaves, p, waves, stream);
     return launch_rows(attn_few_kernel<CAP, BIAS, SINKS>, 2u * kTileBytes + 1024u + 512u, p, waves, stream);
 }
 

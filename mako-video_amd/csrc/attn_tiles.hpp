@@ -212,8 +212,12 @@ struct RangeSeen {
         : lo(w.lo), hi(w.hi), t0(tile), from_lo(tile + 4u * (lane >> 5) - w.lo)
     {
     }
-    // The key of the lane's score i of block b; key j of the tile.
-    __device__ __forceinline__ bool score(int b, int i) const { return from_lo + (32u * b + 8u * (i >> 2) + (i & 3)) < hi - lo; }
+    // The lane's score i of block b, -inf where its key is not one of them.
+    __device__ __forceinline__ float score(float s, int b, int i) const
+    {
+        return from_lo + (32u * b + 8u * (i >> 2) + (i & 3)) < hi - lo ? s : -kInf;
+    }
+    // Whether key j of the tile is.
     __device__ __forceinline__ bool key(uint32_t j) const { return t0 + j >= lo && t0 + j < hi; }
     __device__ __forceinline__ bool any() const { return max(lo, t0) < min(hi, t0 + 64u); }
     // Whether the row's range begins here, in a walk from the last tile to the first where BACKWARD.
@@ -223,6 +227,8 @@ struct RangeSeen {
         return BACKWARD ? hi <= t0 + 64u : lo >= t0;
     }
     __device__ __forceinline__ void note(WaveRows&) const {}
+    // Whether the wave has work in the tile.
+    __device__ __forceinline__ bool meets(const WaveRows& w) const { return w.meets(t0); }
 };
 
 // The bits of a tile's 64 keys, at key t0, that lie in [lo, hi).
@@ -246,7 +252,12 @@ struct BitsSeen {
         : BitsSeen(key_bits(w.lo, w.hi, t0) | key_bits(w.s_lo, w.s_hi, t0), lane)
     {
     }
-    __device__ __forceinline__ bool score(int b, int i) const { return word[b] >> shift & 1u << (8 * (i >> 2) + (i & 3)); }
+    // A bit over a whole register selects: comparisons took two scalar registers each, and the kernels to scratch.
+    __device__ __forceinline__ float score(float s, int b, int i) const
+    {
+        const uint32_t m = uint32_t(__builtin_amdgcn_sbfe(int(word[b] >> shift), 8 * (i >> 2) + (i & 3), 1));
+        return __uint_as_float((__float_as_uint(s) & m) | (0xff800000u & ~m));
+    }
     __device__ __forceinline__ bool key(uint32_t j) const { return word[j >> 5] >> (j & 31u) & 1u; }
     __device__ __forceinline__ bool any() const { return (word[0] | word[1]) != 0u; }
     template <bool BACKWARD>
@@ -255,6 +266,7 @@ struct BitsSeen {
         return !w.begun;
     }
     __device__ __forceinline__ void note(WaveRows& w) const { w.begun |= any(); }
+    __device__ __forceinline__ bool meets(const WaveRows&) const { return __ballot(any()) != 0u; }
 };
 
 // What one of a score as the products (and cap_scores) leave it is in base 2.
@@ -473,7 +485,7 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                s[b][i] = seen.score(b, i) ? s[b][i] : -kInf;
+                s[b][i] = seen.score(s[b][i], b, i);
     }
     // Most tiles raise no maximum by much, and the sum over a lane's 32 keys of a row tells: up to 2^10 no key is above
     // that, and the old maximum serves. That spares the search for the new one in a phase whose vector instructions take 7
@@ -680,6 +692,130 @@ __device__ __forceinline__ bool holds_nonfinite(const char* part, uint32_t lane)
             top = __builtin_elementwise_max(top, __builtin_bit_cast(ushortx2, t[e] & 0x7fff7fffu));
     }
     return __ballot(top[0] >= 0x7f80u || top[1] >= 0x7f80u) != 0u;
+}
+
+// Many rows: eight waves of 32 list rows, in two groups of four, one wave of each group on a SIMD. A group's turn at a
+// tile has two phases, the products (S of this tile, and O of the one before) and the softmax, and the groups are a phase
+// apart, held there by the barriers: while one group's wave has the matrix core of a SIMD the other's has its vector unit.
+// K and V lie in rings of four tiles; a tile's loads go out three of its K (two of its V) ahead of its use, each wave an
+// eighth.
+constexpr uint32_t kPairWaves = 8, kRing = 4;
+
+// tile_output where the tile may have been masked; odd: the eight waves' words from holds_nonfinite for it (null: it was
+// whole).
+template <class Seen>
+__device__ __forceinline__ void masked_output(WaveRows& w, const TileP& pt, bf16x8_t (&frag)[kAhead], const TileReads& rd,
+                                              const char* vt, const Seen& seen, const uint32_t* odd, uint16_t* scratch,
+                                              uint32_t lane)
+{
+    uint32_t any = 0;
+    if (odd) {
+        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(odd), b = *reinterpret_cast<const u32x4_t*>(odd + 4);
+        any = a[0] | a[1] | a[2] | a[3] | b[0] | b[1] | b[2] | b[3];
+    }
+    if (__builtin_amdgcn_readfirstlane(any))
+        tile_output_masked(w, pt, rd, vt, seen, scratch, lane);
+    else
+        tile_output(w, pt, frag, rd, vt);
+}
+
+// A turn of the eight waves, tile t at key t0, of which a row attends the keys that `seen` says, and of the one before it
+// those of `before`. MASKED: this tile or the one before it is not whole for every row of the
+// workgroup, or there is none before it; checked: the turn before was of this form too.
+template <bool CAP, bool BIAS, bool MASKED, class Feed, class Seen>
+__device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Feed& feed, const TileReads& rd,
+                                          floatx16 (&s)[2], bf16x8_t (&frag)[kAhead], TileP& pt, uint16_t* scratch,
+                                          uint32_t* odd, bool checked, uint32_t wave, uint32_t t, uint32_t t0,
+                                          const Seen& seen, const Seen& before, uint32_t lane)
+{
+    // The products.
+    __builtin_amdgcn_s_setprio(1);
+    constexpr bool kSloped = BIAS && !CAP && !MASKED;
+    float* const near_pos = reinterpret_cast<float*>(scratch);
+    int32_t pos = 0;
+    if (kSloped)
+        pos = feed.positions(t)[lane], pos = p.k_pos ? pos : int32_t(t0 + lane);
+    bool near = false;
+    if (!MASKED || seen.meets(w))
+        near = tile_products<!MASKED, kSloped>(w, s, pt, frag, rd, feed.k_tile(t), feed.v_tile(t - 1u), pos, near_pos, lane);
+    if (MASKED) {
+        if (t > 0 && before.meets(w))
+            masked_output(w, pt, frag, rd, feed.v_tile(t - 1u), before,
+                          checked ? odd + kPairWaves * ((t - 1u) % 2u) : nullptr, scratch, lane);
+        // The part of V that this wave loaded: every wave's word is read at the next products, a barrier on.
+        const bool any = holds_nonfinite<2>(feed.v_tile(t) + 2048u * wave, lane);
+        if (lane == 0)
+            odd[kPairWaves * (t % 2u) + wave] = any;
+        wait_lds();
+    }
+    __builtin_amdgcn_s_setprio(0);
+    phase_barrier();
+    // The softmax. With it go out K of tile t + 3, into the slot of tile t - 1, which both groups have read, and V of tile
+    // t + 2 into that of tile t - 2 (among the products they cost 10%: this phase is the shorter one).
+    feed.k();
+    feed.v();
+    if (!MASKED || seen.meets(w))
+        tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, seen, feed.positions(t), near_pos, kSloped, near, lane);
+    // Past the last tile these are some tile's again, and not used.
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        frag[j] = rd.k(feed.k_tile(t + 1u), j);
+    // K of tile t + 2 and V of tile t + 1 have arrived, all but this turn's loads: both groups are past their barriers by
+    // the time that either reads them.
+    wait_vm<Feed::kLoads>();
+    phase_barrier();
+}
+
+// The turns of a workgroup's tiles, of which walk.whole(t) says whether every row of the workgroup attends all of tile t,
+// walk.seen(t) a row's keys of another one (asked for once, in order) and walk.key(t) where it lies; and what is left of
+// the last one's output. The feed has loaded K of three tiles and V of two.
+template <bool CAP, bool BIAS, class Feed, class Walk>
+__device__ __forceinline__ void pair_walk(const DenseParams& p, WaveRows& w, Feed& feed, Walk& walk, const TileReads& rd,
+                                          uint16_t* scratch, uint32_t* odd, uint32_t wave, uint32_t tiles, uint32_t lane)
+{
+    wait_vm<Feed::kLoads>(); // K of tiles 0 and 1, V of tile 0
+    lds_barrier();
+    const bool second = wave >= kPairWaves / 2u;
+    if (second)
+        phase_barrier();
+    floatx16 s[2];
+    bf16x8_t frag[kAhead];
+    TileP pt;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        frag[j] = rd.k(feed.k_tile(0u), j);
+    bool masked = true; // the last turn's form
+    BitsSeen before(0u, lane);
+    // Two loops: one body with both forms copies O between them at every tile.
+    for (uint32_t t = 0; t < tiles;) {
+#pragma unroll 1
+        do {
+            const BitsSeen seen = walk.seen(t);
+            pair_turn<CAP, BIAS, true>(p, w, feed, rd, s, frag, pt, scratch, odd, masked, wave, t, walk.key(t), seen, before,
+                                       lane);
+            before = seen;
+            masked = true, ++t;
+        } while (t < tiles && !(walk.whole(t) && walk.whole(t - 1u)));
+        if (t < tiles) {
+#pragma unroll 1
+            do {
+                pair_turn<CAP, BIAS, false>(p, w, feed, rd, s, frag, pt, scratch, odd, true, wave, t, walk.key(t), before,
+                                            before, lane);
+                ++t;
+            } while (t < tiles && walk.whole(t));
+            masked = false, before = BitsSeen(~uint64_t(0), lane);
+        }
+    }
+    const uint32_t end = tiles - 1u;
+    if (!before.meets(w))
+        ; // nothing of it is this wave's
+    else if (masked)
+        masked_output(w, pt, frag, rd, feed.v_tile(end), before, odd + kPairWaves * (end % 2u), scratch, lane);
+    else
+        tile_output(w, pt, frag, rd, feed.v_tile(end));
+    if (!second)
+        phase_barrier();
+    wait_vm<0>(); // no load into this workgroup's LDS outlives it
 }
 
 // The factors of the scores from `scale` (0: 1 / sqrt(128)) and `cap` (0: none).
