@@ -12,6 +12,8 @@
 // - A tile is four groups of 16 rows, each in one page: four descriptors, of as many rows as there are and none where the
 //   entry is no page, so that nothing else is read and what is missing is zeros. The page numbers of 16 tiles lie in the
 //   lanes of one register, 16 entries read at once, and come out of it by readlane.
+// - With few list rows a stream a workgroup is one wave with 32 of them; with more it is eight waves of 32, which share their
+//   tiles and take turns at products and softmax as in attn_dense.hip.
 // - What a row attends of a tile that is not whole is 64 bits: of ranges, or of the row's line of ancestors. Along it the
 //   rows' numbers fall, and so do the tiles', so a row walks its line once, as far as each tile reaches.
 // - Streams are of any lengths, which the host does not know. All items' tiles are one list, and each of as many workgroups
@@ -33,6 +35,7 @@ struct PagesParams : DenseParams {
     const int32_t* first_rows;
     uint64_t kps, kphs, kprs, vps, vphs, vprs, table_stride; // elements
     uint32_t streams, cols, pages, page_rows, window, workers, slot_rows;
+    uint32_t item_rows; // list rows of an item: a wave's 32, or a workgroup's 256
     FastDiv div_page;
 };
 
@@ -52,7 +55,7 @@ struct Stream {
         near = all - near0;
         front = min((sinks + 63u) / 64u, near0);
         tiles = front + near + (rows + 63u) / 64u;
-        row_tiles = (rows * p.group + 31u) / 32u;
+        row_tiles = (rows * p.group + p.item_rows - 1u) / p.item_rows;
     }
     // The first key of kept tile u.
     __device__ __forceinline__ uint32_t key(uint32_t u) const { return 64u * (u < front ? u : near0 + u - front); }
@@ -144,16 +147,16 @@ struct GroupLoads {
     }
 };
 
-// A workgroup's item, and what a lane has of it.
+// A wave's item, and what a lane has of it.
 struct Item {
     Stream st;
-    uint32_t stream, kvh, list, f0;
+    uint32_t stream, kvh, list, f0; // f0: the wave's first list row
     uint32_t sinks;   // as given: new rows may be among the first ones too
     uint32_t row, up; // the lane's row's number among the new ones; the row of its line that the walk is at (~0: at its end)
     uint32_t place;   // the row's
     uint32_t up_place; // that of `up`
     uint32_t lo;      // kept rows from it on are under the window
-    uint32_t all_lo;  // of every row
+    uint32_t all_lo;  // of every row of the workgroup, or a bound of that
 };
 
 // The row's parent, ~0 for none: a parent lies before its row.
@@ -193,7 +196,9 @@ __device__ __forceinline__ void load_item(const PagesParams& p, Item& it, uint32
     it.place = it.st.kept + depth;
     it.up = it.row, it.up_place = it.place;
     it.lo = p.window && p.window - 1u < it.place ? it.place - (p.window - 1u) : 0u;
-    it.all_lo = wave_max_u32(it.lo);
+    // A row has as many ancestors as there are rows before it, at most.
+    const uint32_t far = it.st.kept + p.div_group.div(min(it.f0 / p.item_rows * p.item_rows + p.item_rows, it.list) - 1u);
+    it.all_lo = p.window && p.window - 1u < far ? far - (p.window - 1u) : 0u;
     w.m_run = -kInf, w.l_run = 0.0f, w.settled = false, w.begun = false;
 }
 
@@ -340,7 +345,7 @@ __device__ __forceinline__ void pages_turn(const PagesParams& p, Item& it, WaveR
 __device__ __forceinline__ void store_item(const PagesParams& p, const Item& it, const WaveRows& w, uint32_t slot,
                                            uint32_t lane)
 {
-    const uint32_t n = lane & 31u, hh = lane >> 5, f = it.f0 + n;
+    const uint32_t hh = lane >> 5, f = it.f0 + (lane & 31u), n = f % p.item_rows;
     const float l = w.l_run + __shfl_xor(w.l_run, 32, kWave);
     if (f >= it.list)
         return;
@@ -369,12 +374,10 @@ __device__ __forceinline__ void store_item(const PagesParams& p, const Item& it,
                       pack_bf16(w.o[db][4 * g + 2] * inv, w.o[db][4 * g + 3] * inv)};
 }
 
-// One wave a workgroup, with a tile of its own in LDS; four of them share a CU.
-template <bool CAP>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void attn_pages_kernel(PagesParams p)
+// A workgroup's run of all items' tiles: item(i, first, last, slot) for each of its parts.
+template <class Part>
+__device__ __forceinline__ void for_parts(const PagesParams& p, uint32_t lane, const Part& part)
 {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    const uint32_t lane = threadIdx.x;
     // Blocks go to the 8 XCDs round-robin; each takes a contiguous part of the list, key head by key head.
     const uint32_t worker = (blockIdx.x % 8u) * (gridDim.x / 8u) + blockIdx.x / 8u;
     Streams streams;
@@ -385,8 +388,6 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         return;
     if (streams.s0 != 0u)
         streams.load(p, 0u, 0u, lane);
-    const TileReads rd(lane);
-    PageFeed feed{{p.kprs, lane}, {p.krs, lane}, {p.vprs, lane}, {p.vrs, lane}, lds, -1};
     while (x < end) {
         while (x >= streams.end)
             streams.load(p, streams.s0 + kWave, streams.end, lane);
@@ -398,7 +399,23 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         const uint32_t first = uint32_t(local - number * st.tiles);
         const uint32_t last = uint32_t(min(uint64_t(st.tiles), first + (end - x)));
         Item it{st, streams.s0 + at, uint32_t(number / st.row_tiles), st.rows * p.group, 0u, sinks, 0u, 0u, 0u, 0u, 0u, 0u};
-        it.f0 = 32u * uint32_t(number - uint64_t(it.kvh) * st.row_tiles);
+        it.f0 = p.item_rows * uint32_t(number - uint64_t(it.kvh) * st.row_tiles);
+        // The item that the run begins with, unless with its first tile, is the first of the workgroup's two parts.
+        const bool cut = first > 0u || last < st.tiles;
+        part(it, first, last, cut ? 2u * worker + (first > 0u ? 0u : 1u) : ~0u);
+        x += last - first;
+    }
+}
+
+// One wave a workgroup, with a tile of its own in LDS; four of them share a CU.
+template <bool CAP>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void attn_pages_kernel(PagesParams p)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t lane = threadIdx.x;
+    const TileReads rd(lane);
+    PageFeed feed{{p.kprs, lane}, {p.krs, lane}, {p.vprs, lane}, {p.vrs, lane}, lds, -1};
+    for_parts(p, lane, [&](Item& it, uint32_t first, uint32_t last, uint32_t slot) {
         WaveRows w;
         feed.numbers(p, it, first & ~15u, lane);
         feed.load<false>(p, it, first);
@@ -412,11 +429,162 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
             for (; u < last && is_whole(it, feed, u); ++u)
                 pages_turn<CAP, false>(p, it, w, feed, rd, u, last, lane);
         }
-        // The item that the share begins with, unless with its first tile, is the first of the worker's two parts.
-        const bool cut = first > 0u || last < st.tiles;
-        store_item(p, it, w, cut ? 2u * worker + (first > 0u ? 0u : 1u) : ~0u, lane);
-        x += last - first;
+        store_item(p, it, w, slot, lane);
+    });
+}
+
+// What a wave of eight loads of a workgroup's tiles, each an eighth: eight rows, which lie in one page.
+struct PairPageFeed {
+    static constexpr int kLoads = 4; // of a turn
+    const PagesParams& p;
+    const Item& it;
+    char* lds;
+    const uint16_t* k_pool; // of the key head
+    const uint16_t* v_pool;
+    const uint16_t* k_rows; // of the stream's new rows
+    const uint16_t* v_rows;
+    uint32_t first, tiles, wave; // the part's first tile, and how many
+    uint32_t k_key, k_chunk, v_key, v_chunk; // the lane's row and bytes of it in its instructions
+    uint32_t base; // lane u % 64 has the page of tile u, of base .. base + 63
+    int32_t ids;
+    uint64_t group_there[4], there_all; // bit u % 64: whether the page of each group of 16 rows is there
+
+    __device__ __forceinline__ PairPageFeed(const PagesParams& params, const Item& item, char* memory, uint32_t part_first,
+                                            uint32_t part_tiles, uint32_t wave_number, uint32_t lane)
+        : p(params), it(item), lds(memory), first(part_first), tiles(part_tiles), wave(wave_number)
+    {
+        k_pool = p.k_pages + it.kvh * p.kphs, v_pool = p.v_pages + it.kvh * p.vphs;
+        k_rows = p.k + it.kvh * p.khs + it.st.q0 * p.krs, v_rows = p.v + it.kvh * p.vhs + it.st.q0 * p.vrs;
+        k_key = lane >> 4, k_chunk = 16u * ((lane & 15u) ^ (8u * (wave & 1u) + k_key));
+        v_key = (lane >> 2) & 3u, v_chunk = 16u * (4u * (lane >> 4) + (lane & 3u));
+        base = first & ~31u;
+        numbers(lane);
     }
+    __device__ __forceinline__ void numbers(uint32_t lane)
+    {
+        const uint32_t u = base + ((lane - base) & 63u);
+        const bool kept = it.st.is_kept(u);
+        const uint32_t key = kept ? it.st.key(u) : 0u;
+        const int32_t* const line = p.table + uint64_t(it.stream) * p.table_stride;
+        ids = -1;
+        there_all = ~uint64_t(0);
+#pragma unroll
+        for (uint32_t g = 0; g < 4u; ++g) {
+            const bool in = kept && key + 16u * g < it.st.kept;
+            const int32_t page = in ? line[p.div_page.div(key + 16u * g)] : -1;
+            const bool there = uint32_t(page) < p.pages;
+            ids = g == wave / 2u && there ? page : ids;
+            group_there[g] = __ballot(there || !in);
+            there_all &= group_there[g];
+        }
+    }
+    __device__ __forceinline__ const char* k_tile(uint32_t t) const { return lds + (t % kRing) * kTileBytes; }
+    __device__ __forceinline__ const char* v_tile(uint32_t t) const { return lds + (kRing + t % kRing) * kTileBytes; }
+    __device__ __forceinline__ int32_t* positions(uint32_t) const { return nullptr; }
+    // The part's tile t, past its end the last one again: every turn has the same count of loads.
+    template <bool VALUE>
+    __device__ __forceinline__ void load(uint32_t t) const
+    {
+        const uint32_t u = first + min(t, tiles - 1u);
+        char* const dst = const_cast<char*>(VALUE ? v_tile(t) : k_tile(t)) + 2048u * wave;
+        const uint16_t* at;
+        uint32_t rows, row;
+        if (it.st.is_kept(u)) {
+            const int32_t page = __builtin_amdgcn_readlane(ids, int(u % 64u));
+            const uint32_t key = it.st.key(u) + 8u * wave, r = key - p.div_page.div(key) * p.page_rows;
+            at = VALUE ? v_pool + uint32_t(max(page, 0)) * p.vps + r * p.vprs : k_pool + uint32_t(max(page, 0)) * p.kps + r * p.kprs;
+            rows = page >= 0 && key < it.st.kept ? min(8u, it.st.kept - key) : 0u;
+            row = uint32_t(VALUE ? p.vprs : p.kprs) * 2u;
+        } else {
+            const uint32_t r = it.st.fresh(u) + 8u * wave;
+            rows = r < it.st.rows ? min(8u, it.st.rows - r) : 0u;
+            at = VALUE ? v_rows + (rows ? r : 0u) * p.vrs : k_rows + (rows ? r : 0u) * p.krs;
+            row = uint32_t(VALUE ? p.vrs : p.krs) * 2u;
+        }
+        u32x4_t b = buffer_words(at, rows ? (rows - 1u) * row + 256u : 0u);
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            b[i] = uint32_t(__builtin_amdgcn_readfirstlane(int(b[i]))); // all of a wave's lanes have the same
+        // Rows 4 of each instruction, of K the chunks swizzled by the row (an instruction on, by four more).
+        load_lds16(b, dst, (VALUE ? v_key : k_key) * row + (VALUE ? v_chunk : k_chunk));
+        load_lds16(b, dst + 1024u, ((VALUE ? v_key : k_key) + 4u) * row + (VALUE ? v_chunk : k_chunk ^ 64u));
+    }
+    __device__ __forceinline__ void next_k(uint32_t t)
+    {
+        if (first + min(t + 3u, tiles - 1u) >= base + 64u) {
+            base += 32u;
+            numbers(threadIdx.x & 63u);
+        }
+        load<false>(t + 3u);
+    }
+    __device__ __forceinline__ void next_v(uint32_t t) { load<true>(t + 2u); }
+    __device__ __forceinline__ bool all_there(uint32_t u) const { return there_all >> (u % 64u) & 1u; }
+    // The bits of the tile's keys whose page is there.
+    __device__ __forceinline__ uint64_t there(uint32_t u) const
+    {
+        uint64_t bits = ~uint64_t(0);
+        if (!all_there(u))
+#pragma unroll
+            for (uint32_t g = 0; g < 4u; ++g)
+                bits &= group_there[g] >> (u % 64u) & 1u ? ~uint64_t(0) : ~(uint64_t(0xffff) << (16u * g));
+        return bits;
+    }
+};
+
+// A part's tiles, as pair_walk asks for them.
+struct PairPageWalk {
+    const PagesParams& p;
+    Item& it;
+    const PairPageFeed& feed;
+    uint32_t lane;
+    __device__ __forceinline__ uint32_t key(uint32_t) const { return 0u; } // only a bias asks where a tile lies
+    __device__ __forceinline__ bool whole(uint32_t t) const
+    {
+        const uint32_t u = feed.first + t;
+        if (!it.st.is_kept(u))
+            return false;
+        const uint32_t t0 = it.st.key(u);
+        return t0 + 64u <= it.st.kept && (t0 >= it.all_lo || t0 + 64u <= it.st.sinks) && feed.all_there(u);
+    }
+    __device__ __forceinline__ BitsSeen seen(uint32_t t)
+    {
+        const uint32_t u = feed.first + t;
+        uint64_t bits;
+        if (it.st.is_kept(u)) {
+            const uint32_t t0 = it.st.key(u);
+            bits = (key_bits(it.lo, it.st.kept, t0) | key_bits(0u, it.st.sinks, t0)) & feed.there(u);
+        } else {
+            bits = fresh_bits(p, it, it.st.fresh(u));
+        }
+        return BitsSeen(it.f0 + (lane & 31u) < it.list ? bits : 0u, lane);
+    }
+};
+
+// Eight waves a workgroup: one to a CU.
+template <bool CAP>
+__global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_pages_pair_kernel(PagesParams p)
+{
+    // K ring, V ring, a wave's scratch (1 KB), and for two tiles whether the waves' parts of V hold an infinity or a NaN.
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kRing * kTileBytes + 1024u * wave);
+    uint32_t* const odd = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + 1024u * kPairWaves);
+    const TileReads rd(lane);
+    for_parts(p, lane, [&](Item& it, uint32_t first, uint32_t last, uint32_t slot) {
+        it.f0 += 32u * wave;
+        PairPageFeed feed(p, it, lds, first, last - first, wave, lane);
+        lds_barrier(); // the part before this one is read
+        feed.load<false>(0u);
+        feed.load<false>(1u);
+        feed.load<true>(0u);
+        feed.load<false>(2u);
+        feed.load<true>(1u);
+        WaveRows w;
+        load_item(p, it, lane, w);
+        PairPageWalk walk{p, it, feed, lane};
+        pair_walk<CAP, false>(p, w, feed, walk, rd, scratch, odd, wave, last - first, lane);
+        store_item(p, it, w, slot, lane);
+    });
 }
 
 // Joins the parts of eight list rows of an item, 32 lanes a row, four values of d each, in the order of the tiles.
@@ -447,12 +615,13 @@ __global__ __launch_bounds__(256) void attn_pages_join_kernel(PagesParams p)
     uint32_t sinks;
     const Stream st = streams.get(p, at, sinks);
     const uint32_t kvh = uint32_t(block / per), f = 8u * uint32_t(block - uint64_t(kvh) * per) + threadIdx.x / 32u;
-    const uint64_t x0 = lane_u64(streams.before, at) + (uint64_t(kvh) * st.row_tiles + f / 32u) * st.tiles, x1 = x0 + st.tiles;
+    const uint64_t x0 = lane_u64(streams.before, at) + (uint64_t(kvh) * st.row_tiles + f / p.item_rows) * st.tiles;
+    const uint64_t x1 = x0 + st.tiles;
     const uint32_t w0 = uint32_t(x0 / share), w1 = uint32_t((x1 - 1u) / share);
     if (f >= st.rows * p.group || w0 == w1)
         return;
     const float2* const ml = reinterpret_cast<const float2*>(p.part + 2ull * p.workers * p.slot_rows * 128u);
-    const uint32_t n = f % 32u, d = 4u * (threadIdx.x & 31u);
+    const uint32_t n = f % p.item_rows, d = 4u * (threadIdx.x & 31u);
     constexpr uint32_t kU = 8;
     float m = -kInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t i0 = w0; i0 <= w1; i0 += kU) {
@@ -498,17 +667,24 @@ namespace {
 
 using namespace mh3;
 
-constexpr size_t kPagesLds = 2u * kTileBytes + 1024u;
+// Which kernel a call takes, from the list rows that its streams have on average.
+struct PagesPlan {
+    uint32_t item_rows, workers, slot_rows; // a part's rows: an item's, or all of the call's where they are fewer
+    uint64_t workspace;
+};
 
-uint32_t workers_of() { return (4u * uint32_t(std::max(host::cu_count(), 1)) + 7u) / 8u * 8u; }
-
-// Rows of a part: an item's, or all of the call's where they are fewer.
-uint32_t slot_rows_of(const MH3PagesAttnArgs& a)
+PagesPlan pages_plan(const MH3PagesAttnArgs& a)
 {
-    return uint32_t(std::min<uint64_t>(32u, uint64_t(a.q_rows) * (a.heads / a.kv_heads)));
+    const uint64_t list = uint64_t(a.q_rows) * (a.heads / a.kv_heads);
+    const bool pair = list > 64ull * a.table.streams;
+    const uint32_t cus = uint32_t(std::max(host::cu_count(), 1));
+    PagesPlan plan;
+    plan.item_rows = pair ? 32u * kPairWaves : 32u;
+    plan.workers = ((pair ? 1u : 4u) * cus + 7u) / 8u * 8u;
+    plan.slot_rows = uint32_t(std::min<uint64_t>(plan.item_rows, list));
+    plan.workspace = 2ull * plan.workers * plan.slot_rows * 130u * 4u;
+    return plan;
 }
-
-uint64_t pages_workspace(const MH3PagesAttnArgs& a) { return 2ull * workers_of() * slot_rows_of(a) * 130u * 4u; }
 
 int check_pages_args(const MH3PagesAttnArgs* args)
 {
@@ -545,14 +721,22 @@ int check_pages_args(const MH3PagesAttnArgs* args)
     return MH3_OK;
 }
 
+template <class Kernel>
+int launch_items(Kernel kernel, uint32_t waves, size_t lds, const PagesParams& p, hipStream_t stream)
+{
+    if (const hipError_t e = host::allow_dynamic_lds(reinterpret_cast<const void*>(kernel), lds); e != hipSuccess)
+        return host::hip_error(e);
+    hipLaunchKernelGGL(kernel, dim3(p.workers), dim3(64u * waves), lds, stream, p);
+    return host::check_launch();
+}
+
 template <bool CAP>
 int launch_pages(const PagesParams& p, hipStream_t stream)
 {
-    const auto kernel = attn_pages_kernel<CAP>;
-    if (const hipError_t e = host::allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kPagesLds); e != hipSuccess)
-        return host::hip_error(e);
-    hipLaunchKernelGGL(kernel, dim3(p.workers), dim3(64), kPagesLds, stream, p);
-    return host::check_launch();
+    if (p.item_rows > 32u)
+        return launch_items(attn_pages_pair_kernel<CAP>, kPairWaves, 2u * kRing * kTileBytes + (1024u + 8u) * kPairWaves, p,
+                            stream);
+    return launch_items(attn_pages_kernel<CAP>, 1u, 2u * kTileBytes + 1024u, p, stream);
 }
 
 } // namespace
@@ -561,7 +745,7 @@ extern "C" int64_t mh3_flash_attn_pages_128_workspace_bytes(const MH3PagesAttnAr
 {
     if (const int rc = check_pages_args(args); rc != MH3_OK)
         return rc;
-    return int64_t(pages_workspace(*args));
+    return int64_t(pages_plan(*args).workspace);
 }
 
 extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint16_t* q, const uint16_t* k,
@@ -576,7 +760,8 @@ extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint
     const MH3PagesArgs& t = a.table;
     if (a.q_rows == 0)
         return MH3_OK;
-    const uint64_t need = pages_workspace(a);
+    const PagesPlan plan = pages_plan(a);
+    const uint64_t need = plan.workspace;
     if (!q || !k || !v || !k_pages || !v_pages || !table || !lengths || !q_off || !workspace || !out)
         return MH3_ERR_POINTER;
     if (workspace_bytes < need)
@@ -628,7 +813,7 @@ extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint
     p.table_stride = t.table_stride, p.streams = t.streams, p.cols = t.cols, p.pages = t.pages;
     p.page_rows = t.page_rows, p.window = a.window, p.div_page = FastDiv::make(t.page_rows);
     p.kv_heads = a.kv_heads, p.group = a.heads / a.kv_heads, p.q_rows = a.q_rows, p.div_group = FastDiv::make(p.group);
-    p.workers = workers_of(), p.slot_rows = slot_rows_of(a);
+    p.workers = plan.workers, p.slot_rows = plan.slot_rows, p.item_rows = plan.item_rows;
     score_factors(a.scale, a.cap, p);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (const int rc = a.cap > 0.0f ? launch_pages<true>(p, s) : launch_pages<false>(p, s); rc != MH3_OK)
