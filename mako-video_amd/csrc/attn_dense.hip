@@ -328,8 +328,7 @@ struct PairFeed {
     PairStream<false, BIAS, SINKS> k;
     PairStream<true, false, SINKS> v;
     // In turn t: K of tile t + 3, V of tile t + 2.
-    __device__ __forceinline__ void next_k(uint32_t) { k(); }
-    __device__ __forceinline__ void next_v(uint32_t) { v(); }
+    __device__ __forceinline__ void next(uint32_t) { k(), v(); }
     __device__ __forceinline__ const char* k_tile(uint32_t t) const { return k.ring + (t % kRing) * kTileBytes; }
     __device__ __forceinline__ const char* v_tile(uint32_t t) const { return v.ring + (t % kRing) * kTileBytes; }
     __device__ __forceinline__ int32_t* positions(uint32_t t) const

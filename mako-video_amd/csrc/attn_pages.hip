@@ -82,32 +82,36 @@ __device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, uint32_t lane)
     return v;
 }
 
-// The streams 64 at a time, one a lane, and the sums of their items' tiles.
+// Stream s of the table, as `sinks` gives it its first rows (which may be new ones too).
+__device__ __forceinline__ Stream stream_of(const PagesParams& p, uint32_t s, uint32_t& sinks)
+{
+    const uint32_t q0 = uint32_t(min(max(p.q_off[s], 0), int32_t(p.q_rows)));
+    const uint32_t rows = uint32_t(min(max(p.q_off[s + 1u], int32_t(q0)), int32_t(p.q_rows))) - q0;
+    const uint32_t kept = uint32_t(min(max(p.lengths[s], 0), int32_t(p.cols * p.page_rows)));
+    sinks = p.first_rows ? min(uint32_t(max(p.first_rows[s], 0)), 1u << 30) : 0u;
+    return Stream(p, q0, rows, kept, min(sinks, kept));
+}
+
+// The streams 64 at a time, one a lane, by the sums of their items' tiles.
 struct Streams {
-    uint32_t s0, q0, rows, kept, sinks;
-    uint64_t before, units, end; // the lane's stream's; end: of the 64
+    uint32_t s0;
+    uint64_t before, some, end; // tiles before the lane's stream; the streams that have any; those up to the 64's end
     __device__ __forceinline__ void load(const PagesParams& p, uint32_t from, uint64_t base, uint32_t lane)
     {
-        s0 = from, q0 = rows = kept = sinks = 0, units = 0;
-        const uint32_t s = from + lane;
-        if (s < p.streams) {
-            const uint32_t a = uint32_t(min(max(p.q_off[s], 0), int32_t(p.q_rows)));
-            q0 = a, rows = uint32_t(min(max(p.q_off[s + 1u], int32_t(a)), int32_t(p.q_rows))) - a;
-            kept = uint32_t(min(max(p.lengths[s], 0), int32_t(p.cols * p.page_rows)));
-            sinks = p.first_rows ? min(uint32_t(max(p.first_rows[s], 0)), 1u << 30) : 0u;
-            const Stream t(p, q0, rows, kept, min(sinks, kept));
+        s0 = from;
+        uint64_t units = 0;
+        if (from + lane < p.streams) {
+            uint32_t sinks;
+            const Stream t = stream_of(p, from + lane, sinks);
             units = uint64_t(t.row_tiles) * p.kv_heads * t.tiles;
         }
+        some = __ballot(units != 0u);
         const uint64_t sum = wave_scan_u64(units, lane);
         before = base + sum - units;
         end = base + lane_u64(sum, kWave - 1);
     }
-    __device__ __forceinline__ Stream get(const PagesParams& p, uint32_t lane, uint32_t& sinks_of) const
-    {
-        const auto of = [&](uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), int(lane))); };
-        sinks_of = of(sinks);
-        return Stream(p, of(q0), of(rows), of(kept), min(sinks_of, of(kept)));
-    }
+    // The last stream that begins at tile x or before it and has tiles, x one of the 64's.
+    __device__ __forceinline__ uint32_t of(uint64_t x) const { return 63u - uint32_t(__builtin_clzll(__ballot(before <= x) & some)); }
 };
 
 // All items' tiles, and a workgroup's share of them.
@@ -123,28 +127,10 @@ __device__ __forceinline__ uint64_t share_of(const PagesParams& p, uint64_t unit
     return max((units + p.workers - 1u) / p.workers, uint64_t(kLeastTiles));
 }
 
-// The offsets of the four instructions that load 16 rows of a K (VALUE false) or V tile, as TileLoads has them.
-template <bool VALUE>
-struct GroupLoads {
-    static constexpr int kOff = VALUE ? 1 : 4;
-    uint32_t row, off[kOff];
-    __device__ __forceinline__ GroupLoads(uint64_t stride, uint32_t lane) : row(uint32_t(stride) * 2u)
-    {
-#pragma unroll
-        for (uint32_t u = 0; u < uint32_t(kOff); ++u) {
-            const uint32_t key = VALUE ? (lane >> 2) & 3u : lane >> 4;
-            const uint32_t chunk = VALUE ? 4u * (lane >> 4) + (lane & 3u) : (lane & 15u) ^ (4u * u + key);
-            off[u] = (4u * u + key) * row + 16u * chunk;
-        }
-    }
-    // Rows 16 g .. of the tile at dst, `rows` of which (the first) lie at `base`; the others are zeros.
-    __device__ __forceinline__ void operator()(char* dst, uint32_t g, const uint16_t* base, uint32_t rows) const
-    {
-        const u32x4_t r = buffer_words(base, rows ? (rows - 1u) * row + 256u : 0u);
-#pragma unroll
-        for (uint32_t u = 0; u < 4u; ++u)
-            load_lds16(r, dst + 4096u * g + 1024u * u, VALUE ? off[0] + 4u * u * row : off[u % uint32_t(kOff)]);
-    }
+// Rows in one piece: where they begin and how many bytes a buffer over them has (none: nothing is read, and zeros come).
+struct Piece {
+    uint64_t at;
+    uint32_t bytes;
 };
 
 // A wave's item, and what a lane has of it.
@@ -164,6 +150,14 @@ __device__ __forceinline__ uint32_t parent_of(const PagesParams& p, const Item& 
 {
     const uint32_t up = row < it.st.rows ? uint32_t(p.parents[it.st.q0 + row]) : ~0u;
     return up < row ? up : ~0u;
+}
+
+// The kept rows that every row of the workgroup has under the window, at least: a row has as many ancestors as there are
+// rows before it, at most.
+__device__ __forceinline__ void bound_window(const PagesParams& p, Item& it)
+{
+    const uint32_t far = it.st.kept + p.div_group.div(min(it.f0 / p.item_rows * p.item_rows + p.item_rows, it.list) - 1u);
+    it.all_lo = p.window && p.window - 1u < far ? far - (p.window - 1u) : 0u;
 }
 
 __device__ __forceinline__ void load_item(const PagesParams& p, Item& it, uint32_t lane, WaveRows& w)
@@ -196,9 +190,6 @@ __device__ __forceinline__ void load_item(const PagesParams& p, Item& it, uint32
     it.place = it.st.kept + depth;
     it.up = it.row, it.up_place = it.place;
     it.lo = p.window && p.window - 1u < it.place ? it.place - (p.window - 1u) : 0u;
-    // A row has as many ancestors as there are rows before it, at most.
-    const uint32_t far = it.st.kept + p.div_group.div(min(it.f0 / p.item_rows * p.item_rows + p.item_rows, it.list) - 1u);
-    it.all_lo = p.window && p.window - 1u < far ? far - (p.window - 1u) : 0u;
     w.m_run = -kInf, w.l_run = 0.0f, w.settled = false, w.begun = false;
 }
 
@@ -220,27 +211,54 @@ __device__ __forceinline__ uint64_t fresh_bits(const PagesParams& p, Item& it, u
     return bits;
 }
 
-// What the workgroup loads, tile by tile.
+// Rows r .. r + n - 1 (of tile u, `row` their first one there) of a part's K (VALUE false) or V, and whether they are there.
+template <bool VALUE>
+__device__ __forceinline__ Piece piece_of(const PagesParams& p, const Item& it, bool kept, uint32_t key, int32_t page,
+                                          uint32_t n)
+{
+    if (kept) {
+        const uint32_t r = key - p.div_page.div(key) * p.page_rows;
+        const uint64_t at = uint64_t(uint32_t(max(page, 0))) * (VALUE ? p.vps : p.kps) + uint64_t(r) * (VALUE ? p.vprs : p.kprs) +
+                            it.kvh * (VALUE ? p.vphs : p.kphs);
+        const uint32_t rows = page >= 0 && key < it.st.kept ? min(n, it.st.kept - key) : 0u;
+        return {reinterpret_cast<uint64_t>((VALUE ? p.v_pages : p.k_pages) + at),
+                rows ? (rows - 1u) * uint32_t(VALUE ? p.vprs : p.kprs) * 2u + 256u : 0u};
+    }
+    const uint32_t rows = key < it.st.rows ? min(n, it.st.rows - key) : 0u;
+    const uint64_t at = uint64_t(it.st.q0 + (rows ? key : 0u)) * (VALUE ? p.vrs : p.krs) + it.kvh * (VALUE ? p.vhs : p.khs);
+    return {reinterpret_cast<uint64_t>((VALUE ? p.v : p.k) + at),
+            rows ? (rows - 1u) * uint32_t(VALUE ? p.vrs : p.krs) * 2u + 256u : 0u};
+}
+
+// The page of kept row `key`, -1 for none.
+__device__ __forceinline__ int32_t page_of(const PagesParams& p, const Item& it, uint32_t key)
+{
+    if (key >= it.st.kept)
+        return -1;
+    const int32_t page = p.table[uint64_t(it.stream) * p.table_stride + p.div_page.div(key)];
+    return uint32_t(page) < p.pages ? page : -1;
+}
+
+// What a workgroup of one wave loads, tile by tile: four pieces of 16 rows, which each lie in one page. Lane 4 (u % 16) + g
+// has those of group g of tile u, for 16 tiles at a time: a page's place takes some 40 scalar instructions to find.
 struct PageFeed {
-    GroupLoads<false> k_page, k_new;
-    GroupLoads<true> v_page, v_new;
     char* lds; // K, V, the wave's scratch (1 KB)
-    int32_t ids;   // lane 4 (u % 16) + g: the page of group g of tile u, -1 where there is none
+    uint32_t k_key, k_chunk, v_key, v_chunk; // the lane's row and bytes of it in its instructions
+    Piece k, v;
+    uint64_t there_bits; // lanes whose page is there
+    __device__ __forceinline__ PageFeed(char* memory, uint32_t lane)
+        : lds(memory), k_key(lane >> 4), k_chunk(16u * ((lane & 15u) ^ (lane >> 4))), v_key((lane >> 2) & 3u),
+          v_chunk(16u * (4u * (lane >> 4) + (lane & 3u)))
+    {
+    }
     __device__ __forceinline__ void numbers(const PagesParams& p, const Item& it, uint32_t u16, uint32_t lane)
     {
-        const uint32_t u = u16 + lane / 4u;
-        ids = -1;
-        if (it.st.is_kept(u)) {
-            const uint32_t key = it.st.key(u) + 16u * (lane % 4u);
-            if (key < it.st.kept) {
-                const int32_t page = p.table[uint64_t(it.stream) * p.table_stride + p.div_page.div(key)];
-                ids = uint32_t(page) < p.pages ? page : -1;
-            }
-        }
-    }
-    __device__ __forceinline__ int32_t number(uint32_t u, uint32_t g) const
-    {
-        return __builtin_amdgcn_readlane(ids, int(4u * (u % 16u) + g));
+        const uint32_t u = u16 + lane / 4u, g = lane % 4u;
+        const bool kept = it.st.is_kept(u);
+        const uint32_t key = 16u * g + (kept ? it.st.key(u) : it.st.fresh(min(u, it.st.tiles - 1u)));
+        const int32_t page = kept ? page_of(p, it, key) : -1;
+        there_bits = __ballot(page >= 0);
+        k = piece_of<false>(p, it, kept, key, page, 16u), v = piece_of<true>(p, it, kept, key, page, 16u);
     }
     // The bits of the tile's keys whose page is there.
     __device__ __forceinline__ uint64_t there(uint32_t u) const
@@ -248,44 +266,36 @@ struct PageFeed {
         uint64_t bits = 0;
 #pragma unroll
         for (uint32_t g = 0; g < 4u; ++g)
-            bits |= number(u, g) >= 0 ? uint64_t(0xffff) << (16u * g) : 0u;
+            bits |= there_bits >> (4u * (u % 16u) + g) & 1u ? uint64_t(0xffff) << (16u * g) : 0u;
         return bits;
     }
+    __device__ __forceinline__ bool all_there(uint32_t u) const { return (there_bits >> (4u * (u % 16u)) & 15u) == 15u; }
     template <bool VALUE>
     __device__ __forceinline__ void load(const PagesParams& p, const Item& it, uint32_t u) const
     {
         char* const dst = lds + (VALUE ? kTileBytes : 0u);
-        if (it.st.is_kept(u)) {
-            const uint32_t t0 = it.st.key(u);
+        const uint32_t row = 2u * uint32_t(it.st.is_kept(u) ? (VALUE ? p.vprs : p.kprs) : (VALUE ? p.vrs : p.krs));
+        const Piece& t = VALUE ? v : k;
+        uint32_t off[4];
 #pragma unroll
-            for (uint32_t g = 0; g < 4u; ++g) {
-                const int32_t page = number(u, g);
-                const uint32_t key = t0 + 16u * g, r = key - p.div_page.div(key) * p.page_rows;
-                const uint64_t at = VALUE ? uint32_t(max(page, 0)) * p.vps + it.kvh * p.vphs + r * p.vprs
-                                          : uint32_t(max(page, 0)) * p.kps + it.kvh * p.kphs + r * p.kprs;
-                const uint32_t rows = page >= 0 ? min(16u, it.st.kept - key) : 0u;
-                if (VALUE)
-                    v_page(dst, g, p.v_pages + at, rows);
-                else
-                    k_page(dst, g, p.k_pages + at, rows);
-            }
-        } else {
-            const uint32_t n0 = it.st.fresh(u);
+        for (uint32_t i = 0; i < 4u; ++i) // rows 4 i of the group, of K the chunks swizzled by the row
+            off[i] = VALUE ? (v_key + 4u * i) * row + v_chunk : (k_key + 4u * i) * row + (k_chunk ^ (64u * i));
 #pragma unroll
-            for (uint32_t g = 0; g < 4u; ++g) {
-                const uint32_t r = n0 + 16u * g, rows = r < it.st.rows ? min(16u, it.st.rows - r) : 0u;
-                const uint64_t row = it.st.q0 + (rows ? r : 0u);
-                if (VALUE)
-                    v_new(dst, g, p.v + it.kvh * p.vhs + row * p.vrs, rows);
-                else
-                    k_new(dst, g, p.k + it.kvh * p.khs + row * p.krs, rows);
-            }
+        for (uint32_t g = 0; g < 4u; ++g) {
+            const int at = int(4u * (u % 16u) + g);
+            const u32x4_t b{uint32_t(__builtin_amdgcn_readlane(int(uint32_t(t.at)), at)),
+                            uint32_t(__builtin_amdgcn_readlane(int(uint32_t(t.at >> 32)), at)) & 0xffffu,
+                            uint32_t(__builtin_amdgcn_readlane(int(t.bytes), at)), uint32_t(kRsrcFlags)};
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i)
+                load_lds16(b, dst + 4096u * g + 1024u * i, off[i]);
         }
     }
 };
 
 // The keys of tile u that the lane's row attends.
-__device__ __forceinline__ uint64_t bits_of(const PagesParams& p, Item& it, const PageFeed& feed, uint32_t u)
+template <class Feed>
+__device__ __forceinline__ uint64_t bits_of(const PagesParams& p, Item& it, const Feed& feed, uint32_t u)
 {
     if (!it.st.is_kept(u))
         return fresh_bits(p, it, it.st.fresh(u));
@@ -293,13 +303,13 @@ __device__ __forceinline__ uint64_t bits_of(const PagesParams& p, Item& it, cons
     return (key_bits(it.lo, it.st.kept, t0) | key_bits(0u, it.st.sinks, t0)) & feed.there(u);
 }
 
-// Whether every row attends all of tile u.
-__device__ __forceinline__ bool is_whole(const Item& it, const PageFeed& feed, uint32_t u)
+// Whether every row attends all of tile u, if its pages are there.
+__device__ __forceinline__ bool is_whole(const Item& it, uint32_t u)
 {
     if (!it.st.is_kept(u))
         return false;
     const uint32_t t0 = it.st.key(u);
-    return t0 + 64u <= it.st.kept && (t0 >= it.all_lo || t0 + 64u <= it.st.sinks) && feed.there(u) == ~uint64_t(0);
+    return t0 + 64u <= it.st.kept && (t0 >= it.all_lo || t0 + 64u <= it.st.sinks);
 }
 
 // A turn of attn_pages_kernel, tile u, as few_turn of attn_dense.hip: a tile's K is on its way from the products before it
@@ -362,9 +372,9 @@ __device__ __forceinline__ void store_item(const PagesParams& p, const Item& it,
             *reinterpret_cast<float2*>(p.part + 2ull * p.workers * p.slot_rows * 128u + at * 2u) = float2{w.m_run, l};
         return;
     }
-    const uint32_t head = it.kvh * p.group + (f - it.row * p.group);
+    const uint32_t row = p.div_group.div(f), head = it.kvh * p.group + (f - row * p.group);
     const float inv = 1.0f / l; // a row attends itself
-    uint16_t* const dst = p.out + uint64_t(head) * p.ohs + uint64_t(it.st.q0 + it.row) * p.ors;
+    uint16_t* const dst = p.out + uint64_t(head) * p.ohs + uint64_t(it.st.q0 + row) * p.ors;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -374,7 +384,7 @@ __device__ __forceinline__ void store_item(const PagesParams& p, const Item& it,
                       pack_bf16(w.o[db][4 * g + 2] * inv, w.o[db][4 * g + 3] * inv)};
 }
 
-// A workgroup's run of all items' tiles: item(i, first, last, slot) for each of its parts.
+// A workgroup's run of all items' tiles: part(item, first, last, slot) for each of its parts.
 template <class Part>
 __device__ __forceinline__ void for_parts(const PagesParams& p, uint32_t lane, const Part& part)
 {
@@ -391,10 +401,9 @@ __device__ __forceinline__ void for_parts(const PagesParams& p, uint32_t lane, c
     while (x < end) {
         while (x >= streams.end)
             streams.load(p, streams.s0 + kWave, streams.end, lane);
-        // The last stream that begins at x or before it and has tiles.
-        const uint32_t at = 63u - uint32_t(__builtin_clzll(__ballot(streams.before <= x && streams.units != 0u)));
+        const uint32_t at = streams.of(x);
         uint32_t sinks;
-        const Stream st = streams.get(p, at, sinks);
+        const Stream st = stream_of(p, streams.s0 + at, sinks);
         const uint64_t local = x - lane_u64(streams.before, at), number = local / st.tiles;
         const uint32_t first = uint32_t(local - number * st.tiles);
         const uint32_t last = uint32_t(min(uint64_t(st.tiles), first + (end - x)));
@@ -414,165 +423,152 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t lane = threadIdx.x;
     const TileReads rd(lane);
-    PageFeed feed{{p.kprs, lane}, {p.krs, lane}, {p.vprs, lane}, {p.vrs, lane}, lds, -1};
+    PageFeed feed(lds, lane);
     for_parts(p, lane, [&](Item& it, uint32_t first, uint32_t last, uint32_t slot) {
         WaveRows w;
+        bound_window(p, it);
         feed.numbers(p, it, first & ~15u, lane);
         feed.load<false>(p, it, first);
         feed.load<true>(p, it, first);
         load_item(p, it, lane, w);
         for (uint32_t u = first; u < last;) {
 #pragma unroll 1
-            for (; u < last && !is_whole(it, feed, u); ++u)
+            for (; u < last && !(is_whole(it, u) && feed.all_there(u)); ++u)
                 pages_turn<CAP, true>(p, it, w, feed, rd, u, last, lane);
 #pragma unroll 1
-            for (; u < last && is_whole(it, feed, u); ++u)
+            for (; u < last && is_whole(it, u) && feed.all_there(u); ++u)
                 pages_turn<CAP, false>(p, it, w, feed, rd, u, last, lane);
         }
         store_item(p, it, w, slot, lane);
     });
 }
 
-// What a wave of eight loads of a workgroup's tiles, each an eighth: eight rows, which lie in one page.
+// What a wave of eight loads of a workgroup's tiles, each an eighth: eight rows, which lie in one page. Their places and
+// sizes are found for 64 tiles at a time, one a lane, every 32 tiles, and lie in LDS: among the softmax's vector
+// instructions there is no time for the some 40 scalar ones that each takes.
 struct PairPageFeed {
     static constexpr int kLoads = 4; // of a turn
     const PagesParams& p;
     const Item& it;
     char* lds;
-    const uint16_t* k_pool; // of the key head
-    const uint16_t* v_pool;
-    const uint16_t* k_rows; // of the stream's new rows
-    const uint16_t* v_rows;
+    u32x4_t* places; // of tile u at u % 64: K's, V's behind all of K's: address, bytes, bytes from a row to the next
     uint32_t first, tiles, wave; // the part's first tile, and how many
     uint32_t k_key, k_chunk, v_key, v_chunk; // the lane's row and bytes of it in its instructions
-    uint32_t base; // lane u % 64 has the page of tile u, of base .. base + 63
-    int32_t ids;
-    uint64_t group_there[4], there_all; // bit u % 64: whether the page of each group of 16 rows is there
+    uint32_t base;         // the places are those of tiles base .. base + 63
+    uint64_t whole;        // bit u % 64: every row attends all of tile u
+    uint64_t group_there[4]; // whether the page of each group of 16 rows is there
 
-    __device__ __forceinline__ PairPageFeed(const PagesParams& params, const Item& item, char* memory, uint32_t part_first,
-                                            uint32_t part_tiles, uint32_t wave_number, uint32_t lane)
-        : p(params), it(item), lds(memory), first(part_first), tiles(part_tiles), wave(wave_number)
+    __device__ __forceinline__ PairPageFeed(const PagesParams& params, const Item& item, char* memory, u32x4_t* list,
+                                            uint32_t part_first, uint32_t part_tiles, uint32_t wave_number, uint32_t lane)
+        : p(params), it(item), lds(memory), places(list), first(part_first), tiles(part_tiles), wave(wave_number)
     {
-        k_pool = p.k_pages + it.kvh * p.kphs, v_pool = p.v_pages + it.kvh * p.vphs;
-        k_rows = p.k + it.kvh * p.khs + it.st.q0 * p.krs, v_rows = p.v + it.kvh * p.vhs + it.st.q0 * p.vrs;
         k_key = lane >> 4, k_chunk = 16u * ((lane & 15u) ^ (8u * (wave & 1u) + k_key));
         v_key = (lane >> 2) & 3u, v_chunk = 16u * (4u * (lane >> 4) + (lane & 3u));
-        base = first & ~31u;
-        numbers(lane);
     }
-    __device__ __forceinline__ void numbers(uint32_t lane)
+    __device__ __forceinline__ void find(uint32_t from)
     {
+        const uint32_t lane = threadIdx.x & 63u;
+        base = from;
         const uint32_t u = base + ((lane - base) & 63u);
         const bool kept = it.st.is_kept(u);
-        const uint32_t key = kept ? it.st.key(u) : 0u;
-        const int32_t* const line = p.table + uint64_t(it.stream) * p.table_stride;
-        ids = -1;
-        there_all = ~uint64_t(0);
+        const uint32_t key = kept ? it.st.key(u) : it.st.fresh(min(u, it.st.tiles - 1u));
+        int32_t mine = -1;
+        whole = __ballot(is_whole(it, u));
 #pragma unroll
         for (uint32_t g = 0; g < 4u; ++g) {
-            const bool in = kept && key + 16u * g < it.st.kept;
-            const int32_t page = in ? line[p.div_page.div(key + 16u * g)] : -1;
-            const bool there = uint32_t(page) < p.pages;
-            ids = g == wave / 2u && there ? page : ids;
-            group_there[g] = __ballot(there || !in);
-            there_all &= group_there[g];
+            const int32_t page = kept ? page_of(p, it, key + 16u * g) : -1;
+            mine = g == wave / 2u ? page : mine;
+            group_there[g] = __ballot(page >= 0);
+            whole &= group_there[g];
         }
+        const Piece k = piece_of<false>(p, it, kept, key + 8u * wave, mine, 8u);
+        const Piece v = piece_of<true>(p, it, kept, key + 8u * wave, mine, 8u);
+        places[lane] = u32x4_t{uint32_t(k.at), uint32_t(k.at >> 32) & 0xffffu, k.bytes, 2u * uint32_t(kept ? p.kprs : p.krs)};
+        places[64u + lane] =
+            u32x4_t{uint32_t(v.at), uint32_t(v.at >> 32) & 0xffffu, v.bytes, 2u * uint32_t(kept ? p.vprs : p.vrs)};
+        asm volatile("" ::: "memory"); // a wave's LDS accesses are in order
     }
     __device__ __forceinline__ const char* k_tile(uint32_t t) const { return lds + (t % kRing) * kTileBytes; }
     __device__ __forceinline__ const char* v_tile(uint32_t t) const { return lds + (kRing + t % kRing) * kTileBytes; }
     __device__ __forceinline__ int32_t* positions(uint32_t) const { return nullptr; }
     // The part's tile t, past its end the last one again: every turn has the same count of loads.
+    __device__ __forceinline__ uint32_t unit(uint32_t t) const { return first + min(t, tiles - 1u); }
+    template <bool VALUE>
+    __device__ __forceinline__ void load(uint32_t t, const u32x4_t& place) const
+    {
+        char* const dst = const_cast<char*>(VALUE ? v_tile(t) : k_tile(t)) + 2048u * wave;
+        const u32x4_t b{uint32_t(__builtin_amdgcn_readfirstlane(int(place[0]))), // all lanes have the same
+                        uint32_t(__builtin_amdgcn_readfirstlane(int(place[1]))),
+                        uint32_t(__builtin_amdgcn_readfirstlane(int(place[2]))), uint32_t(kRsrcFlags)};
+        // Rows 4 of each instruction, of K the chunks swizzled by the row (an instruction on, by four more).
+        const uint32_t off = (VALUE ? v_key : k_key) * place[3] + (VALUE ? v_chunk : k_chunk);
+        load_lds16(b, dst, off);
+        load_lds16(b, dst + 1024u, (VALUE ? off : off ^ 64u) + 4u * place[3]);
+    }
     template <bool VALUE>
     __device__ __forceinline__ void load(uint32_t t) const
     {
-        const uint32_t u = first + min(t, tiles - 1u);
-        char* const dst = const_cast<char*>(VALUE ? v_tile(t) : k_tile(t)) + 2048u * wave;
-        const uint16_t* at;
-        uint32_t rows, row;
-        if (it.st.is_kept(u)) {
-            const int32_t page = __builtin_amdgcn_readlane(ids, int(u % 64u));
-            const uint32_t key = it.st.key(u) + 8u * wave, r = key - p.div_page.div(key) * p.page_rows;
-            at = VALUE ? v_pool + uint32_t(max(page, 0)) * p.vps + r * p.vprs : k_pool + uint32_t(max(page, 0)) * p.kps + r * p.kprs;
-            rows = page >= 0 && key < it.st.kept ? min(8u, it.st.kept - key) : 0u;
-            row = uint32_t(VALUE ? p.vprs : p.kprs) * 2u;
-        } else {
-            const uint32_t r = it.st.fresh(u) + 8u * wave;
-            rows = r < it.st.rows ? min(8u, it.st.rows - r) : 0u;
-            at = VALUE ? v_rows + (rows ? r : 0u) * p.vrs : k_rows + (rows ? r : 0u) * p.krs;
-            row = uint32_t(VALUE ? p.vrs : p.krs) * 2u;
-        }
-        u32x4_t b = buffer_words(at, rows ? (rows - 1u) * row + 256u : 0u);
-#pragma unroll
-        for (int i = 0; i < 3; ++i)
-            b[i] = uint32_t(__builtin_amdgcn_readfirstlane(int(b[i]))); // all of a wave's lanes have the same
-        // Rows 4 of each instruction, of K the chunks swizzled by the row (an instruction on, by four more).
-        load_lds16(b, dst, (VALUE ? v_key : k_key) * row + (VALUE ? v_chunk : k_chunk));
-        load_lds16(b, dst + 1024u, ((VALUE ? v_key : k_key) + 4u) * row + (VALUE ? v_chunk : k_chunk ^ 64u));
+        load<VALUE>(t, places[(VALUE ? 64u : 0u) + unit(t) % 64u]);
     }
-    __device__ __forceinline__ void next_k(uint32_t t)
+    __device__ __forceinline__ void next(uint32_t t)
     {
-        if (first + min(t + 3u, tiles - 1u) >= base + 64u) {
-            base += 32u;
-            numbers(threadIdx.x & 63u);
-        }
-        load<false>(t + 3u);
+        if (unit(t + 3u) >= base + 64u)
+            find(base + 32u);
+        const u32x4_t k = places[unit(t + 3u) % 64u], v = places[64u + unit(t + 2u) % 64u];
+        load<false>(t + 3u, k);
+        load<true>(t + 2u, v);
     }
-    __device__ __forceinline__ void next_v(uint32_t t) { load<true>(t + 2u); }
-    __device__ __forceinline__ bool all_there(uint32_t u) const { return there_all >> (u % 64u) & 1u; }
     // The bits of the tile's keys whose page is there.
     __device__ __forceinline__ uint64_t there(uint32_t u) const
     {
-        uint64_t bits = ~uint64_t(0);
-        if (!all_there(u))
+        uint64_t bits = 0;
 #pragma unroll
-            for (uint32_t g = 0; g < 4u; ++g)
-                bits &= group_there[g] >> (u % 64u) & 1u ? ~uint64_t(0) : ~(uint64_t(0xffff) << (16u * g));
+        for (uint32_t g = 0; g < 4u; ++g)
+            bits |= group_there[g] >> (u % 64u) & 1u ? uint64_t(0xffff) << (16u * g) : 0u;
         return bits;
     }
 };
 
-// A part's tiles, as pair_walk asks for them.
+// A part's tiles, as pair_walk asks for them. What a lane has of its row lies in LDS: only masked turns ask for it.
 struct PairPageWalk {
     const PagesParams& p;
     Item& it;
     const PairPageFeed& feed;
+    uint4* rows; // the wave's: number, place in its line, that place, first kept row under the window
     uint32_t lane;
     __device__ __forceinline__ uint32_t key(uint32_t) const { return 0u; } // only a bias asks where a tile lies
-    __device__ __forceinline__ bool whole(uint32_t t) const
-    {
-        const uint32_t u = feed.first + t;
-        if (!it.st.is_kept(u))
-            return false;
-        const uint32_t t0 = it.st.key(u);
-        return t0 + 64u <= it.st.kept && (t0 >= it.all_lo || t0 + 64u <= it.st.sinks) && feed.all_there(u);
-    }
+    __device__ __forceinline__ bool whole(uint32_t t) const { return feed.whole >> ((feed.first + t) % 64u) & 1u; }
     __device__ __forceinline__ BitsSeen seen(uint32_t t)
     {
-        const uint32_t u = feed.first + t;
-        uint64_t bits;
-        if (it.st.is_kept(u)) {
-            const uint32_t t0 = it.st.key(u);
-            bits = (key_bits(it.lo, it.st.kept, t0) | key_bits(0u, it.st.sinks, t0)) & feed.there(u);
-        } else {
-            bits = fresh_bits(p, it, it.st.fresh(u));
-        }
+        const uint4 r = rows[lane & 31u];
+        it.row = r.x, it.up = r.y, it.up_place = r.z, it.lo = r.w;
+        const uint64_t bits = bits_of(p, it, feed, feed.first + t);
+        if (p.parents)
+            rows[lane & 31u] = uint4{it.row, it.up, it.up_place, it.lo}; // both of a row's lanes the same
         return BitsSeen(it.f0 + (lane & 31u) < it.list ? bits : 0u, lane);
     }
 };
 
 // Eight waves a workgroup: one to a CU.
+constexpr uint32_t kPairWaveBytes = 1024u + 512u + 2048u; // a wave's scratch, its rows, its places
+
 template <bool CAP>
 __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_pages_pair_kernel(PagesParams p)
 {
-    // K ring, V ring, a wave's scratch (1 KB), and for two tiles whether the waves' parts of V hold an infinity or a NaN.
+    // K ring, V ring, the waves' own, and for two tiles whether the waves' parts of V hold an infinity or a NaN.
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint16_t* const scratch = reinterpret_cast<uint16_t*>(lds + 2u * kRing * kTileBytes + 1024u * wave);
-    uint32_t* const odd = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + 1024u * kPairWaves);
+    char* const own = lds + 2u * kRing * kTileBytes + kPairWaveBytes * wave;
+    uint16_t* const scratch = reinterpret_cast<uint16_t*>(own);
+    uint4* const rows = reinterpret_cast<uint4*>(own + 1024u);
+    u32x4_t* const places = reinterpret_cast<u32x4_t*>(own + 1536u);
+    uint32_t* const odd = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + kPairWaveBytes * kPairWaves);
     const TileReads rd(lane);
     for_parts(p, lane, [&](Item& it, uint32_t first, uint32_t last, uint32_t slot) {
         it.f0 += 32u * wave;
-        PairPageFeed feed(p, it, lds, first, last - first, wave, lane);
+        bound_window(p, it);
+        PairPageFeed feed(p, it, lds, places, first, last - first, wave, lane);
+        feed.find(first & ~31u);
         lds_barrier(); // the part before this one is read
         feed.load<false>(0u);
         feed.load<false>(1u);
@@ -581,7 +577,8 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
         feed.load<true>(1u);
         WaveRows w;
         load_item(p, it, lane, w);
-        PairPageWalk walk{p, it, feed, lane};
+        rows[lane & 31u] = uint4{it.row, it.up, it.up_place, it.lo};
+        PairPageWalk walk{p, it, feed, rows, lane};
         pair_walk<CAP, false>(p, w, feed, walk, rd, scratch, odd, wave, last - first, lane);
         store_item(p, it, w, slot, lane);
     });
@@ -599,7 +596,9 @@ __global__ __launch_bounds__(256) void attn_pages_join_kernel(PagesParams p)
     for (uint32_t s0 = 0; s0 < p.streams; s0 += kWave) {
         streams.load(p, s0, base, lane);
         base = streams.end;
-        const uint32_t eights = (streams.rows * p.group + 7u) / 8u;
+        uint32_t sinks;
+        const uint32_t rows = s0 + lane < p.streams ? stream_of(p, s0 + lane, sinks).rows : 0u;
+        const uint32_t eights = (rows * p.group + 7u) / 8u;
         const uint64_t mine = uint64_t(eights) * p.kv_heads, sum = wave_scan_u64(mine, lane);
         const uint64_t all = lane_u64(sum, kWave - 1);
         if (block < all) {
@@ -613,7 +612,7 @@ __global__ __launch_bounds__(256) void attn_pages_join_kernel(PagesParams p)
     if (at == 64u)
         return;
     uint32_t sinks;
-    const Stream st = streams.get(p, at, sinks);
+    const Stream st = stream_of(p, streams.s0 + at, sinks);
     const uint32_t kvh = uint32_t(block / per), f = 8u * uint32_t(block - uint64_t(kvh) * per) + threadIdx.x / 32u;
     const uint64_t x0 = lane_u64(streams.before, at) + (uint64_t(kvh) * st.row_tiles + f / p.item_rows) * st.tiles;
     const uint64_t x1 = x0 + st.tiles;
@@ -734,7 +733,7 @@ template <bool CAP>
 int launch_pages(const PagesParams& p, hipStream_t stream)
 {
     if (p.item_rows > 32u)
-        return launch_items(attn_pages_pair_kernel<CAP>, kPairWaves, 2u * kRing * kTileBytes + (1024u + 8u) * kPairWaves, p,
+        return launch_items(attn_pages_pair_kernel<CAP>, kPairWaves, 2u * kRing * kTileBytes + (kPairWaveBytes + 8u) * kPairWaves, p,
                             stream);
     return launch_items(attn_pages_kernel<CAP>, 1u, 2u * kTileBytes + 1024u, p, stream);
 }

@@ -752,8 +752,7 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Fee
     phase_barrier();
     // The softmax. With it go out K of tile t + 3, into the slot of tile t - 1, which both groups have read, and V of tile
     // t + 2 into that of tile t - 2 (among the products they cost 10%: this phase is the shorter one).
-    feed.next_k(t);
-    feed.next_v(t);
+    feed.next(t);
     if (!MASKED || seen.meets(w))
         tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, seen, feed.positions(t), near_pos, kSloped, near, lane);
     // Past the last tile these are some tile's again, and not used.
