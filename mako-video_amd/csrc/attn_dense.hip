@@ -468,7 +468,7 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     feed.v();
     if (SINKS) {
         PairWalk<BIAS> turns{walk, first, last, all_lo, all_hi, all_s_lo, all_s_hi, rows, lane};
-        pair_walk<CAP, BIAS>(p, w, feed, turns, rd, scratch, odd, wave, tiles, lane);
+        pair_walk<CAP, BIAS>(p, w, feed, turns, rd, scratch, odd, wave, tiles, f0 < p.list, lane);
         const uint4 r = rows[lane & 31u];
         w.lo = r.x, w.hi = r.y;
         store_rows(p, w, kvh, f0, split, lane);

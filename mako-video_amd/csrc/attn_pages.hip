@@ -19,7 +19,8 @@
 // - Streams are of any lengths, which the host does not know. All items' tiles are one list, and each of as many workgroups
 //   as the chip holds takes an equal run of it, whichever items that cuts: it writes the items that are its own and leaves
 //   parts (O, the maximum, the sum) of the two at its ends. A second kernel joins those in the order of the tiles. Where the
-//   cuts lie follows from the lengths alone.
+//   cuts lie follows from the lengths alone. If all streams' items have as many row tiles, that many workgroups take the
+//   same run, one row tile each, so that what one of them has read the others find in their XCD's L2.
 #include "attn_tiles.hpp"
 
 namespace mh3 {
@@ -71,9 +72,17 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t v, uint32_t lane)
            uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), int(lane)))) << 32;
 }
 
+// a / b and ceil(a / b), of 32 bits where a has no more: 64 take some hundred instructions.
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint32_t b)
+{
+    return a >> 32 ? a / b : uint64_t(uint32_t(a) / b);
+}
+
 // The sum of v over the lanes up to this one.
 __device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, uint32_t lane)
 {
+    if (!__ballot(v >> 26)) // so 64 of them are below 2^32
+        return wave_excl_scan_u32(uint32_t(v)) + v;
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
         const uint64_t o = __shfl_up(static_cast<unsigned long long>(v), d, kWave);
@@ -96,36 +105,62 @@ __device__ __forceinline__ Stream stream_of(const PagesParams& p, uint32_t s, ui
 struct Streams {
     uint32_t s0;
     uint64_t before, some, end; // tiles before the lane's stream; the streams that have any; those up to the 64's end
-    __device__ __forceinline__ void load(const PagesParams& p, uint32_t from, uint64_t base, uint32_t lane)
+    // together: row tiles that a run takes at once, if all have as many; else 1, and they count one by one.
+    __device__ __forceinline__ void sum(const PagesParams& p, uint32_t from, uint64_t base, const Stream& t, uint32_t together,
+                                        uint32_t lane)
     {
         s0 = from;
-        uint64_t units = 0;
-        if (from + lane < p.streams) {
-            uint32_t sinks;
-            const Stream t = stream_of(p, from + lane, sinks);
-            units = uint64_t(t.row_tiles) * p.kv_heads * t.tiles;
-        }
+        const uint64_t units = uint64_t(together > 1u ? min(t.row_tiles, 1u) : t.row_tiles) * p.kv_heads * t.tiles;
         some = __ballot(units != 0u);
-        const uint64_t sum = wave_scan_u64(units, lane);
-        before = base + sum - units;
-        end = base + lane_u64(sum, kWave - 1);
+        const uint64_t to = wave_scan_u64(units, lane);
+        before = base + to - units;
+        end = base + lane_u64(to, kWave - 1);
+    }
+    __device__ __forceinline__ static Stream of_lane(const PagesParams& p, uint32_t from, uint32_t lane)
+    {
+        uint32_t sinks;
+        return from + lane < p.streams ? stream_of(p, from + lane, sinks) : Stream(p, 0u, 0u, 0u, 0u);
+    }
+    __device__ __forceinline__ void load(const PagesParams& p, uint32_t from, uint64_t base, uint32_t together, uint32_t lane)
+    {
+        sum(p, from, base, of_lane(p, from, lane), together, lane);
     }
     // The last stream that begins at tile x or before it and has tiles, x one of the 64's.
     __device__ __forceinline__ uint32_t of(uint64_t x) const { return 63u - uint32_t(__builtin_clzll(__ballot(before <= x) & some)); }
 };
 
-// All items' tiles, and a workgroup's share of them.
-__device__ __forceinline__ uint64_t all_units(const PagesParams& p, Streams& st, uint32_t lane)
-{
-    st.load(p, 0u, 0u, lane);
-    while (st.s0 + kWave < p.streams)
-        st.load(p, st.s0 + kWave, st.end, lane);
-    return st.end;
-}
-__device__ __forceinline__ uint64_t share_of(const PagesParams& p, uint64_t units)
-{
-    return max((units + p.workers - 1u) / p.workers, uint64_t(kLeastTiles));
-}
+// How the items' tiles are shared out: runs of `share`, each taken by `together` workgroups, a row tile each.
+struct Shares {
+    uint64_t units, share;
+    uint32_t together;
+    // Leaves the streams at their first 64.
+    __device__ __forceinline__ Shares(const PagesParams& p, Streams& st, uint32_t lane)
+    {
+        const Stream mine = Streams::of_lane(p, 0u, lane);
+        uint32_t least = wave_min_u32(mine.rows ? mine.row_tiles : ~0u), most = wave_max_u32(mine.row_tiles);
+        for (uint32_t s0 = kWave; s0 < p.streams; s0 += kWave) {
+            const Stream t = Streams::of_lane(p, s0, lane);
+            least = min(least, wave_min_u32(t.rows ? t.row_tiles : ~0u)), most = max(most, wave_max_u32(t.row_tiles));
+        }
+        together = least == most && most <= p.workers ? most : 1u;
+        st.sum(p, 0u, 0u, mine, together, lane);
+        while (st.s0 + kWave < p.streams)
+            st.load(p, st.s0 + kWave, st.end, together, lane);
+        units = st.end;
+        const uint32_t runs = p.workers / together;
+        share = max(quotient(units + runs - 1u, runs), uint64_t(kLeastTiles));
+        if (st.s0 != 0u)
+            st.sum(p, 0u, 0u, mine, together, lane);
+    }
+};
+
+// What the join has to know of an item that runs cut, left by the workgroup whose run is the first to begin inside it.
+struct Cut {
+    uint32_t rows; // list rows, 0: the workgroup leaves none
+    uint32_t q0, f0, kvh;
+    uint32_t run, last; // the parts are those of runs run - 1 .. last
+    uint32_t together, row_tile;
+};
 
 // Rows in one piece: where they begin and how many bytes a buffer over them has (none: nothing is read, and zeros come).
 struct Piece {
@@ -351,6 +386,9 @@ __device__ __forceinline__ void pages_turn(const PagesParams& p, Item& it, WaveR
         feed.load<true>(p, it, u + 1u);
 }
 
+// The parts behind the cuts.
+__device__ __forceinline__ float* parts_of(const PagesParams& p) { return p.part + uint64_t(p.workers) * (sizeof(Cut) / 4u); }
+
 // Writes an item's rows, or with `slot` a part of them: O [slot][row][128], behind all slots' the maxima and sums.
 __device__ __forceinline__ void store_item(const PagesParams& p, const Item& it, const WaveRows& w, uint32_t slot,
                                            uint32_t lane)
@@ -361,7 +399,7 @@ __device__ __forceinline__ void store_item(const PagesParams& p, const Item& it,
         return;
     if (slot != ~0u) {
         const uint64_t at = uint64_t(slot) * p.slot_rows + n;
-        float* const dst = p.part + at * 128u;
+        float* const dst = parts_of(p) + at * 128u;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -369,7 +407,7 @@ __device__ __forceinline__ void store_item(const PagesParams& p, const Item& it,
                 *reinterpret_cast<float4*>(dst + 32 * db + 8 * g + 4u * hh) =
                     float4{w.o[db][4 * g], w.o[db][4 * g + 1], w.o[db][4 * g + 2], w.o[db][4 * g + 3]};
         if (hh == 0)
-            *reinterpret_cast<float2*>(p.part + 2ull * p.workers * p.slot_rows * 128u + at * 2u) = float2{w.m_run, l};
+            *reinterpret_cast<float2*>(parts_of(p) + 2ull * p.workers * p.slot_rows * 128u + at * 2u) = float2{w.m_run, l};
         return;
     }
     const uint32_t row = p.div_group.div(f), head = it.kvh * p.group + (f - row * p.group);
@@ -391,29 +429,38 @@ __device__ __forceinline__ void for_parts(const PagesParams& p, uint32_t lane, c
     // Blocks go to the 8 XCDs round-robin; each takes a contiguous part of the list, key head by key head.
     const uint32_t worker = (blockIdx.x % 8u) * (gridDim.x / 8u) + blockIdx.x / 8u;
     Streams streams;
-    const uint64_t units = all_units(p, streams, lane), share = share_of(p, units);
-    uint64_t x = share * worker;
-    const uint64_t end = min(units, x + share);
-    if (x >= end)
-        return;
-    if (streams.s0 != 0u)
-        streams.load(p, 0u, 0u, lane);
-    while (x < end) {
+    const Shares shares(p, streams, lane);
+    const uint32_t run = worker / shares.together, row_tile = worker - run * shares.together;
+    const uint64_t begin = shares.share * run, end = min(shares.units, begin + shares.share);
+    Cut cut{};
+    for (uint64_t x = begin; x < end;) {
         while (x >= streams.end)
-            streams.load(p, streams.s0 + kWave, streams.end, lane);
-        const uint32_t at = streams.of(x);
+            streams.load(p, streams.s0 + kWave, streams.end, shares.together, lane);
+        const uint32_t at = streams.of(x), stream = streams.s0 + at;
         uint32_t sinks;
-        const Stream st = stream_of(p, streams.s0 + at, sinks);
-        const uint64_t local = x - lane_u64(streams.before, at), number = local / st.tiles;
+        const Stream st = stream_of(p, stream, sinks);
+        const uint64_t local = x - lane_u64(streams.before, at), number = quotient(local, st.tiles);
         const uint32_t first = uint32_t(local - number * st.tiles);
         const uint32_t last = uint32_t(min(uint64_t(st.tiles), first + (end - x)));
-        Item it{st, streams.s0 + at, uint32_t(number / st.row_tiles), st.rows * p.group, 0u, sinks, 0u, 0u, 0u, 0u, 0u, 0u};
-        it.f0 = p.item_rows * uint32_t(number - uint64_t(it.kvh) * st.row_tiles);
+        const uint32_t kvh = uint32_t(shares.together > 1u ? number : quotient(number, st.row_tiles));
+        Item it{st, stream, kvh, st.rows * p.group, 0u, sinks, 0u, 0u, 0u, 0u, 0u, 0u};
+        it.f0 = p.item_rows * (shares.together > 1u ? row_tile : uint32_t(number - uint64_t(kvh) * st.row_tiles));
         // The item that the run begins with, unless with its first tile, is the first of the workgroup's two parts.
-        const bool cut = first > 0u || last < st.tiles;
-        part(it, first, last, cut ? 2u * worker + (first > 0u ? 0u : 1u) : ~0u);
+        const bool whole = first == 0u && last == st.tiles;
+        if (first > 0u && shares.share >= first) // the run before this one begins with the item or ahead of it
+            cut = Cut{min(p.item_rows, it.list - min(it.f0, it.list)),
+                      st.q0,
+                      it.f0,
+                      kvh,
+                      run,
+                      uint32_t(quotient(x - first + st.tiles - 1u, uint32_t(min(shares.share, uint64_t(~0u))))),
+                      shares.together,
+                      row_tile};
+        part(it, first, last, whole ? ~0u : 2u * worker + (first > 0u ? 0u : 1u));
         x += last - first;
     }
+    if (threadIdx.x == 0)
+        reinterpret_cast<Cut*>(p.part)[worker] = cut;
 }
 
 // One wave a workgroup, with a tile of its own in LDS; four of them share a CU.
@@ -579,84 +626,84 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
         load_item(p, it, lane, w);
         rows[lane & 31u] = uint4{it.row, it.up, it.up_place, it.lo};
         PairPageWalk walk{p, it, feed, rows, lane};
-        pair_walk<CAP, false>(p, w, feed, walk, rd, scratch, odd, wave, last - first, lane);
+        pair_walk<CAP, false>(p, w, feed, walk, rd, scratch, odd, wave, last - first, it.f0 < it.list, lane);
         store_item(p, it, w, slot, lane);
     });
 }
 
-// Joins the parts of eight list rows of an item, 32 lanes a row, four values of d each, in the order of the tiles.
-__global__ __launch_bounds__(256) void attn_pages_join_kernel(PagesParams p)
+// Joins the parts of the items that the runs cut, in the order of the tiles: `blocks` blocks a cut, for some of its rows
+// each. 32 lanes a row, four values of d each; with SPLIT 4 a row's parts are taken by four waves, every fourth each, and
+// these meet in LDS.
+template <uint32_t SPLIT>
+__global__ __launch_bounds__(256) void attn_pages_join_kernel(PagesParams p, uint32_t blocks)
 {
-    const uint32_t lane = threadIdx.x & 63u;
-    Streams streams;
-    const uint64_t units = all_units(p, streams, lane), share = share_of(p, units);
-    // The stream of this block's rows: kv_heads ceil(list / 8) blocks each.
-    uint64_t block = blockIdx.x, base = 0;
-    uint32_t at = 64u, per = 0;
-    for (uint32_t s0 = 0; s0 < p.streams; s0 += kWave) {
-        streams.load(p, s0, base, lane);
-        base = streams.end;
-        uint32_t sinks;
-        const uint32_t rows = s0 + lane < p.streams ? stream_of(p, s0 + lane, sinks).rows : 0u;
-        const uint32_t eights = (rows * p.group + 7u) / 8u;
-        const uint64_t mine = uint64_t(eights) * p.kv_heads, sum = wave_scan_u64(mine, lane);
-        const uint64_t all = lane_u64(sum, kWave - 1);
-        if (block < all) {
-            at = uint32_t(__builtin_ctzll(__ballot(block < sum)));
-            block -= lane_u64(sum - mine, at);
-            per = uint32_t(__builtin_amdgcn_readlane(int(eights), int(at)));
-            break;
-        }
-        block -= all;
-    }
-    if (at == 64u)
-        return;
-    uint32_t sinks;
-    const Stream st = stream_of(p, streams.s0 + at, sinks);
-    const uint32_t kvh = uint32_t(block / per), f = 8u * uint32_t(block - uint64_t(kvh) * per) + threadIdx.x / 32u;
-    const uint64_t x0 = lane_u64(streams.before, at) + (uint64_t(kvh) * st.row_tiles + f / p.item_rows) * st.tiles;
-    const uint64_t x1 = x0 + st.tiles;
-    const uint32_t w0 = uint32_t(x0 / share), w1 = uint32_t((x1 - 1u) / share);
-    if (f >= st.rows * p.group || w0 == w1)
-        return;
-    const float2* const ml = reinterpret_cast<const float2*>(p.part + 2ull * p.workers * p.slot_rows * 128u);
-    const uint32_t n = f % p.item_rows, d = 4u * (threadIdx.x & 31u);
-    constexpr uint32_t kU = 8;
-    float m = -kInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t i0 = w0; i0 <= w1; i0 += kU) {
-        float2 t[kU];
-        float4 v[kU];
-#pragma unroll
-        for (uint32_t u = 0; u < kU; ++u) {
-            const uint32_t i = i0 + u;
-            t[u] = float2{-kInf, 0.0f}, v[u] = float4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (i <= w1) {
-                const uint64_t slot = (2ull * i + (share * i <= x0 ? 1u : 0u)) * p.slot_rows + n;
-                t[u] = ml[slot], v[u] = *reinterpret_cast<const float4*>(p.part + slot * 128u + d);
+    __shared__ float met[SPLIT][8 / SPLIT][6][32];
+    const Cut cut = reinterpret_cast<const Cut*>(p.part)[blockIdx.x / blocks];
+    const float* const parts = parts_of(p);
+    const float2* const ml = reinterpret_cast<const float2*>(parts + 2ull * p.workers * p.slot_rows * 128u);
+    constexpr uint32_t kRows = 8u / SPLIT, kU = 8;
+    const uint32_t sub = threadIdx.x / 32u, which = sub / kRows, d = 4u * (threadIdx.x & 31u);
+    for (uint32_t n0 = blockIdx.x % blocks * kRows; n0 < cut.rows; n0 += blocks * kRows) {
+        const uint32_t n = n0 + sub % kRows;
+        const bool mine = n < cut.rows;
+        float m = -kInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const auto meet = [&](const float2* t, const float4* v, uint32_t count) {
+            float m_new = m;
+            for (uint32_t u = 0; u < count; ++u)
+                m_new = fmaxf(m_new, t[u].x);
+            // A part without a key of this row has left zeros and -inf. (A NaN of its scores is in its sum and its O.)
+            const float old = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+            l *= old, m = m_new;
+            for (int c = 0; c < 4; ++c)
+                o[c] *= old;
+            for (uint32_t u = 0; u < count; ++u) {
+                const float e = t[u].x == -kInf ? 1.0f : __builtin_amdgcn_exp2f(t[u].x - m_new);
+                l = fmaf(t[u].y, e, l);
+                o[0] = fmaf(v[u].x, e, o[0]), o[1] = fmaf(v[u].y, e, o[1]);
+                o[2] = fmaf(v[u].z, e, o[2]), o[3] = fmaf(v[u].w, e, o[3]);
             }
+        };
+        for (uint32_t i0 = cut.run - 1u + which; i0 <= cut.last; i0 += SPLIT * kU) {
+            float2 t[kU];
+            float4 v[kU];
+#pragma unroll
+            for (uint32_t u = 0; u < kU; ++u) {
+                const uint32_t i = i0 + SPLIT * u;
+                t[u] = float2{-kInf, 0.0f}, v[u] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (mine && i <= cut.last) {
+                    const uint64_t slot =
+                        (2ull * (i * cut.together + cut.row_tile) + (i < cut.run ? 1u : 0u)) * p.slot_rows + n;
+                    t[u] = ml[slot], v[u] = *reinterpret_cast<const float4*>(parts + slot * 128u + d);
+                }
+            }
+            meet(t, v, kU);
         }
-        float m_new = m;
-#pragma unroll
-        for (uint32_t u = 0; u < kU; ++u)
-            m_new = fmaxf(m_new, t[u].x);
-        // A part without a key of this row has left zeros and -inf. (A NaN of its scores is in its sum and its O.)
-        const float old = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-        l *= old, m = m_new;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            o[c] *= old;
-#pragma unroll
-        for (uint32_t u = 0; u < kU; ++u) {
-            const float e = t[u].x == -kInf ? 1.0f : __builtin_amdgcn_exp2f(t[u].x - m_new);
-            l = fmaf(t[u].y, e, l);
-            o[0] = fmaf(v[u].x, e, o[0]), o[1] = fmaf(v[u].y, e, o[1]);
-            o[2] = fmaf(v[u].z, e, o[2]), o[3] = fmaf(v[u].w, e, o[3]);
+        if (SPLIT > 1u) {
+            float(&mark)[6][32] = met[which][sub % kRows];
+            mark[0][d / 4u] = m, mark[1][d / 4u] = l;
+            for (int c = 0; c < 4; ++c)
+                mark[2 + c][d / 4u] = o[c];
+            __syncthreads();
+            if (which == 0u) {
+                float2 t[SPLIT];
+                float4 v[SPLIT];
+                for (uint32_t i = 0; i < SPLIT; ++i) {
+                    const float(&from)[6][32] = met[i][sub % kRows];
+                    t[i] = float2{from[0][d / 4u], from[1][d / 4u]};
+                    v[i] = float4{from[2][d / 4u], from[3][d / 4u], from[4][d / 4u], from[5][d / 4u]};
+                }
+                m = -kInf, l = 0.0f, o[0] = o[1] = o[2] = o[3] = 0.0f;
+                meet(t, v, SPLIT);
+            }
+            __syncthreads();
         }
+        if (!mine || which != 0u)
+            continue;
+        const float inv = 1.0f / l;
+        const uint32_t f = cut.f0 + n, row = p.div_group.div(f), head = cut.kvh * p.group + (f - row * p.group);
+        *reinterpret_cast<uint2*>(p.out + uint64_t(head) * p.ohs + uint64_t(cut.q0 + row) * p.ors + d) =
+            uint2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
     }
-    const float inv = 1.0f / l;
-    const uint32_t row = p.div_group.div(f), head = kvh * p.group + (f - row * p.group);
-    *reinterpret_cast<uint2*>(p.out + uint64_t(head) * p.ohs + uint64_t(st.q0 + row) * p.ors + d) =
-        uint2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
 }
 
 } // namespace
@@ -681,7 +728,7 @@ PagesPlan pages_plan(const MH3PagesAttnArgs& a)
     plan.item_rows = pair ? 32u * kPairWaves : 32u;
     plan.workers = ((pair ? 1u : 4u) * cus + 7u) / 8u * 8u;
     plan.slot_rows = uint32_t(std::min<uint64_t>(plan.item_rows, list));
-    plan.workspace = 2ull * plan.workers * plan.slot_rows * 130u * 4u;
+    plan.workspace = uint64_t(plan.workers) * (sizeof(Cut) + 2ull * plan.slot_rows * 130u * 4u);
     return plan;
 }
 
@@ -797,10 +844,6 @@ extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint
     const host::Span o[] = {{out, span(a.heads, a.out_head_stride, a.out_row_stride)}, {workspace, need}};
     if (host::any_overlap(in, o))
         return MH3_ERR_PARAM;
-    // A block of the join for every eight list rows of a key head, and one more a stream for what is left of eight.
-    const uint64_t blocks = uint64_t(a.kv_heads) * (uint64_t(a.q_rows) * (a.heads / a.kv_heads) / 8u + t.streams);
-    if (blocks >= (1ull << 31))
-        return MH3_ERR_SHAPE;
     PagesParams p{};
     p.q = q, p.k = k, p.v = v, p.out = out, p.k_pages = k_pages, p.v_pages = v_pages;
     p.table = table, p.lengths = lengths, p.q_off = q_off, p.parents = parents, p.first_rows = sinks;
@@ -817,6 +860,13 @@ extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (const int rc = a.cap > 0.0f ? launch_pages<true>(p, s) : launch_pages<false>(p, s); rc != MH3_OK)
         return rc;
-    hipLaunchKernelGGL(attn_pages_join_kernel, dim3(uint32_t(blocks)), dim3(256), 0, s, p);
+    // Blocks a cut item: for the four waves' rows four passes at most, for the eight waves' eight.
+    if (p.item_rows > 32u) {
+        const uint32_t blocks = (p.slot_rows + 63u) / 64u;
+        hipLaunchKernelGGL(attn_pages_join_kernel<1u>, dim3(p.workers * blocks), dim3(256), 0, s, p, blocks);
+    } else {
+        const uint32_t blocks = (p.slot_rows + 7u) / 8u;
+        hipLaunchKernelGGL(attn_pages_join_kernel<4u>, dim3(p.workers * blocks), dim3(256), 0, s, p, blocks);
+    }
     return host::check_launch();
 }

@@ -726,7 +726,7 @@ template <bool CAP, bool BIAS, bool MASKED, class Feed, class Seen>
 __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Feed& feed, const TileReads& rd,
                                           floatx16 (&s)[2], bf16x8_t (&frag)[kAhead], TileP& pt, uint16_t* scratch,
                                           uint32_t* odd, bool checked, uint32_t wave, uint32_t t, uint32_t t0,
-                                          const Seen& seen, const Seen& before, uint32_t lane)
+                                          const Seen& seen, const Seen& before, uint32_t lane, bool works = true)
 {
     // The products.
     __builtin_amdgcn_s_setprio(1);
@@ -736,7 +736,7 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Fee
     if (kSloped)
         pos = feed.positions(t)[lane], pos = p.k_pos ? pos : int32_t(t0 + lane);
     bool near = false;
-    if (!MASKED || seen.meets(w))
+    if (MASKED ? seen.meets(w) : works)
         near = tile_products<!MASKED, kSloped>(w, s, pt, frag, rd, feed.k_tile(t), feed.v_tile(t - 1u), pos, near_pos, lane);
     if (MASKED) {
         if (t > 0 && before.meets(w))
@@ -753,7 +753,7 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Fee
     // The softmax. With it go out K of tile t + 3, into the slot of tile t - 1, which both groups have read, and V of tile
     // t + 2 into that of tile t - 2 (among the products they cost 10%: this phase is the shorter one).
     feed.next(t);
-    if (!MASKED || seen.meets(w))
+    if (MASKED ? seen.meets(w) : works)
         tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, seen, feed.positions(t), near_pos, kSloped, near, lane);
     // Past the last tile these are some tile's again, and not used.
 #pragma unroll
@@ -767,10 +767,12 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Fee
 
 // The turns of a workgroup's tiles, of which walk.whole(t) says whether every row of the workgroup attends all of tile t,
 // walk.seen(t) a row's keys of another one (asked for once, in order) and walk.key(t) where it lies; and what is left of
-// the last one's output. The feed has loaded K of three tiles and V of two.
+// the last one's output. The feed has loaded K of three tiles and V of two. works: the wave has rows; one without only
+// loads.
 template <bool CAP, bool BIAS, class Feed, class Walk>
 __device__ __forceinline__ void pair_walk(const DenseParams& p, WaveRows& w, Feed& feed, Walk& walk, const TileReads& rd,
-                                          uint16_t* scratch, uint32_t* odd, uint32_t wave, uint32_t tiles, uint32_t lane)
+                                          uint16_t* scratch, uint32_t* odd, uint32_t wave, uint32_t tiles, bool works,
+                                          uint32_t lane)
 {
     wait_vm<Feed::kLoads>(); // K of tiles 0 and 1, V of tile 0
     lds_barrier();
@@ -799,10 +801,10 @@ __device__ __forceinline__ void pair_walk(const DenseParams& p, WaveRows& w, Fee
 #pragma unroll 1
             do {
                 pair_turn<CAP, BIAS, false>(p, w, feed, rd, s, frag, pt, scratch, odd, true, wave, t, walk.key(t), before,
-                                            before, lane);
+                                            before, lane, works);
                 ++t;
             } while (t < tiles && walk.whole(t));
-            masked = false, before = BitsSeen(~uint64_t(0), lane);
+            masked = false, before = BitsSeen(works ? ~uint64_t(0) : 0u, lane);
         }
     }
     const uint32_t end = tiles - 1u;
