@@ -283,41 +283,68 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     store_rows(p, w, kvh, tile * 32u, split, lane);
 }
 
-// What a wave loads of a workgroup's tiles, a call a tile: its eighth of K (with all of the tile's key positions, into the
-// wave's own ring) or of V. After the workgroup's last tile the same again, so that every turn has the same count of loads;
-// these are not read. The state is scalar and moves by additions.
+// What a wave loads of a workgroup's tiles, a call a tile: its quarter of K, or of V. After the workgroup's last tile the
+// same again, so that every turn has the same count of loads; these are not read. The state is scalar and moves by
+// additions.
 // With JUMP, between the tile after which `jump` more are to come and the next one, the gap between the two parts of a walk.
-template <bool VALUE, bool POS, bool JUMP>
+template <bool JUMP>
 struct PairStream {
-    TileLoads<2, VALUE> ld;
+    uint32_t row, off[4];     // bytes from a key to the next; the lane's in its four instructions
+    char* quarter;            // of the ring's first tile
+    uint32_t slot;            // byte offset in the ring
     const uint16_t* at;       // the next tile's first key
     int64_t step;             // elements to the one after it
     uint32_t left, left_step; // keys from it on
     uint32_t more;            // tiles after it
-    char* ring;
-    uint32_t slot; // byte offset in the ring
-    const int32_t* pos;
-    char* pos_ring;
-    uint32_t lane;
-    uint32_t jump, gap; // keys more to the next tile's
-    uint64_t stride;    // elements from a key to the next
+    uint32_t jump, gap;       // keys more to the next tile's
+    __device__ __forceinline__ PairStream(bool value, uint64_t stride, uint32_t wave, uint32_t lane, char* ring,
+                                          const uint16_t* first, uint32_t keys, bool back, uint32_t tiles, uint32_t jump_at,
+                                          uint32_t gap_keys)
+        : row(uint32_t(stride) * 2u), quarter(ring + 4096u * (wave % kHalf)), slot(0u), at(first),
+          step((back ? -64 : 64) * int64_t(stride)), left(keys), left_step(back ? 64u : -64u), more(tiles - 1u), jump(jump_at),
+          gap(gap_keys)
+    {
+        // As TileLoads: instruction i holds keys 4 i .. 4 i + 3, and 4 (wave % 4) is the first.
+        const uint32_t key = value ? (lane >> 2) & 3u : lane >> 4;
+#pragma unroll
+        for (uint32_t u = 0; u < 4u; ++u) {
+            const uint32_t chunk = value ? 4u * (lane >> 4) + (lane & 3u) : (lane & 15u) ^ (4u * u + key);
+            off[u] = (16u * (wave % kHalf) + 4u * u + key) * row + 16u * chunk;
+        }
+    }
     __device__ __forceinline__ void operator()()
     {
-        ld(ring + slot, at, left);
-        if (POS) // no positions: no records, and zeros
-            load_lds4(buffer_words(pos, pos ? left * 4u : 0u), pos_ring + slot / 64u, 4u * lane);
+        const u32x4_t r = buffer_words(at, (min(64u, left) - 1u) * row + 256u);
+#pragma unroll
+        for (uint32_t u = 0; u < 4u; ++u)
+            load_lds16(r, quarter + slot + 1024u * u, off[u]);
         slot = (slot + kTileBytes) & (kRing * kTileBytes - 1u);
         at += more ? step : 0;
         left += more ? left_step : 0u;
-        if (POS)
-            pos -= more && pos ? int32_t(left_step) : 0;
         if (JUMP && more == jump) {
             const bool back = step < 0;
-            at += back ? -int64_t(gap * stride) : int64_t(gap * stride);
+            at += (back ? -int64_t(gap) : int64_t(gap)) * int64_t(row / 2u);
             left += back ? gap : -gap;
-            if (POS)
-                pos -= pos ? (back ? int64_t(gap) : -int64_t(gap)) : 0;
         }
+        more -= more ? 1u : 0u;
+    }
+};
+
+// Under a bias each wave loads all of a tile's key positions into a ring of its own, a turn's with those of K.
+template <bool JUMP>
+struct PosStream {
+    char* ring;
+    uint32_t slot;
+    const int32_t* pos; // null: no records, and zeros
+    uint32_t left, more, jump, gap, lane;
+    __device__ __forceinline__ void operator()()
+    {
+        load_lds4(buffer_words(pos, pos ? left * 4u : 0u), ring + slot, 4u * lane);
+        slot = (slot + 256u) & (kRing * 256u - 1u);
+        // From the last tile to the first.
+        const uint32_t back = (more ? 64u : 0u) + (JUMP && more == jump ? gap : 0u);
+        pos -= pos ? back : 0u;
+        left += back;
         more -= more ? 1u : 0u;
     }
 };
@@ -325,15 +352,21 @@ struct PairStream {
 template <bool BIAS, bool SINKS>
 struct PairFeed {
     static constexpr int kLoads = BIAS ? 5 : 4; // of a turn
-    PairStream<false, BIAS, SINKS> k;
-    PairStream<true, false, SINKS> v;
-    // In turn t: K of tile t + 3, V of tile t + 2.
-    __device__ __forceinline__ void next(uint32_t) { k(), v(); }
-    __device__ __forceinline__ const char* k_tile(uint32_t t) const { return k.ring + (t % kRing) * kTileBytes; }
-    __device__ __forceinline__ const char* v_tile(uint32_t t) const { return v.ring + (t % kRing) * kTileBytes; }
+    PairStream<SINKS> stream;
+    PosStream<SINKS> pos;
+    char* lds;
+    __device__ __forceinline__ const char* k_tile(uint32_t t) const { return lds + (t % kRing) * kTileBytes; }
+    __device__ __forceinline__ const char* v_tile(uint32_t t) const { return lds + (kRing + t % kRing) * kTileBytes; }
     __device__ __forceinline__ int32_t* positions(uint32_t t) const
     {
-        return reinterpret_cast<int32_t*>(k.pos_ring + (t % kRing) * 256u);
+        return reinterpret_cast<int32_t*>(pos.ring + (t % kRing) * 256u);
+    }
+    // In turn t: K of tile t + 3 or V of tile t + 2, and the positions of tile t + 3.
+    __device__ __forceinline__ void next(uint32_t)
+    {
+        stream();
+        if (BIAS)
+            pos();
     }
 };
 
@@ -380,8 +413,8 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     const uint32_t f0 = (tile * kPairWaves + wave) * 32u;
     WaveRows w;
     load_rows<CAP, BIAS, SINKS>(p, kvh, f0, lane, w);
-    uint32_t* const odd = span + 4u * kPairWaves; // [2][kPairWaves]: a masked tile's V holds an infinity or a NaN
-    uint32_t* const s_span = odd + 2u * kPairWaves; // SINKS
+    uint32_t* const odd = span + 4u * kPairWaves; // [2][kHalf]: a masked tile's V holds an infinity or a NaN
+    uint32_t* const s_span = odd + 2u * kHalf;     // SINKS
     // SINKS: the rows' ranges, out of the registers: only masked turns ask for them.
     uint4* const rows = reinterpret_cast<uint4*>(scratch + 1024u);
     if (SINKS && lane < 32u)
@@ -431,41 +464,25 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     const uint32_t gap = both ? walk.k0 - walk.s0 - 64u * walk.front : 0u;
     const uint32_t jump = both ? (BIAS ? walk.front - first : last - walk.front) : ~0u;
     const TileReads rd(lane);
-    const uint32_t from = key_of(0), left_step = BIAS ? 64u : -64u;
-    const auto stride = [](uint64_t row) { return (BIAS ? -64 : 64) * int64_t(row); };
-    PairFeed<BIAS, SINKS> feed{{{p.krs, 2u * wave, lane},
-                         p.k + uint64_t(kvh) * p.khs + uint64_t(from) * p.krs,
-                         stride(p.krs),
-                         p.kv_rows - from,
-                         left_step,
-                         tiles - 1u,
-                         lds,
-                         0u,
-                         p.k_pos ? p.k_pos + from : nullptr,
-                         reinterpret_cast<char*>(scratch) + 1024,
-                         lane,
-                         jump,
-                         gap,
-                         p.krs},
-                        {{p.vrs, 2u * wave, lane},
-                         p.v + uint64_t(kvh) * p.vhs + uint64_t(from) * p.vrs,
-                         stride(p.vrs),
-                         p.kv_rows - from,
-                         left_step,
-                         tiles - 1u,
-                         lds + kRing * kTileBytes,
-                         0u,
-                         nullptr,
-                         nullptr,
-                         lane,
-                         jump,
-                         gap,
-                         p.vrs}};
-    feed.k();
-    feed.k();
-    feed.v();
-    feed.k();
-    feed.v();
+    const uint32_t from = key_of(0);
+    const bool second = wave >= kHalf;
+    const uint64_t head = uint64_t(kvh) * (second ? p.vhs : p.khs), row = second ? p.vrs : p.krs;
+    PairFeed<BIAS, SINKS> feed{{second, row, wave, lane, lds + (second ? kRing * kTileBytes : 0u),
+                                (second ? p.v : p.k) + head + uint64_t(from) * row, p.kv_rows - from, BIAS, tiles, jump, gap},
+                               {reinterpret_cast<char*>(scratch) + 1024, 0u, p.k_pos ? p.k_pos + from : nullptr,
+                                p.kv_rows - from, tiles - 1u, jump, gap, lane},
+                               lds};
+    // K of tiles 0, 1 and 2, or V of tiles 0 and 1, each turn's loads together.
+    if (second) {
+        if (BIAS)
+            feed.pos();
+        feed.next(0u);
+        feed.next(0u);
+    } else {
+        feed.next(0u);
+        feed.next(0u);
+        feed.next(0u);
+    }
     if (SINKS) {
         PairWalk<BIAS> turns{walk, first, last, all_lo, all_hi, all_s_lo, all_s_hi, rows, lane};
         pair_walk<CAP, BIAS>(p, w, feed, turns, rd, scratch, odd, wave, tiles, f0 < p.list, lane);
@@ -474,9 +491,8 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
         store_rows(p, w, kvh, f0, split, lane);
         return;
     }
-    wait_vm<PairFeed<BIAS, SINKS>::kLoads>(); // K of tiles 0 and 1, V of tile 0
+    wait_vm<2 * PairFeed<BIAS, SINKS>::kLoads>(); // K of tile 0
     lds_barrier();
-    const bool second = wave >= kPairWaves / 2u;
     if (second)
         phase_barrier();
     floatx16 s[2];
@@ -511,7 +527,7 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     if (!w.meets(key_of(end)))
         ; // nothing of it is this wave's
     else if (b < tiles || a == tiles) // the last turn was of the masked form
-        masked_output(w, pt, frag, rd, feed.v_tile(end), seen(end), odd + kPairWaves * (end % 2u), scratch, lane);
+        masked_output(w, pt, frag, rd, feed.v_tile(end), seen(end), odd + kHalf * (end % 2u), scratch, lane);
     else
         tile_output(w, pt, frag, rd, feed.v_tile(end));
     if (!second)
@@ -787,7 +803,7 @@ int launch_form(const DenseParams& p, uint32_t waves, hipStream_t stream)
 {
     if (waves == kPairWaves)
         return launch_rows(attn_pair_kernel<CAP, BIAS, SINKS>,
-                           2u * kRing * kTileBytes + (2048u + 16u + 8u + (SINKS ? 512u + 16u : 0u)) * kPairWaves, p, waves, stream);
+                           2u * kRing * kTileBytes + (2048u + 16u + 4u + (SINKS ? 512u + 16u : 0u)) * kPairWaves, p, waves, stream);
     return launch_rows(attn_few_kernel<CAP, BIAS, SINKS>, 2u * kTileBytes + 1024u + 512u, p, waves, stream);
 }
 

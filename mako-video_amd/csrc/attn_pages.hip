@@ -490,17 +490,17 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     });
 }
 
-// What a wave of eight loads of a workgroup's tiles, each an eighth: eight rows, which lie in one page. Their places and
-// sizes are found for 64 tiles at a time, one a lane, every 32 tiles, and lie in LDS: among the softmax's vector
+// What a wave of eight loads of a workgroup's tiles, K or V, each a quarter: a group of 16 rows, which lie in one page. Their
+// places and sizes are found for 64 tiles at a time, one a lane, every 32 tiles, and lie in LDS: among the softmax's vector
 // instructions there is no time for the some 40 scalar ones that each takes.
 struct PairPageFeed {
     static constexpr int kLoads = 4; // of a turn
     const PagesParams& p;
     const Item& it;
     char* lds;
-    u32x4_t* places; // of tile u at u % 64: K's, V's behind all of K's: address, bytes, bytes from a row to the next
+    u32x4_t* places; // of tile u at u % 64: address, bytes, bytes from a row to the next
     uint32_t first, tiles, wave; // the part's first tile, and how many
-    uint32_t k_key, k_chunk, v_key, v_chunk; // the lane's row and bytes of it in its instructions
+    uint32_t key, chunk; // the lane's row and bytes of it in its instructions
     uint32_t base;         // the places are those of tiles base .. base + 63
     uint64_t whole;        // bit u % 64: every row attends all of tile u
     uint64_t group_there[4]; // whether the page of each group of 16 rows is there
@@ -509,8 +509,8 @@ struct PairPageFeed {
                                             uint32_t part_first, uint32_t part_tiles, uint32_t wave_number, uint32_t lane)
         : p(params), it(item), lds(memory), places(list), first(part_first), tiles(part_tiles), wave(wave_number)
     {
-        k_key = lane >> 4, k_chunk = 16u * ((lane & 15u) ^ (8u * (wave & 1u) + k_key));
-        v_key = (lane >> 2) & 3u, v_chunk = 16u * (4u * (lane >> 4) + (lane & 3u));
+        key = wave < kHalf ? lane >> 4 : (lane >> 2) & 3u;
+        chunk = 16u * (wave < kHalf ? (lane & 15u) ^ (lane >> 4) : 4u * (lane >> 4) + (lane & 3u));
     }
     __device__ __forceinline__ void find(uint32_t from)
     {
@@ -518,52 +518,46 @@ struct PairPageFeed {
         base = from;
         const uint32_t u = base + ((lane - base) & 63u);
         const bool kept = it.st.is_kept(u);
-        const uint32_t key = kept ? it.st.key(u) : it.st.fresh(min(u, it.st.tiles - 1u));
+        const uint32_t k0 = kept ? it.st.key(u) : it.st.fresh(min(u, it.st.tiles - 1u));
         int32_t mine = -1;
         whole = __ballot(is_whole(it, u));
 #pragma unroll
         for (uint32_t g = 0; g < 4u; ++g) {
-            const int32_t page = kept ? page_of(p, it, key + 16u * g) : -1;
-            mine = g == wave / 2u ? page : mine;
+            const int32_t page = kept ? page_of(p, it, k0 + 16u * g) : -1;
+            mine = g == wave % kHalf ? page : mine;
             group_there[g] = __ballot(page >= 0);
             whole &= group_there[g];
         }
-        const Piece k = piece_of<false>(p, it, kept, key + 8u * wave, mine, 8u);
-        const Piece v = piece_of<true>(p, it, kept, key + 8u * wave, mine, 8u);
-        places[lane] = u32x4_t{uint32_t(k.at), uint32_t(k.at >> 32) & 0xffffu, k.bytes, 2u * uint32_t(kept ? p.kprs : p.krs)};
-        places[64u + lane] =
-            u32x4_t{uint32_t(v.at), uint32_t(v.at >> 32) & 0xffffu, v.bytes, 2u * uint32_t(kept ? p.vprs : p.vrs)};
+        const uint32_t k = k0 + 16u * (wave % kHalf);
+        const Piece t = wave < kHalf ? piece_of<false>(p, it, kept, k, mine, 16u) : piece_of<true>(p, it, kept, k, mine, 16u);
+        const uint64_t row = wave < kHalf ? (kept ? p.kprs : p.krs) : (kept ? p.vprs : p.vrs);
+        places[lane] = u32x4_t{uint32_t(t.at), uint32_t(t.at >> 32) & 0xffffu, t.bytes, 2u * uint32_t(row)};
         asm volatile("" ::: "memory"); // a wave's LDS accesses are in order
     }
     __device__ __forceinline__ const char* k_tile(uint32_t t) const { return lds + (t % kRing) * kTileBytes; }
     __device__ __forceinline__ const char* v_tile(uint32_t t) const { return lds + (kRing + t % kRing) * kTileBytes; }
     __device__ __forceinline__ int32_t* positions(uint32_t) const { return nullptr; }
     // The part's tile t, past its end the last one again: every turn has the same count of loads.
-    __device__ __forceinline__ uint32_t unit(uint32_t t) const { return first + min(t, tiles - 1u); }
-    template <bool VALUE>
-    __device__ __forceinline__ void load(uint32_t t, const u32x4_t& place) const
+    __device__ __forceinline__ void load(uint32_t t) const
     {
-        char* const dst = const_cast<char*>(VALUE ? v_tile(t) : k_tile(t)) + 2048u * wave;
+        const u32x4_t place = places[(first + min(t, tiles - 1u)) % 64u];
+        char* const dst = const_cast<char*>(wave < kHalf ? k_tile(t) : v_tile(t)) + 4096u * (wave % kHalf);
         const u32x4_t b{uint32_t(__builtin_amdgcn_readfirstlane(int(place[0]))), // all lanes have the same
                         uint32_t(__builtin_amdgcn_readfirstlane(int(place[1]))),
                         uint32_t(__builtin_amdgcn_readfirstlane(int(place[2]))), uint32_t(kRsrcFlags)};
-        // Rows 4 of each instruction, of K the chunks swizzled by the row (an instruction on, by four more).
-        const uint32_t off = (VALUE ? v_key : k_key) * place[3] + (VALUE ? v_chunk : k_chunk);
-        load_lds16(b, dst, off);
-        load_lds16(b, dst + 1024u, (VALUE ? off : off ^ 64u) + 4u * place[3]);
-    }
-    template <bool VALUE>
-    __device__ __forceinline__ void load(uint32_t t) const
-    {
-        load<VALUE>(t, places[(VALUE ? 64u : 0u) + unit(t) % 64u]);
+        const uint32_t four = 4u * uint32_t(__builtin_amdgcn_readfirstlane(int(place[3])));
+        const uint32_t flip = wave < kHalf ? 64u : 0u; // of K the chunks are swizzled by the row, 4 u + key
+        const uint32_t at = key * (four / 4u);
+#pragma unroll
+        for (uint32_t u = 0; u < 4u; ++u)
+            load_lds16(b, dst + 1024u * u, at + u * four + (chunk ^ u * flip));
     }
     __device__ __forceinline__ void next(uint32_t t)
     {
-        if (unit(t + 3u) >= base + 64u)
+        const uint32_t ahead = t + (wave < kHalf ? 3u : 2u);
+        if (first + min(ahead, tiles - 1u) >= base + 64u)
             find(base + 32u);
-        const u32x4_t k = places[unit(t + 3u) % 64u], v = places[64u + unit(t + 2u) % 64u];
-        load<false>(t + 3u, k);
-        load<true>(t + 2u, v);
+        load(ahead);
     }
     // The bits of the tile's keys whose page is there.
     __device__ __forceinline__ uint64_t there(uint32_t u) const
@@ -597,7 +591,7 @@ struct PairPageWalk {
 };
 
 // Eight waves a workgroup: one to a CU.
-constexpr uint32_t kPairWaveBytes = 1024u + 512u + 2048u; // a wave's scratch, its rows, its places
+constexpr uint32_t kPairWaveBytes = 1024u + 512u + 1024u; // a wave's scratch, its rows, its places
 
 template <bool CAP>
 __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_pages_pair_kernel(PagesParams p)
@@ -617,11 +611,10 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
         PairPageFeed feed(p, it, lds, places, first, last - first, wave, lane);
         feed.find(first & ~31u);
         lds_barrier(); // the part before this one is read
-        feed.load<false>(0u);
-        feed.load<false>(1u);
-        feed.load<true>(0u);
-        feed.load<false>(2u);
-        feed.load<true>(1u);
+        feed.load(0u);
+        feed.load(1u);
+        if (wave < kHalf)
+            feed.load(2u);
         WaveRows w;
         load_item(p, it, lane, w);
         rows[lane & 31u] = uint4{it.row, it.up, it.up_place, it.lo};
@@ -780,7 +773,7 @@ template <bool CAP>
 int launch_pages(const PagesParams& p, hipStream_t stream)
 {
     if (p.item_rows > 32u)
-        return launch_items(attn_pages_pair_kernel<CAP>, kPairWaves, 2u * kRing * kTileBytes + (kPairWaveBytes + 8u) * kPairWaves, p,
+        return launch_items(attn_pages_pair_kernel<CAP>, kPairWaves, 2u * kRing * kTileBytes + (kPairWaveBytes + 4u) * kPairWaves, p,
                             stream);
     return launch_items(attn_pages_kernel<CAP>, 1u, 2u * kTileBytes + 1024u, p, stream);
 }

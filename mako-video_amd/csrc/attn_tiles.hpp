@@ -697,12 +697,13 @@ __device__ __forceinline__ bool holds_nonfinite(const char* part, uint32_t lane)
 // Many rows: eight waves of 32 list rows, in two groups of four, one wave of each group on a SIMD. A group's turn at a
 // tile has two phases, the products (S of this tile, and O of the one before) and the softmax, and the groups are a phase
 // apart, held there by the barriers: while one group's wave has the matrix core of a SIMD the other's has its vector unit.
-// K and V lie in rings of four tiles; a tile's loads go out three of its K (two of its V) ahead of its use, each wave an
-// eighth.
-constexpr uint32_t kPairWaves = 8, kRing = 4;
+// K and V lie in rings of four tiles. The first group loads K and the second V, each wave a quarter: a tile's loads go out
+// three turns of K (two of V) ahead of its use and have a turn and a half to arrive, as the group that loads what the other
+// reads first is the one that is ahead with K and behind with V. (Each wave an eighth of both: one turn. 256 heads of 256
+// rows and 8192 keys each, K and V from HBM: 287 us and 277.)
+constexpr uint32_t kPairWaves = 8, kHalf = kPairWaves / 2, kRing = 4;
 
-// tile_output where the tile may have been masked; odd: the eight waves' words from holds_nonfinite for it (null: it was
-// whole).
+// tile_output where the tile may have been masked; odd: four waves' words from holds_nonfinite for it (null: it was whole).
 template <class Seen>
 __device__ __forceinline__ void masked_output(WaveRows& w, const TileP& pt, bf16x8_t (&frag)[kAhead], const TileReads& rd,
                                               const char* vt, const Seen& seen, const uint32_t* odd, uint16_t* scratch,
@@ -710,8 +711,8 @@ __device__ __forceinline__ void masked_output(WaveRows& w, const TileP& pt, bf16
 {
     uint32_t any = 0;
     if (odd) {
-        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(odd), b = *reinterpret_cast<const u32x4_t*>(odd + 4);
-        any = a[0] | a[1] | a[2] | a[3] | b[0] | b[1] | b[2] | b[3];
+        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(odd);
+        any = a[0] | a[1] | a[2] | a[3];
     }
     if (__builtin_amdgcn_readfirstlane(any))
         tile_output_masked(w, pt, rd, vt, seen, scratch, lane);
@@ -741,17 +742,23 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Fee
     if (MASKED) {
         if (t > 0 && before.meets(w))
             masked_output(w, pt, frag, rd, feed.v_tile(t - 1u), before,
-                          checked ? odd + kPairWaves * ((t - 1u) % 2u) : nullptr, scratch, lane);
-        // The part of V that this wave loaded: every wave's word is read at the next products, a barrier on.
-        const bool any = holds_nonfinite<2>(feed.v_tile(t) + 2048u * wave, lane);
+                          checked ? odd + kHalf * ((t - 1u) % 2u) : nullptr, scratch, lane);
+        wait_lds();
+    }
+    // The first group's K of tile t + 1 has arrived, the second's V of tile t, all but the last turn's loads: the first
+    // reader of either is the first group, of K at this turn's end and of V at its next products, past the barrier here.
+    wait_vm<Feed::kLoads>();
+    if (MASKED && wave >= kHalf) { // the part of V that this wave loaded
+        const bool any = holds_nonfinite<4>(feed.v_tile(t) + 4096u * (wave - kHalf), lane);
         if (lane == 0)
-            odd[kPairWaves * (t % 2u) + wave] = any;
+            odd[kHalf * (t % 2u) + wave - kHalf] = any;
         wait_lds();
     }
     __builtin_amdgcn_s_setprio(0);
     phase_barrier();
-    // The softmax. With it go out K of tile t + 3, into the slot of tile t - 1, which both groups have read, and V of tile
-    // t + 2 into that of tile t - 2 (among the products they cost 10%: this phase is the shorter one).
+    // The softmax. With it go out the first group's K of tile t + 3, into the slot of tile t - 1, which both groups have
+    // read, and the second's V of tile t + 2 into that of tile t - 2 (among the products they cost 10%: this phase is the
+    // shorter one).
     feed.next(t);
     if (MASKED ? seen.meets(w) : works)
         tile_softmax<CAP, BIAS, MASKED>(p, w, s, pt, t0, seen, feed.positions(t), near_pos, kSloped, near, lane);
@@ -759,24 +766,21 @@ __device__ __forceinline__ void pair_turn(const DenseParams& p, WaveRows& w, Fee
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
         frag[j] = rd.k(feed.k_tile(t + 1u), j);
-    // K of tile t + 2 and V of tile t + 1 have arrived, all but this turn's loads: both groups are past their barriers by
-    // the time that either reads them.
-    wait_vm<Feed::kLoads>();
     phase_barrier();
 }
 
 // The turns of a workgroup's tiles, of which walk.whole(t) says whether every row of the workgroup attends all of tile t,
 // walk.seen(t) a row's keys of another one (asked for once, in order) and walk.key(t) where it lies; and what is left of
-// the last one's output. The feed has loaded K of three tiles and V of two. works: the wave has rows; one without only
+// the last one's output. The feed has loaded K of three tiles, or V of two. works: the wave has rows; one without only
 // loads.
 template <bool CAP, bool BIAS, class Feed, class Walk>
 __device__ __forceinline__ void pair_walk(const DenseParams& p, WaveRows& w, Feed& feed, Walk& walk, const TileReads& rd,
                                           uint16_t* scratch, uint32_t* odd, uint32_t wave, uint32_t tiles, bool works,
                                           uint32_t lane)
 {
-    wait_vm<Feed::kLoads>(); // K of tiles 0 and 1, V of tile 0
+    wait_vm<2 * Feed::kLoads>(); // K of tile 0
     lds_barrier();
-    const bool second = wave >= kPairWaves / 2u;
+    const bool second = wave >= kHalf;
     if (second)
         phase_barrier();
     floatx16 s[2];
@@ -811,7 +815,7 @@ __device__ __forceinline__ void pair_walk(const DenseParams& p, WaveRows& w, Fee
     if (!before.meets(w))
         ; // nothing of it is this wave's
     else if (masked)
-        masked_output(w, pt, frag, rd, feed.v_tile(end), before, odd + kPairWaves * (end % 2u), scratch, lane);
+        masked_output(w, pt, frag, rd, feed.v_tile(end), before, odd + kHalf * (end % 2u), scratch, lane);
     else
         tile_output(w, pt, frag, rd, feed.v_tile(end));
     if (!second)
