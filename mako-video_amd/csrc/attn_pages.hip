@@ -41,6 +41,7 @@ struct PagesParams : DenseParams {
 };
 
 constexpr uint32_t kLeastTiles = 3; // of a workgroup: below it the join costs more than the tiles
+constexpr uint32_t kBegin = 3;      // tiles that take as long as the begin of a part
 
 // A stream: its new rows q0 .. q0 + rows - 1, kept rows, and the tiles of its items.
 struct Stream {
@@ -101,19 +102,36 @@ __device__ __forceinline__ Stream stream_of(const PagesParams& p, uint32_t s, ui
     return Stream(p, q0, rows, kept, min(sinks, kept));
 }
 
-// The streams 64 at a time, one a lane, by the sums of their items' tiles.
+// How the items' tiles are shared out: runs of `share` pieces, each taken by `together` workgroups, a row tile each (if all
+// streams' items have as many row tiles; else 1, and row tiles count one by one). A piece is a tile, or with `size` an
+// item's equal part of so many tiles at most.
+struct Sharing {
+    uint32_t together, size;
+    __device__ __forceinline__ uint32_t pieces(uint32_t tiles) const { return size ? (tiles + size - 1u) / size : tiles; }
+    // Those of a lane's stream, and of all lanes': 2^32 - 1 for more than a few million.
+    __device__ __forceinline__ uint64_t of(const PagesParams& p, const Stream& t) const
+    {
+        return uint64_t(together > 1u ? min(t.row_tiles, 1u) : t.row_tiles) * p.kv_heads * pieces(t.tiles);
+    }
+    __device__ __forceinline__ uint32_t of_all(const PagesParams& p, const Stream& t) const
+    {
+        const uint64_t n = of(p, t);
+        return __ballot(n >> 20) ? ~0u : wave_sum_u32(uint32_t(n));
+    }
+};
+
+// The streams 64 at a time, one a lane, by the sums of their items' pieces.
 struct Streams {
     uint32_t s0;
-    uint64_t before, some, end; // tiles before the lane's stream; the streams that have any; those up to the 64's end
-    // together: row tiles that a run takes at once, if all have as many; else 1, and they count one by one.
-    __device__ __forceinline__ void sum(const PagesParams& p, uint32_t from, uint64_t base, const Stream& t, uint32_t together,
-                                        uint32_t lane)
+    uint64_t before, some, end; // pieces before the lane's stream; the streams that have any; those up to the 64's end
+    __device__ __forceinline__ void sum(const PagesParams& p, uint32_t from, uint64_t base, const Stream& t,
+                                        const Sharing& sharing, uint32_t lane)
     {
         s0 = from;
-        const uint64_t units = uint64_t(together > 1u ? min(t.row_tiles, 1u) : t.row_tiles) * p.kv_heads * t.tiles;
-        some = __ballot(units != 0u);
-        const uint64_t to = wave_scan_u64(units, lane);
-        before = base + to - units;
+        const uint64_t pieces = sharing.of(p, t);
+        some = __ballot(pieces != 0u);
+        const uint64_t to = wave_scan_u64(pieces, lane);
+        before = base + to - pieces;
         end = base + lane_u64(to, kWave - 1);
     }
     __device__ __forceinline__ static Stream of_lane(const PagesParams& p, uint32_t from, uint32_t lane)
@@ -121,18 +139,17 @@ struct Streams {
         uint32_t sinks;
         return from + lane < p.streams ? stream_of(p, from + lane, sinks) : Stream(p, 0u, 0u, 0u, 0u);
     }
-    __device__ __forceinline__ void load(const PagesParams& p, uint32_t from, uint64_t base, uint32_t together, uint32_t lane)
+    __device__ __forceinline__ void load(const PagesParams& p, uint32_t from, uint64_t base, const Sharing& sharing,
+                                         uint32_t lane)
     {
-        sum(p, from, base, of_lane(p, from, lane), together, lane);
+        sum(p, from, base, of_lane(p, from, lane), sharing, lane);
     }
-    // The last stream that begins at tile x or before it and has tiles, x one of the 64's.
+    // The last stream that begins at piece x or before it and has any, x one of the 64's.
     __device__ __forceinline__ uint32_t of(uint64_t x) const { return 63u - uint32_t(__builtin_clzll(__ballot(before <= x) & some)); }
 };
 
-// How the items' tiles are shared out: runs of `share`, each taken by `together` workgroups, a row tile each.
-struct Shares {
+struct Shares : Sharing {
     uint64_t units, share;
-    uint32_t together;
     // Leaves the streams at their first 64.
     __device__ __forceinline__ Shares(const PagesParams& p, Streams& st, uint32_t lane)
     {
@@ -142,15 +159,32 @@ struct Shares {
             const Stream t = Streams::of_lane(p, s0, lane);
             least = min(least, wave_min_u32(t.rows ? t.row_tiles : ~0u)), most = max(most, wave_max_u32(t.row_tiles));
         }
-        together = least == most && most <= p.workers ? most : 1u;
-        st.sum(p, 0u, 0u, mine, together, lane);
+        together = least == most && most <= p.workers ? most : 1u, size = 0u;
+        st.sum(p, 0u, 0u, mine, *this, lane);
         while (st.s0 + kWave < p.streams)
-            st.load(p, st.s0 + kWave, st.end, together, lane);
+            st.load(p, st.s0 + kWave, st.end, *this, lane);
         units = st.end;
         const uint32_t runs = p.workers / together;
         share = max(quotient(units + runs - 1u, runs), uint64_t(kLeastTiles));
-        if (st.s0 != 0u)
-            st.sum(p, 0u, 0u, mine, together, lane);
+        // Where cutting each item into equal parts gives every run one of them, hardly longer than its share: a run that
+        // goes on into another item begins anew there, which takes as long as some tiles.
+        for (uint32_t i = 0; i <= kBegin && size == 0u && share < (1u << 20); ++i) {
+            const Sharing parts{together, uint32_t(share) + i};
+            uint64_t n = parts.of_all(p, mine);
+            for (uint32_t s0 = kWave; s0 < p.streams && n <= runs; s0 += kWave)
+                n += parts.of_all(p, Streams::of_lane(p, s0, lane));
+            if (n <= runs)
+                size = parts.size;
+        }
+        if (size || st.s0 != 0u)
+            st.sum(p, 0u, 0u, mine, *this, lane);
+        while (size && st.s0 + kWave < p.streams)
+            st.load(p, st.s0 + kWave, st.end, *this, lane);
+        if (size) {
+            units = st.end, share = 1u;
+            if (st.s0 != 0u)
+                st.sum(p, 0u, 0u, mine, *this, lane);
+        }
     }
 };
 
@@ -435,29 +469,31 @@ __device__ __forceinline__ void for_parts(const PagesParams& p, uint32_t lane, c
     Cut cut{};
     for (uint64_t x = begin; x < end;) {
         while (x >= streams.end)
-            streams.load(p, streams.s0 + kWave, streams.end, shares.together, lane);
+            streams.load(p, streams.s0 + kWave, streams.end, shares, lane);
         const uint32_t at = streams.of(x), stream = streams.s0 + at;
         uint32_t sinks;
         const Stream st = stream_of(p, stream, sinks);
-        const uint64_t local = x - lane_u64(streams.before, at), number = quotient(local, st.tiles);
-        const uint32_t first = uint32_t(local - number * st.tiles);
-        const uint32_t last = uint32_t(min(uint64_t(st.tiles), first + (end - x)));
+        const uint32_t pieces = shares.pieces(st.tiles);
+        const uint64_t local = x - lane_u64(streams.before, at), number = quotient(local, pieces);
+        const uint32_t a = uint32_t(local - number * pieces), b = uint32_t(min(uint64_t(pieces), a + (end - x)));
         const uint32_t kvh = uint32_t(shares.together > 1u ? number : quotient(number, st.row_tiles));
         Item it{st, stream, kvh, st.rows * p.group, 0u, sinks, 0u, 0u, 0u, 0u, 0u, 0u};
         it.f0 = p.item_rows * (shares.together > 1u ? row_tile : uint32_t(number - uint64_t(kvh) * st.row_tiles));
-        // The item that the run begins with, unless with its first tile, is the first of the workgroup's two parts.
-        const bool whole = first == 0u && last == st.tiles;
-        if (first > 0u && shares.share >= first) // the run before this one begins with the item or ahead of it
+        // The item that the run begins with, unless with its first piece, is the first of the workgroup's two parts.
+        const bool whole = a == 0u && b == pieces;
+        if (a > 0u && shares.share >= a) // the run before this one begins with the item or ahead of it
             cut = Cut{min(p.item_rows, it.list - min(it.f0, it.list)),
                       st.q0,
                       it.f0,
                       kvh,
                       run,
-                      uint32_t(quotient(x - first + st.tiles - 1u, uint32_t(min(shares.share, uint64_t(~0u))))),
+                      uint32_t(quotient(x - a + pieces - 1u, uint32_t(min(shares.share, uint64_t(~0u))))),
                       shares.together,
                       row_tile};
-        part(it, first, last, whole ? ~0u : 2u * worker + (first > 0u ? 0u : 1u));
-        x += last - first;
+        const uint32_t first = shares.size ? uint32_t(uint64_t(st.tiles) * a / pieces) : a;
+        const uint32_t last = shares.size ? uint32_t(uint64_t(st.tiles) * b / pieces) : b;
+        part(it, first, last, whole ? ~0u : 2u * worker + (a > 0u ? 0u : 1u));
+        x += b - a;
     }
     if (threadIdx.x == 0)
         reinterpret_cast<Cut*>(p.part)[worker] = cut;
