@@ -212,14 +212,41 @@ struct Item {
     uint32_t up_place; // that of `up`
     uint32_t lo;      // kept rows from it on are under the window
     uint32_t all_lo;  // of every row of the workgroup, or a bound of that
+    const int32_t* parents; // in LDS, of streams of up to kParents rows
 };
 
-// The row's parent, ~0 for none: a parent lies before its row.
+constexpr uint32_t kParents = 1024;
+
+// The row's parent, ~0 for none: a parent lies before its row. (A line of them read from memory takes half a us a step.)
 __device__ __forceinline__ uint32_t parent_of(const PagesParams& p, const Item& it, uint32_t row)
 {
-    const uint32_t up = row < it.st.rows ? uint32_t(p.parents[it.st.q0 + row]) : ~0u;
+    uint32_t up = ~0u;
+    if (row < it.st.rows)
+        up = uint32_t(it.st.rows <= kParents ? it.parents[row] : p.parents[it.st.q0 + row]);
     return up < row ? up : ~0u;
 }
+
+// The parents of the item's stream into LDS, by all `threads` of the workgroup.
+__device__ __forceinline__ void load_parents(const PagesParams& p, const Item& it, int32_t* to, uint32_t threads)
+{
+    if (p.parents && it.st.rows <= kParents)
+        for (uint32_t i = threadIdx.x; i < it.st.rows; i += threads)
+            to[i] = p.parents[it.st.q0 + i];
+}
+
+// A wave's rows of q as they lie in memory, so that they are on their way while other things are looked up.
+struct RawRows {
+    uint4 t[8];
+    __device__ __forceinline__ RawRows(const PagesParams& p, const Item& it, uint32_t lane)
+    {
+        const uint32_t f = it.f0 + (lane & 31u), fc = min(f, it.list - 1u), row = p.div_group.div(fc);
+        const uint32_t head = it.kvh * p.group + (fc - row * p.group);
+        const uint16_t* const src = p.q + uint64_t(head) * p.qhs + uint64_t(it.st.q0 + row) * p.qrs + 8u * (lane >> 5);
+#pragma unroll
+        for (int dc = 0; dc < 8; ++dc)
+            t[dc] = f < it.list ? *reinterpret_cast<const uint4*>(src + 16 * dc) : uint4{0u, 0u, 0u, 0u};
+    }
+};
 
 // The kept rows that every row of the workgroup has under the window, at least: a row has as many ancestors as there are
 // rows before it, at most.
@@ -229,17 +256,12 @@ __device__ __forceinline__ void bound_window(const PagesParams& p, Item& it)
     it.all_lo = p.window && p.window - 1u < far ? far - (p.window - 1u) : 0u;
 }
 
-__device__ __forceinline__ void load_item(const PagesParams& p, Item& it, uint32_t lane, WaveRows& w)
+__device__ __forceinline__ void begin_item(const PagesParams& p, Item& it, const RawRows& raw, uint32_t lane, WaveRows& w)
 {
-    const uint32_t n = lane & 31u, hh = lane >> 5, f = it.f0 + n;
-    const uint32_t fc = min(f, it.list - 1u);
-    it.row = p.div_group.div(fc);
-    const uint32_t head = it.kvh * p.group + (fc - it.row * p.group);
-    const uint16_t* const src = p.q + uint64_t(head) * p.qhs + uint64_t(it.st.q0 + it.row) * p.qrs;
+    it.row = p.div_group.div(min(it.f0 + (lane & 31u), it.list - 1u));
 #pragma unroll
     for (int dc = 0; dc < 8; ++dc) {
-        const uint4 t = f < it.list ? *reinterpret_cast<const uint4*>(src + 16 * dc + 8u * hh) : uint4{0u, 0u, 0u, 0u};
-        uint32_t x[4] = {t.x, t.y, t.z, t.w};
+        uint32_t x[4] = {raw.t[dc].x, raw.t[dc].y, raw.t[dc].z, raw.t[dc].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             x[e] = pack_bf16(bf16_lo(x[e]) * p.q_pow, bf16_hi(x[e]) * p.q_pow);
@@ -477,7 +499,7 @@ __device__ __forceinline__ void for_parts(const PagesParams& p, uint32_t lane, c
         const uint64_t local = x - lane_u64(streams.before, at), number = quotient(local, pieces);
         const uint32_t a = uint32_t(local - number * pieces), b = uint32_t(min(uint64_t(pieces), a + (end - x)));
         const uint32_t kvh = uint32_t(shares.together > 1u ? number : quotient(number, st.row_tiles));
-        Item it{st, stream, kvh, st.rows * p.group, 0u, sinks, 0u, 0u, 0u, 0u, 0u, 0u};
+        Item it{st, stream, kvh, st.rows * p.group, 0u, sinks, 0u, 0u, 0u, 0u, 0u, 0u, nullptr};
         it.f0 = p.item_rows * (shares.together > 1u ? row_tile : uint32_t(number - uint64_t(kvh) * st.row_tiles));
         // The item that the run begins with, unless with its first piece, is the first of the workgroup's two parts.
         const bool whole = a == 0u && b == pieces;
@@ -507,13 +529,17 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     const uint32_t lane = threadIdx.x;
     const TileReads rd(lane);
     PageFeed feed(lds, lane);
+    int32_t* const parents = reinterpret_cast<int32_t*>(lds + 2u * kTileBytes + 1024u);
     for_parts(p, lane, [&](Item& it, uint32_t first, uint32_t last, uint32_t slot) {
         WaveRows w;
         bound_window(p, it);
+        const RawRows raw(p, it, lane);
+        load_parents(p, it, parents, kWave);
+        it.parents = parents;
         feed.numbers(p, it, first & ~15u, lane);
         feed.load<false>(p, it, first);
         feed.load<true>(p, it, first);
-        load_item(p, it, lane, w);
+        begin_item(p, it, raw, lane, w);
         for (uint32_t u = first; u < last;) {
 #pragma unroll 1
             for (; u < last && !(is_whole(it, u) && feed.all_there(u)); ++u)
@@ -632,7 +658,7 @@ constexpr uint32_t kPairWaveBytes = 1024u + 512u + 1024u; // a wave's scratch, i
 template <bool CAP>
 __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_pages_pair_kernel(PagesParams p)
 {
-    // K ring, V ring, the waves' own, and for two tiles whether the waves' parts of V hold an infinity or a NaN.
+    // K ring, V ring, the waves' own, for two tiles whether the waves' parts of V hold an infinity or a NaN, and a tree.
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     char* const own = lds + 2u * kRing * kTileBytes + kPairWaveBytes * wave;
@@ -640,10 +666,12 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     uint4* const rows = reinterpret_cast<uint4*>(own + 1024u);
     u32x4_t* const places = reinterpret_cast<u32x4_t*>(own + 1536u);
     uint32_t* const odd = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + kPairWaveBytes * kPairWaves);
+    int32_t* const parents = reinterpret_cast<int32_t*>(odd + 2u * kHalf);
     const TileReads rd(lane);
     for_parts(p, lane, [&](Item& it, uint32_t first, uint32_t last, uint32_t slot) {
         it.f0 += 32u * wave;
         bound_window(p, it);
+        const RawRows raw(p, it, lane);
         PairPageFeed feed(p, it, lds, places, first, last - first, wave, lane);
         feed.find(first & ~31u);
         lds_barrier(); // the part before this one is read
@@ -651,8 +679,11 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
         feed.load(1u);
         if (wave < kHalf)
             feed.load(2u);
+        load_parents(p, it, parents, 64u * kPairWaves);
+        it.parents = parents;
+        lds_barrier();
         WaveRows w;
-        load_item(p, it, lane, w);
+        begin_item(p, it, raw, lane, w);
         rows[lane & 31u] = uint4{it.row, it.up, it.up_place, it.lo};
         PairPageWalk walk{p, it, feed, rows, lane};
         pair_walk<CAP, false>(p, w, feed, walk, rd, scratch, odd, wave, last - first, it.f0 < it.list, lane);
@@ -809,9 +840,9 @@ template <bool CAP>
 int launch_pages(const PagesParams& p, hipStream_t stream)
 {
     if (p.item_rows > 32u)
-        return launch_items(attn_pages_pair_kernel<CAP>, kPairWaves, 2u * kRing * kTileBytes + (kPairWaveBytes + 4u) * kPairWaves, p,
+        return launch_items(attn_pages_pair_kernel<CAP>, kPairWaves, 2u * kRing * kTileBytes + (kPairWaveBytes + 4u) * kPairWaves + 4u * kParents, p,
                             stream);
-    return launch_items(attn_pages_kernel<CAP>, 1u, 2u * kTileBytes + 1024u, p, stream);
+    return launch_items(attn_pages_kernel<CAP>, 1u, 2u * kTileBytes + 1024u + 4u * kParents, p, stream);
 }
 
 } // namespace
@@ -889,9 +920,9 @@ extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (const int rc = a.cap > 0.0f ? launch_pages<true>(p, s) : launch_pages<false>(p, s); rc != MH3_OK)
         return rc;
-    // Blocks a cut item: for the four waves' rows four passes at most, for the eight waves' eight.
+    // Blocks a workgroup of the others', for a few passes over its cut item's rows each.
     if (p.item_rows > 32u) {
-        const uint32_t blocks = (p.slot_rows + 63u) / 64u;
+        const uint32_t blocks = (p.slot_rows + 15u) / 16u;
         hipLaunchKernelGGL(attn_pages_join_kernel<1u>, dim3(p.workers * blocks), dim3(256), 0, s, p, blocks);
     } else {
         const uint32_t blocks = (p.slot_rows + 7u) / 8u;
