@@ -36,12 +36,13 @@ struct PagesParams : DenseParams {
     const int32_t* first_rows;
     uint64_t kps, kphs, kprs, vps, vphs, vprs, table_stride; // elements
     uint32_t streams, cols, pages, page_rows, window, workers, slot_rows;
-    uint32_t item_rows; // list rows of an item: a wave's 32, or a workgroup's 256
+    uint32_t item_rows; // list rows of an item: a wave's 32, or up to eight waves'
+    uint32_t begin;     // tiles that take as long as the begin of a part
+    FastDiv div_item;
     FastDiv div_page;
 };
 
 constexpr uint32_t kLeastTiles = 3; // of a workgroup: below it the join costs more than the tiles
-constexpr uint32_t kBegin = 3;      // tiles that take as long as the begin of a part
 
 // A stream: its new rows q0 .. q0 + rows - 1, kept rows, and the tiles of its items.
 struct Stream {
@@ -57,7 +58,7 @@ struct Stream {
         near = all - near0;
         front = min((sinks + 63u) / 64u, near0);
         tiles = front + near + (rows + 63u) / 64u;
-        row_tiles = (rows * p.group + p.item_rows - 1u) / p.item_rows;
+        row_tiles = p.div_item.div(rows * p.group + p.item_rows - 1u);
     }
     // The first key of kept tile u.
     __device__ __forceinline__ uint32_t key(uint32_t u) const { return 64u * (u < front ? u : near0 + u - front); }
@@ -168,7 +169,7 @@ struct Shares : Sharing {
         share = max(quotient(units + runs - 1u, runs), uint64_t(kLeastTiles));
         // Where cutting each item into equal parts gives every run one of them, hardly longer than its share: a run that
         // goes on into another item begins anew there, which takes as long as some tiles.
-        for (uint32_t i = 0; i <= kBegin && size == 0u && share < (1u << 20); ++i) {
+        for (uint32_t i = 0; i <= p.begin && size == 0u && share < (1u << 20); ++i) {
             const Sharing parts{together, uint32_t(share) + i};
             uint64_t n = parts.of_all(p, mine);
             for (uint32_t s0 = kWave; s0 < p.streams && n <= runs; s0 += kWave)
@@ -205,7 +206,8 @@ struct Piece {
 // A wave's item, and what a lane has of it.
 struct Item {
     Stream st;
-    uint32_t stream, kvh, list, f0; // f0: the wave's first list row
+    uint32_t stream, kvh;
+    uint32_t begin, list, f0; // the item's list rows, up to `list`, and the wave's first one
     uint32_t sinks;   // as given: new rows may be among the first ones too
     uint32_t row, up; // the lane's row's number among the new ones; the row of its line that the walk is at (~0: at its end)
     uint32_t place;   // the row's
@@ -252,7 +254,7 @@ struct RawRows {
 // rows before it, at most.
 __device__ __forceinline__ void bound_window(const PagesParams& p, Item& it)
 {
-    const uint32_t far = it.st.kept + p.div_group.div(min(it.f0 / p.item_rows * p.item_rows + p.item_rows, it.list) - 1u);
+    const uint32_t far = it.st.kept + p.div_group.div(it.list - 1u);
     it.all_lo = p.window && p.window - 1u < far ? far - (p.window - 1u) : 0u;
 }
 
@@ -449,7 +451,7 @@ __device__ __forceinline__ float* parts_of(const PagesParams& p) { return p.part
 __device__ __forceinline__ void store_item(const PagesParams& p, const Item& it, const WaveRows& w, uint32_t slot,
                                            uint32_t lane)
 {
-    const uint32_t hh = lane >> 5, f = it.f0 + (lane & 31u), n = f % p.item_rows;
+    const uint32_t hh = lane >> 5, f = it.f0 + (lane & 31u), n = f - it.begin;
     const float l = w.l_run + __shfl_xor(w.l_run, 32, kWave);
     if (f >= it.list)
         return;
@@ -499,14 +501,16 @@ __device__ __forceinline__ void for_parts(const PagesParams& p, uint32_t lane, c
         const uint64_t local = x - lane_u64(streams.before, at), number = quotient(local, pieces);
         const uint32_t a = uint32_t(local - number * pieces), b = uint32_t(min(uint64_t(pieces), a + (end - x)));
         const uint32_t kvh = uint32_t(shares.together > 1u ? number : quotient(number, st.row_tiles));
-        Item it{st, stream, kvh, st.rows * p.group, 0u, sinks, 0u, 0u, 0u, 0u, 0u, 0u, nullptr};
-        it.f0 = p.item_rows * (shares.together > 1u ? row_tile : uint32_t(number - uint64_t(kvh) * st.row_tiles));
+        const uint32_t from = p.item_rows * (shares.together > 1u ? row_tile : uint32_t(number - uint64_t(kvh) * st.row_tiles));
+        Item it{st};
+        it.stream = stream, it.kvh = kvh, it.sinks = sinks;
+        it.begin = it.f0 = from, it.list = min(from + p.item_rows, st.rows * p.group);
         // The item that the run begins with, unless with its first piece, is the first of the workgroup's two parts.
         const bool whole = a == 0u && b == pieces;
         if (a > 0u && shares.share >= a) // the run before this one begins with the item or ahead of it
-            cut = Cut{min(p.item_rows, it.list - min(it.f0, it.list)),
+            cut = Cut{it.list - from,
                       st.q0,
-                      it.f0,
+                      from,
                       kvh,
                       run,
                       uint32_t(quotient(x - a + pieces - 1u, uint32_t(min(shares.share, uint64_t(~0u))))),
@@ -669,7 +673,8 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     int32_t* const parents = reinterpret_cast<int32_t*>(odd + 2u * kHalf);
     const TileReads rd(lane);
     for_parts(p, lane, [&](Item& it, uint32_t first, uint32_t last, uint32_t slot) {
-        it.f0 += 32u * wave;
+        // Few rows go to as many waves of either group, and to each SIMD before one gets two.
+        it.f0 += 32u * (wave < kHalf ? 2u * wave : 2u * (kPairWaves - 1u - wave) + 1u);
         bound_window(p, it);
         const RawRows raw(p, it, lane);
         PairPageFeed feed(p, it, lds, places, first, last - first, wave, lane);
@@ -773,19 +778,24 @@ namespace {
 
 using namespace mh3;
 
-// Which kernel a call takes, from the list rows that its streams have on average.
+// Tiles that take as long as the begin of a part, of one wave and of eight.
+constexpr uint32_t kBegin = 3, kPairBegin = 12;
+
+// Which kernel a call takes, and how many rows an item has, from the list rows that its streams have on average.
 struct PagesPlan {
-    uint32_t item_rows, workers, slot_rows; // a part's rows: an item's, or all of the call's where they are fewer
+    uint32_t item_rows, workers, slot_rows; // slot_rows: a part's, an item's or all of the call's where they are fewer
     uint64_t workspace;
 };
 
 PagesPlan pages_plan(const MH3PagesAttnArgs& a)
 {
     const uint64_t list = uint64_t(a.q_rows) * (a.heads / a.kv_heads);
-    const bool pair = list > 64ull * a.table.streams;
+    const uint64_t rows = (list + a.table.streams - 1u) / a.table.streams; // of a stream
+    const bool pair = rows > 64u;
     const uint32_t cus = uint32_t(std::max(host::cu_count(), 1));
     PagesPlan plan;
-    plan.item_rows = pair ? 32u * kPairWaves : 32u;
+    const uint64_t items = (rows + 32u * kPairWaves - 1u) / (32u * kPairWaves);
+    plan.item_rows = pair ? uint32_t((rows + items - 1u) / items + 31u) / 32u * 32u : 32u;
     plan.workers = ((pair ? 1u : 4u) * cus + 7u) / 8u * 8u;
     plan.slot_rows = uint32_t(std::min<uint64_t>(plan.item_rows, list));
     plan.workspace = uint64_t(plan.workers) * (sizeof(Cut) + 2ull * plan.slot_rows * 130u * 4u);
@@ -916,6 +926,7 @@ extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint
     p.page_rows = t.page_rows, p.window = a.window, p.div_page = FastDiv::make(t.page_rows);
     p.kv_heads = a.kv_heads, p.group = a.heads / a.kv_heads, p.q_rows = a.q_rows, p.div_group = FastDiv::make(p.group);
     p.workers = plan.workers, p.slot_rows = plan.slot_rows, p.item_rows = plan.item_rows;
+    p.div_item = FastDiv::make(plan.item_rows), p.begin = plan.item_rows > 32u ? kPairBegin : kBegin;
     score_factors(a.scale, a.cap, p);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (const int rc = a.cap > 0.0f ? launch_pages<true>(p, s) : launch_pages<false>(p, s); rc != MH3_OK)
