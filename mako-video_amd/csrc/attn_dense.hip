@@ -412,7 +412,10 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
     uint32_t* const span = reinterpret_cast<uint32_t*>(lds + 2u * kRing * kTileBytes + kWaveBytes * kPairWaves);
     const uint32_t f0 = (tile * kPairWaves + wave) * 32u;
     WaveRows w;
-    load_rows<CAP, BIAS, SINKS>(p, kvh, f0, lane, w);
+    if (SINKS)
+        load_ranges<CAP, BIAS, true>(p, kvh, f0, lane, w); // the queries when the first tiles are on their way
+    else
+        load_rows<CAP, BIAS, false>(p, kvh, f0, lane, w);
     uint32_t* const odd = span + 4u * kPairWaves; // [2][kHalf]: a masked tile's V holds an infinity or a NaN
     uint32_t* const s_span = odd + 2u * kHalf;     // SINKS
     // SINKS: the rows' ranges, out of the registers: only masked turns ask for them.
@@ -450,6 +453,8 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
         tiles_of(p, k0, k1, split, first, last);
     }
     if (first >= last) { // the same for every wave
+        if (SINKS)
+            load_queries(p, kvh, f0, lane, w); // for its zeros
         store_rows(p, w, kvh, f0, split, lane);
         return;
     }
@@ -484,6 +489,7 @@ __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu
         feed.next(0u);
     }
     if (SINKS) {
+        load_queries(p, kvh, f0, lane, w);
         PairWalk<BIAS> turns{walk, first, last, all_lo, all_hi, all_s_lo, all_s_hi, rows, lane};
         pair_walk<CAP, BIAS>(p, w, feed, turns, rd, scratch, odd, wave, tiles, f0 < p.list, lane);
         const uint4 r = rows[lane & 31u];

@@ -278,8 +278,8 @@ __device__ __forceinline__ float score_unit(const DenseParams& p)
 
 __device__ __forceinline__ bool is_near(int32_t rel) { return rel > -(1 << 23) && rel < (1 << 23); }
 
-template <bool CAP, bool BIAS, bool SINKS>
-__device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, uint32_t f0, uint32_t lane, WaveRows& w)
+// The query fragments of a wave's rows, and zeros for their output.
+__device__ __forceinline__ void load_queries(const DenseParams& p, uint32_t kvh, uint32_t f0, uint32_t lane, WaveRows& w)
 {
     const uint32_t n = lane & 31u, hh = lane >> 5, f = f0 + n;
     const uint32_t fc = min(f, p.list - 1u), row = p.div_group.div(fc), head = kvh * p.group + (fc - row * p.group);
@@ -298,6 +298,14 @@ __device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, ui
 #pragma unroll
         for (int e = 0; e < 16; ++e)
             w.o[b][e] = 0.0f;
+}
+
+// The keys of a wave's rows, and what their bias goes by.
+template <bool CAP, bool BIAS, bool SINKS>
+__device__ __forceinline__ void load_ranges(const DenseParams& p, uint32_t kvh, uint32_t f0, uint32_t lane, WaveRows& w)
+{
+    const uint32_t f = f0 + (lane & 31u);
+    const uint32_t fc = min(f, p.list - 1u), row = p.div_group.div(fc), head = kvh * p.group + (fc - row * p.group);
     range_of(p, f, row, w.lo, w.hi);
     if (SINKS) {
         sinks_of(p, f, row, w.lo, w.hi, w.s_lo, w.s_hi);
@@ -322,6 +330,13 @@ __device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, ui
         w.steep = __ballot(!(fabsf(w.slope_unit) <= 0x1p80f)) != 0;
         w.q_near = !w.steep && !__ballot(!is_near(rel));
     }
+}
+
+template <bool CAP, bool BIAS, bool SINKS>
+__device__ __forceinline__ void load_rows(const DenseParams& p, uint32_t kvh, uint32_t f0, uint32_t lane, WaveRows& w)
+{
+    load_queries(p, kvh, f0, lane, w);
+    load_ranges<CAP, BIAS, SINKS>(p, kvh, f0, lane, w);
 }
 
 // Scores x under a cap, without their factor and but for a constant, which a softmax does not see: tanh(u) =

@@ -837,21 +837,17 @@ def attn_window_ranges(q_off, k_off, q_rows, kv_rows, window, *, sinks=None, cau
         raise ValueError("q_off: at least one document")
     if not 1 <= window <= 0xffffffff:
         raise ValueError("window: at least one key, the row's own")
-    _need(q_off, "q_off", torch.int32, docs + 1)
-    _need(k_off, "k_off", torch.int32, docs + 1)
-    if sinks is not None:
-        _need(sinks, "sinks", torch.int32, docs)
-    both = torch.empty((2, q_rows, 2), dtype=torch.int32, device=q_off.device) if ranges is None and first is None else None
-    ranges = (both[0] if both is not None else torch.empty((q_rows, 2), dtype=torch.int32, device=q_off.device)) \
-        if ranges is None else ranges
-    first = (both[1] if both is not None else torch.empty((q_rows, 2), dtype=torch.int32, device=q_off.device)) \
-        if first is None else first
-    _need(ranges, "ranges", torch.int32, 2 * q_rows)
-    _need(first, "first", torch.int32, 2 * q_rows)
-    a = WindowArgs(q_rows, kv_rows, docs, int(bool(causal)), window, 0)
-    _on(_one_device(q_off=q_off, k_off=k_off, sinks=sinks, ranges=ranges, first=first), "attn_window_ranges",
-        lib.mh3_attn_window_ranges, C.byref(a), q_off.data_ptr(), k_off.data_ptr(), _ptr(sinks), ranges.data_ptr(),
-        first.data_ptr())
+    if ranges is None and first is None:
+        ranges, first = torch.empty((2, q_rows, 2), dtype=torch.int32, device=q_off.device).unbind(0)
+    elif ranges is None or first is None:
+        made = torch.empty((q_rows, 2), dtype=torch.int32, device=q_off.device)
+        ranges, first = (made, first) if ranges is None else (ranges, made)
+    device = _operands((q_off, "q_off", torch.int32, docs + 1), (k_off, "k_off", torch.int32, docs + 1),
+                       (sinks, "sinks", torch.int32, docs), (ranges, "ranges", torch.int32, 2 * q_rows),
+                       (first, "first", torch.int32, 2 * q_rows))
+    _on(device, "attn_window_ranges", lib.mh3_attn_window_ranges,
+        C.byref(WindowArgs(q_rows, kv_rows, docs, int(bool(causal)), window, 0)), q_off.data_ptr(), k_off.data_ptr(),
+        _ptr(sinks), ranges.data_ptr(), first.data_ptr())
     return ranges, first
 
 
@@ -972,26 +968,26 @@ def _pools(pools, pages=None):
     return held, len(pools), pages, pools
 
 
-def _one_device_of(pools, **tensors) -> int:
-    return _one_device(**tensors, **{f"pools[{i}]": t for i, t in enumerate(pools)})
-
-
-def _missing(missing, device):
-    if missing is None:
-        return torch.empty(1, dtype=torch.int32, device=torch.device("cuda", device))
-    _need(missing, "missing", torch.int32, 1)
-    return missing
+def _page_lists(table, refs, pages, *lists, pools=()) -> int:
+    """The GPU that a table, its counts, lists (as for _operands) and pools are on, all checked."""
+    device = _operands((refs, "refs", torch.int32, pages), *lists)
+    others = _one_device(table=table) if not pools else \
+        _one_device(table=table, **{f"pools[{i}]": t for i, t in enumerate(pools)})
+    if others != device:
+        raise ValueError(f"table: on GPU {others}, other operands on GPU {device}")
+    return device
 
 
 def pages_take(table, refs, first, last, *, missing=None):
     """Gives the entries first[s] .. last[s] - 1 (int32 [streams]) of each stream's row of `table` (int32
     [streams][entries], -1: no page) that are -1 a page each, the lowest free ones (refs int32 [pages], 0: free) in the
     order (stream, entry), and counts them. Returns `missing`, int32 [1]: how many found none and stay -1."""
-    a = _page_table(table, _counts(refs))
-    _need(first, "first", torch.int32, a.streams)
-    _need(last, "last", torch.int32, a.streams)
-    device = _one_device(table=table, refs=refs, first=first, last=last, missing=missing)
-    missing = _missing(missing, device)
+    pages = _counts(refs)
+    a = _page_table(table, pages)
+    if missing is None:
+        missing = torch.empty(1, dtype=torch.int32, device=refs.device)
+    device = _page_lists(table, refs, pages, (first, "first", torch.int32, a.streams),
+                         (last, "last", torch.int32, a.streams), (missing, "missing", torch.int32, 1))
     _on(device, "pages_take", lib.mh3_pages_take, C.byref(a), table.data_ptr(), refs.data_ptr(), first.data_ptr(),
         last.data_ptr(), missing.data_ptr())
     return missing
@@ -999,11 +995,12 @@ def pages_take(table, refs, first, last, *, missing=None):
 
 def pages_free(table, refs, first, last):
     """Clears the entries first[s] .. last[s] - 1 of each stream to -1; their pages' counts fall."""
-    a = _page_table(table, _counts(refs))
-    _need(first, "first", torch.int32, a.streams)
-    _need(last, "last", torch.int32, a.streams)
-    _on(_one_device(table=table, refs=refs, first=first, last=last), "pages_free", lib.mh3_pages_free, C.byref(a),
-        table.data_ptr(), refs.data_ptr(), first.data_ptr(), last.data_ptr())
+    pages = _counts(refs)
+    a = _page_table(table, pages)
+    device = _page_lists(table, refs, pages, (first, "first", torch.int32, a.streams),
+                         (last, "last", torch.int32, a.streams))
+    _on(device, "pages_free", lib.mh3_pages_free, C.byref(a), table.data_ptr(), refs.data_ptr(), first.data_ptr(),
+        last.data_ptr())
 
 
 def pages_fork(pools, table, refs, parents, rows, page_rows, *, new_table=None, missing=None, workspace=None):
@@ -1019,18 +1016,17 @@ def pages_fork(pools, table, refs, parents, rows, page_rows, *, new_table=None, 
     b = _page_table(new_table, pages, page_rows, "new_table")
     if (b.streams, b.cols, b.table_stride) != (a.streams, a.cols, a.table_stride):
         raise ValueError("new_table: laid out as table")
-    _need(parents, "parents", torch.int32, a.streams)
-    _need(rows, "rows", torch.int32, a.streams)
-    device = _one_device_of(pools, table=table, refs=refs, parents=parents, rows=rows, new_table=new_table,
-                            missing=missing, workspace=workspace)
-    missing = _missing(missing, device)
     ref = C.byref(a)
     nbytes = lib.mh3_pages_fork_workspace_bytes(ref)
     if nbytes < 0:
         _check(nbytes, "pages_fork")
     if workspace is None:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=table.device)
-    _need(workspace, "workspace", torch.uint8, nbytes)
+    if missing is None:
+        missing = torch.empty(1, dtype=torch.int32, device=table.device)
+    device = _page_lists(table, refs, pages, (parents, "parents", torch.int32, a.streams),
+                         (rows, "rows", torch.int32, a.streams), (missing, "missing", torch.int32, 1),
+                         (workspace, "workspace", torch.uint8, nbytes), pools=[new_table, *pools])
     _on(device, "pages_fork", lib.mh3_pages_fork, ref, held, n_pools, table.data_ptr(), refs.data_ptr(),
         parents.data_ptr(), rows.data_ptr(), new_table.data_ptr(), missing.data_ptr(), workspace.data_ptr(),
         workspace.numel())
@@ -1042,15 +1038,17 @@ def pages_copy(pools, src, dst):
     ...], or one). A pair is passed over if either is no page, if the call also copies from its dst, or if an earlier pair
     has the same dst."""
     held, n_pools, pages, pools = _pools(pools)
-    n = src.numel()
-    _need(src, "src", torch.int32, n)
-    _need(dst, "dst", torch.int32, n)
-    if dst.numel() != n:
-        raise ValueError("src and dst: as many pages")
     if not n_pools:
         raise ValueError("pools: at least one")
-    _on(_one_device_of(pools, src=src, dst=dst), "pages_copy", lib.mh3_pages_copy, held, n_pools, pages, src.data_ptr(),
-        dst.data_ptr(), n)
+    if not isinstance(src, torch.Tensor) or not isinstance(dst, torch.Tensor):
+        raise TypeError("src and dst: expected tensors")
+    n = src.numel()
+    if dst.numel() != n:
+        raise ValueError("src and dst: as many pages")
+    device = _operands((src, "src", torch.int32, n), (dst, "dst", torch.int32, n))
+    if _one_device(**{f"pools[{i}]": t for i, t in enumerate(pools)}) != device:
+        raise ValueError(f"pools: not on GPU {device}, where src is")
+    _on(device, "pages_copy", lib.mh3_pages_copy, held, n_pools, pages, src.data_ptr(), dst.data_ptr(), n)
 
 
 def pages_compact(pools, table, refs, *, map=None, used=None, workspace=None):
@@ -1062,17 +1060,15 @@ def pages_compact(pools, table, refs, *, map=None, used=None, workspace=None):
     dev = table.device
     map = torch.empty(pages, dtype=torch.int32, device=dev) if map is None else map
     used = torch.empty(1, dtype=torch.int32, device=dev) if used is None else used
-    _need(map, "map", torch.int32, pages)
-    _need(used, "used", torch.int32, 1)
     ref = C.byref(a)
     nbytes = lib.mh3_pages_compact_workspace_bytes(ref)
     if nbytes < 0:
         _check(nbytes, "pages_compact")
     if workspace is None:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _need(workspace, "workspace", torch.uint8, nbytes)
-    _on(_one_device_of(pools, table=table, refs=refs, map=map, used=used, workspace=workspace), "pages_compact",
-        lib.mh3_pages_compact, ref, held, n_pools, table.data_ptr(), refs.data_ptr(), map.data_ptr(), used.data_ptr(),
+    device = _page_lists(table, refs, pages, (map, "map", torch.int32, pages), (used, "used", torch.int32, 1),
+                         (workspace, "workspace", torch.uint8, nbytes), pools=pools)
+    _on(device, "pages_compact", lib.mh3_pages_compact, ref, held, n_pools, table.data_ptr(), refs.data_ptr(), map.data_ptr(), used.data_ptr(),
         workspace.data_ptr(), workspace.numel())
     return map, used
 
@@ -1119,11 +1115,14 @@ def pages_write(k, v, k_pages, v_pages, table, starts, off, *, rows=None, layout
     a = PagesWriteArgs(_page_table(table, pages, page_rows), kv_heads, 128, n_rows, n_rows, khs, krs, vhs, vrs, *k_strides,
                        *shape[3:])
     if rows is not None:
+        if not isinstance(rows, torch.Tensor):
+            raise TypeError("rows: expected a tensor")
         a.n = rows.numel()
-        _need(rows, "rows", torch.int32, a.n)
-    _need(starts, "starts", torch.int32, a.table.streams)
-    _need(off, "off", torch.int32, a.table.streams + 1)
-    device = _one_device(k=k, v=v, k_pages=k_pages, v_pages=v_pages, table=table, starts=starts, off=off, rows=rows)
+    streams = a.table.streams
+    device = _operands((starts, "starts", torch.int32, streams), (off, "off", torch.int32, streams + 1),
+                       (rows, "rows", torch.int32, a.n))
+    if _one_device(k=k, v=v, k_pages=k_pages, v_pages=v_pages, table=table) != device:
+        raise ValueError(f"k: not on GPU {device}, where starts is")
     _on(device, "pages_write", lib.mh3_pages_write, C.byref(a), k.data_ptr(), v.data_ptr(), k_pages.data_ptr(),
         v_pages.data_ptr(), table.data_ptr(), starts.data_ptr(), off.data_ptr(), _ptr(rows))
 
@@ -1170,8 +1169,7 @@ def flash_attn_pages_128(q, k, v, k_pages, v_pages, table, lengths, q_off, *, pa
         raise ValueError("layout is 'heads' or 'rows'")
     a = _pages_attn_args(q, k, v, k_pages, v_pages, table, window, scale, cap, layout, page_layout)
     heads, q_rows, streams = a.heads, a.q_rows, a.table.streams
-    device = _one_device(q=q, k=k, v=v, k_pages=k_pages, v_pages=v_pages, table=table, lengths=lengths, q_off=q_off,
-                         parents=parents, sinks=sinks, out=out, workspace=workspace)
+    device = _one_device(q=q, k=k, v=v, k_pages=k_pages, v_pages=v_pages, table=table, out=out)
     if device != torch._C._cuda_getDevice():  # the workspace's size is of the current device
         with torch.cuda.device(device):
             return flash_attn_pages_128(q, k, v, k_pages, v_pages, table, lengths, q_off, parents=parents, window=window,
@@ -1183,19 +1181,16 @@ def flash_attn_pages_128(q, k, v, k_pages, v_pages, table, lengths, q_off, *, pa
     out_heads, out_rows, a.out_head_stride, a.out_row_stride = _head_rows(out, "out", out_layout)
     if out_heads != heads or out_rows != q_rows:
         raise ValueError("out: q's heads and rows")
-    _need(lengths, "lengths", torch.int32, streams)
-    _need(q_off, "q_off", torch.int32, streams + 1)
-    if parents is not None:
-        _need(parents, "parents", torch.int32, q_rows)
-    if sinks is not None:
-        _need(sinks, "sinks", torch.int32, streams)
     ref = C.byref(a)
     nbytes = lib.mh3_flash_attn_pages_128_workspace_bytes(ref)
     if nbytes < 0:
         _check(nbytes, "flash_attn_pages_128")
     if workspace is None:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _need(workspace, "workspace", torch.uint8, nbytes)
+    if _operands((lengths, "lengths", torch.int32, streams), (q_off, "q_off", torch.int32, streams + 1),
+                 (parents, "parents", torch.int32, q_rows), (sinks, "sinks", torch.int32, streams),
+                 (workspace, "workspace", torch.uint8, nbytes)) != device:
+        raise ValueError(f"lengths: not on GPU {device}, where q is")
     _on(device, "flash_attn_pages_128", lib.mh3_flash_attn_pages_128, ref, q.data_ptr(), k.data_ptr(), v.data_ptr(),
         k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), q_off.data_ptr(), _ptr(parents),
         _ptr(sinks), workspace.data_ptr(), workspace.numel(), out.data_ptr())
