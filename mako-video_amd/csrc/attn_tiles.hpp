@@ -217,6 +217,8 @@ struct RangeSeen {
     {
         return from_lo + (32u * b + 8u * (i >> 2) + (i & 3)) < hi - lo ? s : -kInf;
     }
+    // Whether a row of the wave attends not all of block b's 32 keys (not asked here).
+    __device__ __forceinline__ bool masks(int) const { return true; }
     // Whether key j of the tile is.
     __device__ __forceinline__ bool key(uint32_t j) const { return t0 + j >= lo && t0 + j < hi; }
     __device__ __forceinline__ bool any() const { return max(lo, t0) < min(hi, t0 + 64u); }
@@ -258,6 +260,7 @@ struct BitsSeen {
         const uint32_t m = uint32_t(__builtin_amdgcn_sbfe(int(word[b] >> shift), 8 * (i >> 2) + (i & 3), 1));
         return __uint_as_float((__float_as_uint(s) & m) | (0xff800000u & ~m));
     }
+    __device__ __forceinline__ bool masks(int b) const { return __ballot(word[b] != ~0u) != 0u; }
     __device__ __forceinline__ bool key(uint32_t j) const { return word[j >> 5] >> (j & 31u) & 1u; }
     __device__ __forceinline__ bool any() const { return (word[0] | word[1]) != 0u; }
     template <bool BACKWARD>
@@ -498,9 +501,10 @@ __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, 
     if (MASKED) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
+            if (seen.masks(b))
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                s[b][i] = seen.score(s[b][i], b, i);
+                for (int i = 0; i < 16; ++i)
+                    s[b][i] = seen.score(s[b][i], b, i);
     }
     // Most tiles raise no maximum by much, and the sum over a lane's 32 keys of a row tells: up to 2^10 no key is above
     // that, and the old maximum serves. That spares the search for the new one in a phase whose vector instructions take 7
