@@ -134,6 +134,8 @@ CASES = [
     (7, 1, 112, [2000, 1999], [33, 2]), (8, 8, 64, [4096], [100]), (2, 2, 16, [10] * 70, 1), (6, 3, 256, [3000, 77], 7),
     (16, 2, 1024, [5000, 1024, 1023], 4), (2, 1, 16, [20000], [200]), (12, 2, 32, [50] * 130 + [9000], 2),
     (64, 1, 16, [100, 3000], [1, 70]), (4, 4, 64, [0, 0], [300, 1]),
+    # Runs of more tiles than either kernel looks up at a time.
+    (64, 64, 16, [20000], [70]), (64, 64, 32, [20000, 5], 1), (48, 48, 128, [9000, 9001], [33, 100]),
 ]
 
 
@@ -221,21 +223,26 @@ def test_a_row_is_its_own_stream(dev):
     assert torch.equal(one, wide)
 
 
-def test_layouts_strides_and_slices(dev):
-    """Heads side by side in wider rows, one layer's slices of pages that hold several, a table in a wider one."""
-    st = streams(6, dev, tree=True)
+@pytest.mark.parametrize("i,gap", [(6, 32), (6, 8), (8, 8), (4, 24)])
+def test_layouts_strides_and_slices(dev, i, gap):
+    """Heads side by side in wider rows (by 8 elements, and by 64), one layer's slices of pages that hold several, a table in
+    a wider one; with streams of many rows and of few."""
+    st = streams(i, dev, tree=True)
     want = st.run()
     rows = st.q.shape[1]
-    wide = [torch.full((rows, x.shape[0] * 128 + 64), NAN, dtype=torch.bfloat16, device=dev) for x in (st.q, st.k, st.v)]
-    q, k, v = (w[:, 32:-32] for w in wide)
+    wide = [torch.full((rows, x.shape[0] * 128 + 2 * gap), NAN, dtype=torch.bfloat16, device=dev) for x in (st.q, st.k, st.v)]
+    q, k, v = (w[:, gap:-gap] for w in wide)
     for t, x in zip((q, k, v), (st.q, st.k, st.v)):
         t.copy_(x.transpose(0, 1).reshape(rows, -1))
-    pool = torch.full((st.pages, 3, 2, *st.k_pages.shape[1:]), NAN, dtype=torch.bfloat16, device=dev)
-    pool[:, 1, 0], pool[:, 1, 1] = st.k_pages, st.v_pages
+    heads, page = st.k_pages.shape[1:3]
+    pool = torch.full((st.pages, 3, 2, page, heads, 128 + gap), NAN, dtype=torch.bfloat16, device=dev)
+    k_pages, v_pages = (pool[:, 1, x, :, :, :128].transpose(2, 1) for x in range(2))     # rows of heads, each wider
+    k_pages.copy_(st.k_pages)
+    v_pages.copy_(st.v_pages)
     table = torch.full((len(st.lines), len(st.lines[0]) + 9), 1, dtype=torch.int32, device=dev)
     table[:, 4:-5] = ints(st.lines, dev)
     out = torch.zeros((rows, st.q.shape[0] * 128), dtype=torch.bfloat16, device=dev)
-    mh.flash_attn_pages_128(q, k, v, pool[:, 1, 0], pool[:, 1, 1], table[:, 4:-5], ints(st.kept, dev), ints(st.q_off, dev),
+    mh.flash_attn_pages_128(q, k, v, k_pages, v_pages, table[:, 4:-5], ints(st.kept, dev), ints(st.q_off, dev),
                             parents=ints(st.parents, dev), layout="rows", out=out)
     assert torch.equal(out.view(rows, -1, 128).transpose(0, 1), want)
 
