@@ -500,7 +500,8 @@ int mh3_pages_write(const MH3PagesWriteArgs* args, const uint16_t* k, const uint
  *   window:  0: none. sinks: int32 [streams], how many first rows stay in sight (NULL: none).
  * A kept row whose entry is no page is not attended. scale, cap, the strides and rounding are mh3_flash_attn_128's, the pools'
  * strides mh3_pages_write's; page_rows is a multiple of 16. What lies in rows that a row does not attend, in pages past a
- * stream's length among them, has no effect on any of its bits. Rows of no stream keep what out holds.
+ * stream's length among them, has no effect on any of its bits. Rows of no stream (before q_off[0], and from
+ * q_off[streams] on) become zero or keep what out holds (zero_rest).
  *   workspace: mh3_flash_attn_pages_128_workspace_bytes(args) bytes; the call overwrites it, so calls that overlap in time,
  *            two captured graphs among them, need their own.
  * out may not overlap an input, the pools or the workspace (MH3_ERR_PARAM). */
@@ -513,7 +514,7 @@ typedef struct MH3PagesAttnArgs {
     uint32_t window;
     float scale; /* score scale, up to 2^100; 0 means 1 / sqrt(128) */
     float cap;   /* tanh cap, 2^-60 .. 1024; 0: none */
-    uint32_t reserved;
+    uint32_t zero_rest; /* 1: rows of no stream become zero; 0: they keep what out holds */
     uint64_t q_head_stride, q_row_stride, k_head_stride, k_row_stride;
     uint64_t v_head_stride, v_row_stride, out_head_stride, out_row_stride;
     uint64_t k_page_stride, k_page_head_stride, k_page_row_stride;

@@ -38,6 +38,7 @@ struct PagesParams : DenseParams {
     uint32_t streams, cols, pages, page_rows, window, workers, slot_rows;
     uint32_t item_rows; // list rows of an item: a wave's 32, or up to eight waves'
     uint32_t begin;     // tiles that take as long as the begin of a part
+    uint32_t zero_rest; // rows of no stream become zero
     FastDiv div_item;
     FastDiv div_page;
 };
@@ -703,6 +704,17 @@ template <uint32_t SPLIT>
 __global__ __launch_bounds__(256) void attn_pages_join_kernel(PagesParams p, uint32_t blocks)
 {
     __shared__ float met[SPLIT][8 / SPLIT][6][32];
+    if (p.zero_rest) {
+        const uint32_t from = uint32_t(min(max(p.q_off[p.streams], 0), int32_t(p.q_rows)));
+        const uint32_t before = min(uint32_t(max(p.q_off[0], 0)), from), rest = before + p.q_rows - from;
+        const uint32_t heads = p.kv_heads * p.group;
+        for (uint64_t i = blockIdx.x * 8u + threadIdx.x / 32u; i < uint64_t(rest) * heads; i += gridDim.x * 8u) {
+            const uint32_t n = uint32_t(i / heads), head = uint32_t(i - uint64_t(n) * heads);
+            const uint32_t row = n < before ? n : from + (n - before);
+            *reinterpret_cast<uint2*>(p.out + uint64_t(head) * p.ohs + uint64_t(row) * p.ors + 4u * (threadIdx.x & 31u)) =
+                uint2{0u, 0u};
+        }
+    }
     const Cut cut = reinterpret_cast<const Cut*>(p.part)[blockIdx.x / blocks];
     const float* const parts = parts_of(p);
     const float2* const ml = reinterpret_cast<const float2*>(parts + 2ull * p.workers * p.slot_rows * 128u);
@@ -812,7 +824,7 @@ int check_pages_args(const MH3PagesAttnArgs* args)
         return MH3_ERR_SHAPE;
     if (a.head_dim != 128u)
         return MH3_ERR_UNSUPPORTED;
-    if (!(a.scale >= 0.0f && a.scale <= 0x1p100f) || !(a.cap == 0.0f || (a.cap >= 0x1p-60f && a.cap <= 1024.0f)))
+    if (a.zero_rest > 1u || !(a.scale >= 0.0f && a.scale <= 0x1p100f) || !(a.cap == 0.0f || (a.cap >= 0x1p-60f && a.cap <= 1024.0f)))
         return MH3_ERR_PARAM;
     if (t.streams == 0 || t.streams > MH3_MAX_STREAMS || t.cols == 0 || t.cols >= (1u << 24) || t.pages == 0 ||
         t.pages >= (1u << 24) || t.table_stride < t.cols || t.table_stride >= (1ull << 32) || t.page_rows == 0 ||
@@ -926,7 +938,7 @@ extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint
     p.page_rows = t.page_rows, p.window = a.window, p.div_page = FastDiv::make(t.page_rows);
     p.kv_heads = a.kv_heads, p.group = a.heads / a.kv_heads, p.q_rows = a.q_rows, p.div_group = FastDiv::make(p.group);
     p.workers = plan.workers, p.slot_rows = plan.slot_rows, p.item_rows = plan.item_rows;
-    p.div_item = FastDiv::make(plan.item_rows), p.begin = plan.item_rows > 32u ? kPairBegin : kBegin;
+    p.zero_rest = a.zero_rest, p.div_item = FastDiv::make(plan.item_rows), p.begin = plan.item_rows > 32u ? kPairBegin : kBegin;
     score_factors(a.scale, a.cap, p);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (const int rc = a.cap > 0.0f ? launch_pages<true>(p, s) : launch_pages<false>(p, s); rc != MH3_OK)

@@ -97,7 +97,7 @@ class PagesWriteArgs(C.Structure):
 class PagesAttnArgs(C.Structure):
     _fields_ = [("table", PagesArgs), ("heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
                 ("q_rows", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float), ("cap", C.c_float),
-                ("reserved", C.c_uint32)] + \
+                ("zero_rest", C.c_uint32)] + \
                [(f"{t}_{d}_stride", C.c_uint64) for t in ("q", "k", "v", "out") for d in ("head", "row")] + \
                [(f"{t}_{d}_stride", C.c_uint64) for t in ("k", "v") for d in ("page", "page_head", "page_row")]
 
@@ -1176,7 +1176,8 @@ def flash_attn_pages_128(q, k, v, k_pages, v_pages, table, lengths, q_off, *, pa
                                         sinks=sinks, scale=scale, cap=cap, layout=layout, page_layout=page_layout, out=out,
                                         out_layout=out_layout, workspace=workspace)
     if out is None:
-        out = torch.zeros((heads, q_rows, 128) if out_layout == "heads" else (q_rows, heads * 128),
+        a.zero_rest = 1
+        out = torch.empty((heads, q_rows, 128) if out_layout == "heads" else (q_rows, heads * 128),
                           dtype=torch.bfloat16, device=device)
     out_heads, out_rows, a.out_head_stride, a.out_row_stride = _head_rows(out, "out", out_layout)
     if out_heads != heads or out_rows != q_rows:

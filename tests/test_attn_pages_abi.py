@@ -31,7 +31,8 @@ def test_shapes():
     for kw in ({"streams": 0}, {"streams": 4097}, {"cols": 0}, {"pages": 0}, {"pages": 1 << 24}, {"table_stride": 4},
                {"page_rows": 0}, {"page_rows": 24}, {"page_rows": 8}, {"page_rows": 1 << 28}):
         assert call(attn_args(args(**kw))) == mh.ERR_SHAPE, kw
-    for kw in ({"scale": -1.0}, {"scale": float("nan")}, {"cap": -1.0}, {"cap": 1025.0}, {"cap": float("inf")}):
+    for kw in ({"scale": -1.0}, {"scale": float("nan")}, {"cap": -1.0}, {"cap": 1025.0}, {"cap": float("inf")},
+               {"zero_rest": 2}):
         assert call(attn_args(**kw)) == mh.ERR_PARAM, kw
     for t in ("q", "k", "v", "out"):
         assert call(attn_args(**{f"{t}_row_stride": 132})) == call(attn_args(**{f"{t}_head_stride": 4})) == mh.ERR_ALIGN

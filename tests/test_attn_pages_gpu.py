@@ -135,7 +135,7 @@ CASES = [
     (16, 2, 1024, [5000, 1024, 1023], 4), (2, 1, 16, [20000], [200]), (12, 2, 32, [50] * 130 + [9000], 2),
     (64, 1, 16, [100, 3000], [1, 70]), (4, 4, 64, [0, 0], [300, 1]),
     # Runs of more tiles than either kernel looks up at a time.
-    (64, 64, 16, [20000], [70]), (64, 64, 32, [20000, 5], 1), (48, 48, 128, [9000, 9001], [33, 100]),
+    (2, 2, 16, [40], [1100]), (64, 64, 16, [20000], [70]), (64, 64, 32, [20000, 5], 1), (48, 48, 128, [9000, 9001], [33, 100]),
 ]
 
 
@@ -281,5 +281,7 @@ def test_nothing_to_do(dev):
     t, n = ints(st.lines, dev), ints(st.kept, dev)
     mh.flash_attn_pages_128(st.q, st.k, st.v, st.k_pages, st.v_pages, t, n, ints([5, 5], dev), out=out)
     assert bool((out == 3).all())
+    out = mh.flash_attn_pages_128(st.q, st.k, st.v, st.k_pages, st.v_pages, t, n, ints([5, 5], dev))
+    assert not bool(out.any())
     e = st.q[:, :0], st.k[:, :0], st.v[:, :0]
     assert mh.flash_attn_pages_128(*e, st.k_pages, st.v_pages, t, n, ints([0, 0], dev)).shape == (5, 0, 128)
