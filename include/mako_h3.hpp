@@ -207,6 +207,47 @@ struct Scores {
     const int32_t* sinks = nullptr; // a second range of each row's, with ranges (attn_window_ranges)
 };
 
+// Streams' kept rows in pages: the table int32 [streams][cols] (stride ints from a stream's entries to the next one's; 0:
+// cols), over pools of `pages` pages of page_rows rows.
+struct Pages {
+    uint32_t streams = 0, cols = 0, pages = 0, page_rows = 0;
+    uint64_t stride = 0;
+
+    MH3PagesArgs args() const { return MH3PagesArgs{streams, cols, pages, page_rows, stride ? stride : cols}; }
+};
+
+// The shape of a call over kept rows: heads, new rows, and where head rows and the pools' lie. Zero kv_heads: as many as
+// heads; zero strides: [heads][rows][128], and pools [pages][kv_heads][page_rows][128].
+struct PagesAttn {
+    struct Pool {
+        uint64_t page = 0, head = 0, row = 0;
+    };
+    Pages table;
+    uint32_t heads = 0, kv_heads = 0, q_rows = 0, window = 0;
+    float scale = 0.0f, cap = 0.0f; // 0: 1 / sqrt(128); no cap
+    bool zero_rest = false;         // rows of no stream become zero
+    Dense::Strides q, k, v, out;
+    Pool k_pages, v_pages;
+
+    MH3PagesAttnArgs args() const
+    {
+        const uint32_t kv = kv_heads ? kv_heads : heads;
+        Dense d;
+        d.heads = heads, d.kv_heads = kv, d.q_rows = d.kv_rows = q_rows, d.q = q, d.k = k, d.v = v, d.out = out;
+        const MH3DenseAttnArgs r = d.args();
+        const auto pool = [&](const Pool& p) {
+            const uint64_t head = uint64_t(table.page_rows) * 128;
+            return p.page || p.head || p.row ? p : Pool{head * kv, head, 128};
+        };
+        const Pool kp = pool(k_pages), vp = pool(v_pages);
+        return MH3PagesAttnArgs{table.args(),    heads,           kv,           128,          q_rows,         window,
+                                scale,           cap,             zero_rest,    r.q_head_stride, r.q_row_stride,
+                                r.k_head_stride, r.k_row_stride,  r.v_head_stride, r.v_row_stride, r.out_head_stride,
+                                r.out_row_stride, kp.page,        kp.head,      kp.row,       vp.page,        vp.head,
+                                vp.row};
+    }
+};
+
 inline std::optional<uint32_t> parse_int8(const std::string& text)
 {
     uint32_t mask = 0;
@@ -412,6 +453,99 @@ public:
         const MH3RangeArgs a{q_rows, kv_rows, docs, causal ? 1u : 0u};
         check(mh3_attn_ranges(&a, q_off, k_off, prefix, ranges, s_), "attn_ranges");
     }
+    // Scores::ranges and Scores::sinks of documents whose rows attend a window of keys and the first sinks[d] (may be null)
+    // of their document.
+    void attn_window_ranges(uint32_t q_rows, uint32_t kv_rows, uint32_t docs, uint32_t window, bool causal,
+                            const int32_t* q_off, const int32_t* k_off, const int32_t* sinks, int32_t* ranges,
+                            int32_t* first) const
+    {
+        const MH3WindowArgs a{q_rows, kv_rows, docs, causal ? 1u : 0u, window, 0};
+        check(mh3_attn_window_ranges(&a, q_off, k_off, sinks, ranges, first, s_), "attn_window_ranges");
+    }
+
+    // Kept rows in pages (mako_h3.h has the rules). missing, used: device int32, may be null.
+    void pages_take(const Pages& t, int32_t* table, int32_t* refs, const int32_t* first, const int32_t* last,
+                    int32_t* missing = nullptr) const
+    {
+        const MH3PagesArgs a = t.args();
+        check(mh3_pages_take(&a, table, refs, first, last, missing, s_), "pages_take");
+    }
+    void pages_free(const Pages& t, int32_t* table, int32_t* refs, const int32_t* first, const int32_t* last) const
+    {
+        const MH3PagesArgs a = t.args();
+        check(mh3_pages_free(&a, table, refs, first, last, s_), "pages_free");
+    }
+    static uint64_t pages_fork_workspace_bytes(const Pages& t)
+    {
+        const MH3PagesArgs a = t.args();
+        return bytes(mh3_pages_fork_workspace_bytes(&a), "pages_fork");
+    }
+    void pages_fork(const Pages& t, const std::vector<MH3Pool>& pools, const int32_t* table, int32_t* refs,
+                    const int32_t* parents, const int32_t* rows, int32_t* new_table, void* workspace,
+                    uint64_t workspace_bytes, int32_t* missing = nullptr) const
+    {
+        const MH3PagesArgs a = t.args();
+        check(mh3_pages_fork(&a, pools.data(), uint32_t(pools.size()), table, refs, parents, rows, new_table, missing,
+                             workspace, workspace_bytes, s_),
+              "pages_fork");
+    }
+    void pages_copy(const std::vector<MH3Pool>& pools, uint32_t pages, const int32_t* src, const int32_t* dst,
+                    uint32_t n) const
+    {
+        check(mh3_pages_copy(pools.data(), uint32_t(pools.size()), pages, src, dst, n, s_), "pages_copy");
+    }
+    static uint64_t pages_compact_workspace_bytes(const Pages& t)
+    {
+        const MH3PagesArgs a = t.args();
+        return bytes(mh3_pages_compact_workspace_bytes(&a), "pages_compact");
+    }
+    void pages_compact(const Pages& t, const std::vector<MH3Pool>& pools, int32_t* table, int32_t* refs, int32_t* map,
+                       void* workspace, uint64_t workspace_bytes, int32_t* used = nullptr) const
+    {
+        const MH3PagesArgs a = t.args();
+        check(mh3_pages_compact(&a, pools.data(), uint32_t(pools.size()), table, refs, map, used, workspace,
+                                workspace_bytes, s_),
+              "pages_compact");
+    }
+    // The shape's q_rows new rows of k and v, or the n that `rows` says, to kept rows starts[s] + j - off[s].
+    void pages_write(const PagesAttn& d, const uint16_t* k, const uint16_t* v, uint16_t* k_pages, uint16_t* v_pages,
+                     const int32_t* table, const int32_t* starts, const int32_t* off, const int32_t* rows = nullptr,
+                     uint32_t n = 0) const
+    {
+        const MH3PagesAttnArgs a = d.args();
+        const MH3PagesWriteArgs w{a.table,
+                                  a.kv_heads,
+                                  128,
+                                  a.q_rows,
+                                  rows ? n : a.q_rows,
+                                  a.k_head_stride,
+                                  a.k_row_stride,
+                                  a.v_head_stride,
+                                  a.v_row_stride,
+                                  a.k_page_stride,
+                                  a.k_page_head_stride,
+                                  a.k_page_row_stride,
+                                  a.v_page_stride,
+                                  a.v_page_head_stride,
+                                  a.v_page_row_stride};
+        check(mh3_pages_write(&w, k, v, k_pages, v_pages, table, starts, off, rows, s_), "pages_write");
+    }
+    // Attention of the streams' new rows over their kept ones and themselves (parents, sinks: may be null).
+    static uint64_t flash_attn_pages_128_workspace_bytes(const PagesAttn& d)
+    {
+        const MH3PagesAttnArgs a = d.args();
+        return bytes(mh3_flash_attn_pages_128_workspace_bytes(&a), "flash_attn_pages_128");
+    }
+    void flash_attn_pages_128(const PagesAttn& d, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                              const uint16_t* k_pages, const uint16_t* v_pages, const int32_t* table,
+                              const int32_t* lengths, const int32_t* q_off, const int32_t* parents, const int32_t* sinks,
+                              void* workspace, uint64_t workspace_bytes, uint16_t* out) const
+    {
+        const MH3PagesAttnArgs a = d.args();
+        check(mh3_flash_attn_pages_128(&a, q, k, v, k_pages, v_pages, table, lengths, q_off, parents, sinks, workspace,
+                                       workspace_bytes, out, s_),
+              "flash_attn_pages_128");
+    }
     // Flash attention over the pass lists idx / cnt of cube_select (or cube_topk) and the dense rows
     // [dense_row0, dense_row0 + n_dense); q, k, v and out in c's cube geometry. scale 0: 1 / sqrt(128).
     void flash_attn_sparse_128(const Cubes& c, const uint16_t* q, const uint16_t* k, const uint16_t* v,
@@ -523,6 +657,11 @@ public:
     }
 
 private:
+    static uint64_t bytes(int64_t n, const char* what)
+    {
+        check(n < 0 ? int(n) : MH3_OK, what);
+        return uint64_t(n);
+    }
     static MH3RowsArgs rows_args(uint32_t rows, uint32_t dim, uint32_t dtype, const Modulation& m, float eps,
                                  uint32_t flags = 0)
     {
