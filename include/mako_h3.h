@@ -4,7 +4,8 @@
  * `swiglu_rows`, the `--sparse` cube selector (`cube_pool`, `cube_scores`, `cube_topk`, fused `cube_select`),
  * the `--int8` weight quantizer (`quant_rows_i8`) and the int8 weight-only fc1 GEMM with its SwiGLU epilogue; and of
  * the dense path beside it: rotary positions on several axes (`rotary_axes`), attention over whole rows
- * (`flash_attn_128`) and 4-bit microscaled products (`gemm_mx4`).
+ * (`flash_attn_128`), under a window too, streams whose kept rows lie in pages (`pages_*`, `flash_attn_pages_128`), and
+ * 4-bit microscaled products (`gemm_mx4`).
  *
  * The reference runs these as Metal kernels looked up by name in mako-common's TransformerRuntime
  * (`dispatch(enc, name, {buffers}, &args, sizeof args, grid, tg)`, the in-repo instance being
@@ -397,9 +398,9 @@ int mh3_flash_attn_128_sinks(const MH3DenseAttnArgs* args, const uint16_t* q, co
  * row i has key place own = k_off[d + 1] - q_off[d + 1] + i. It attends the document's keys in (own - window, own] with
  * causal 1, in (own - window, own + window) with causal 0, and of the document's first sinks[d] keys (int32 [docs], or
  * NULL: none) those up to own with causal 1, all of them with causal 0. ranges takes the window's part, first those of
- * the first keys that lie before the window (all of them, if it ends among them; 0 and 0 where it covers them); both int32 [q_rows][2], 8-byte
- * aligned. Rows of no document have two empty ranges. Neither output may overlap an input or the other
- * (MH3_ERR_PARAM). */
+ * the first keys that lie before the window (all of them, if it ends among them; 0 and 0 where it covers them); both
+ * int32 [q_rows][2], 8-byte aligned. Rows of no document have two empty ranges. Neither output may overlap an input or
+ * the other (MH3_ERR_PARAM). */
 typedef struct MH3WindowArgs {
     uint32_t q_rows;
     uint32_t kv_rows; /* the ranges are cut off at 0 and kv_rows */
@@ -420,8 +421,8 @@ int mh3_attn_window_ranges(const MH3WindowArgs* args, const int32_t* q_off, cons
  * every call follow from its inputs: nothing depends on the order in which the GPU gets to it.
  * A pool is `pages` pages of page_bytes, each in one piece, page_stride bytes apart (multiples of 16, the base 16-byte
  * aligned): of whatever a program keeps by rows, say a layer's keys, or all layers' keys and values. Calls take up to
- * MH3_MAX_POOLS pools (a host array), which may not overlap each other, the table, refs or another list (MH3_ERR_PARAM;
- * so for all in- and outputs below). int32 lists and tables are 4-byte aligned, workspaces 16; a call that overlaps
+ * MH3_MAX_POOLS pools (a host array), which may not overlap each other, the table, refs or another list, each taken as
+ * the span from its first page to its last one's end (MH3_ERR_PARAM; so for all in- and outputs below). int32 lists and tables are 4-byte aligned, workspaces 16; a call that overlaps
  * another in time needs its own workspace. */
 enum { MH3_MAX_POOLS = 64, MH3_MAX_STREAMS = 4096, MH3_MAX_PAIRS = 16384 };
 typedef struct MH3PagesArgs {
@@ -436,8 +437,8 @@ typedef struct MH3Pool {
     uint64_t page_bytes;
     uint64_t page_stride;
 } MH3Pool;
-/* Gives the entries first[s] .. last[s] - 1 of each stream s that are negative a page each, the lowest free ones in the
- * order (stream, entry), and counts them (refs 1). Entries that find no page stay; *missing (NULL: not wanted) says how
+/* Gives the entries first[s] .. last[s] - 1 of each stream s that are no page a page each, the lowest free ones in the
+ * order (stream, entry), and counts them (refs 1). Entries that find no page become -1; *missing (NULL: not wanted) says how
  * many. first and last: int32 [streams], clamped to [0, cols]. */
 int mh3_pages_take(const MH3PagesArgs* args, int32_t* table, int32_t* refs, const int32_t* first, const int32_t* last,
                    int32_t* missing, mh3_stream_t stream);

@@ -6,7 +6,11 @@
 // order (stream, entry); counts change by integer atomics, whose order does not show. Entries that are no page of the pool
 // (negative, or past its end) are no page to any kernel, so a bad table reads and writes nothing outside the pool.
 // A program calls them once a step (fork, free, compact: now and then), for all layers: what bounds them is the launches
-// and, where pages move, HBM.
+// (take and write 4.5 us each, a fork of eight streams 4.3 to plan and 4.3 to do) and, where pages move, HBM: 512 pages of
+// 262 KB copied in 54 us, 5 TB/s, two of five streams' pages freed and 510 MB moved in 96.
+// Planning is one workgroup's for take and fork: 1024 entries and 8192 counts in each of its passes. The plan of a compaction
+// is a workgroup's per 8192 pages, each of which counts all pages itself: pages^2 / 1024 bytes in all, mostly from L2, 0.1 MB
+// for ten thousand pages and 1 GB for a million.
 #include "mh3_common.hpp"
 
 #include <algorithm>
@@ -172,7 +176,7 @@ __global__ __launch_bounds__(kTakers) void pages_take_kernel(Table t, int32_t* r
         return t.at(a, start[a] + j - begin[a]);
     };
     const uint32_t none = take_lowest(
-        refs, t.pages, n, sh, [&](uint32_t j) { return entry(j) < 0; },
+        refs, t.pages, n, sh, [&](uint32_t j) { return !t.page(entry(j)); },
         [&](uint32_t j, int32_t page) {
             entry(j) = page;
             if (page >= 0)

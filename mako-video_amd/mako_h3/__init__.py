@@ -2,9 +2,10 @@
 
 The op names are the reference's kernel names (mako-common's `rms_mod_rows`, `gate_add_rows`, `swiglu_rows`,
 `cube_pool`, `cube_scores`, `cube_topk`, `quant_rows_i8`; fc1's `gemm_i8` + `swiglu_rows` as `gemm_w8a16_swiglu`),
-with the dense path beside them (`rotary_axes`, `heads_partial_axes`, `flash_attn_128`, `attn_ranges`, `quant_rows_mx4`,
-`gemm_mx4*`, which also run on the GPU that their tensors are on where it is not the current one), and errors raise RuntimeError as the reference's host code throws std::runtime_error on a bad call
-(src/video/audio_vae.cpp:231-232). Every call checks the tensors against the sizes the kernel will touch before it
+with the dense path beside them (`rotary_axes`, `heads_partial_axes`, `flash_attn_128`, `attn_ranges`,
+`attn_window_ranges`, `quant_rows_mx4`, `gemm_mx4*`, and for streams over pages `pages_*` and `flash_attn_pages_128`, which
+also run on the GPU that their tensors are on where it is not the current one), and errors raise RuntimeError as the
+reference's host code throws std::runtime_error on a bad call (src/video/audio_vae.cpp:231-232). Every call checks the tensors against the sizes the kernel will touch before it
 reaches the library, launches on torch's current stream, and returns without synchronizing.
 
 torch is used here only for device memory and streams; the compute is the library's HIP kernels. There is no
@@ -980,7 +981,7 @@ def _page_lists(table, refs, pages, *lists, pools=()) -> int:
 
 def pages_take(table, refs, first, last, *, missing=None):
     """Gives the entries first[s] .. last[s] - 1 (int32 [streams]) of each stream's row of `table` (int32
-    [streams][entries], -1: no page) that are -1 a page each, the lowest free ones (refs int32 [pages], 0: free) in the
+    [streams][entries], -1: no page) that are no page a page each, the lowest free ones (refs int32 [pages], 0: free) in the
     order (stream, entry), and counts them. Returns `missing`, int32 [1]: how many found none and stay -1."""
     pages = _counts(refs)
     a = _page_table(table, pages)

@@ -129,6 +129,14 @@ def test_take_and_free(dev, streams, cols, pages, seed):
         m.same(table, refs)
 
 
+def test_take_where_no_page_of_the_pool_is(dev):
+    """Entries outside the pool are no page, whichever side they lie on; those that find none end as -1."""
+    table = ints([[1, 9, -7, 2**31 - 1, -2**31, 4]], dev)
+    refs = ints([0, 1, 2, 0], dev)
+    assert int(mh.pages_take(table, refs, ints([0], dev), ints([6], dev))) == 3
+    assert table.tolist() == [[1, 0, 3, -1, -1, -1]] and refs.tolist() == [1, 1, 2, 1]
+
+
 def test_take_at_the_int_range(dev):
     """Bounds at the ends of int32, more wants than a workgroup has threads, and a pool that runs out in their midst."""
     m = Model(random.Random(5), 3, 3001, 5000, fill=0.1, share=0.0)
