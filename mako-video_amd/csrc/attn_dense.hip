@@ -1,8 +1,9 @@
 // `flash_attn_128`: flash attention over whole rows, head_dim 128, bf16 in and out: what a block runs without the sparse
 // selection, for any count of query and key rows, shared key heads, a range of keys for each query row (documents packed
-// into one batch, a prefix, causal rows), a tanh cap on the scores and a bias that falls with the distance.
+// into one batch, a prefix, causal rows), a second range (what a window has left behind and still keeps in sight), a tanh cap
+// on the scores and a bias that falls with the distance.
 //   s[i][j] = cap tanh(scale q_i . k_j / cap) - slope |q_pos_i - k_pos_j|   (without a cap: scale q_i . k_j)
-//   out_i = sum_j softmax_j(s[i][lo_i .. hi_i)) v_j;   a row without keys is zero.
+//   out_i = sum_j softmax_j(s[i][j], j in [lo_i, hi_i) or [lo'_i, hi'_i)) v_j;   a row without keys is zero.
 // The reference's counterpart of the plain case is mako-common's flash_attn_coop_128_32 (docs/performance.md).
 //
 // Design (gfx950, v_mfma_f32_32x32x16_bf16), the fragments and LDS images of attn.hip:
@@ -24,14 +25,23 @@
 // - A row's bits come from its own scores, its keys' values and the ranges. Waves and workgroups decide together what to
 //   skip, never how a row rounds: that a neighbour attends an infinity or a far position leaves no trace. (One decision for
 //   the wave's 32 rows instead: the same time within 2%.)
+// - Of two ranges a workgroup walks the tiles of both, not those between them, and a row's keys of a masked tile are 64 bits
+//   instead of two bounds: one pair of bounds is compared key by key in the scalar registers of each compare, and a second
+//   pair's did not fit beside them. Which turns are masked is decided tile by tile: a walk's first and last of each range.
+// - Eight waves load a tile together: the first four K three tiles ahead, the others V two, each a quarter, as soon as half
+//   of a turn has made room (all eight waves loading K and then V: 945 rows of 56 heads 40.8 us for 39.6 now, 960 x 544
+//   8,507 and 8,419, the packed clips below 1,503 and 1,474, 2 x 4096 causal rows of 40 heads on 8 under a bias 450 and 430).
 // - Few rows leave the chip idle: their keys are then split over workgroups, each leaves its part of O, the maximum and the
 //   sum in the workspace, and a second kernel joins them in a fixed order.
-// What bounds it: many rows, the chip's power (960 x 544, 56 heads, 19,305 rows: 8.65 .. 8.9 ms, 1200 .. 1230 TFLOP/s, the
+// What bounds it: many rows, the chip's power (960 x 544, 56 heads, 19,305 rows: 8.4 .. 8.9 ms, 1200 .. 1270 TFLOP/s, the
 // clock at 1.65 to 1.7 GHz and the matrix cores busy 72% of it); under a cap also the vector unit's transcendentals (five
-// clips packed into 14,925 rows of 40 heads 1490 us, without a cap 1230, with a multiplication in the place of the cap's
-// exponential and reciprocal 1260); few rows, the one pass over K and V (129,536 keys of 8 heads in 95 us, 5.5 TB/s).
-// Under a bias the eight-wave kernels hold five or six registers in scratch, read between the loops, in masked turns and in
-// rare paths, never in the loop of whole tiles.
+// clips packed into 14,925 rows of 40 heads 1475 us, without a cap 1230, with a multiplication in the place of the cap's
+// exponential and reciprocal 1260); under a window also the turns that are masked and each workgroup's begin (960 x 544,
+// 4080 keys back and the 435 first: 2159 us for 75 tiles a workgroup, 1.74 us a whole turn, 2.9 a masked one of which there are
+// some nine, 4.7 the first, 5.8 before it, and 5 until the CU has its next workgroup); few rows, the one pass over K and V
+// (129,536 keys of 8 heads in 95 us, 5.5 TB/s).
+// Under a bias the eight-wave kernels hold six or seven registers in scratch, read between the loops, in masked turns and in
+// rare paths, never in the loop of whole tiles; with a second range twenty, six of which each turn reads.
 #include "attn_tiles.hpp"
 
 #include <type_traits>

@@ -20,7 +20,18 @@
 //   as the chip holds takes an equal run of it, whichever items that cuts: it writes the items that are its own and leaves
 //   parts (O, the maximum, the sum) of the two at its ends. A second kernel joins those in the order of the tiles. Where the
 //   cuts lie follows from the lengths alone. If all streams' items have as many row tiles, that many workgroups take the
-//   same run, one row tile each, so that what one of them has read the others find in their XCD's L2.
+//   same run, one row tile each, so that what one of them has read the others find in their XCD's L2 (two frames of 510
+//   rows, 56 heads, 4080 rows back and the 435 first: 209 us, and 188 since).
+// What bounds it, by what a call has most of (5 TB/s is what a copy of 1 GiB reaches here):
+// - One new row a stream: the one pass over K and V. 129,536 kept rows of three streams, 40 heads on 8: 95 us, 5.6 TB/s, and 7
+//   for the join; of 64 streams under a window of 1020 rows, 240 MB: 49 and 7.
+// - Small trees: a part's begin (the streams' sums, the pages' numbers, the rows' lines) beside few turns: eight rows after
+//   2985 kept, 56 heads, 23 us and 9 for the join, the pass over K and V alone 17.
+// - Larger trees: the turns. Five of 63 rows after 129,536 kept in all, 40 heads on 8: 160 list rows an item leave three of
+//   eight waves without rows; 127 turns of 1.55 us and some 20 to begin and to join: 226.
+// - Chunks: products and softmax in turn, K and V from HBM: those frames' 79 turns take 2 us each, the clock at 1.8 .. 2.1 GHz
+//   and the matrix cores busy 38 .. 43% of it.
+// Most of the eight-wave kernel's 38 registers in scratch are those of the list of parts; the loop of whole tiles reads none.
 #include "attn_tiles.hpp"
 
 namespace mh3 {
