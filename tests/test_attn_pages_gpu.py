@@ -285,3 +285,66 @@ def test_nothing_to_do(dev):
     assert not bool(out.any())
     e = st.q[:, :0], st.k[:, :0], st.v[:, :0]
     assert mh.flash_attn_pages_128(*e, st.k_pages, st.v_pages, t, n, ints([0, 0], dev)).shape == (5, 0, 128)
+
+
+def test_most_streams(dev):
+    """As many streams as a call takes, a few of them without kept or new rows."""
+    n = mh.MAX_STREAMS
+    st = Streams(77, dev, 2, 1, 16, [(7 * s) % 41 for s in range(n)], [0 if s % 97 == 5 else 1 + (s % 50 == 0) for s in range(n)])
+    out = torch.zeros_like(st.q)
+    st.run(out=out, window=20)
+    check(out, *st.want(window=20))
+
+
+def far_pool(like, dev, storage):
+    """A pool of `like`'s pages, 2.5 GB from one to the next."""
+    step = 1_250_000_008
+    pool = storage.as_strided(like.shape, (step, *like.stride()[1:]))
+    pool.copy_(like)
+    return pool
+
+
+def test_pages_past_32_bits_of_offsets(dev):
+    """Pages that lie gigabytes apart: attention, rows into them, copies, forks and compactions are those of close ones."""
+    st = Streams(5, dev, 4, 2, 32, [70], [3])
+    assert st.pages == 6
+    size = 5 * 1_250_000_008 + st.k_pages[0].numel()
+    k_far = far_pool(st.k_pages, dev, torch.empty(size, dtype=torch.bfloat16, device=dev))
+    v_far = far_pool(st.v_pages, dev, torch.empty(size, dtype=torch.bfloat16, device=dev))
+    near, far = [st.k_pages, st.v_pages], [k_far, v_far]
+    same = lambda: all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(near, far))  # noqa: E731
+    want = st.run()
+    st.k_pages, st.v_pages = far
+    assert torch.equal(st.run(), want)
+    table, off = ints([st.lines[0] * 1, [-1] * len(st.lines[0])], dev), ints([0, 5, 5], dev)
+    for pools in (near, far):
+        refs = torch.zeros(6, dtype=torch.int32, device=dev)
+        refs[ints(st.lines[0][:3], dev).long()] = 1
+        t = table.clone()
+        mh.pages_write(st.k[:, :5].contiguous(), st.v[:, :5].contiguous(), *pools, t, ints([62, 0], dev), off)
+        t, missing = mh.pages_fork(pools, t, refs, ints([0, 0], dev), ints([0, 67], dev), 32)
+        assert int(missing) == 0
+        mh.pages_copy(pools, t[0, :1].contiguous(), t[1, 2:3].contiguous())
+        mh.pages_free(t, refs, ints([0, 0], dev), ints([3, 0], dev))
+        mh.pages_compact(pools, t, refs)
+    assert same()
+
+
+def test_two_at_once(dev):
+    """Two calls on two streams, each with a workspace of its own, again and again."""
+    sts = [streams(i, dev, tree=True) for i in (7, 17)]
+    want = [st.run(window=90) for st in sts]
+    side = [torch.cuda.Stream() for _ in sts]
+    ws = [torch.empty(mh.flash_attn_pages_128_workspace_bytes(st.q, st.k, st.v, st.k_pages, st.v_pages, ints(st.lines, dev)),
+                      dtype=torch.uint8, device=dev) for st in sts]
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for n, st in enumerate(sts):
+            with torch.cuda.stream(side[n]):
+                got[n].append(st.run(window=90, workspace=ws[n]))
+    torch.cuda.synchronize()
+    for n in (0, 1):
+        for out in got[n]:
+            assert torch.equal(out, want[n])
