@@ -792,18 +792,21 @@ def _head_rows(t, name, layout):
         raise TypeError(f"{name}: expected a tensor")
     if t.dtype != torch.bfloat16:
         raise ValueError(f"{name}: dtype {t.dtype}, expected {torch.bfloat16}")
-    if t.dim() != (3 if layout == "heads" else 2):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != (3 if layout == "heads" else 2):
         raise ValueError(f"{name}: [heads][rows][128] for layout 'heads', [rows][heads * 128] for 'rows'")
-    if t.shape[-1] and t.stride(-1) != 1:
+    if stride[-1] != 1 and shape[-1]:
         raise ValueError(f"{name}: the last dimension must be contiguous")
+    # A dimension of one element may carry any stride: it is never stepped over.
     if layout == "heads":
-        if t.shape[2] != 128:
+        heads, rows, width = shape
+        if width != 128:
             raise ValueError(f"{name}: rows of 128 values")
-        # A dimension of one element may carry any stride: it is never stepped over.
-        return (t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 128)
-    if t.shape[1] == 0 or t.shape[1] % 128:
+        return heads, rows, stride[0] if heads > 1 else 0, stride[1] if rows > 1 else 128
+    rows, width = shape
+    if width == 0 or width % 128:
         raise ValueError(f"{name}: rows of heads * 128 values")
-    return t.shape[1] // 128, t.shape[0], 128, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return width // 128, rows, 128, stride[0] if rows > 1 else width
 
 
 def attn_ranges(q_off, k_off, q_rows, kv_rows, *, prefix=None, causal=False, ranges=None):
