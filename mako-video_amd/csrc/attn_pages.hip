@@ -981,14 +981,17 @@ extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (const int rc = a.cap > 0.0f ? launch_pages<true>(p, s) : launch_pages<false>(p, s); rc != MH3_OK)
         return rc;
-    // As many workgroups as there may be pieces, of one a CU to four (five cases at one, two and four, us: 6.2, 6.4 and 7.1;
-    // 11.4, 8.0 and 7.3; 4.2, 4.4 and 5.0; 10.0, 7.9 and 7.0; 5.2, 5.2 and 5.3).
+    // Waves to a row's parts where items have many (eight parts or so), and as many workgroups as there may be pieces of
+    // rows, of one a CU to four (five cases at one, two and four, us: 6.2, 6.4 and 7.1; 11.4, 8.0 and 7.3; 4.2, 4.4 and 5.0;
+    // 10.0, 7.9 and 7.0; 5.2, 5.2 and 5.3).
     const uint64_t cus = uint64_t(std::max(host::cu_count(), 1)), list = uint64_t(a.q_rows) * p.group;
-    const uint64_t pieces = p.kv_heads * (list / (p.item_rows > 32u ? 8u : 2u) + list / p.item_rows + t.streams);
+    const uint64_t items = p.kv_heads * (list / p.item_rows + std::min(t.streams, a.q_rows));
+    const bool split = p.workers > 8u * items;
+    const uint64_t pieces = items + p.kv_heads * list / (split ? 2u : 8u);
     const uint32_t joiners = uint32_t(std::min(std::max(pieces, cus), 4u * cus));
-    if (p.item_rows > 32u)
-        hipLaunchKernelGGL(attn_pages_join_kernel<1u>, dim3(joiners), dim3(256), 0, s, p);
-    else
+    if (split)
         hipLaunchKernelGGL(attn_pages_join_kernel<4u>, dim3(joiners), dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL(attn_pages_join_kernel<1u>, dim3(joiners), dim3(256), 0, s, p);
     return host::check_launch();
 }
