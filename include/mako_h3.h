@@ -422,8 +422,8 @@ int mh3_attn_window_ranges(const MH3WindowArgs* args, const int32_t* q_off, cons
  * A pool is `pages` pages of page_bytes, each in one piece, page_stride bytes apart (multiples of 16, the base 16-byte
  * aligned): of whatever a program keeps by rows, say a layer's keys, or all layers' keys and values. Calls take up to
  * MH3_MAX_POOLS pools (a host array), which may not overlap each other, the table, refs or another list, each taken as
- * the span from its first page to its last one's end (MH3_ERR_PARAM; so for all in- and outputs below). int32 lists and tables are 4-byte aligned, workspaces 16; a call that overlaps
- * another in time needs its own workspace. */
+ * the span from its first page to its last one's end (MH3_ERR_PARAM; so for all in- and outputs below). int32 lists and
+ * tables are 4-byte aligned, workspaces 16; a call that overlaps another in time needs its own workspace. */
 enum { MH3_MAX_POOLS = 64, MH3_MAX_STREAMS = 4096, MH3_MAX_PAIRS = 16384 };
 typedef struct MH3PagesArgs {
     uint32_t streams;      /* 1 .. MH3_MAX_STREAMS */

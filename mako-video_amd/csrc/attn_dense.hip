@@ -819,7 +819,8 @@ int launch_form(const DenseParams& p, uint32_t waves, hipStream_t stream)
 {
     if (waves == kPairWaves)
         return launch_rows(attn_pair_kernel<CAP, BIAS, SINKS>,
-                           2u * kRing * kTileBytes + (2048u + 16u + 4u + (SINKS ? 512u + 16u : 0u)) * kPairWaves, p, waves, stream);
+                           2u * kRing * kTileBytes + (2048u + 16u + 4u + (SINKS ? 512u + 16u : 0u)) * kPairWaves, p, waves,
+                           stream);
     return launch_rows(attn_few_kernel<CAP, BIAS, SINKS>, 2u * kTileBytes + 1024u + 512u, p, waves, stream);
 }
 
@@ -897,7 +898,8 @@ extern "C" int mh3_flash_attn_128_sinks(const MH3DenseAttnArgs* args, const uint
         if (plan.tiles * a.kv_heads * plan.splits * plan.waves * 64u >= (1ull << 31))
             return MH3_ERR_SHAPE;
     DenseParams p{};
-    p.q = q, p.k = k, p.v = v, p.out = out, p.ranges = ranges, p.sinks = sinks, p.slopes = slopes, p.q_pos = q_pos, p.k_pos = k_pos;
+    p.q = q, p.k = k, p.v = v, p.out = out, p.ranges = ranges, p.sinks = sinks, p.slopes = slopes;
+    p.q_pos = q_pos, p.k_pos = k_pos;
     p.part = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kHeader) : nullptr;
     p.qhs = a.q_head_stride, p.qrs = a.q_row_stride, p.khs = a.k_head_stride, p.krs = a.k_row_stride;
     p.vhs = a.v_head_stride, p.vrs = a.v_row_stride, p.ohs = a.out_head_stride, p.ors = a.out_row_stride;

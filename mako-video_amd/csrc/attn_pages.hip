@@ -23,13 +23,14 @@
 //   same run, one row tile each, so that what one of them has read the others find in their XCD's L2 (two frames of 510
 //   rows, 56 heads, 4080 rows back and the 435 first: 209 us, and 188 since).
 // What bounds it, by what a call has most of (5 TB/s is what a copy of 1 GiB reaches here):
-// - One new row a stream: the one pass over K and V. 129,536 kept rows of three streams, 40 heads on 8: 95 us, 5.6 TB/s, and 7
-//   for the join; of 64 streams under a window of 1020 rows, 240 MB: 49 and 7.
+// - One new row a stream: the one pass over K and V. 129,536 kept rows of three streams, 40 heads on 8: 97 us, 5.5 TB/s, and 6
+//   for the join; of 64 streams under a window of 1020 rows, 240 MB: 49 and 5.
 // - Small trees: a part's begin (the streams' sums, the pages' numbers, the rows' lines) beside few turns: eight rows after
-//   2985 kept, 56 heads, 23 us and 9 for the join, the pass over K and V alone 17.
+//   2985 kept, 56 heads, 24 us and 4 for the join, the pass over K and V alone 17.
 // - Larger trees: the turns. Five of 63 rows after 129,536 kept in all, 40 heads on 8: 160 list rows an item leave three of
-//   eight waves without rows; 127 turns of 1.55 us and some 20 to begin and to join: 226.
-// - Chunks: products and softmax in turn, K and V from HBM: those frames' 79 turns take 2 us each, the clock at 1.8 .. 2.1 GHz
+//   eight waves without rows; 136 turns of 1.5 us or more, by the card and its clock (with zeros for all values 203 us for
+//   241), and some 25 to begin and to join: 226 .. 275.
+// - Chunks: products and softmax in turn, K and V from HBM: those frames' 80 turns take 2 us each, the clock at 1.8 .. 2.1 GHz
 //   and the matrix cores busy 38 .. 43% of it.
 // Most of the eight-wave kernel's 38 registers in scratch are those of the list of parts; the loop of whole tiles reads none.
 #include "attn_tiles.hpp"
@@ -158,7 +159,10 @@ struct Streams {
         sum(p, from, base, of_lane(p, from, lane), sharing, lane);
     }
     // The last stream that begins at piece x or before it and has any, x one of the 64's.
-    __device__ __forceinline__ uint32_t of(uint64_t x) const { return 63u - uint32_t(__builtin_clzll(__ballot(before <= x) & some)); }
+    __device__ __forceinline__ uint32_t of(uint64_t x) const
+    {
+        return 63u - uint32_t(__builtin_clzll(__ballot(before <= x) & some));
+    }
 };
 
 struct Shares : Sharing {
@@ -323,8 +327,8 @@ __device__ __forceinline__ Piece piece_of(const PagesParams& p, const Item& it, 
 {
     if (kept) {
         const uint32_t r = key - p.div_page.div(key) * p.page_rows;
-        const uint64_t at = uint64_t(uint32_t(max(page, 0))) * (VALUE ? p.vps : p.kps) + uint64_t(r) * (VALUE ? p.vprs : p.kprs) +
-                            it.kvh * (VALUE ? p.vphs : p.kphs);
+        const uint64_t at = uint64_t(uint32_t(max(page, 0))) * (VALUE ? p.vps : p.kps) +
+                            uint64_t(r) * (VALUE ? p.vprs : p.kprs) + it.kvh * (VALUE ? p.vphs : p.kphs);
         const uint32_t rows = page >= 0 && key < it.st.kept ? min(n, it.st.kept - key) : 0u;
         return {reinterpret_cast<uint64_t>((VALUE ? p.v_pages : p.k_pages) + at),
                 rows ? (rows - 1u) * uint32_t(VALUE ? p.vprs : p.kprs) * 2u + 256u : 0u};
@@ -862,7 +866,8 @@ int check_pages_args(const MH3PagesAttnArgs* args)
         return MH3_ERR_SHAPE;
     if (a.head_dim != 128u)
         return MH3_ERR_UNSUPPORTED;
-    if (a.zero_rest > 1u || !(a.scale >= 0.0f && a.scale <= 0x1p100f) || !(a.cap == 0.0f || (a.cap >= 0x1p-60f && a.cap <= 1024.0f)))
+    if (a.zero_rest > 1u || !(a.scale >= 0.0f && a.scale <= 0x1p100f) ||
+        !(a.cap == 0.0f || (a.cap >= 0x1p-60f && a.cap <= 1024.0f)))
         return MH3_ERR_PARAM;
     if (t.streams == 0 || t.streams > MH3_MAX_STREAMS || t.cols == 0 || t.cols >= (1u << 24) || t.pages == 0 ||
         t.pages >= (1u << 24) || t.table_stride < t.cols || t.table_stride >= (1ull << 32) || t.page_rows == 0 ||
@@ -900,8 +905,8 @@ template <bool CAP>
 int launch_pages(const PagesParams& p, hipStream_t stream)
 {
     if (p.item_rows > 32u)
-        return launch_items(attn_pages_pair_kernel<CAP>, kPairWaves, 2u * kRing * kTileBytes + (kPairWaveBytes + 4u) * kPairWaves + 4u * kParents, p,
-                            stream);
+        return launch_items(attn_pages_pair_kernel<CAP>, kPairWaves,
+                            2u * kRing * kTileBytes + (kPairWaveBytes + 4u) * kPairWaves + 4u * kParents, p, stream);
     return launch_items(attn_pages_kernel<CAP>, 1u, 2u * kTileBytes + 1024u + 4u * kParents, p, stream);
 }
 
@@ -981,9 +986,9 @@ extern "C" int mh3_flash_attn_pages_128(const MH3PagesAttnArgs* args, const uint
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (const int rc = a.cap > 0.0f ? launch_pages<true>(p, s) : launch_pages<false>(p, s); rc != MH3_OK)
         return rc;
-    // Waves to a row's parts where items have many (eight parts or so), and as many workgroups as there may be pieces of
-    // rows, of one a CU to four (five cases at one, two and four, us: 6.2, 6.4 and 7.1; 11.4, 8.0 and 7.3; 4.2, 4.4 and 5.0;
-    // 10.0, 7.9 and 7.0; 5.2, 5.2 and 5.3).
+    // Four waves to a row's parts where items have many (with two parts an item, 64 streams' single rows, 7.2 us, and 5.4 with
+    // one wave), and as many workgroups as there may be pieces of rows, of one a CU to four (five cases at one, two and four,
+    // us: 6.2, 6.4 and 7.1; 11.4, 8.0 and 7.3; 4.2, 4.4 and 5.0; 10.0, 7.9 and 7.0; 5.2, 5.2 and 5.3).
     const uint64_t cus = uint64_t(std::max(host::cu_count(), 1)), list = uint64_t(a.q_rows) * p.group;
     const uint64_t items = p.kv_heads * (list / p.item_rows + std::min(t.streams, a.q_rows));
     const bool split = p.workers > 8u * items;

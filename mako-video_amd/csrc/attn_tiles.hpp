@@ -469,9 +469,9 @@ __device__ __forceinline__ float tile_exponentials(const floatx16 (&s)[2], TileP
     return sum[0] + sum[1];
 }
 
-// The softmax of a tile at key t0 (MASKED: not every row attends all of it, but the keys that `seen` says): P^T, and the rows' maxima, sums and (where a
-// maximum moved) rescaled O. BIAS: kp and near_pos are LDS for the tile's positions; sloped: tile_products has taken the
-// bias off, if the positions are near.
+// The softmax of a tile at key t0 (MASKED: not every row attends all of it, but the keys that `seen` says): P^T, and the
+// rows' maxima, sums and (where a maximum moved) rescaled O. BIAS: kp and near_pos are LDS for the tile's positions; sloped:
+// tile_products has taken the bias off, if the positions are near.
 template <bool CAP, bool BIAS, bool MASKED, class Seen>
 __device__ __forceinline__ void tile_softmax(const DenseParams& p, WaveRows& w, floatx16 (&s)[2], TileP& pt, uint32_t t0,
                                              const Seen& seen, const int32_t* kp, float* near_pos, bool sloped, bool near,

@@ -5,8 +5,9 @@ The op names are the reference's kernel names (mako-common's `rms_mod_rows`, `ga
 with the dense path beside them (`rotary_axes`, `heads_partial_axes`, `flash_attn_128`, `attn_ranges`,
 `attn_window_ranges`, `quant_rows_mx4`, `gemm_mx4*`, and for streams over pages `pages_*` and `flash_attn_pages_128`, which
 also run on the GPU that their tensors are on where it is not the current one), and errors raise RuntimeError as the
-reference's host code throws std::runtime_error on a bad call (src/video/audio_vae.cpp:231-232). Every call checks the tensors against the sizes the kernel will touch before it
-reaches the library, launches on torch's current stream, and returns without synchronizing.
+reference's host code throws std::runtime_error on a bad call (src/video/audio_vae.cpp:231-232). Every call checks the
+tensors against the sizes the kernel will touch before it reaches the library, launches on torch's current stream, and
+returns without synchronizing.
 
 torch is used here only for device memory and streams; the compute is the library's HIP kernels. There is no
 fallback: if libmako_h3.so is missing, importing this module raises.
@@ -1072,8 +1073,8 @@ def pages_compact(pools, table, refs, *, map=None, used=None, workspace=None):
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     device = _page_lists(table, refs, pages, (map, "map", torch.int32, pages), (used, "used", torch.int32, 1),
                          (workspace, "workspace", torch.uint8, nbytes), pools=pools)
-    _on(device, "pages_compact", lib.mh3_pages_compact, ref, held, n_pools, table.data_ptr(), refs.data_ptr(), map.data_ptr(), used.data_ptr(),
-        workspace.data_ptr(), workspace.numel())
+    _on(device, "pages_compact", lib.mh3_pages_compact, ref, held, n_pools, table.data_ptr(), refs.data_ptr(),
+        map.data_ptr(), used.data_ptr(), workspace.data_ptr(), workspace.numel())
     return map, used
 
 
