@@ -348,3 +348,17 @@ def test_two_at_once(dev):
     for n in (0, 1):
         for out in got[n]:
             assert torch.equal(out, want[n])
+
+
+def test_lengths_and_offsets_past_their_ends(dev):
+    """Lengths below zero and past the table, and offsets before the first row and past the last, are those ends'."""
+    st = streams(8, dev)  # two streams
+    table, rows = ints(st.lines, dev), st.q.shape[1]
+    full = len(st.lines[0]) * st.page
+    run = lambda n, off: mh.flash_attn_pages_128(st.q, st.k, st.v, st.k_pages, st.v_pages, table, ints(n, dev),  # noqa: E731
+                                                 ints(off, dev), window=300, sinks=ints([5, 5], dev))
+    assert torch.equal(run([-5, 0], [0, 7, rows]), run([0, 0], [0, 7, rows]))
+    assert torch.equal(run([-2 ** 31, 64], [-9, 7, rows + 100]), run([0, 64], [0, 7, rows]))
+    # What the pages hold past the rows that were kept is NaN, so that only finite places are compared.
+    st.k_pages, st.v_pages = st.k_pages.nan_to_num(0.25), st.v_pages.nan_to_num(0.25)
+    assert torch.equal(run([2 ** 31 - 1, full + 1], [0, 7, rows]), run([full, full], [0, 7, rows]))

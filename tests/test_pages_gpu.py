@@ -366,3 +366,26 @@ def test_captured(dev):
         torch.cuda.synchronize()
         m.same(table, refs)
         assert torch.equal(pool, want)
+
+
+def test_nothing_to_do(dev):
+    """Empty lists and spans, streams that go on from themselves, pages that lie together: everything stays as it is."""
+    g = torch.Generator(device=dev).manual_seed(9)
+    pool = torch.randn((6, 2, 16, 128), generator=g, device=dev).to(torch.bfloat16)
+    pools, want = [pool, pool.clone()], pool.clone()
+    table, refs = ints([[0, 2, -1], [1, -1, -1]], dev), ints([1, 1, 1, 0, 0, 0], dev)
+    table0, refs0 = table.clone(), refs.clone()
+    assert int(mh.pages_take(table, refs, ints([3, 2], dev), ints([1, 2], dev))) == 0
+    mh.pages_free(table, refs, ints([2, 9], dev), ints([2, 3], dev))
+    mh.pages_copy(pools, ints([], dev), ints([], dev))
+    off = ints([0, 0, 0], dev)
+    rows = torch.zeros((2, 4, 128), dtype=torch.bfloat16, device=dev)
+    mh.pages_write(rows, rows, *pools, table, ints([0, 0], dev), off)
+    mh.pages_write(rows, rows, *pools, table, ints([0, 0], dev), off, rows=ints([], dev))
+    mh.pages_write(rows[:, :0], rows[:, :0], *pools, table, ints([0, 0], dev), off)
+    fresh, missing = mh.pages_fork(pools, table, refs, ints([0, 1], dev), ints([1000, -4], dev), 16)
+    moved, used = mh.pages_compact(pools, table, refs)
+    assert int(missing) == 0 and int(used) == 3 and moved.tolist() == [0, 1, 2, -1, -1, -1]
+    for t in (table, fresh):
+        assert torch.equal(t, table0)
+    assert torch.equal(refs, refs0) and all(torch.equal(p, want) for p in pools)
