@@ -474,8 +474,10 @@ int mh3_pages_compact(const MH3PagesArgs* args, const MH3Pool* pools, uint32_t n
  * the n_rows rows of k and v that is, for the accepted ones of drafted rows. k and v are bf16 heads as in
  * mh3_flash_attn_128; element (page, head, row, d) of the pools k_pages and v_pages lies at page * page_stride + head *
  * page_head_stride + row * page_row_stride + d of each (elements, multiples of 8; rows 128 .. 2^23 - 1 apart), so pages of
- * head tiles, of [page_rows][kv_heads * 128] rows, and one layer's slices of pages that hold several, are all taken. A row
- * whose place or page does not exist is passed over. Two streams that write the same row of a shared page leave either's. */
+ * head tiles, of [page_rows][kv_heads * 128] rows, and one layer's slices of pages that hold several, are all taken. A
+ * pool's rows lie apart (from the smallest stride to the largest, each steps over all that the smaller ones span) and, if both
+ * have the same strides, apart from the other pool's; else MH3_ERR_PARAM. A row whose place or page does not exist is passed
+ * over. Two streams that write the same row of a shared page leave either's. */
 typedef struct MH3PagesWriteArgs {
     MH3PagesArgs table;
     uint32_t kv_heads;

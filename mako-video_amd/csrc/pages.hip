@@ -547,6 +547,49 @@ bool in_pools(const Pools& pools, uint32_t pages, const host::Span (&spans)[N])
     return false;
 }
 
+// How often something repeats, and elements from one to the next.
+struct Repeat {
+    uint64_t n, stride;
+};
+
+// Whether rows of 128 elements that repeat so lie apart: from the smallest stride to the largest, each steps over all that
+// the smaller ones span. The other layouts without a shared element (strides that miss each other by their factors) are no
+// nest of dimensions, and count as none.
+template <size_t N>
+bool rows_apart(Repeat (&dims)[N])
+{
+    std::sort(dims, dims + N, [](const Repeat& a, const Repeat& b) { return a.stride < b.stride; });
+    uint64_t span = 128;
+    for (const Repeat& d : dims) {
+        if (d.n <= 1u)
+            continue;
+        if (d.stride < span)
+            return false;
+        span += (d.n - 1u) * d.stride;
+    }
+    return true;
+}
+
+// Whether two pools of the same strides, `offset` elements apart, share none: a pair of such rows repeats as they do, and
+// seen from any repetition of the largest stride the other pool's rows are its remainder on, or as many short of the next.
+bool pools_apart(uint64_t pages, uint64_t page, uint64_t heads, uint64_t head, uint64_t rows, uint64_t row, uint64_t offset)
+{
+    Repeat dims[] = {{pages, page}, {heads, head}, {rows, row}};
+    uint64_t largest = 0, span = 128;
+    for (const Repeat& d : dims)
+        if (d.n > 1u)
+            largest = std::max(largest, d.stride), span += (d.n - 1u) * d.stride;
+    if (offset >= span)
+        return true;
+    const uint64_t on = largest ? offset % largest : offset;
+    for (const uint64_t step : {on, largest > on ? largest - on : on}) {
+        Repeat all[] = {{2u, step}, dims[0], dims[1], dims[2]};
+        if (rows_apart(all))
+            return true;
+    }
+    return false;
+}
+
 uint32_t copy_blocks(uint64_t items) { return uint32_t(std::min<uint64_t>(items, 8u * uint64_t(host::cu_count()))); }
 
 } // namespace
@@ -724,10 +767,22 @@ extern "C" int mh3_pages_write(const MH3PagesWriteArgs* args, const uint16_t* k,
         if (s >= (1ull << 36))
             return MH3_ERR_SHAPE;
     }
+    // A pool's rows apart from each other, as out's of the attention.
+    Repeat kd[] = {{a.table.pages, a.k_page_stride}, {a.kv_heads, a.k_page_head_stride}, {a.table.page_rows, a.k_page_row_stride}};
+    Repeat vd[] = {{a.table.pages, a.v_page_stride}, {a.kv_heads, a.v_page_head_stride}, {a.table.page_rows, a.v_page_row_stride}};
+    if (!rows_apart(kd) || !rows_apart(vd))
+        return MH3_ERR_PARAM;
     if (a.n == 0 || a.n_rows == 0)
         return MH3_OK;
     if (!k || !v || !k_pages || !v_pages || !table || !starts || !off)
         return MH3_ERR_POINTER;
+    // And from the other pool's, where both have the same strides; else only the same pool twice is told.
+    const uint64_t from = reinterpret_cast<uintptr_t>(k_pages), to = reinterpret_cast<uintptr_t>(v_pages);
+    if (from == to || (a.k_page_stride == a.v_page_stride && a.k_page_head_stride == a.v_page_head_stride &&
+                       a.k_page_row_stride == a.v_page_row_stride &&
+                       !pools_apart(a.table.pages, a.k_page_stride, a.kv_heads, a.k_page_head_stride, a.table.page_rows,
+                                    a.k_page_row_stride, (from < to ? to - from : from - to) / 2u)))
+        return MH3_ERR_PARAM;
     if (!host::aligned16(k) || !host::aligned16(v) || !host::aligned16(k_pages) || !host::aligned16(v_pages) ||
         !aligned4(table) || !aligned4(starts) || !aligned4(off) || !aligned4(rows))
         return MH3_ERR_ALIGN;
@@ -744,7 +799,7 @@ extern "C" int mh3_pages_write(const MH3PagesWriteArgs* args, const uint16_t* k,
     // Each pool by itself: those of a layer's keys and values may lie in one another's gaps.
     const host::Span ko[] = {{k_pages, pool(a.k_page_stride, a.k_page_head_stride, a.k_page_row_stride)}};
     const host::Span vo[] = {{v_pages, pool(a.v_page_stride, a.v_page_head_stride, a.v_page_row_stride)}};
-    if (k_pages == v_pages || host::any_overlap(in, ko) || host::any_overlap(in, vo))
+    if (host::any_overlap(in, ko) || host::any_overlap(in, vo))
         return MH3_ERR_PARAM;
     WriteParams p{};
     p.k = k, p.v = v, p.k_pages = k_pages, p.v_pages = v_pages;
