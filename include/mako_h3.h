@@ -418,7 +418,8 @@ int mh3_attn_window_ranges(const MH3WindowArgs* args, const int32_t* q_off, cons
  * [streams][cols], table_stride ints from a stream's first entry to the next one's; an entry of -1 is no page, and every
  * call takes other numbers outside [0, pages) for none too. refs is int32 [pages]: how many of the table's entries name
  * each page; a page is free if that is zero, and nothing else is kept of it. Streams may share pages (fork). The results of
- * every call follow from its inputs: nothing depends on the order in which the GPU gets to it.
+ * every call follow from its inputs, and nothing depends on the order in which the GPU gets to it, with one exception: rows
+ * that one mh3_pages_write writes twice.
  * A pool is `pages` pages of page_bytes, each in one piece, page_stride bytes apart (multiples of 16, the base 16-byte
  * aligned): of whatever a program keeps by rows, say a layer's keys, or all layers' keys and values. Calls take up to
  * MH3_MAX_POOLS pools (a host array), which may not overlap each other, the table, refs or another list, each taken as
@@ -477,7 +478,9 @@ int mh3_pages_compact(const MH3PagesArgs* args, const MH3Pool* pools, uint32_t n
  * head tiles, of [page_rows][kv_heads * 128] rows, and one layer's slices of pages that hold several, are all taken. A
  * pool's rows lie apart (from the smallest stride to the largest, each steps over all that the smaller ones span) and, if both
  * have the same strides, apart from the other pool's; else MH3_ERR_PARAM. A row whose place or page does not exist is passed
- * over. Two streams that write the same row of a shared page leave either's. */
+ * over. A row of a page that a call writes more than once (by two streams that share the page, or by one whose table names it
+ * twice) holds pieces of 16 bytes of any of those writes afterwards, K's and V's independently: streams that go on from a
+ * shared row fork first. */
 typedef struct MH3PagesWriteArgs {
     MH3PagesArgs table;
     uint32_t kv_heads;

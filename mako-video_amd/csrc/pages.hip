@@ -3,8 +3,10 @@
 // the entries that name page p, and a page is free if that is zero, so the table and refs are all of the state.
 //
 // What the calls decide is a function of their inputs alone: free pages are taken lowest first, for the entries in the
-// order (stream, entry); counts change by integer atomics, whose order does not show. Entries that are no page of the pool
-// (negative, or past its end) are no page to any kernel, so a bad table reads and writes nothing outside the pool.
+// order (stream, entry); counts change by integer atomics, whose order does not show. (Only rows that one pages_write writes
+// twice, into a page that two entries name, are any mixture of the two: finding them would take a look at the other streams'
+// entries for each row.) Entries that are no page of the pool (negative, or past its end) are no page to any kernel, so a
+// bad table reads and writes nothing outside the pool.
 // A program calls them once a step (fork, free, compact: now and then), for all layers: what bounds them is the launches
 // (take and write 4.5 us each, a fork of eight streams 4.3 to plan and 4.3 to do) and, where pages move, HBM: 512 pages of
 // 262 KB copied in 54 us, 5 TB/s, two of five streams' pages freed and 510 MB moved in 96.

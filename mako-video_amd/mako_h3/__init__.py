@@ -1105,8 +1105,9 @@ def pages_write(k, v, k_pages, v_pages, table, starts, off, *, rows=None, layout
     """New rows into their pages: of the rows j, those of stream s are off[s] .. off[s + 1] - 1 (int32 [streams + 1]), and
     row j goes to kept row starts[s] + j - off[s] (int32 [streams]) of its stream. rows (int32 [n]): which row of k and v
     row j is (None: j itself). k, v bf16 heads as flash_attn_128 takes them (`layout`); the pools bf16
-    [pages][heads][page rows][128] ("heads") or [pages][page rows][heads * 128] ("rows"), slices of wider pages too. A row
-    whose page is missing is passed over."""
+    [pages][heads][page rows][128] ("heads") or [pages][page rows][heads * 128] ("rows"), slices of wider pages too; their
+    rows may not lie over each other. A row whose page is missing is passed over; one that two streams of a shared page both
+    write is any mixture of the two (pages_fork gives each its own)."""
     if layout not in ("heads", "rows") or page_layout not in ("heads", "rows"):
         raise ValueError("layout is 'heads' or 'rows'")
     kv_heads, n_rows, khs, krs = _head_rows(k, "k", layout)
