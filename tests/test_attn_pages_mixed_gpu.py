@@ -134,3 +134,26 @@ def test_infinities_that_rows_attend(dev, i):
         assert torch.equal(got[:, ~rows, column], clean[:, ~rows, column])
     others = [d for d in range(128) if d not in (5, 9)]
     assert torch.equal(got[:, :, others], clean[:, :, others])
+
+
+@pytest.mark.parametrize("scale,cap", [(2.0 ** 20, 0.0), (2.0 ** 100, 0.0), (2.0 ** -40, 0.0), (2.0 ** 30, 7.0), (0.1, 2.0 ** -60),
+                                       (0.1, 1024.0)])
+@pytest.mark.parametrize("heads,kv_heads,kept,new", [(8, 2, [700, 33], [3, 40]), (16, 2, [1500], [90])])
+def test_scores_to_the_ends_of_their_range(dev, heads, kv_heads, kept, new, scale, cap):
+    """Values of -1, 0 and 1 make the products exact and tie many of them: with a large scale the ties of each row's maximum
+    share its probability, whichever tile or part they lie in; with a tiny one, or under a tiny cap, all keys do."""
+    st = Mixed(9, dev, heads, kv_heads, 32, kept, new, sinks=[20] * len(kept))
+    for x in (st.q, st.k, st.k_pages):
+        x.copy_(x.nan_to_num(0.0).clamp(-1.4, 1.4).round())
+    for window in (0, 200):
+        check(st.run(window=window, scale=scale, cap=cap), *st.want(window=window, scale=scale, cap=cap))
+    # The same rows in one piece, under the same window.
+    s = len(kept) - 1
+    mine = slice(st.q_off[s], st.q_off[s + 1])
+    k, v = (torch.cat([st.kept_rows(p, s)[0], x[:, mine]], 1) for p, x in ((st.k_pages, st.k), (st.v_pages, st.v)))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    ranges, first = mh.attn_window_ranges(ints([0, new[s]]), ints([0, kept[s] + new[s]]), new[s], kept[s] + new[s], 200,
+                                          sinks=ints([20]))
+    want, mag = st.want(window=200, scale=scale, cap=cap)
+    check(mh.flash_attn_128(st.q[:, mine].contiguous(), k, v, ranges=ranges, sinks=first, scale=scale, cap=cap),
+          want[:, mine], mag[:, mine])
