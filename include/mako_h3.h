@@ -510,7 +510,11 @@ int mh3_pages_write(const MH3PagesWriteArgs* args, const uint16_t* k, const uint
  * q_off[streams] on) become zero or keep what out holds (zero_rest).
  *   workspace: mh3_flash_attn_pages_128_workspace_bytes(args) bytes; the call overwrites it, so calls that overlap in time,
  *            two captured graphs among them, need their own.
- * out may not overlap an input, the pools or the workspace (MH3_ERR_PARAM). */
+ * out may not overlap an input, the pools or the workspace (MH3_ERR_PARAM).
+ * What it is fast for is streams with about as many new rows each, up to some hundreds. The host does not see q_off: the kernel
+ * is chosen by the new rows that a stream of the table has on average, those without any included, so a few long runs in a
+ * table of many idle streams take up to twice as long as in a table of their own rows; and the work of a run of new rows
+ * grows with their square under any window. */
 typedef struct MH3PagesAttnArgs {
     MH3PagesArgs table;
     uint32_t heads; /* query heads, a multiple of kv_heads */

@@ -37,8 +37,8 @@
 // clock at 1.65 to 1.7 GHz and the matrix cores busy 72% of it); under a cap also the vector unit's transcendentals (five
 // clips packed into 14,925 rows of 40 heads 1475 us, without a cap 1230, with a multiplication in the place of the cap's
 // exponential and reciprocal 1260); under a window also the turns that are masked and each workgroup's begin (960 x 544,
-// 4080 keys back and the 435 first: 2159 us for 75 tiles a workgroup, 1.74 us a whole turn, 2.9 a masked one of which there are
-// some nine, 4.7 the first, 5.8 before it, and 5 until the CU has its next workgroup); few rows, the one pass over K and V
+// 4080 keys back and the 435 first: 2160 .. 2290 us by card for 75 tiles a workgroup, 1.74 us a whole turn, 2.9 a masked one of
+// which there are some nine, 4.7 the first, 5.8 before it, and 5 until the CU has its next workgroup); few rows, the one pass over K and V
 // (129,536 keys of 8 heads in 95 us, 5.5 TB/s).
 // Under a bias the eight-wave kernels hold six or seven registers in scratch, read between the loops, in masked turns and in
 // rare paths, never in the loop of whole tiles; with a second range twenty, six of which each turn reads.
@@ -748,6 +748,10 @@ Plan plan_of(const MH3DenseAttnArgs& a, uint32_t waves)
 // plan: more of them than plan_of's is faster there too, or costs little (us, plan_of's splits and these: 56, 51 x 14,922 4
 // 100 and 9 90; 16, 39 x 29,920 16 54 and 32 45; 392 on 56, 9 x 11,066 4 79 and 9 70; 35 on 7, 11 x 69,694 36 67 and
 // 73 70; 7, 34 x 75,312 36 72 and 73 74).
+// Nor do calls with a second range of keys, as few_has_less counts one a row: they take the first plan, made as if each row
+// attended all keys, where the same rows with one range may find the other kernel or be held up by the look (us, both ranges
+// of a window of 1020 keys and 16 first ones, and the window's alone; documents of 1024 keys each, 40 on 8: 64 x 1 124 and 77,
+// 8 x 64 69 and 85).
 struct Plans {
     Plan first, second;
     uint64_t list;

@@ -119,6 +119,12 @@ __device__ __forceinline__ Stream stream_of(const PagesParams& p, uint32_t s, ui
 // How the items' tiles are shared out: runs of `share` pieces, each taken by `together` workgroups, a row tile each (if all
 // streams' items have as many row tiles; else 1, and row tiles count one by one). A piece is a tile, or with `size` an
 // item's equal part of so many tiles at most.
+// An item's tiles are its stream's: those that its own rows do not see (new rows behind its last one, and under a window kept
+// and new ones that it has left behind) take masked turns that add nothing. That is little for the trees and frames that this
+// is for, but long chunks grow with the square of their rows (40 heads on 8, 4096 kept, a window of 64, 510 / 1000 / 2000 /
+// 4000 new rows 36 / 51 / 115 / 332 us, and in one piece through flash_attn_128 47 / 17 / 33 / 49). Nor do all
+// workgroups have work where as many of a run's row tiles as go together do not divide them (without the window, 64 / 69 / 86 /
+// 130 / 254 row tiles on 256 workgroups: 526 / 710 / 1177 / 3161 / 5301 us, 724 / 590 / 482 / 320 / 532 TFLOP/s).
 struct Sharing {
     uint32_t together, size;
     __device__ __forceinline__ uint32_t pieces(uint32_t tiles) const { return size ? (tiles + size - 1u) / size : tiles; }
@@ -838,7 +844,8 @@ constexpr uint32_t kBegin = 3, kPairBegin = 12;
 // Which kernel a call takes, and how many rows an item has, from the list rows that its streams have on average. (One wave a
 // workgroup and eight, us, 40 heads on 8: five streams of 129,536 kept rows in all and 60 list rows each 118 and 128, 65 139
 // and 128, 100 169 and 130; three of 14,925 and 60 rows 33 and 36, 90 36 and 37, 125 41 and 40; one of 2985 within 3 of each
-// other up to 150.)
+// other up to 150.) Streams without new rows count too, as the host does not see them: two of 510 rows over 4515 kept ones take
+// 171 us in a table of two and 337 in one of 64 (56 heads; 40 on 8 136 and 222).
 struct PagesPlan {
     uint32_t item_rows, workers, slot_rows; // slot_rows: a part's, an item's or all of the call's where they are fewer
     uint64_t workspace;
